@@ -501,6 +501,116 @@ int nsmlp_absmax_dq_dequantize(const uint8_t* q, long long n, int dq_block, cons
  * pinned buffers and H2D copies, RT:3437-3493, safetensor_loader.py:172-201). */
 int nsmlp_host_device_pointer(const void* host, void** device_ptr);
 
+/* --------------------------------------------- paged K/V cache in 8 bits
+ * The attention side of a decoder layer: a cache of K and V rows in blocks of
+ * `block_tokens` tokens (16, 32 or 64), 8 bits per value with one fp32 scale
+ * per (block, K/V head) for K and one for V, the bookkeeping that hands the
+ * blocks out, and the attention that reads it.  No reference counterpart (the
+ * reference's attention and its K/V cache are torch code, RT:5927-7142).
+ *
+ * Formats: NSMLP_KV_INT8: code in -127..127, scale = largest magnitude / 127.
+ * NSMLP_KV_E4M3: OCP e4m3, scale = the smallest power of two that keeps the
+ * largest magnitude within 448.  value = code * scale.  A (block, head)'s scale
+ * never shrinks while the block is filled and is 2^-100 at least; where a call
+ * raises it, the stored codes are rewritten as code'(code * old / new), rounded
+ * to nearest even like new values.  A call that writes a block's first token
+ * starts its scale anew.  A value that is not finite makes the (block, head)'s
+ * scale NaN until then.
+ * data: [num_blocks][kv_heads][2][block_tokens * head_dim] bytes in an order of
+ * the library's own; scale: [num_blocks][kv_heads][2] (K, V).  Both are zeroed
+ * once by the caller.  head_dim 64 or 128; 16-byte aligned. */
+#define NSMLP_DTYPE_F16 0
+#define NSMLP_DTYPE_BF16 1
+#define NSMLP_KV_INT8 0
+#define NSMLP_KV_E4M3 1
+
+typedef struct nsmlp_kv_cache {
+  int num_blocks, kv_heads, head_dim, block_tokens, format;
+  uint8_t* data;
+  float* scale;
+} nsmlp_kv_cache;
+
+/* Stores K and V rows k, v [n][kv_heads][head_dim] (strides in elements,
+ * multiples of 8; the last dimension contiguous) at slots[n] (block *
+ * block_tokens + offset; a slot outside the cache, such as -1, stores nothing).
+ * The tokens of one block stand next to each other in the call, in the order
+ * of their offsets, as nsmlp_kv_plan lists them. */
+int nsmlp_kv_append(const nsmlp_kv_cache* cache, const void* k, long long k_row_stride, long long k_head_stride,
+                    const void* v, long long v_row_stride, long long v_head_stride, int dtype, const int64_t* slots, int n,
+                    void* stream);
+
+/* The stored values at slots[n], rounded to dtype: k_out, v_out
+ * [n][kv_heads][head_dim], contiguous; zeros for a slot outside the cache. */
+int nsmlp_kv_read(const nsmlp_kv_cache* cache, const int64_t* slots, int n, void* k_out, void* v_out, int dtype,
+                  void* stream);
+
+/* A batch of requests (at most 4096) on the device: their cached tokens
+ * cached[requests] (at most 2^29 each), their blocks table[requests][max_blocks] (block j of a
+ * request holds its tokens j * block_tokens ...), and the free blocks: a ring
+ * of num_blocks ids whose entries state[0], state[0] + 1, ... (modulo
+ * num_blocks), state[1] of them, are free.  q_heads and kv_heads size the
+ * attention's schedule; the attention wants q_heads a multiple of kv_heads. */
+typedef struct nsmlp_kv_batch {
+  int requests, max_blocks, num_blocks, block_tokens, q_heads, kv_heads;
+  int32_t* cached;
+  int32_t* table;
+  int32_t* ring;
+  int32_t* state;
+} nsmlp_kv_batch;
+
+/* One step of a batch.  total: tokens of the step's tensors; max_new: the most
+ * new tokens of a request (0: not known).  slots[total], q_start[requests + 1],
+ * kv_len[requests], next[requests], info[4] and the schedule
+ * (nsmlp_kv_schedule_bytes) are written by nsmlp_kv_plan. */
+typedef struct nsmlp_kv_step {
+  int total, max_new;
+  int64_t* slots;
+  int32_t* q_start;
+  int32_t* kv_len;
+  int32_t* next;
+  int32_t* info;
+  int32_t* schedule;
+  size_t schedule_bytes;
+} nsmlp_kv_step;
+
+size_t nsmlp_kv_schedule_bytes(const nsmlp_kv_batch* batch, int total, int max_new); /* 0: invalid arguments */
+
+/* Plans a step that adds new_tokens[requests] tokens: request r takes
+ * ceil((cached + new) / block_tokens) - ceil(cached / block_tokens) blocks from
+ * the ring's front, requests in order, and its table entries are written.
+ * slots: the step's tokens, request by request; q_start: where each request's
+ * tokens start; kv_len: cached + new.  A request is refused (slots -1, kv_len
+ * 0, nothing taken) where its blocks would exceed max_blocks, its new tokens
+ * max_new, or the blocks asked for up to and with it the free ones.  info:
+ * the ring's (head, count) after the step, requests refused, the sum of
+ * new_tokens.  Tokens of the step past that sum get slot -1.  The batch's
+ * lengths and ring stay as they are until nsmlp_kv_commit, so that a plan can
+ * be made again.  The schedule lists the attention's work. */
+int nsmlp_kv_plan(const nsmlp_kv_batch* batch, const int32_t* new_tokens, const nsmlp_kv_step* step, void* stream);
+
+/* Makes a step's lengths and ring state the batch's (step NULL: they stay),
+ * then ends the requests with finished[r] != 0 (NULL: none): their blocks go to
+ * the ring's end in the order of requests and of their tables, their entries
+ * become -1 and their lengths 0. */
+int nsmlp_kv_commit(const nsmlp_kv_batch* batch, const nsmlp_kv_step* step, const int32_t* finished, void* stream);
+
+/* Attention of a planned step's queries over the cache.  q [total][q_heads]
+ * [head_dim] (strides in elements, multiples of 8); query head h reads K/V head
+ * h / (q_heads / kv_heads).  Token i of a request with n new tokens sees its
+ * first kv_len - n + i + 1 keys:
+ *   out = sum_j softmax_j(scale q . k_j) v_j     [total][q_heads][head_dim]
+ *   lse = log sum_j exp(scale q . k_j)           [total][q_heads] fp32, nullable
+ * A token that sees no key (a refused request's) gets zeros and -inf; rows past
+ * the step's tokens are left as they are.  A table entry that is not a block
+ * (or past max_blocks) hides its keys and sets
+ * NSMLP_STATUS_BLOCK_UNAVAILABLE in the workspace's status word.  fp32 sums;
+ * the result does not depend on how the work is scheduled, only on the batch's
+ * lengths.  scale > 0. */
+size_t nsmlp_paged_attention_workspace_bytes(const nsmlp_kv_batch* batch, int total, int max_new, int head_dim);
+int nsmlp_paged_attention(const nsmlp_kv_cache* cache, const nsmlp_kv_batch* batch, const nsmlp_kv_step* step, const void* q,
+                          long long q_row_stride, long long q_head_stride, int dtype, float scale, void* out, float* lse,
+                          void* ws, size_t ws_bytes, void* stream);
+
 /* -------------------------------------------------------- synthetic data
  * Seeded synthetic weights for benchmarks (counter-based; the value of
  * element i depends only on (seed, i)):

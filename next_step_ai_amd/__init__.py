@@ -5,6 +5,7 @@ Modules:
               entry points (same names and signatures)
   router      the learned-basis router on the GPU (route_sparse_mlp)
   slot_table  the HBM hot-block slot table and the one-call decode layer
+  kv_cache    paged K/V cache in 8 bits, its block tables and its attention
   layout      block-bank layout contract and the active-block layout
   synth       seeded synthetic NF4 layers generated on the GPU
 """

@@ -30,6 +30,10 @@ NSMLP_DOWN_GATHERED = 1
 NSMLP_CACHE_GROW_ONLY = 1
 NSMLP_STATUS_BLOCK_UNAVAILABLE = 1
 NSMLP_STATUS_FIXED_RANGE = 2
+NSMLP_DTYPE_F16 = 0
+NSMLP_DTYPE_BF16 = 1
+NSMLP_KV_INT8 = 0
+NSMLP_KV_E4M3 = 1
 
 
 class SlotTable(ctypes.Structure):
@@ -79,6 +83,33 @@ class CacheState(ctypes.Structure):
     _fields_ = [("capacity", I32), ("lookup", P), ("slot_block", P), ("slot_score", P), ("active_count", P)]
 
 
+class KvCacheView(ctypes.Structure):
+    """Mirror of ``nsmlp_kv_cache``."""
+
+    _fields_ = [
+        ("num_blocks", I32), ("kv_heads", I32), ("head_dim", I32), ("block_tokens", I32), ("format", I32),
+        ("data", P), ("scale", P),
+    ]
+
+
+class KvBatchView(ctypes.Structure):
+    """Mirror of ``nsmlp_kv_batch``."""
+
+    _fields_ = [
+        ("requests", I32), ("max_blocks", I32), ("num_blocks", I32), ("block_tokens", I32), ("q_heads", I32),
+        ("kv_heads", I32), ("cached", P), ("table", P), ("ring", P), ("state", P),
+    ]
+
+
+class KvStepView(ctypes.Structure):
+    """Mirror of ``nsmlp_kv_step``."""
+
+    _fields_ = [
+        ("total", I32), ("max_new", I32), ("slots", P), ("q_start", P), ("kv_len", P), ("next", P), ("info", P),
+        ("schedule", P), ("schedule_bytes", SZ),
+    ]
+
+
 # name -> (restype, argtypes)
 SIGNATURES: dict[str, tuple] = {
     "nsmlp_last_error": (ctypes.c_char_p, []),
@@ -124,6 +155,14 @@ SIGNATURES: dict[str, tuple] = {
     "nsmlp_cache_workspace_bytes": (SZ, [I32]),
     "nsmlp_cache_promote": (I32, [ctypes.POINTER(SlotTable), ctypes.POINTER(CacheState), P, I32, I32, P, P, SZ, P]),
     "nsmlp_cache_record_f32": (I32, [P, I32, P, I32, I32, P, P]),
+    "nsmlp_kv_append": (I32, [ctypes.POINTER(KvCacheView), P, I64, I64, P, I64, I64, I32, P, I32, P]),
+    "nsmlp_kv_read": (I32, [ctypes.POINTER(KvCacheView), P, I32, P, P, I32, P]),
+    "nsmlp_kv_schedule_bytes": (SZ, [ctypes.POINTER(KvBatchView), I32, I32]),
+    "nsmlp_kv_plan": (I32, [ctypes.POINTER(KvBatchView), P, ctypes.POINTER(KvStepView), P]),
+    "nsmlp_kv_commit": (I32, [ctypes.POINTER(KvBatchView), ctypes.POINTER(KvStepView), P, P]),
+    "nsmlp_paged_attention_workspace_bytes": (SZ, [ctypes.POINTER(KvBatchView), I32, I32, I32]),
+    "nsmlp_paged_attention": (I32, [ctypes.POINTER(KvCacheView), ctypes.POINTER(KvBatchView), ctypes.POINTER(KvStepView),
+                                    P, I64, I64, I32, F32, P, P, P, SZ, P]),
     "nsmlp_host_device_pointer": (I32, [P, ctypes.POINTER(P)]),
     "nsmlp_synth_normal_f16": (I32, [U64, I64, F32, P, P]),
     "nsmlp_synth_normal_f32": (I32, [U64, I64, F32, P, P]),

@@ -17,23 +17,8 @@ namespace {
 
 thread_local char g_err[512] = "";
 
-constexpr size_t kAlign = 256;
-// Fixed counter region at the start of every workspace (zeroed once by
-// nsmlp_workspace_init, restored to zero by the kernels that use it).
-constexpr size_t kStatusOff = 0;
-constexpr size_t kServedOff = 16;  // [2] u32 block counts: HBM slots, host copies
-constexpr size_t kBlkCountOff = 256;
-constexpr int kMaxK = 32768;
-constexpr size_t kRowCountOff = kBlkCountOff + (size_t)kMaxK * sizeof(int);
-constexpr int kMaxRowChunks = 1024;
-constexpr size_t kCounterBytes = kRowCountOff + (size_t)kMaxRowChunks * sizeof(int) + 256;
-
 constexpr int kRowsPerChunk = 256;
 constexpr int kMaxGroups = 64;
-
-size_t align_up(size_t v) { return (v + kAlign - 1) / kAlign * kAlign; }
-
-bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
 int env_int(const char* name, int dflt) {
   const char* v = getenv(name);
@@ -146,7 +131,8 @@ const char* fault_kind_name(int code) {
   }
 }
 
-// Called first by every compute entry point: NSMLP_OK unless a rule fires.
+}  // namespace
+
 int fault_point(const char* name) {
   if (g_fault_armed.load(std::memory_order_acquire) == 0) return NSMLP_OK;
   std::lock_guard<std::mutex> lk(g_fault_mu);
@@ -161,11 +147,7 @@ int fault_point(const char* name) {
   return NSMLP_OK;
 }
 
-#define NSMLP_FAULT_POINT(name)             \
-  do {                                      \
-    const int fault_rc_ = fault_point(name); \
-    if (fault_rc_) return fault_rc_;        \
-  } while (0)
+namespace {
 
 // NF4 code values (QLoRA normal-float 4-bit table).
 const float kNF4[16] = {
@@ -565,7 +547,7 @@ extern "C" {
 
 const char* nsmlp_last_error(void) { return g_err; }
 
-int nsmlp_version(void) { return 106; }
+int nsmlp_version(void) { return 107; }
 
 int nsmlp_fault_inject(const char* spec) { return fault_set(spec); }
 

@@ -17,6 +17,29 @@ constexpr int kMaxSelect = 65535;  // selection keys pack the index in 16 bits
 // ---------------------------------------------------------------- errors --
 int set_error(int code, const char* fmt, ...);
 int check_launch(const char* what);
+// Called first by every compute entry point: NSMLP_OK unless an armed fault
+// rule fires (nsmlp_fault_inject).
+int fault_point(const char* name);
+#define NSMLP_FAULT_POINT(name)              \
+  do {                                       \
+    const int fault_rc_ = fault_point(name); \
+    if (fault_rc_) return fault_rc_;         \
+  } while (0)
+
+// ------------------------------------------------------------ workspaces --
+constexpr size_t kAlign = 256;
+// Fixed counter region at the start of every workspace (zeroed once by
+// nsmlp_workspace_init, restored to zero by the kernels that use it).
+constexpr size_t kStatusOff = 0;
+constexpr size_t kServedOff = 16;  // [2] u32 block counts: HBM slots, host copies
+constexpr size_t kBlkCountOff = 256;
+constexpr int kMaxK = 32768;
+constexpr size_t kRowCountOff = kBlkCountOff + (size_t)kMaxK * sizeof(int);
+constexpr int kMaxRowChunks = 1024;
+constexpr size_t kCounterBytes = kRowCountOff + (size_t)kMaxRowChunks * sizeof(int) + 256;
+
+inline size_t align_up(size_t v) { return (v + kAlign - 1) / kAlign * kAlign; }
+inline bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
 // ------------------------------------------------------------------ fp16 --
 __device__ __forceinline__ float h2f(uint16_t h) { return (float)__builtin_bit_cast(_Float16, h); }

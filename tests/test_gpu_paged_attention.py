@@ -1,0 +1,283 @@
+"""Attention over the paged 8-bit cache against the formula in 64 bits on the
+cache's own codes and scales."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+
+class Served:
+    """Requests with (cached, new) tokens, their K and V in a cache and in the plain one."""
+
+    def __init__(self, dev, lengths, Hq, H, D, block, fmt, dtype, seed=0, spread=1.0, max_new=None):
+        from next_step_ai_amd.kv_cache import KvBatch, KvCache
+
+        self.rng = np.random.RandomState(seed)
+        self.dev, self.dtype, self.lengths, self.D, self.fmt = dev, dtype, lengths, D, fmt
+        pool = sum(-(-(c + n) // block) for c, n in lengths) + 3
+        width = max(-(-(c + n) // block) for c, n in lengths) + 1
+        order = self.rng.permutation(pool)
+        self.batch = KvBatch(pool, block, max_requests=len(lengths), max_blocks=max(width, 1), q_heads=Hq, kv_heads=H,
+                             head_dim=D, free_blocks=torch.from_numpy(order))
+        self.cache = KvCache(pool, H, D, block_tokens=block, fmt=fmt)
+        self.plain = ref.PlainCache(pool, H, D, block, fmt)
+        where = ref.PlainBatch(pool, block, len(lengths), width, order)
+        for phase in (0, 1):
+            new = [x[phase] for x in lengths]
+            total = sum(new)
+            if phase == 0 and total == 0:
+                continue
+            self.step = self.batch.plan(torch.tensor(new, dtype=torch.int32, device=dev), total,
+                                        max_new=max(new) if max_new is None else max_new * phase)
+            slots = where.plan(new, total)["slots"]
+            k, v = (torch.from_numpy(self.rng.standard_normal((total, H, D))
+                                     * np.exp2(self.rng.uniform(-spread, spread, (total, H, 1)))).to(dtype) for _ in range(2))
+            self.cache.append(k.to(dev), v.to(dev), self.step.slots)
+            self.plain.append(k.float().numpy(), v.float().numpy(), slots)
+            if phase == 0:
+                self.batch.commit()
+                where.commit()
+        self.where = where._next[0] if where._next else where.blocks
+        self.total, self.block = total, block
+        self.q = torch.from_numpy(self.rng.standard_normal((total, Hq, D)) * 1.5).to(dtype).to(dev)
+
+    def slots_of(self, r, n):
+        return [self.where[r][p // self.block] * self.block + p % self.block for p in range(n)]
+
+    def check(self, out, lse, q=None, scale=None, hide=()):
+        """Per element: the output's rounding, the weights' rounding to fp16 (2^-11 each at most, and 2^-25 of the largest
+        weight where it is subnormal) and fp32 scores (2^-24 per operation, |score| up to 64: 2^-16)."""
+        q = (self.q if q is None else q).cpu()
+        scale = self.D ** -0.5 if scale is None else scale
+        u = 2.0 ** -11 if self.dtype == torch.float16 else 2.0 ** -8
+        t0 = 0
+        for r, (c, n) in enumerate(self.lengths):
+            if n == 0:
+                continue
+            keep = [p for p in range(c + n) if (r, p // self.block) not in hide]
+            slots = [self.slots_of(r, c + n)[p] for p in keep]
+            k, v = self.plain.values(slots, 0), self.plain.values(slots, 1)
+            want, wl, spread = ref.attention(q[t0: t0 + n].double(), k, v, n, len(keep), scale)
+            got, gl = out[t0: t0 + n].cpu().double(), lse[t0: t0 + n].cpu().double()
+            most = float(np.abs(v).max()) if v.size else 0.0
+            bound = u * want.abs() + (2.0 ** -11 + 2.0 ** -15) * spread + (c + n) * 2.0 ** -25 * most + 2.0 ** -24
+            worst = ((got - want).abs() / bound).max().item()
+            assert worst <= 1.0, (r, c, n, worst)
+            empty = wl == -np.inf
+            assert torch.equal(gl == -np.inf, empty)
+            assert ((gl - wl).abs()[~empty] <= 2.0 ** -14 + 2.0 ** -20 * wl.abs()[~empty]).all()
+            t0 += n
+
+    def run(self, q=None, **kw):
+        from next_step_ai_amd.kv_cache import paged_attention
+
+        q = self.q if q is None else q
+        lse = torch.full(q.shape[:2], 7.0, device=self.dev)
+        out = paged_attention(q, self.cache, self.step, lse=lse, **kw)
+        return out, lse
+
+
+@pytest.mark.parametrize("fmt,dtype", [("int8", torch.float16), ("e4m3", torch.bfloat16)])
+@pytest.mark.parametrize("Hq,H,D,block", [(4, 4, 64, 16), (16, 1, 128, 16), (14, 2, 128, 32), (6, 2, 64, 64), (40, 2, 128, 16)])
+def test_decode(gpu, fmt, dtype, Hq, H, D, block):
+    """One token each at lengths around a tile, a block and a workgroup's share, the first token of a request among them."""
+    lengths = [(0, 1), (1, 1), (14, 1), (15, 1), (16, 1), (0, 0), (31, 1), (32, 1), (63, 1), (64, 1), (127, 1), (130, 1), (400, 1)]
+    s = Served(gpu, lengths, Hq, H, D, block, fmt, dtype, seed=Hq + D)
+    s.check(*s.run())
+
+
+@pytest.mark.parametrize("fmt,dtype", [("e4m3", torch.float16), ("int8", torch.bfloat16)])
+@pytest.mark.parametrize("Hq,H,D,block,lengths", [
+    (4, 1, 128, 16, [(0, 5), (7, 4), (100, 2), (33, 1)]),
+    (6, 2, 64, 32, [(50, 7), (0, 1), (0, 40), (129, 3), (1, 0)]),
+    (16, 1, 128, 16, [(20, 37), (300, 1), (0, 65)]),
+    (2, 2, 128, 64, [(0, 130), (257, 65)]),
+    (3, 1, 64, 16, [(5, 200)]),
+])
+def test_several_tokens(gpu, fmt, dtype, Hq, H, D, block, lengths):
+    """Drafts, prompts and chunks next to single tokens: every row's own end."""
+    s = Served(gpu, lengths, Hq, H, D, block, fmt, dtype, seed=len(lengths))
+    s.check(*s.run())
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_keys_shared_out(gpu, fmt):
+    """Few rows and many keys: partial results joined, more than 64 blocks per wave, in both lists."""
+    s = Served(gpu, [(9001, 1)], 4, 1, 128, 16, fmt, torch.float16, seed=9)
+    s.check(*s.run())
+    s = Served(gpu, [(5000, 1), (3, 1), (2600, 1)], 4, 2, 64, 16, fmt, torch.float16, seed=10)
+    s.check(*s.run())
+    s = Served(gpu, [(4000, 33), (700, 1)], 8, 1, 128, 32, fmt, torch.bfloat16, seed=11)
+    s.check(*s.run())
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_scales_that_differ(gpu, fmt):
+    """K and V magnitudes 2^-12 to 2^12 from token to token: blocks' scales far apart, weights from 1 down to nothing."""
+    s = Served(gpu, [(300, 1), (70, 20), (1500, 1)], 4, 2, 64, 16, fmt, torch.bfloat16, seed=12, spread=12.0)
+    q = s.q * 2.0 ** -8
+    s.check(*s.run(q), q=q)
+
+
+def test_strides_scale_and_buffers(gpu):
+    from next_step_ai_amd.kv_cache import paged_attention
+
+    s = Served(gpu, [(40, 3), (200, 1)], 8, 2, 64, 16, "int8", torch.float16, seed=13)
+    want, lse = s.run(scale=0.3)
+    s.check(want, lse, scale=0.3)
+    fused = torch.zeros(4, 12, 64, dtype=torch.float16, device=gpu)
+    fused[:, 2:10] = s.q
+    out = torch.empty_like(want)
+    assert paged_attention(fused[:, 2:10], s.cache, s.step, scale=0.3, out=out) is out
+    assert torch.equal(out, want)
+    odd = torch.zeros(4, 8, 65, dtype=torch.float16, device=gpu)[:, :, 1:]
+    odd.copy_(s.q)
+    assert torch.equal(s.run(odd, scale=0.3)[0], want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out2, _ = s.run(scale=0.3)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(out2, want)
+    for _ in range(3):
+        assert torch.equal(s.run(scale=0.3)[0], want)
+
+
+def test_rows_that_see_nothing(gpu):
+    """A refused request's tokens: zeros and -inf; padding rows are left alone."""
+    from next_step_ai_amd.kv_cache import KvBatch, KvCache, paged_attention
+
+    for group, most in ((2, 0), (8, 0), (2, 6)):
+        b = KvBatch(2, 16, max_requests=3, max_blocks=4, q_heads=2 * group, kv_heads=2)
+        c = KvCache(2, 2, 128)
+        new = torch.tensor([5, 6, 40], dtype=torch.int32, device=gpu)
+        if most:
+            new[2] = 6
+            b.cached[2] = 60  # longer than the table
+        total = int(new.sum())
+        st = b.plan(new, total + 2, max_new=most)
+        assert int(st.info[2]) == 1
+        x = torch.randn(total + 2, 2, 128, device=gpu).half()
+        c.append(x, x, st.slots)
+        q = torch.randn(total + 2, 2 * group, 128, device=gpu).half()
+        out, lse = torch.full_like(q, 3.0), torch.full(q.shape[:2], 3.0, device=gpu)
+        paged_attention(q, c, st, out=out, lse=lse)
+        assert (out[11:total] == 0).all() and (lse[11:total] == -float("inf")).all()
+        assert (out[:11].abs().sum(-1) > 0).all()
+        assert (out[total:] == 3).all() and (lse[total:] == 3).all()
+
+
+@pytest.mark.parametrize("fmt,dtype", [("int8", torch.float16), ("e4m3", torch.bfloat16)])
+def test_garbage_past_the_end(gpu, fmt, dtype):
+    """Bytes that no token has filled, e4m3 NaN codes and infinite codes of other formats among them, and scales of unused blocks do not matter."""
+    s = Served(gpu, [(17, 1), (40, 9), (100, 33)], 8, 2, 128, 32, fmt, dtype, seed=14)
+    want, lse = s.run()
+    used = {x for r, (c, n) in enumerate(s.lengths) for x in s.slots_of(r, c + n)}
+    data = s.cache.data.view(s.cache.num_blocks, 2, 2, -1)
+    probe = s.cache.data.clone()
+    free = [x for x in range(s.cache.num_blocks * 32) if x not in used]
+    # overwrite the unused tail tokens of the last blocks in place: K tile [D/16][16][16], V tile [D/64][4][64][4]
+    for x in free:
+        b, t = x // 32, x % 32
+        tile = data[b].view(2, 2, 2, 16 * 128)[:, :, t // 16]  # [heads, k/v, bytes of a tile]
+        tile[:, 0].view(2, 8, 16, 16)[:, :, t % 16] = 0x7F
+        tile[:, 1].view(2, 2, 4, 64, 4)[:, :, t % 16 // 4, :, t % 4] = 0xFF
+    assert not torch.equal(s.cache.data, probe)
+    unused = [b for b in range(s.cache.num_blocks) if all(b * 32 + t not in used for t in range(32))]
+    for b in unused:
+        s.cache.scale[b] = float("nan")
+    again, lse2 = s.run()
+    assert torch.equal(again, want) and torch.equal(lse, lse2)
+
+
+def test_values_that_are_not_finite(gpu):
+    """A NaN block poisons the rows that see it and no others; a NaN query its own row."""
+    s = Served(gpu, [(20, 40), (30, 1)], 4, 2, 64, 16, "int8", torch.float16, seed=15)
+    want, lse = s.run()
+    s.cache.scale[s.where[0][3], 0, 1] = float("nan")  # V of tokens 48..63 of request 0, head 0: seen from token 28 on
+    got, _ = s.run()
+    assert torch.equal(got[:28], want[:28]) and torch.equal(got[40:], want[40:])
+    assert got[28:40, :2].isnan().all() and torch.equal(got[28:40, 2:], want[28:40, 2:])
+    s.cache.scale[s.where[0][3], 0, 1] = 1.0
+    s.cache.scale[s.where[0][3], 1, 0] = float("nan")  # K
+    got, _ = s.run()
+    assert got[28:40, 2:].isnan().all() and torch.equal(got[:28], want[:28])
+    s.cache.scale[s.where[0][3], 1, 0] = 1.0
+    q = s.q.clone()
+    q[40, 1, 3] = float("inf")
+    q[41 - 2, 0, 3] = float("nan")
+    got, _ = s.run(q)
+    assert got[40, 1].isnan().all() and got[39, 0].isnan().all()
+    assert torch.equal(got[40, 0], s.run()[0][40, 0]) and torch.equal(got[:39], s.run()[0][:39])
+
+
+def test_table_entry_that_is_no_block(gpu):
+    """Its keys are hidden and the status word says so."""
+    from next_step_ai_amd import _lib
+    from next_step_ai_amd._runtime import StatusWord, workspace
+
+    s = Served(gpu, [(100, 1), (60, 30)], 4, 1, 64, 16, "e4m3", torch.float16, seed=16)
+    word = StatusWord(gpu, "paged attention")
+    ws = workspace(1 << 20, gpu)
+    word.clear(ws)
+    s.run(ws=None)
+    word.take(workspace(1 << 20, gpu))
+    word.check()
+    s.batch.table[0, 2], s.batch.table[1, 1] = -1, s.cache.num_blocks + 5
+    out, lse = s.run()
+    s.check(out, lse, hide={(0, 2), (1, 1)})
+    word.take(workspace(1 << 20, gpu))
+    with pytest.raises(RuntimeError, match="out of range"):
+        word.check()
+    assert _lib.NSMLP_STATUS_BLOCK_UNAVAILABLE == 1
+
+
+def test_offsets_past_32_bits(gpu):
+    """Blocks whose bytes lie past 2^32."""
+    from next_step_ai_amd.kv_cache import KvBatch, KvCache, paged_attention
+
+    blocks = (1 << 32) // (8 * 2 * 64 * 128) + 40
+    small = None
+    for first in (blocks - 5, 0):
+        c = KvCache(blocks, 8, 128, block_tokens=64) if small is None else KvCache(5, 8, 128, block_tokens=64)
+        n = c.num_blocks
+        order = torch.arange(first, first + 5) if small is None else torch.arange(5)
+        b = KvBatch(n, 64, max_requests=1, max_blocks=8, q_heads=16, kv_heads=8, free_blocks=order)
+        g = torch.Generator(device=gpu).manual_seed(3)
+        x, y, q = (torch.randn(300, h, 128, device=gpu, generator=g).half() for h in (8, 8, 16))
+        st = b.plan(torch.tensor([300], dtype=torch.int32, device=gpu), 300)
+        c.append(x, y, st.slots)
+        got = paged_attention(q, c, st), c.read(st.slots)["v"]
+        if small is None:
+            small = got
+        else:
+            assert torch.equal(got[0], small[0]) and torch.equal(got[1], small[1])
+
+
+def test_refusals(gpu):
+    from next_step_ai_amd.kv_cache import KvBatch, KvCache, paged_attention
+
+    s = Served(gpu, [(5, 2)], 4, 2, 64, 16, "int8", torch.float16, seed=17)
+    q = s.q
+    for bad in (q.float(), q[:1], q[:, :2], q.cpu()):
+        with pytest.raises(RuntimeError):
+            paged_attention(bad, s.cache, s.step)
+    for kw in (dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(out=torch.empty_like(q).float()),
+               dict(out=torch.empty(2, 4, 65, dtype=q.dtype, device=gpu)[:, :, 1:]), dict(lse=torch.empty(2, 4, device=gpu).half()),
+               dict(ws=torch.empty(64, dtype=torch.uint8, device=gpu))):
+        with pytest.raises(RuntimeError):
+            paged_attention(q, s.cache, s.step, **kw)
+    for other in (KvCache(s.cache.num_blocks + 1, 2, 64), KvCache(s.cache.num_blocks, 4, 64),
+                  KvCache(s.cache.num_blocks, 2, 64, block_tokens=32)):
+        with pytest.raises(RuntimeError, match="the batch"):
+            paged_attention(q, other, s.step)
+    uneven = KvBatch(s.cache.num_blocks, 16, max_requests=1, max_blocks=4, q_heads=3, kv_heads=2)
+    step = uneven.plan(torch.full((1,), 2, dtype=torch.int32, device=gpu), 2)
+    with pytest.raises(RuntimeError, match="multiple of kv_heads"):
+        paged_attention(q[:, :3], s.cache, step)
+    other = KvBatch(s.cache.num_blocks, 16, max_requests=1, max_blocks=4, q_heads=4, kv_heads=2)
+    with pytest.raises(RuntimeError, match="another batch"):
+        other.plan(torch.ones(1, dtype=torch.int32, device=gpu), 2, step=s.step)
