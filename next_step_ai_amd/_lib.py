@@ -205,8 +205,9 @@ def check(rc: int, what: str) -> None:
 
 def call(name: str, *args) -> None:
     """Call a status-returning entry point; raise RuntimeError on failure."""
-    rc = getattr(lib(), name)(*args)
-    check(int(rc), name)
+    rc = getattr(_lib if _lib is not None else lib(), name)(*args)
+    if rc != 0:
+        check(int(rc), name)
 
 
 def fault_inject(spec: str | None) -> None:

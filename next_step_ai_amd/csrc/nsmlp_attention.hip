@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(256) k_attn_join(KvAttnArgs a, const KvSplit* 
 }
 
 template <int D, int kFmt, bool kBf16>
-void launch_typed(const KvAttnArgs& a, bool list_b, hipStream_t s) {
+void attention_typed(const KvAttnArgs& a, hipStream_t s) {
   const KvUnit* ua = reinterpret_cast<const KvUnit*>(a.sched + a.s.off_units_a);
   const KvUnit* ub = reinterpret_cast<const KvUnit*>(a.sched + a.s.off_units_b);
   const KvSplit* sa = reinterpret_cast<const KvSplit*>(a.sched + a.s.off_splits_a);
@@ -412,7 +412,7 @@ void launch_typed(const KvAttnArgs& a, bool list_b, hipStream_t s) {
   if (a.s.max_splits_a > 0)
     k_attn_join<D, kBf16><<<join_grid(a.s.max_splits_a, a.s.rows_a), dim3(256), 0, s>>>(a, sa, a.sched + 1, a.s.rows_a,
                                                                                        a.acc_a, a.ml_a);
-  if (list_b) {
+  if (a.list_b) {
     k_attn_stream<D, kFmt, kBf16, 1><<<grid(a.s.max_units_b), dim3(kStreamThreads), 0, s>>>(a, ub, a.sched + 2, a.s.max_units_b, a.s.rows_b,
                                                                                            a.acc_b, a.ml_b);
     if (a.s.max_splits_b > 0)
@@ -433,15 +433,8 @@ size_t kv_attn_partial_floats(const KvSchedule& s, int kv_heads, int D, size_t (
   return at;
 }
 
-void launch_kv_attention(const KvAttnArgs& a, bool bf16, bool list_b, hipStream_t s) {
-  const bool i8 = a.c.fmt == NSMLP_KV_INT8;
-  if (a.c.D == 128) {
-    if (i8) bf16 ? launch_typed<128, NSMLP_KV_INT8, true>(a, list_b, s) : launch_typed<128, NSMLP_KV_INT8, false>(a, list_b, s);
-    else bf16 ? launch_typed<128, NSMLP_KV_E4M3, true>(a, list_b, s) : launch_typed<128, NSMLP_KV_E4M3, false>(a, list_b, s);
-  } else {
-    if (i8) bf16 ? launch_typed<64, NSMLP_KV_INT8, true>(a, list_b, s) : launch_typed<64, NSMLP_KV_INT8, false>(a, list_b, s);
-    else bf16 ? launch_typed<64, NSMLP_KV_E4M3, true>(a, list_b, s) : launch_typed<64, NSMLP_KV_E4M3, false>(a, list_b, s);
-  }
+void launch_kv_attention(const KvAttnArgs& a, bool bf16, hipStream_t s) {
+  NSMLP_KV_BY_TYPE(attention_typed, a, bf16, s);
 }
 
 }  // namespace nsmlp

@@ -45,19 +45,6 @@ __device__ __forceinline__ float kv_decode1(uint32_t byte) {
   else return __builtin_amdgcn_cvt_f32_fp8(byte, 0);
 }
 
-template <int kFmt>
-__device__ __forceinline__ uint32_t kv_encode1(float x) {  // x = value / scale; non-finite: code 0
-  if constexpr (kFmt == NSMLP_KV_INT8) {
-    if (!(fabsf(x) < 1e30f)) x = 0.0f;
-    const float r = rintf(fminf(fmaxf(x, -127.0f), 127.0f));
-    return (uint32_t)((int)r + 128);
-  } else {
-    if (!(fabsf(x) < 1e30f)) x = 0.0f;
-    const float r = fminf(fmaxf(x, -448.0f), 448.0f);
-    return __builtin_amdgcn_cvt_pk_fp8_f32(r, r, 0, false) & 0xFFu;
-  }
-}
-
 // four codes of a dword as fp16, in byte order
 template <int kFmt>
 __device__ __forceinline__ uint2 kv_half4(uint32_t w) {
@@ -97,6 +84,7 @@ struct KvAppendArgs {
   long long k_row, k_head, v_row, v_head;  // strides in elements
   const int64_t* slots;
   int n;
+  int take;  // tokens that a wave looks at (set by the launch)
 };
 void launch_kv_append(const KvAppendArgs& a, bool bf16, hipStream_t s);
 
@@ -137,7 +125,7 @@ struct KvSchedule {  // sizes, from the host's knowledge of a step (kv_schedule)
 KvSchedule kv_schedule(int requests, int total, int max_new, int group, int kv_heads);
 
 struct KvPlanArgs {
-  int R, total, max_new, max_blocks, num_blocks, B, b_shift, group;
+  int R, total, max_new, row_limit, max_blocks, num_blocks, B, b_shift, group;
   const int32_t *cached, *fresh;     // [R]
   int32_t* table;                    // [R][max_blocks]
   const int32_t *ring, *state;       // [num_blocks] free blocks, (head, count)
@@ -160,12 +148,12 @@ struct KvAttnArgs {
   float scale_log2;  // softmax scale times log2(e)
   float *acc_a, *ml_a, *acc_b, *ml_b;  // partial results of either list: [parts][kv_heads][rows][D], [..][4] (m, l, x)
   int* status;
+  bool list_b;  // whether a request can be long enough for the second list
   KvSchedule s;
 };
 // floats of the partial results, and where acc_a, ml_a, acc_b, ml_b start
 size_t kv_attn_partial_floats(const KvSchedule& s, int kv_heads, int D, size_t (&off)[4]);
-// list_b: whether a request can be long enough for the second list
-void launch_kv_attention(const KvAttnArgs& a, bool bf16, bool list_b, hipStream_t s);
+void launch_kv_attention(const KvAttnArgs& a, bool bf16, hipStream_t s);
 
 struct KvCommitArgs {
   int R, max_blocks, num_blocks, b_shift, B;
@@ -174,5 +162,18 @@ struct KvCommitArgs {
   const int32_t* finished;  // [R] or NULL
 };
 void launch_kv_commit(const KvCommitArgs& a, hipStream_t s);
+
+// f<D, format, bf16>(args) for the cache's head size and format
+#define NSMLP_KV_BY_TYPE(f, a, bf16, s)                                                            \
+  do {                                                                                             \
+    const bool i8_ = (a).c.fmt == NSMLP_KV_INT8;                                                   \
+    if ((a).c.D == 128) {                                                                          \
+      if (i8_) (bf16) ? f<128, NSMLP_KV_INT8, true>(a, s) : f<128, NSMLP_KV_INT8, false>(a, s);    \
+      else (bf16) ? f<128, NSMLP_KV_E4M3, true>(a, s) : f<128, NSMLP_KV_E4M3, false>(a, s);        \
+    } else {                                                                                       \
+      if (i8_) (bf16) ? f<64, NSMLP_KV_INT8, true>(a, s) : f<64, NSMLP_KV_INT8, false>(a, s);      \
+      else (bf16) ? f<64, NSMLP_KV_E4M3, true>(a, s) : f<64, NSMLP_KV_E4M3, false>(a, s);          \
+    }                                                                                              \
+  } while (0)
 
 }  // namespace nsmlp

@@ -16,200 +16,178 @@ namespace {
 // blocks, the ring's entries head + (sum of need before r) ...; it is refused
 // (no slots, kv_len 0, lengths unchanged) where its blocks exceed the table's
 // width or the running sum the free count.
-constexpr int kPlanThreads = 1024;
-constexpr int kPlanWaves = kPlanThreads / kWave;
-
-__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    const int o = __shfl_up(v, d, kWave);
-    if (lane >= d) v += o;
-  }
+//
+// What bounds it: latency.  8 requests write 224 bytes, 4096 requests 0.7 MB; a
+// step is a chain of one load of the lengths, two scans, one load of the
+// ring's entries and the stores.  Sums within a wave go through DPP adds (a
+// few cycles each; exchanges through LDS took most of the time before), the
+// waves' sums meet in LDS once per scan, and the workgroup is no wider than
+// the requests need: 64 threads need no barrier between waves at all.
+__device__ __forceinline__ int wave_scan(int v) {  // inclusive
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row 0 -> 1, 2 -> 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // rows 0, 1 -> 2, 3
   return v;
 }
 
 // Exclusive sums of N values over the workgroup's threads, totals in `total`.
-template <int N>
-__device__ __forceinline__ void block_scan(int (&v)[N], int (&total)[N], int (*wsum)[kPlanWaves], int tid) {
-  const int lane = tid & (kWave - 1), wave = tid >> 6;
+template <int N, int kThreads>
+__device__ __forceinline__ void block_scan(int (&v)[N], int (&total)[N], int (*wsum)[16], int tid) {
+  constexpr int kWaves = kThreads / kWave;
+  const int lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int inc[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    inc[i] = wave_scan(v[i], lane);
-    if (lane == kWave - 1) wsum[i][wave] = inc[i];
-  }
-  __syncthreads();
+  for (int i = 0; i < N; ++i) inc[i] = wave_scan(v[i]);
+  if constexpr (kWaves == 1) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    int before = 0, all = 0;
-    for (int w = 0; w < kPlanWaves; ++w) {
-      const int x = wsum[i][w];
-      before += w < wave ? x : 0;
-      all += x;
+    for (int i = 0; i < N; ++i) total[i] = __builtin_amdgcn_readlane(inc[i], kWave - 1), v[i] = inc[i] - v[i];
+  } else {
+    if (lane == kWave - 1) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) wsum[i][wave] = inc[i];
     }
-    v[i] = before + inc[i] - v[i];
-    total[i] = all;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int all = wave_scan(lane < kWaves ? wsum[i][lane & 15] : 0);
+      total[i] = __builtin_amdgcn_readlane(all, kWaves - 1);
+      v[i] = inc[i] - v[i] + (wave == 0 ? 0 : __builtin_amdgcn_readlane(all, wave == 0 ? 0 : wave - 1));
+    }
+    __syncthreads();
   }
-  __syncthreads();
 }
 
 __device__ __forceinline__ int clip_len(int v) { return min(max(v, 0), 1 << 29); }
 
-constexpr int kPer = kKvMaxRequests / kPlanThreads;
-
 // keys per part, so that about `target` units share the list's `work` keys
 __device__ __forceinline__ int part_keys(long long work, int target, int least) {
   if (target <= 0) return 1 << 30;  // more than any request's
-  const long long each = (work + target - 1) / target;
-  const long long up = (each + 127) / 128 * 128;
-  return up < least ? least : up > (1 << 30) ? 1 << 30 : (int)up;
+  const double each = ceil((double)work / target);  // exact: below 2^53, and a quotient's ceiling does not round down
+  const double up = ceil(each * (1.0 / 128)) * 128;
+  return up < least ? least : up > (double)(1 << 30) ? 1 << 30 : (int)up;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) k_kv_plan(KvPlanArgs a) {
+constexpr int kPlanSums = 7;
+
+template <int kThreads, int kPer>
+__global__ void __launch_bounds__(kThreads) k_kv_plan(KvPlanArgs a) {
   extern __shared__ __attribute__((aligned(16))) int lds[];
-  __shared__ int wsum[4][kPlanWaves];
-  __shared__ long long wsum2[2][kPlanWaves];
-  __shared__ int refused_s;
-  int* q_start = lds;           // [R + 1]
+  __shared__ int wsum[kPlanSums][16];
+  int* q_start = lds;             // [R + 1]
   int* base = q_start + a.R + 1;  // [R] blocks granted before the request; -1: refused
   int* first = base + a.R;        // [R] first unit of its list
   int* split = first + a.R;       // [R] first split tile of its list
   int* partial = split + a.R;     // [R] first partial
+  int* len_s = partial + a.R;     // [R] cached tokens
+  kernarg_warm<sizeof(KvPlanArgs)>();
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid >> 6;
-  const int per = (a.R + kPlanThreads - 1) / kPlanThreads;
+  const int per = kPer == 1 ? 1 : (a.R + kThreads - 1) / kThreads;
   const int r0 = tid * per;
   const unsigned N = (unsigned)a.num_blocks;
-  const int head = (int)((unsigned)a.state[0] % N), count = min(max(a.state[1], 0), a.num_blocks);
-  if (tid == 0) refused_s = 0;
 
   int cached[kPer], fresh[kPer], need[kPer];
-  int sum[2] = {0, 0}, total[2];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int r = r0 + i;
     const bool in = i < per && r < a.R;
     cached[i] = in ? clip_len(a.cached[r]) : 0;
     fresh[i] = in ? min(max(a.fresh[r], 0), 1 << 28) : 0;
+  }
+  const int head = (int)((unsigned)a.state[0] % N), count = min(max(a.state[1], 0), a.num_blocks);
+  int sum[2] = {0, 0}, total[2];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
     const int have = (cached[i] + a.B - 1) >> a.b_shift, tot = (cached[i] + fresh[i] + a.B - 1) >> a.b_shift;
     need[i] = tot <= a.max_blocks ? tot - have : -1;  // -1: longer than the table
     sum[0] += fresh[i];
     sum[1] += max(need[i], 0);
   }
-  block_scan(sum, total, wsum, tid);
-  // granted requests, and the work of either list
-  int at = sum[0], used = sum[1], refused = 0, kv[kPer];
+  block_scan<2, kThreads>(sum, total, wsum, tid);
+  // granted requests, and the work (tiles of rows times keys) of either list,
+  // summed exactly in three pieces of 20 bits (1024 of them stay in 30)
+  int at = sum[0], used = sum[1], kv[kPer], tiles[kPer];  // tiles < 0: list a
   long long work[2] = {0, 0};
+  int cnt[kPlanSums] = {};  // units a, units b, split tiles a, b, partials a, b, blocks granted
+  int refused = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int r = r0 + i;
-    if (i < per && r < a.R) {
-      const int n = max(need[i], 0);
-      const bool ok = need[i] >= 0 && (n == 0 || used + n <= count) && fresh[i] <= a.max_new;
+    const bool in = i < per && r < a.R;
+    const int n = max(need[i], 0);
+    const bool ok = need[i] >= 0 && (n == 0 || used + n <= count) && fresh[i] <= a.max_new;
+    kv[i] = in && ok ? cached[i] + fresh[i] : 0;
+    if (in) {
       q_start[r] = at;
+      len_s[r] = cached[i];
       base[r] = ok ? used : -1;
-      kv[i] = ok ? cached[i] + fresh[i] : 0;
-      refused += !ok && fresh[i] > 0;
-      used += n;
-      at += fresh[i];
-      const long long rows = (long long)fresh[i] * a.group;
-      if (rows > a.s.rows_a) work[1] += (rows + a.s.rows_b - 1) / a.s.rows_b * kv[i];
-      else if (rows > 0) work[0] += kv[i];
-    } else {
-      kv[i] = 0;
+      if (blockIdx.x == 0) {
+        a.q_start[r] = at;
+        a.kv_len[r] = kv[i];
+        a.next[r] = ok ? cached[i] + fresh[i] : cached[i];
+      }
     }
+    refused += in && !ok && fresh[i] > 0;
+    cnt[6] += in && ok ? n : 0;
+    used += n;
+    at += fresh[i];
+    const int rows = min(fresh[i], a.row_limit) * a.group;
+    const bool b = rows > a.s.rows_a;
+    tiles[i] = b ? (rows + a.s.rows_b - 1) / a.s.rows_b : rows > 0 ? -1 : 0;
+    work[b ? 1 : 0] += (long long)kv[i] * abs(tiles[i]);
   }
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const long long w = wave_sum(work[i]);
-    if (lane == 0) wsum2[i][wave] = w;
-  }
-  if (refused) atomicAdd(&refused_s, refused);
-  if (tid == 0) q_start[a.R] = total[0];
-  __syncthreads();
-  long long all[2] = {0, 0};
-  for (int w = 0; w < kPlanWaves; ++w) {
-    all[0] += wsum2[0][w];
-    all[1] += wsum2[1][w];
+  long long all[2];
+  {
+    int piece[kPlanSums] = {(int)(work[0] & 0xFFFFF), (int)((work[0] >> 20) & 0xFFFFF), (int)(work[0] >> 40),
+                            (int)(work[1] & 0xFFFFF), (int)((work[1] >> 20) & 0xFFFFF), (int)(work[1] >> 40), refused};
+    int sums[kPlanSums];
+    block_scan<kPlanSums, kThreads>(piece, sums, wsum, tid);
+    all[0] = sums[0] + ((long long)sums[1] << 20) + ((long long)sums[2] << 40);
+    all[1] = sums[3] + ((long long)sums[4] << 20) + ((long long)sums[5] << 40);
+    refused = sums[6];
   }
   const int keys_a = part_keys(all[0], a.s.target_a, a.s.min_a), keys_b = part_keys(all[1], a.s.target_b, a.s.min_b);
   // units of each request: tiles of rows times parts of its keys
-  int cnt[4] = {0, 0, 0, 0}, cnt_total[4];  // units a, units b, split tiles a, split tiles b
-  int parts_b_sum[1] = {0}, parts_b_total[1];
+  int parts[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const long long rows = (long long)fresh[i] * a.group;
-    if (rows == 0) continue;
-    if (rows > a.s.rows_a) {
-      const int tiles = (int)((rows + a.s.rows_b - 1) / a.s.rows_b), parts = max(1, (kv[i] + keys_b - 1) / keys_b);
-      cnt[1] += tiles * parts;
-      if (parts > 1) {
-        cnt[3] += tiles;
-        parts_b_sum[0] += tiles * parts;
-      }
-    } else {
-      const int parts = max(1, (kv[i] + keys_a - 1) / keys_a);
-      cnt[0] += parts;
-      if (parts > 1) cnt[2] += 1;
-    }
+    const bool b = tiles[i] > 0;
+    const int n = abs(tiles[i]), keys = b ? keys_b : keys_a;
+    parts[i] = max(1, (int)(((unsigned)kv[i] + (unsigned)keys - 1) / (unsigned)keys));
+    const int u = n * parts[i], s = parts[i] > 1 ? n : 0, p = parts[i] > 1 ? u : 0;
+    cnt[0] += b ? 0 : u, cnt[1] += b ? u : 0;
+    cnt[2] += b ? 0 : s, cnt[3] += b ? s : 0;
+    cnt[4] += b ? 0 : p, cnt[5] += b ? p : 0;
   }
-  int parts_a_sum[1] = {0}, parts_a_total[1];
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const long long rows = (long long)fresh[i] * a.group;
-    if (rows > 0 && rows <= a.s.rows_a) {
-      const int parts = max(1, (kv[i] + keys_a - 1) / keys_a);
-      if (parts > 1) parts_a_sum[0] += parts;
-    }
-  }
-  block_scan(cnt, cnt_total, wsum, tid);
-  block_scan(parts_a_sum, parts_a_total, wsum, tid);
-  block_scan(parts_b_sum, parts_b_total, wsum, tid);
-  int ua = cnt[0], ub = cnt[1], sa = cnt[2], sb = cnt[3], pa = parts_a_sum[0], pb = parts_b_sum[0];
+  int cnt_total[kPlanSums];
+  block_scan<kPlanSums, kThreads>(cnt, cnt_total, wsum, tid);
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int r = r0 + i;
     if (i >= per || r >= a.R) continue;
-    const long long rows = (long long)fresh[i] * a.group;
-    if (rows > a.s.rows_a) {
-      const int tiles = (int)((rows + a.s.rows_b - 1) / a.s.rows_b), parts = max(1, (kv[i] + keys_b - 1) / keys_b);
-      first[r] = ub, split[r] = sb, partial[r] = pb;
-      ub += tiles * parts;
-      if (parts > 1) sb += tiles, pb += tiles * parts;
-    } else {
-      const int parts = rows == 0 ? 0 : max(1, (kv[i] + keys_a - 1) / keys_a);
-      first[r] = ua, split[r] = sa, partial[r] = pa;
-      ua += parts;
-      if (parts > 1) sa += 1, pa += parts;
-    }
-    if (blockIdx.x == 0) {
-      a.q_start[r] = q_start[r];
-      a.kv_len[r] = kv[i];
-      a.next[r] = base[r] >= 0 ? cached[i] + fresh[i] : cached[i];
-    }
+    const bool b = tiles[i] > 0;
+    const int n = abs(tiles[i]), u = n * parts[i];
+    first[r] = b ? cnt[1] : cnt[0], split[r] = b ? cnt[3] : cnt[2], partial[r] = b ? cnt[5] : cnt[4];
+    cnt[b ? 1 : 0] += u;
+    if (parts[i] > 1) cnt[b ? 3 : 2] += n, cnt[b ? 5 : 4] += u;
   }
+  if (tid == 0) q_start[a.R] = total[0];
   if (blockIdx.x == 0 && tid == 0) {
     a.q_start[a.R] = total[0];
-    // blocks used: the needs of granted requests (a refused one takes none)
-    a.info[2] = refused_s;
+    a.info[0] = (int)(((unsigned)head + (unsigned)cnt_total[6]) % N);
+    a.info[1] = count - cnt_total[6];
+    a.info[2] = refused;
     a.info[3] = total[0];
     a.sched[0] = min(cnt_total[0], a.s.max_units_a);
     a.sched[1] = min(cnt_total[2], a.s.max_splits_a);
     a.sched[2] = min(cnt_total[1], a.s.max_units_b);
     a.sched[3] = min(cnt_total[3], a.s.max_splits_b);
   }
-  {
-    int granted[1] = {0}, granted_total[1];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (i < per && r0 + i < a.R && base[r0 + i] >= 0) granted[0] += max(need[i], 0);
-    block_scan(granted, granted_total, wsum, tid);  // its barriers also publish the LDS arrays
-    if (blockIdx.x == 0 && tid == 0) {
-      a.info[0] = (int)(((unsigned)head + (unsigned)granted_total[0]) % N);
-      a.info[1] = count - granted_total[0];
-    }
-  }
+  __syncthreads();
   // slots: one thread per token; a block's first token also writes its entry
-  for (long long t = (long long)blockIdx.x * kPlanThreads + tid; t < a.total; t += (long long)gridDim.x * kPlanThreads) {
+  for (int t = (int)blockIdx.x * kThreads + tid; t < a.total; t += (int)gridDim.x * kThreads) {
     int lo = 0, hi = a.R;  // the last request with q_start <= t
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -218,8 +196,8 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_plan(KvPlanArgs a) {
     }
     long long slot = -1;
     if (t < q_start[a.R] && base[lo] >= 0) {
-      const int c = clip_len(a.cached[lo]);
-      const int have = (c + a.B - 1) >> a.b_shift, p = c + (int)t - q_start[lo], j = p >> a.b_shift;
+      const int c = len_s[lo];
+      const int have = (c + a.B - 1) >> a.b_shift, p = c + t - q_start[lo], j = p >> a.b_shift;
       int32_t* entry = a.table + (long long)lo * a.max_blocks + j;
       int id;
       if (j < have) {
@@ -237,43 +215,47 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_plan(KvPlanArgs a) {
   KvUnit* units_b = reinterpret_cast<KvUnit*>(a.sched + a.s.off_units_b);
   KvSplit* splits_a = reinterpret_cast<KvSplit*>(a.sched + a.s.off_splits_a);
   KvSplit* splits_b = reinterpret_cast<KvSplit*>(a.sched + a.s.off_splits_b);
-  for (int r = (int)blockIdx.x * kPlanWaves + wave; r < a.R; r += (int)gridDim.x * kPlanWaves) {
-    const int q = q_start[r + 1] - q_start[r];
-    if (q == 0) continue;
-    const int c = clip_len(a.cached[r]), len = base[r] >= 0 ? c + q : 0;
-    const long long rows = (long long)q * a.group;
-    const bool b = rows > a.s.rows_a;
-    const int per_tile = b ? a.s.rows_b : a.s.rows_a, keys = b ? keys_b : keys_a;
-    const int tiles = (int)((rows + per_tile - 1) / per_tile), parts = max(1, (len + keys - 1) / keys);
-    KvUnit* units = b ? units_b : units_a;
-    KvSplit* splits = b ? splits_b : splits_a;
+  auto write = [&](int r, int i, int q, int len, bool b, int tiles_r, int parts_r) {
+    const int per_tile = b ? a.s.rows_b : a.s.rows_a;
     const int max_units = b ? a.s.max_units_b : a.s.max_units_a, max_splits = b ? a.s.max_splits_b : a.s.max_splits_a,
               max_parts = b ? a.s.max_parts_b : a.s.max_parts_a;
-    for (int i = lane; i < tiles * parts; i += kWave) {
-      // the last tile sees the most keys: it goes first
-      const int tile = tiles - 1 - i / parts, part = i % parts;
-      const int last = (int)min((long long)q, ((long long)(tile + 1) * per_tile + a.group - 1) / a.group);
-      const int keys_seen = max(0, len - q + last);  // of the tile's last row
-      const int each = ((keys_seen + parts - 1) / parts + 63) & ~63;
-      KvUnit u;
-      u.req = r;
-      u.row = tile * per_tile;
-      u.kv_begin = min(part * each, keys_seen);
-      u.kv_end = min((part + 1) * each, keys_seen);
-      u.part = parts > 1 ? partial[r] + i : -1;
-      u.pad[0] = u.pad[1] = u.pad[2] = 0;
-      if (first[r] + i < max_units && u.part < max_parts) units[first[r] + i] = u;
-      if (parts > 1 && part == 0 && split[r] + i / parts < max_splits)
-        splits[split[r] + i / parts] = KvSplit{r, u.row, u.part, parts};
-    }
+    // the last tile sees the most keys: it goes first
+    const int nth = parts_r == 1 ? i : (int)((unsigned)i / (unsigned)parts_r), part = i - nth * parts_r;
+    const int tile = tiles_r - 1 - nth;
+    const int last = min(q, (int)(((unsigned)(tile + 1) * (unsigned)per_tile + a.group - 1) / (unsigned)a.group));
+    const int keys_seen = max(0, len - q + last);  // of the tile's last row
+    const int each = parts_r == 1 ? keys_seen : ((int)((unsigned)(keys_seen + parts_r - 1) / (unsigned)parts_r) + 63) & ~63;
+    KvUnit u;
+    u.req = r;
+    u.row = tile * per_tile;
+    u.kv_begin = min(part * each, keys_seen);
+    u.kv_end = min((part + 1) * each, keys_seen);
+    u.part = parts_r > 1 ? partial[r] + i : -1;
+    u.pad[0] = u.pad[1] = u.pad[2] = 0;
+    if (first[r] + i < max_units && u.part < max_parts) (b ? units_b : units_a)[first[r] + i] = u;
+    if (parts_r > 1 && part == 0 && split[r] + nth < max_splits)
+      (b ? splits_b : splits_a)[split[r] + nth] = KvSplit{r, u.row, u.part, parts_r};
+  };
+  constexpr int kWaves = kThreads / kWave;
+  for (int r = (int)blockIdx.x * kWaves + wave; r < a.R; r += (int)gridDim.x * kWaves) {
+    const int q = q_start[r + 1] - q_start[r];
+    if (q == 0) continue;
+    const int len = base[r] >= 0 ? len_s[r] + q : 0;
+    const int rows = min(q, a.row_limit) * a.group;
+    const bool b = rows > a.s.rows_a;
+    const int n = b ? (rows + a.s.rows_b - 1) / a.s.rows_b : 1, keys = b ? keys_b : keys_a;
+    const int parts_r = max(1, (int)(((unsigned)len + (unsigned)keys - 1) / (unsigned)keys));
+    for (int i = lane; i < n * parts_r; i += kWave) write(r, i, q, len, b, n, parts_r);
   }
 }
+
+constexpr int kPlanThreads = 1024;
 
 // Lengths, ring state and (for finished requests) the table after a step.  A
 // finished request's blocks return to the ring's end in the order of requests
 // and of their tables; one workgroup, as the order is a running sum.
 __global__ void __launch_bounds__(kPlanThreads) k_kv_commit(KvCommitArgs a) {
-  __shared__ int wsum[1][kPlanWaves];
+  __shared__ int wsum[1][16];
   const int tid = threadIdx.x;
   const int per = (a.R + kPlanThreads - 1) / kPlanThreads, r0 = tid * per;
   const unsigned N = (unsigned)a.num_blocks;
@@ -287,7 +269,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_commit(KvCommitArgs a) {
     if (a.finished != nullptr && a.finished[r] != 0)
       mine[0] += min((max(len, 0) + a.B - 1) >> a.b_shift, a.max_blocks);
   }
-  block_scan(mine, total, wsum, tid);
+  block_scan<1, kPlanThreads>(mine, total, wsum, tid);
   int at = mine[0];
   for (int i = 0; i < per; ++i) {
     const int r = r0 + i;
@@ -315,199 +297,283 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_commit(KvCommitArgs a) {
 
 // ---------------------------------------------------------------- append --
 // One wave per (run, head, K or V): a run is the tokens of one block, which
-// stand next to each other in the call.  The wave of a run's first token does
-// it; the others leave.  Two passes over the run's rows (the second from the
-// caches): the largest magnitude, then the codes.
+// stand next to each other in the call.  A wave looks at kTake tokens for the
+// first of a run; where there are few tokens it takes one.  A run's rows are
+// loaded once, all loads in flight together, and stay in registers between the
+// search for the largest magnitude and the coding.
+//
+// K: a lane holds 16 dims of a token (16 code bytes).  V: a lane holds 4 dims
+// of 4 tokens, which is how V's codes lie; the wave owns the block's V, so
+// bytes of other tokens in a piece of 16 are read and written back.
 constexpr int kAppendThreads = 256;
 
 template <bool kBf16>
-__device__ __forceinline__ float in_value(uint16_t h) {
-  if constexpr (kBf16) return __uint_as_float((uint32_t)h << 16);
-  else return h2f(h);
+__device__ __forceinline__ float in_value(uint32_t h) {
+  if constexpr (kBf16) return __uint_as_float(h << 16);
+  else return h2f((uint16_t)h);
+}
+template <bool kBf16>
+__device__ __forceinline__ float in_lo(uint32_t w) { return in_value<kBf16>(w & 0xFFFFu); }
+template <bool kBf16>
+__device__ __forceinline__ float in_hi(uint32_t w) {
+  if constexpr (kBf16) return __uint_as_float(w & 0xFFFF0000u);
+  else return in_value<kBf16>(w >> 16);
 }
 
-template <int D, int kFmt, bool kBf16>
-__global__ void __launch_bounds__(kAppendThreads) k_kv_append(KvAppendArgs a) {
-  constexpr int kChunks = D / 16, kTok = kWave / kChunks;  // 16-dim pieces of a token, tokens of a pass
-  const int lane = threadIdx.x & (kWave - 1);
-  const long long item = (long long)blockIdx.x * (kAppendThreads / kWave) + (threadIdx.x >> 6);
-  const int two_heads = 2 * a.c.heads;
-  const int t = (int)(item / two_heads), hk = (int)(item % two_heads), h = hk >> 1;
-  const bool is_v = hk & 1;
-  if (t >= a.n) return;
-  const long long limit = (long long)a.c.num_blocks * a.c.B;
-  const long long slot = a.slots[t];
-  if (slot < 0 || slot >= limit) return;
-  const long long blk = slot >> a.c.b_shift;
-  if (t > 0) {
-    const long long prev = a.slots[t - 1];
-    if (prev >= 0 && prev < limit && prev == slot - 1 && (prev >> a.c.b_shift) == blk) return;
+// Codes of four values under scale s (r = 1 / s rounded), in byte order.  The
+// int8 quotient is rounded as a division: x r corrected by its residual (a
+// correctly rounded r makes the corrected product the correctly rounded
+// quotient); adding 1.5 2^23 + 128 rounds it to an integer, to even, and leaves
+// code + 128 in the low byte (|x / s| < 127.5, as s is at least the largest
+// magnitude / 127).  An e4m3 scale is a power of two: x r is exact.
+template <int kFmt>
+__device__ __forceinline__ uint32_t kv_encode4(const float (&x)[4], float s, float r) {
+  if constexpr (kFmt == NSMLP_KV_INT8) {
+    uint32_t c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float q = x[i] * r;
+      const float y = __builtin_fmaf(__builtin_fmaf(-q, s, x[i]), r, q);
+      c[i] = __float_as_uint(y + 12583040.0f);
+    }
+    const uint32_t lo = __builtin_amdgcn_perm(c[1], c[0], 0x0C0C0400u), hi = __builtin_amdgcn_perm(c[3], c[2], 0x04000C0Cu);
+    return lo | hi;
+  } else {
+    (void)s;
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * r, x[1] * r, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2] * r, x[3] * r, w, true);
   }
-  const int o0 = (int)(slot & (a.c.B - 1));  // first new offset
-  // run length: B <= 64 lanes look at the following tokens
-  const long long mine = t + lane < a.n && lane < a.c.B - o0 ? a.slots[t + lane] : -1;
-  const unsigned long long same = __ballot(mine == slot + lane);
-  const int n = same == ~0ull ? 64 : __builtin_ctzll(~same);
+}
 
-  const uint16_t* x = is_v ? a.v + (long long)t * a.v_row + (long long)h * a.v_head
-                           : a.k + (long long)t * a.k_row + (long long)h * a.k_head;
-  const long long row = is_v ? a.v_row : a.k_row;
+// A stored dword's codes under a larger scale.
+template <int kFmt>
+__device__ __forceinline__ uint32_t kv_recode4(uint32_t w, float s_old, float s, float r) {
+  float x[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = kv_decode1<kFmt>((w >> (8 * i)) & 0xFFu) * s_old;
+  return kv_encode4<kFmt>(x, s, r);
+}
+
+__device__ __forceinline__ uint32_t top16(uint32_t top, uint32_t w) {
+  return max(top, max(w & 0x7FFFu, (w >> 16) & 0x7FFFu));
+}
+
+template <int D, int B, int kFmt, bool kBf16>
+__device__ __forceinline__ void append_run(const KvAppendArgs& a, int t, long long slot, int n, int h, bool is_v, int lane) {
+  const long long blk = slot / B;
+  const int o0 = (int)(slot & (B - 1));  // first new offset
   float* sp = a.c.scale + (blk * a.c.heads + h) * 2 + (is_v ? 1 : 0);
+  uint8_t* dst = a.c.data + ((blk * a.c.heads + h) * 2 + (is_v ? 1 : 0)) * (long long)(B * D);
   const float s_old = o0 == 0 ? 0.0f : *sp;
-  uint8_t* dst = a.c.data + ((blk * a.c.heads + h) * 2 + (is_v ? 1 : 0)) * (long long)(a.c.B * D);
-
-  // largest magnitude, as bits (a NaN or infinity is above every finite value)
-  const int tl = lane / kChunks, c = lane % kChunks;
-  uint32_t top = 0;
-  for (int i = tl; i < n; i += kTok) {
-    const uint4* p = reinterpret_cast<const uint4*>(x + i * row + c * 16);
-    const uint4 u0 = p[0], u1 = p[1];
-    const uint32_t w[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
+  const auto settle = [&](uint32_t top, float& s, float& r, bool& recode) {
+    // largest magnitude, as bits (a NaN or infinity is above every finite value)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, max(w[j] & 0x7FFFu, (w[j] >> 16) & 0x7FFFu));
-  }
-#pragma unroll
-  for (int m = kWave / 2; m >= 1; m >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m, kWave));
-  const float need = kv_scale_of<kFmt>(in_value<kBf16>((uint16_t)top));
-  // a NaN on either side stays until the block is started anew
-  const float s_new = need != need || s_old != s_old ? __uint_as_float(0x7FC00000u) : fmaxf(s_old, need);
-  const bool recode = o0 > 0 && s_new != s_old;
-  if (lane == 0) *sp = s_new;
-
+    for (int m = kWave / 2; m >= 1; m >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m, kWave));
+    const float need = kv_scale_of<kFmt>(in_value<kBf16>(top));
+    // a NaN on either side stays until the block is started anew
+    s = need != need || s_old != s_old ? __uint_as_float(0x7FC00000u) : fmaxf(s_old, need);
+    r = 1.0f / s;
+    recode = o0 > 0 && s != s_old;
+    if (lane == 0) *sp = s;
+  };
+  float s, r;
+  bool recode;
   if (!is_v) {
+    constexpr int kChunks = D / 16, kTok = kWave / kChunks, kPass = B / kTok;  // tokens of a pass
+    const int tl = lane / kChunks, c = lane % kChunks;
+    const uint16_t* x = a.k + (long long)t * a.k_row + (long long)h * a.k_head + c * 16;
+    uint4 u[kPass][2];
+    uint32_t top = 0;
+#pragma unroll
+    for (int p = 0; p < kPass; ++p) {
+      const int i = p * kTok + tl;
+      u[p][0] = u[p][1] = uint4{0, 0, 0, 0};
+      if (i < n) {
+        const uint4* q = reinterpret_cast<const uint4*>(x + i * a.k_row);
+        u[p][0] = q[0], u[p][1] = q[1];
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < kPass; ++p)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) top = top16(top16(top16(top16(top, u[p][j].x), u[p][j].y), u[p][j].z), u[p][j].w);
+    settle(top, s, r, recode);
     if (recode) {
       for (int i = tl; i < o0; i += kTok) {
-        uint32_t* q = reinterpret_cast<uint32_t*>(dst + kv_k_off(D, i, c * 16));
+        uint4* q = reinterpret_cast<uint4*>(dst + kv_k_off(D, i, c * 16));
+        const uint4 w = *q;
+        *q = uint4{kv_recode4<kFmt>(w.x, s_old, s, r), kv_recode4<kFmt>(w.y, s_old, s, r), kv_recode4<kFmt>(w.z, s_old, s, r),
+                   kv_recode4<kFmt>(w.w, s_old, s, r)};
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < kPass; ++p) {
+      const int i = p * kTok + tl;
+      if (i < n) {
+        uint32_t o[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t w = q[j];
-          uint32_t r = 0;
-#pragma unroll
-          for (int b = 0; b < 4; ++b)
-            r |= kv_encode1<kFmt>(kv_decode1<kFmt>((w >> (8 * b)) & 0xFFu) * s_old / s_new) << (8 * b);
-          q[j] = r;
+          const uint4& v = u[p][j >> 1];
+          const uint32_t w0 = j & 1 ? v.z : v.x, w1 = j & 1 ? v.w : v.y;
+          const float e[4] = {in_lo<kBf16>(w0), in_hi<kBf16>(w0), in_lo<kBf16>(w1), in_hi<kBf16>(w1)};
+          o[j] = kv_encode4<kFmt>(e, s, r);
         }
+        *reinterpret_cast<uint4*>(dst + kv_k_off(D, o0 + i, c * 16)) = uint4{o[0], o[1], o[2], o[3]};
       }
-    }
-    for (int i = tl; i < n; i += kTok) {
-      const uint4* p = reinterpret_cast<const uint4*>(x + i * row + c * 16);
-      const uint4 u0 = p[0], u1 = p[1];
-      const uint32_t w[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
-      uint32_t r[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        r[j] = kv_encode1<kFmt>(in_value<kBf16>((uint16_t)w[2 * j]) / s_new) |
-               kv_encode1<kFmt>(in_value<kBf16>((uint16_t)(w[2 * j] >> 16)) / s_new) << 8 |
-               kv_encode1<kFmt>(in_value<kBf16>((uint16_t)w[2 * j + 1]) / s_new) << 16 |
-               kv_encode1<kFmt>(in_value<kBf16>((uint16_t)(w[2 * j + 1] >> 16)) / s_new) << 24;
-      }
-      *reinterpret_cast<uint4*>(dst + kv_k_off(D, o0 + i, c * 16)) = uint4{r[0], r[1], r[2], r[3]};
     }
   } else {
-    // pieces of 4 tokens by 4 dims, 16 bytes; the wave owns the block's V, so
-    // a piece's other tokens are read and written back
-    constexpr int kPieces = D / 4, kGroups = kWave / kPieces;
+    constexpr int kPieces = D / 4, kGroups = kWave / kPieces, kPass = B / 4 / kGroups;
     const int gl = lane / kPieces, d0 = lane % kPieces * 4;
-    const int g_end = (o0 + n + 3) >> 2;
-    for (int g = (recode ? 0 : o0 >> 2) + gl; g < g_end; g += kGroups) {
-      uint4* q = reinterpret_cast<uint4*>(dst + kv_v_off(D, 4 * g, d0));
-      const bool all_new = 4 * g >= o0 && 4 * g + 4 <= o0 + n;
-      uint4 old = uint4{0, 0, 0, 0};
-      if (!all_new) old = *q;
-      uint32_t w[4] = {old.x, old.y, old.z, old.w};
+    const uint16_t* x = a.v + ((long long)t - o0) * a.v_row + (long long)h * a.v_head + d0;
+    uint2 u[kPass][4];
+    uint32_t top = 0;
 #pragma unroll
-      for (int tt = 0; tt < 4; ++tt) {
-        const int off = 4 * g + tt;
-        if (off >= o0 && off < o0 + n) {
-          const uint2 u = *reinterpret_cast<const uint2*>(x + (off - o0) * row + d0);
-          const uint32_t e[2] = {u.x, u.y};
+    for (int p = 0; p < kPass; ++p)
 #pragma unroll
-          for (int d = 0; d < 4; ++d)
-            w[d] = (w[d] & ~(0xFFu << (8 * tt))) |
-                   kv_encode1<kFmt>(in_value<kBf16>((uint16_t)(e[d >> 1] >> (16 * (d & 1)))) / s_new) << (8 * tt);
-        } else if (off < o0 && recode) {
-#pragma unroll
-          for (int d = 0; d < 4; ++d)
-            w[d] = (w[d] & ~(0xFFu << (8 * tt))) |
-                   kv_encode1<kFmt>(kv_decode1<kFmt>((w[d] >> (8 * tt)) & 0xFFu) * s_old / s_new) << (8 * tt);
-        }
+      for (int i = 0; i < 4; ++i) {
+        const int off = 4 * (p * kGroups + gl) + i;
+        u[p][i] = uint2{0, 0};
+        if (off >= o0 && off < o0 + n) u[p][i] = *reinterpret_cast<const uint2*>(x + off * a.v_row);
       }
-      *q = uint4{w[0], w[1], w[2], w[3]};
+#pragma unroll
+    for (int p = 0; p < kPass; ++p)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = top16(top16(top, u[p][i].x), u[p][i].y);
+    settle(top, s, r, recode);
+#pragma unroll
+    for (int p = 0; p < kPass; ++p) {
+      const int first = 4 * (p * kGroups + gl);
+      if (first >= o0 + n || (!recode && first + 4 <= o0)) continue;
+      uint4* q = reinterpret_cast<uint4*>(dst + kv_v_off(D, first, d0));
+      // bytes of tokens before, in and after the run
+      const int lo = min(max(o0 - first, 0), 4), hi = min(o0 + n - first, 4);
+      const uint32_t before = lo == 4 ? ~0u : (1u << (8 * lo)) - 1u, upto = hi == 4 ? ~0u : (1u << (8 * hi)) - 1u;
+      uint4 old = uint4{0, 0, 0, 0};
+      if (lo > 0 || hi < 4) old = *q;
+      const uint32_t w[4] = {old.x, old.y, old.z, old.w};
+      uint32_t o[4];
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        float e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t v = d < 2 ? u[p][i].x : u[p][i].y;
+          e[i] = d & 1 ? in_hi<kBf16>(v) : in_lo<kBf16>(v);
+        }
+        const uint32_t kept = recode && lo > 0 ? kv_recode4<kFmt>(w[d], s_old, s, r) : w[d];
+        o[d] = (kept & before) | (kv_encode4<kFmt>(e, s, r) & upto & ~before) | (w[d] & ~upto);
+      }
+      *q = uint4{o[0], o[1], o[2], o[3]};
     }
+  }
+}
+
+template <int D, int B, int kFmt, bool kBf16>
+__global__ void __launch_bounds__(kAppendThreads, B == 64 ? 2 : 4) k_kv_append(KvAppendArgs a) {
+  kernarg_warm<sizeof(KvAppendArgs)>();
+  const int lane = threadIdx.x & (kWave - 1);
+  const int item = (int)blockIdx.x * (kAppendThreads / kWave) + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int two_heads = 2 * a.c.heads;
+  const int t0 = item / two_heads * a.take, hk = item % two_heads;
+  if (t0 >= a.n) return;
+  const long long limit = (long long)a.c.num_blocks * B;
+  // Slots of the wave's tokens and of the 64 after them, in one round trip:
+  // which start a run, and which go on with the one before them.
+  const auto slot_at = [&](int t) -> long long {
+    const long long v = t >= 0 && t < a.n ? a.slots[t] : -1;
+    return v < limit ? v : -1;
+  };
+  const long long s0 = slot_at(t0 + lane), s1 = slot_at(t0 + kWave + lane), p0 = slot_at(t0 + lane - 1), p1 = slot_at(t0 + kWave + lane - 1);
+  const bool on0 = s0 >= 0 && p0 == s0 - 1 && (s0 & (B - 1)) != 0, on1 = s1 >= 0 && p1 == s1 - 1 && (s1 & (B - 1)) != 0;
+  const unsigned long long go0 = __ballot(on0), go1 = __ballot(on1);
+  unsigned long long todo = __ballot(lane < a.take && s0 >= 0 && !on0);
+  while (todo != 0) {
+    const int i = __builtin_ctzll(todo);
+    todo &= todo - 1;
+    // tokens i + 1 ... that go on: at most B - 1 <= 63 of them
+    const unsigned long long after = i == kWave - 1 ? go1 : (go0 >> (i + 1)) | (go1 << (kWave - 1 - i));
+    const int n = after == ~0ull ? kWave : 1 + __builtin_ctzll(~after);
+    const long long slot = ((long long)__builtin_amdgcn_readlane((int)(s0 >> 32), i) << 32) |
+                           (uint32_t)__builtin_amdgcn_readlane((int)s0, i);
+    append_run<D, B, kFmt, kBf16>(a, t0 + i, slot, min(n, B - (int)(slot & (B - 1))), hk >> 1, hk & 1, lane);
   }
 }
 
 // ------------------------------------------------------------------ read --
-// One thread per 8 dims of a (slot, head): values code * scale, rounded once.
+// One thread per 16 dims of a (slot, head): values code * scale, rounded once.
+// The token's V bytes lie one in each dword of 4 pieces of 16; the threads of
+// the group's other tokens find the same pieces in the caches.
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack_out(float a, float b) {
+  if constexpr (kBf16) return __builtin_bit_cast(uint16_t, (__bf16)a) | (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)b) << 16;
+  else return f2h(a) | (uint32_t)f2h(b) << 16;
+}
+
 template <int D, int kFmt, bool kBf16>
 __global__ void __launch_bounds__(256) k_kv_read(KvReadArgs a) {
-  const long long item = (long long)blockIdx.x * 256 + threadIdx.x;
-  const int per = D / 8;
-  const int d0 = (int)(item % per) * 8;
-  const long long th = item / per;
-  const int h = (int)(th % a.c.heads);
-  const long long t = th / a.c.heads;
+  kernarg_warm<sizeof(KvReadArgs)>();
+  constexpr int kPer = D / 16;
+  const unsigned item = blockIdx.x * 256u + threadIdx.x;
+  const int c = (int)(item % kPer);
+  const unsigned th = item / kPer;
+  const int h = (int)(th % (unsigned)a.c.heads);
+  const int t = (int)(th / (unsigned)a.c.heads);
   if (t >= a.n) return;
   const long long slot = a.slots[t];
-  uint32_t out[2][4] = {};
+  uint32_t ko[8] = {}, vo[8] = {};
   if (slot >= 0 && slot < (long long)a.c.num_blocks * a.c.B) {
     const long long bh = (slot >> a.c.b_shift) * a.c.heads + h;
-    const int off = (int)(slot & (a.c.B - 1));
+    const int off = (int)(slot & (a.c.B - 1)), sh = 8 * (off & 3);
     const uint8_t* kb = a.c.data + bh * 2 * (long long)(a.c.B * D);
-    const uint8_t* vb = kb + a.c.B * D;
-    const float ks = a.c.scale[bh * 2], vs = a.c.scale[bh * 2 + 1];
-    const uint2 kw = *reinterpret_cast<const uint2*>(kb + kv_k_off(D, off, d0));
-    const uint8_t* vp = vb + kv_v_off(D, off, d0);
+    const uint4 kw = *reinterpret_cast<const uint4*>(kb + kv_k_off(D, off, c * 16));
+    const uint4* vp = reinterpret_cast<const uint4*>(kb + a.c.B * D + kv_v_off(D, off & ~3, c * 16));
+    const uint4 vw[4] = {vp[0], vp[1], vp[2], vp[3]};
+    const float2 s = *reinterpret_cast<const float2*>(a.c.scale + bh * 2);
+    const uint32_t kd[4] = {kw.x, kw.y, kw.z, kw.w};
 #pragma unroll
-    for (int d = 0; d < 8; ++d) {
-      const uint32_t kc = ((d < 4 ? kw.x : kw.y) >> (8 * (d & 3))) & 0xFFu;
-      const float kx = kv_decode1<kFmt>(kc) * ks, vx = kv_decode1<kFmt>(vp[4 * d]) * vs;
-      uint32_t kh, vh;
-      if constexpr (kBf16) {
-        kh = __builtin_bit_cast(uint16_t, (__bf16)kx), vh = __builtin_bit_cast(uint16_t, (__bf16)vx);
-      } else {
-        kh = f2h(kx), vh = f2h(vx);
+    for (int j = 0; j < 4; ++j) {
+      float k[4], v[4];
+      const uint32_t vd[4] = {vw[j].x, vw[j].y, vw[j].z, vw[j].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        k[i] = kv_decode1<kFmt>((kd[j] >> (8 * i)) & 0xFFu) * s.x;
+        v[i] = kv_decode1<kFmt>((vd[i] >> sh) & 0xFFu) * s.y;
       }
-      out[0][d >> 1] |= kh << (16 * (d & 1));
-      out[1][d >> 1] |= vh << (16 * (d & 1));
+      ko[2 * j] = pack_out<kBf16>(k[0], k[1]), ko[2 * j + 1] = pack_out<kBf16>(k[2], k[3]);
+      vo[2 * j] = pack_out<kBf16>(v[0], v[1]), vo[2 * j + 1] = pack_out<kBf16>(v[2], v[3]);
     }
   }
-  const long long o = (t * a.c.heads + h) * D + d0;
-  *reinterpret_cast<uint4*>(a.k + o) = uint4{out[0][0], out[0][1], out[0][2], out[0][3]};
-  *reinterpret_cast<uint4*>(a.v + o) = uint4{out[1][0], out[1][1], out[1][2], out[1][3]};
-}
-
-template <template <int, int, bool> class L, class A>
-void by_type(const A& a, bool bf16, hipStream_t s) {
-  const bool i8 = a.c.fmt == NSMLP_KV_INT8, d128 = a.c.D == 128;
-  if (d128) {
-    if (i8) bf16 ? L<128, NSMLP_KV_INT8, true>::go(a, s) : L<128, NSMLP_KV_INT8, false>::go(a, s);
-    else bf16 ? L<128, NSMLP_KV_E4M3, true>::go(a, s) : L<128, NSMLP_KV_E4M3, false>::go(a, s);
-  } else {
-    if (i8) bf16 ? L<64, NSMLP_KV_INT8, true>::go(a, s) : L<64, NSMLP_KV_INT8, false>::go(a, s);
-    else bf16 ? L<64, NSMLP_KV_E4M3, true>::go(a, s) : L<64, NSMLP_KV_E4M3, false>::go(a, s);
-  }
+  const long long o = ((long long)t * a.c.heads + h) * D + c * 16;
+  uint4 *kp = reinterpret_cast<uint4*>(a.k + o), *vp = reinterpret_cast<uint4*>(a.v + o);
+  kp[0] = uint4{ko[0], ko[1], ko[2], ko[3]}, kp[1] = uint4{ko[4], ko[5], ko[6], ko[7]};
+  vp[0] = uint4{vo[0], vo[1], vo[2], vo[3]}, vp[1] = uint4{vo[4], vo[5], vo[6], vo[7]};
 }
 
 template <int D, int kFmt, bool kBf16>
-struct AppendLaunch {
-  static void go(const KvAppendArgs& a, hipStream_t s) {
-    const long long waves = (long long)a.n * a.c.heads * 2, per = kAppendThreads / kWave;
-    k_kv_append<D, kFmt, kBf16><<<dim3((unsigned)((waves + per - 1) / per)), dim3(kAppendThreads), 0, s>>>(a);
-  }
-};
+void append_typed(KvAppendArgs a, hipStream_t s) {
+  // Most tokens of a long call are a prompt's, and the waves that find no first
+  // token of a run cost a round trip each: several tokens per wave where even
+  // then every CU has a dozen waves.  More would leave single tokens that stand
+  // next to each other to one wave, one after the other.
+  const long long pairs = (long long)a.n * a.c.heads * 2;
+  a.take = pairs >= 128 * 1024 ? 16 : pairs >= 32 * 1024 ? 8 : 1;
+  const long long waves = (long long)((a.n + a.take - 1) / a.take) * a.c.heads * 2, per = kAppendThreads / kWave;
+  const dim3 grid((unsigned)((waves + per - 1) / per)), block(kAppendThreads);
+  if (a.c.B == 16) k_kv_append<D, 16, kFmt, kBf16><<<grid, block, 0, s>>>(a);
+  else if (a.c.B == 32) k_kv_append<D, 32, kFmt, kBf16><<<grid, block, 0, s>>>(a);
+  else k_kv_append<D, 64, kFmt, kBf16><<<grid, block, 0, s>>>(a);
+}
+
 template <int D, int kFmt, bool kBf16>
-struct ReadLaunch {
-  static void go(const KvReadArgs& a, hipStream_t s) {
-    const long long items = (long long)a.n * a.c.heads * (D / 8);
-    k_kv_read<D, kFmt, kBf16><<<dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s>>>(a);
-  }
-};
+void read_typed(const KvReadArgs& a, hipStream_t s) {
+  const long long items = (long long)a.n * a.c.heads * (D / 16);
+  k_kv_read<D, kFmt, kBf16><<<dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s>>>(a);
+}
 
 }  // namespace
 
-void launch_kv_append(const KvAppendArgs& a, bool bf16, hipStream_t s) { by_type<AppendLaunch>(a, bf16, s); }
-void launch_kv_read(const KvReadArgs& a, bool bf16, hipStream_t s) { by_type<ReadLaunch>(a, bf16, s); }
+void launch_kv_append(const KvAppendArgs& a, bool bf16, hipStream_t s) { NSMLP_KV_BY_TYPE(append_typed, a, bf16, s); }
+void launch_kv_read(const KvReadArgs& a, bool bf16, hipStream_t s) { NSMLP_KV_BY_TYPE(read_typed, a, bf16, s); }
 
 KvSchedule kv_schedule(int requests, int total, int max_new, int group, int kv_heads) {
   (void)max_new;
@@ -534,15 +600,24 @@ KvSchedule kv_schedule(int requests, int total, int max_new, int group, int kv_h
   return s;
 }
 
-void launch_kv_plan(const KvPlanArgs& a, hipStream_t s) {
+template <int kThreads, int kPer>
+static void launch_plan(const KvPlanArgs& a, hipStream_t s) {
   static std::once_flag once;
-  constexpr int kMost = (5 * kKvMaxRequests + 1) * (int)sizeof(int);
+  constexpr int kMost = (6 * kThreads * kPer + 1) * (int)sizeof(int);
   std::call_once(once, [] {
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k_kv_plan), hipFuncAttributeMaxDynamicSharedMemorySize, kMost);
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k_kv_plan<kThreads, kPer>),
+                              hipFuncAttributeMaxDynamicSharedMemorySize, kMost);
   });
-  int groups = max((a.total + 2047) / 2048, (a.R + 63) / 64);
-  groups = min(max(groups, 1), 64);
-  k_kv_plan<<<dim3(groups), dim3(kPlanThreads), (5 * a.R + 1) * sizeof(int), s>>>(a);
+  // two tokens per thread, and at most 128 workgroups scan the lengths
+  const int groups = min(max((a.total + 2 * kThreads - 1) / (2 * kThreads), (a.R + 63) / 64), 128);
+  k_kv_plan<kThreads, kPer><<<dim3(max(groups, 1)), dim3(kThreads), (6 * a.R + 1) * sizeof(int), s>>>(a);
+}
+
+void launch_kv_plan(const KvPlanArgs& a, hipStream_t s) {
+  if (a.R <= 64) launch_plan<64, 1>(a, s);
+  else if (a.R <= 256) launch_plan<256, 1>(a, s);
+  else if (a.R <= 1024) launch_plan<1024, 1>(a, s);
+  else launch_plan<1024, kKvMaxRequests / 1024>(a, s);
 }
 
 void launch_kv_commit(const KvCommitArgs& a, hipStream_t s) {

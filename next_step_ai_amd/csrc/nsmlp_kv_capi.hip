@@ -115,7 +115,8 @@ int nsmlp_kv_append(const nsmlp_kv_cache* cache, const void* k, long long k_row_
   KvAppendArgs a;
   int rc = cache_view(cache, a.c);
   if (rc || (rc = check_dtype(dtype))) return rc;
-  if (n < 0 || n > kMaxTokens) return set_error(NSMLP_EINVAL, "n = %d out of range [0, 2^24]", n);
+  if (n < 0 || n > kMaxTokens || (long long)n * a.c.heads > (1 << 28))
+    return set_error(NSMLP_EINVAL, "n = %d rows of %d heads: at most 2^24 rows and 2^28 heads' rows", n, a.c.heads);
   if (n == 0) return NSMLP_OK;
   if (slots == nullptr) return set_error(NSMLP_EINVAL, "slots must be non-NULL");
   if ((rc = check_rows("k", k, k_row_stride, k_head_stride)) || (rc = check_rows("v", v, v_row_stride, v_head_stride))) return rc;
@@ -135,7 +136,8 @@ int nsmlp_kv_read(const nsmlp_kv_cache* cache, const int64_t* slots, int n, void
   KvReadArgs a;
   int rc = cache_view(cache, a.c);
   if (rc || (rc = check_dtype(dtype))) return rc;
-  if (n < 0 || n > kMaxTokens) return set_error(NSMLP_EINVAL, "n = %d out of range [0, 2^24]", n);
+  if (n < 0 || n > kMaxTokens || (long long)n * a.c.heads > (1 << 28))
+    return set_error(NSMLP_EINVAL, "n = %d rows of %d heads: at most 2^24 rows and 2^28 heads' rows", n, a.c.heads);
   if (n == 0) return NSMLP_OK;
   if (slots == nullptr) return set_error(NSMLP_EINVAL, "slots must be non-NULL");
   if ((rc = check_rows("k_out", k_out, 0, 0)) || (rc = check_rows("v_out", v_out, 0, 0))) return rc;
@@ -179,6 +181,7 @@ int nsmlp_kv_plan(const nsmlp_kv_batch* batch, const int32_t* new_tokens, const 
   a.info = step->info;
   a.sched = step->schedule;
   a.max_new = step->max_new == 0 ? 1 << 30 : step->max_new;
+  a.row_limit = (1 << 28) / a.group;  // rows of a request fit 32 bits
   launch_kv_plan(a, (hipStream_t)stream);
   return check_launch("nsmlp_kv_plan");
 }
@@ -252,8 +255,8 @@ int nsmlp_paged_attention(const nsmlp_kv_cache* cache, const nsmlp_kv_batch* bat
   a.scale_log2 = (float)((double)scale * 1.4426950408889634);
   // requests of few rows are on one list, the others on the second: empty where no request can be that long
   const int longest = step->max_new == 0 || step->max_new > step->total ? step->total : step->max_new;
-  const bool list_b = (long long)longest * a.group > a.s.rows_a;
-  launch_kv_attention(a, dtype == NSMLP_DTYPE_BF16, list_b, (hipStream_t)stream);
+  a.list_b = (long long)longest * a.group > a.s.rows_a;
+  launch_kv_attention(a, dtype == NSMLP_DTYPE_BF16, (hipStream_t)stream);
   return check_launch("nsmlp_paged_attention");
 }
 

@@ -18,7 +18,6 @@ attention and K/V cache are torch code in ``streaming_llama_runtime.py``
 from __future__ import annotations
 
 import ctypes
-import math
 
 import torch
 
@@ -35,18 +34,24 @@ def _device(device) -> torch.device:
     return require_device(torch.empty(0, device="cuda" if device is None else device), "cache")
 
 
-def _rows(t: torch.Tensor, what: str, heads: int, dim: int, device: torch.device) -> torch.Tensor:
-    """[tokens, heads, dim] in fp16 or bf16 that the kernels can read in 16-byte pieces; a copy where the strides do not allow it."""
+def _rows(t: torch.Tensor, what: str, heads: int, dim: int, device: torch.device) -> tuple[torch.Tensor, int, int, int]:
+    """(tensor, address, row and head stride) of [tokens, heads, dim] in fp16 or
+    bf16 that the kernels can read in 16-byte pieces; a copy where the strides
+    do not allow it."""
     if t.dtype not in _DTYPES:
         raise RuntimeError(f"{what} must be fp16 or bf16, got {t.dtype}")
-    if t.dim() != 3 or tuple(t.shape[1:]) != (heads, dim):
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim:
         raise RuntimeError(f"{what} must be [tokens, {heads}, {dim}], got {tuple(t.shape)}")
     if t.device != device:
-        raise RuntimeError(f"{what} must be on {device}, got {t.device}")
-    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
+        raise RuntimeError(f"{what} must be a GPU tensor on {device}, got {t.device}")
+    row, head, one = t.stride()
+    p = t.data_ptr()
+    if one != 1 or row % 8 or head % 8 or p % 16:
         t = t.contiguous()
         t = t if t.data_ptr() % 16 == 0 else t.clone()
-    return t
+        row, head, _ = t.stride()
+        p = t.data_ptr()
+    return t, p, row, head
 
 
 def _slots(t: torch.Tensor, device: torch.device) -> torch.Tensor:
@@ -77,21 +82,22 @@ class KvCache:
         self._view = _lib.KvCacheView(num_blocks=self.num_blocks, kv_heads=self.kv_heads, head_dim=self.head_dim,
                                       block_tokens=self.block_tokens, format=_FORMATS[fmt], data=ptr(self.data),
                                       scale=ptr(self.scale))
+        self._ref = ctypes.byref(self._view)
 
     def append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         """Store the rows ``k``, ``v`` [tokens, kv_heads, head_dim] at ``slots``
         (a plan's: a block's tokens stand next to each other, in order; a slot
         of -1 stores nothing).  Where the new rows exceed a block's scale its
         stored codes are rewritten under the larger one."""
-        k = _rows(k, "k", self.kv_heads, self.head_dim, self.device)
-        v = _rows(v, "v", self.kv_heads, self.head_dim, self.device)
+        k, kp, k_row, k_head = _rows(k, "k", self.kv_heads, self.head_dim, self.device)
+        v, vp, v_row, v_head = _rows(v, "v", self.kv_heads, self.head_dim, self.device)
         slots = _slots(slots, self.device)
-        n = int(slots.numel())
-        if k.dtype != v.dtype or int(k.shape[0]) != n or int(v.shape[0]) != n:
+        n = slots.shape[0]
+        if k.dtype != v.dtype or k.shape[0] != n or v.shape[0] != n:
             raise RuntimeError(f"k, v and slots must be of the same length and k and v of one dtype: got {tuple(k.shape)} "
                                f"{k.dtype}, {tuple(v.shape)} {v.dtype} and {n} slots")
-        _lib.call("nsmlp_kv_append", ctypes.byref(self._view), ptr(k), k.stride(0), k.stride(1), ptr(v), v.stride(0),
-                  v.stride(1), _DTYPES[k.dtype], ptr(slots), n, stream_handle(self.device))
+        _lib.call("nsmlp_kv_append", self._ref, kp, k_row, k_head, vp, v_row, v_head, _DTYPES[k.dtype], slots.data_ptr(), n,
+                  stream_handle(self.device))
 
     def read(self, slots: torch.Tensor, dtype: torch.dtype = torch.float16) -> dict[str, torch.Tensor]:
         """The stored rows at ``slots``: ``{"k": ..., "v": ...}`` of [tokens,
@@ -99,11 +105,25 @@ class KvCache:
         if dtype not in _DTYPES:
             raise RuntimeError(f"dtype must be fp16 or bf16, got {dtype}")
         slots = _slots(slots, self.device)
-        n = int(slots.numel())
-        out = torch.empty(2, n, self.kv_heads, self.head_dim, dtype=dtype, device=self.device)
-        _lib.call("nsmlp_kv_read", ctypes.byref(self._view), ptr(slots), n, ptr(out[0]), ptr(out[1]), _DTYPES[dtype],
+        n = slots.shape[0]
+        shape = (n, self.kv_heads, self.head_dim)
+        k, v = torch.empty(shape, dtype=dtype, device=self.device), torch.empty(shape, dtype=dtype, device=self.device)
+        _lib.call("nsmlp_kv_read", self._ref, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), _DTYPES[dtype],
                   stream_handle(self.device))
-        return {"k": out[0], "v": out[1]}
+        return {"k": k, "v": v}
+
+
+class _StepLayout:
+    """Sizes of a step's buffers, which depend on its total and max_new alone."""
+
+    __slots__ = ("ints", "schedule_bytes", "ws_bytes")
+
+    def __init__(self, batch: "KvBatch", total: int, max_new: int):
+        self.schedule_bytes = int(_lib.lib().nsmlp_kv_schedule_bytes(batch._ref, total, max_new))
+        if self.schedule_bytes == 0:
+            raise RuntimeError(f"nsmlp_kv_schedule_bytes: {_lib.last_error()}")
+        self.ints = (3 * batch.requests + 5 + 3) // 4 * 4
+        self.ws_bytes: dict[int, int] = {}
 
 
 class KvStep:
@@ -113,38 +133,40 @@ class KvStep:
     block table.  ``info`` and the others are device tensors: reading them
     waits for the stream."""
 
+    __slots__ = ("batch", "total", "max_new", "slots", "_buf", "_layout", "_view", "_ref")
+
     def __init__(self, batch: "KvBatch", total: int, max_new: int):
-        R, dev = batch.requests, batch.device
-        self.batch, self.total, self.max_new = batch, int(total), int(max_new)
-        nbytes = int(_lib.lib().nsmlp_kv_schedule_bytes(ctypes.byref(batch._view), self.total, self.max_new))
-        if nbytes == 0:
-            raise RuntimeError(f"nsmlp_kv_schedule_bytes: {_lib.last_error()}")
-        # one allocation: slots, then q_start, kv_len, next and info, then the schedule
-        head = 8 * self.total
-        ints = (3 * R + 5 + 3) // 4 * 4
-        pad = -head % 16
-        buf = torch.empty(head + pad + 4 * ints + nbytes, dtype=torch.uint8, device=dev)
-        self.slots = buf[:head].view(torch.int64)
-        v = buf[head + pad: head + pad + 4 * ints].view(torch.int32)
-        self.q_start, self.kv_len, self._next, self.info = v[:R + 1], v[R + 1: 2 * R + 1], v[2 * R + 1: 3 * R + 1], \
-            v[3 * R + 1: 3 * R + 5]
-        base = ptr(buf) + head + pad
-        self._buf = buf
-        self._view = _lib.KvStepView(total=self.total, max_new=self.max_new, slots=ptr(buf), q_start=base,
-                                     kv_len=base + 4 * (R + 1), next=base + 4 * (2 * R + 1), info=base + 4 * (3 * R + 1),
-                                     schedule=base + 4 * ints, schedule_bytes=nbytes)
-        self._ws_bytes: dict[int, int] = {}
+        lay = batch._layout(total, max_new)
+        self.batch, self.total, self.max_new, self._layout = batch, total, max_new, lay
+        self.slots = torch.empty(total, dtype=torch.int64, device=batch.device)
+        # q_start, kv_len, next and info, then the schedule at the next 16 bytes
+        self._buf = torch.empty(lay.ints + lay.schedule_bytes // 4, dtype=torch.int32, device=batch.device)
+        base, R = self._buf.data_ptr(), batch.requests
+        self._view = _lib.KvStepView(total, max_new, self.slots.data_ptr(), base, base + 4 * (R + 1), base + 4 * (2 * R + 1),
+                                     base + 4 * (3 * R + 1), base + 4 * lay.ints, lay.schedule_bytes)
+        self._ref = ctypes.byref(self._view)
+
+    @property
+    def q_start(self) -> torch.Tensor:
+        return self._buf.narrow(0, 0, self.batch.requests + 1)
+
+    @property
+    def kv_len(self) -> torch.Tensor:
+        return self._buf.narrow(0, self.batch.requests + 1, self.batch.requests)
+
+    @property
+    def info(self) -> torch.Tensor:
+        return self._buf.narrow(0, 3 * self.batch.requests + 1, 4)
 
     @property
     def table(self) -> torch.Tensor:
         return self.batch.table
 
     def workspace_bytes(self, head_dim: int) -> int:
-        n = self._ws_bytes.get(head_dim)
+        n = self._layout.ws_bytes.get(head_dim)
         if n is None:
-            n = int(_lib.lib().nsmlp_paged_attention_workspace_bytes(ctypes.byref(self.batch._view), self.total, self.max_new,
-                                                                    head_dim))
-            self._ws_bytes[head_dim] = n
+            n = int(_lib.lib().nsmlp_paged_attention_workspace_bytes(self.batch._ref, self.total, self.max_new, head_dim))
+            self._layout.ws_bytes[head_dim] = n
         return n
 
     def check(self) -> None:
@@ -187,9 +209,18 @@ class KvBatch:
                                       block_tokens=self.block_tokens, q_heads=self.q_heads, kv_heads=self.kv_heads,
                                       cached=ptr(self.cached), table=ptr(self.table), ring=ptr(self.ring),
                                       state=ptr(self.state))
-        if int(_lib.lib().nsmlp_kv_schedule_bytes(ctypes.byref(self._view), 1, 0)) == 0:
-            raise RuntimeError(f"KvBatch: {_lib.last_error()}")
+        self._ref = ctypes.byref(self._view)
+        self._layouts: dict[tuple[int, int], _StepLayout] = {}
+        self._layout(1, 0)  # checks the arguments
         self._step: KvStep | None = None
+
+    def _layout(self, total: int, max_new: int) -> _StepLayout:
+        lay = self._layouts.get((total, max_new))
+        if lay is None:
+            if len(self._layouts) >= 1024:
+                self._layouts.clear()
+            lay = self._layouts[(total, max_new)] = _StepLayout(self, total, max_new)
+        return lay
 
     def plan(self, new_tokens: torch.Tensor, total: int, *, max_new: int = 0, step: KvStep | None = None) -> KvStep:
         """Place the step's tokens: ``new_tokens`` [requests] int32 on the
@@ -199,15 +230,15 @@ class KvBatch:
         are until :meth:`commit`; a plan that is not committed can be made
         again.  ``step``: an earlier step of the same ``total`` and ``max_new``
         whose buffers are written again (a captured graph's)."""
-        if new_tokens.dtype != torch.int32 or new_tokens.device != self.device or int(new_tokens.numel()) != self.requests \
+        total, max_new = int(total), int(max_new)
+        if new_tokens.dtype != torch.int32 or new_tokens.device != self.device or new_tokens.numel() != self.requests \
                 or not new_tokens.is_contiguous():
             raise RuntimeError(f"new_tokens must be a contiguous int32 [{self.requests}] tensor on {self.device}")
         if step is None:
             step = KvStep(self, total, max_new)
-        elif step.batch is not self or step.total != int(total) or step.max_new != int(max_new):
+        elif step.batch is not self or step.total != total or step.max_new != max_new:
             raise RuntimeError("the step to plan into belongs to another batch, total or max_new")
-        _lib.call("nsmlp_kv_plan", ctypes.byref(self._view), ptr(new_tokens), ctypes.byref(step._view),
-                  stream_handle(self.device))
+        _lib.call("nsmlp_kv_plan", self._ref, new_tokens.data_ptr(), step._ref, stream_handle(self.device))
         self._step = step
         return step
 
@@ -218,8 +249,7 @@ class KvBatch:
                                      or int(finished.numel()) != self.requests or not finished.is_contiguous()):
             raise RuntimeError(f"finished must be a contiguous int32 [{self.requests}] tensor on {self.device}")
         st, self._step = self._step, None
-        _lib.call("nsmlp_kv_commit", ctypes.byref(self._view), None if st is None else ctypes.byref(st._view), ptr(finished),
-                  stream_handle(self.device))
+        _lib.call("nsmlp_kv_commit", self._ref, None if st is None else st._ref, ptr(finished), stream_handle(self.device))
 
 
 def paged_attention(q: torch.Tensor, cache: KvCache, step: KvStep, *, scale: float | None = None,
@@ -230,26 +260,25 @@ def paged_attention(q: torch.Tensor, cache: KvCache, step: KvStep, *, scale: flo
     K and V are appended before the call).  ``scale`` defaults to
     1/sqrt(head_dim).  Returns ``out`` [total, q_heads, head_dim]; ``lse``
     ([total, q_heads] fp32) receives the log of the softmax sums."""
-    device = require_device(q, "q")
-    b = step.batch
-    if cache.device != device or b.device != device:
-        raise RuntimeError(f"q is on {device}, the cache on {cache.device} and the batch on {b.device}")
-    q = _rows(q, "q", b.q_heads, cache.head_dim, device)
-    if int(q.shape[0]) != step.total:
-        raise RuntimeError(f"q holds {int(q.shape[0])} tokens, the step {step.total}")
-    shape = (step.total, b.q_heads, cache.head_dim)
+    b, device, dim = step.batch, cache.device, cache.head_dim
+    if b.device != device:
+        raise RuntimeError(f"the cache is on {device} and the batch on {b.device}")
+    total, heads = step.total, b.q_heads
+    q, qp, q_row, q_head = _rows(q, "q", heads, dim, device)
+    if q.shape[0] != total:
+        raise RuntimeError(f"q holds {q.shape[0]} tokens, the step {total}")
+    dtype = q.dtype
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=device)
-    elif out.dtype != q.dtype or out.device != device or tuple(out.shape) != shape or not out.is_contiguous() \
+        out = torch.empty((total, heads, dim), dtype=dtype, device=device)
+    elif out.dtype != dtype or out.device != device or tuple(out.shape) != (total, heads, dim) or not out.is_contiguous() \
             or out.data_ptr() % 16:
-        raise RuntimeError(f"out must be a contiguous, 16-byte aligned {q.dtype} tensor {shape} on {device}")
-    if lse is not None and (lse.dtype != torch.float32 or lse.device != device or tuple(lse.shape) != shape[:2]
+        raise RuntimeError(f"out must be a contiguous, 16-byte aligned {dtype} tensor {(total, heads, dim)} on {device}")
+    if lse is not None and (lse.dtype != torch.float32 or lse.device != device or tuple(lse.shape) != (total, heads)
                             or not lse.is_contiguous()):
-        raise RuntimeError(f"lse must be a contiguous fp32 tensor {shape[:2]} on {device}")
+        raise RuntimeError(f"lse must be a contiguous fp32 tensor {(total, heads)} on {device}")
     if ws is None:
-        ws = workspace(step.workspace_bytes(cache.head_dim), device)
-    _lib.call("nsmlp_paged_attention", ctypes.byref(cache._view), ctypes.byref(b._view), ctypes.byref(step._view), ptr(q),
-              q.stride(0), q.stride(1), _DTYPES[q.dtype],
-              1.0 / math.sqrt(cache.head_dim) if scale is None else float(scale), ptr(out), ptr(lse), ptr(ws), ws.numel(),
-              stream_handle(device))
+        ws = workspace(step.workspace_bytes(dim), device)
+    _lib.call("nsmlp_paged_attention", cache._ref, b._ref, step._ref, qp, q_row, q_head, _DTYPES[dtype],
+              dim ** -0.5 if scale is None else float(scale), out.data_ptr(), None if lse is None else lse.data_ptr(),
+              ws.data_ptr(), ws.numel(), stream_handle(device))
     return out
