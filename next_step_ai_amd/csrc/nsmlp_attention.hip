@@ -14,6 +14,9 @@
 // maxima between lanes; a weight is then at most 2^8, far inside fp16.
 // acc, l, m and the scores are fp32; a weight is rounded to fp16 once, as the
 // products' operand (relative 2^-12, averaged over the keys).
+#include <mutex>
+#include <type_traits>
+
 #include "nsmlp_kv.h"
 
 namespace nsmlp {
@@ -39,6 +42,22 @@ template <bool kBf16>
 __device__ __forceinline__ uint16_t to_out(float x) {
   if constexpr (kBf16) return __builtin_bit_cast(uint16_t, (__bf16)x);
   else return f2h(x);
+}
+
+// bf16 queries become fp16 under a power of two of the row's own: its largest
+// magnitude (bits `top`) lands in [1, 2), what it loses is below 2^-24 of that.
+__device__ __forceinline__ int row_exponent(uint32_t top) { return min(max((int)(top >> 7), 1), 254) - 127; }
+
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+__device__ __forceinline__ uint4 bf16_to_f16(const uint4& raw, int e) {
+  uint32_t o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = word(raw, i);
+    o[i] = pack_f16(ldexpf(__uint_as_float(w << 16), -e), ldexpf(__uint_as_float(w & 0xFFFF0000u), -e));
+  }
+  return uint4{o[0], o[1], o[2], o[3]};
 }
 
 // Pages of a range of keys, held one per lane: 64 pages from page `first`.
@@ -99,8 +118,6 @@ __device__ __forceinline__ void load_tile(StreamTile<D, kFmt>& t, const KvAttnAr
   }
 }
 
-__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
-
 template <int D, int kFmt, bool kBf16, int NB>
 __global__ void __launch_bounds__(kStreamThreads) k_attn_stream(KvAttnArgs a, const KvUnit* units, const int32_t* n_units,
                                                                 int max_units, int rows_of_unit, float* acc_out, float* ml_out) {
@@ -133,30 +150,17 @@ __global__ void __launch_bounds__(kStreamThreads) k_attn_stream(KvAttnArgs a, co
         raw[s] = in ? *reinterpret_cast<const uint4*>(src + 64 * (s >> 1) + 16 * grp + 8 * (s & 1)) : uint4{0, 0, 0, 0};
       rowf[b] = a.scale_log2;
       if constexpr (kBf16) {
-        // bf16 queries become fp16 under a power of two of the row's own: its
-        // largest magnitude lands in [1, 2), what it loses is below 2^-24 of it
         uint32_t top = 0;
 #pragma unroll
         for (int s = 0; s < KS; ++s)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t w = word(raw[s], i);
-            top = max(top, max(w & 0x7FFFu, (w >> 16) & 0x7FFFu));
-          }
+          for (int i = 0; i < 4; ++i) top = max(top, max(word(raw[s], i) & 0x7FFFu, (word(raw[s], i) >> 16) & 0x7FFFu));
         top = max(top, (uint32_t)__shfl_xor((int)top, 16, kWave));
         top = max(top, (uint32_t)__shfl_xor((int)top, 32, kWave));
-        const int e = min(max((int)(top >> 7), 1), 254) - 127;  // exponent of the largest
+        const int e = row_exponent(top);
         rowf[b] *= ldexpf(1.0f, e);
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          uint32_t o[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t w = word(raw[s], i);
-            o[i] = pack_f16(ldexpf(__uint_as_float(w << 16), -e), ldexpf(__uint_as_float(w & 0xFFFF0000u), -e));
-          }
-          q[b][s] = as_h8(uint4{o[0], o[1], o[2], o[3]});
-        }
+        for (int s = 0; s < KS; ++s) q[b][s] = as_h8(bf16_to_f16(raw[s], e));
       } else {
 #pragma unroll
         for (int s = 0; s < KS; ++s) q[b][s] = as_h8(raw[s]);
@@ -227,10 +231,10 @@ __global__ void __launch_bounds__(kStreamThreads) k_attn_stream(KvAttnArgs a, co
               if (masked && !((seen >> (4 * s + i)) & 1)) e[s][i] = kLowest;
               top = fmaxf(top, e[s][i]);
             }
-          if (__any(top > m[b] + kLazy)) {
+          if (__builtin_expect_with_probability(__any(top > m[b] + kLazy), 0, 0.99)) {
             top = fmaxf(top, m[b]);
             top = fmaxf(top, __shfl_xor(top, 16, kWave));
-            top = fmaxf(top, __shfl_xor(top, 32, kWave));
+            top = ceilf(fmaxf(top, __shfl_xor(top, 32, kWave)));  // an integer: rescaling is exact
             const float scale = exp2_fast(m[b] - top);
             m[b] = top;
             l[b] *= scale, x[b] *= scale;
@@ -357,6 +361,328 @@ __global__ void __launch_bounds__(kStreamThreads) k_attn_stream(KvAttnArgs a, co
   }
 }
 
+// ----------------------------------------------------------------- tiles --
+// Prompts and chunks: NW waves of 32 query rows each against tiles of 64 keys
+// that the workgroup decodes to fp16 once, in LDS, as the operands of
+// v_mfma_f32_32x32x16_f16 (A rows: keys or dims, B columns: queries):
+//   K fragment (32 keys, 16 dims): lane l: key l % 32, dims 16 (2 a + l / 32) + 8 u + 0..7
+//   V fragment (32 dims, 16 keys): lane l: keys 4 h + 0..3 and 8 + 4 h + 0..3, h = l / 32
+// so that the scores of a query stay in its two lanes, in the order in which
+// the second product wants the weights.
+//
+// A tile's weights are taken under the reference as it stands; their sums, kept
+// anyway, tell whether one was too large for it (the first tile, and seldom
+// after), and only then is the maximum looked for.  References are integers,
+// so that rescaling is exact.
+constexpr int kTileKeys = 64;
+constexpr float kSumLimit = 4096.0f;  // 16 weights of a lane: none above 2^12, far inside fp16
+
+__device__ __forceinline__ float max16(const float16_t& s, int at) {
+  return fmaxf(fmaxf(fmaxf(s[at], s[at + 1]), fmaxf(s[at + 2], s[at + 3])),
+               fmaxf(fmaxf(s[at + 4], s[at + 5]), fmaxf(s[at + 6], s[at + 7])));
+}
+
+// What the products of a tile need to know of its blocks, per 16 keys.
+struct TileMeta {
+  float4_t ks, lv, iv;
+  int bad[4];
+};
+
+template <int D, int kFmt, bool kBf16, int NW, bool kLse>
+__global__ void __launch_bounds__(NW* kWave, 2) k_attn_tile(KvAttnArgs a, const KvUnit* units, const int32_t* n_units,
+                                                            int max_units, float* acc_out, float* ml_out) {
+  constexpr int KS = D / 16, ND = D / 32, NJ = D / 64, kRows = 32 * NW;
+  constexpr int kKBytes = 2 * KS * 1024, kVBytes = 4 * ND * 1024;  // fragments of a tile: 1 KB each
+  constexpr int kBuf = kKBytes + kVBytes + 64;
+  extern __shared__ __attribute__((aligned(16))) char lds[];  // [2][K fragments, V fragments, TileMeta]
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  // the 16 keys of a tile that this wave decodes: K, V or (4 waves) both
+  const int part = wave & 3;
+  const bool does_k = NW == 4 || wave < 4, does_v = NW == 4 || wave >= 4;
+  const int items = min(*n_units, max_units) * a.c.heads;
+  for (int item = blockIdx.x; item < items; item += gridDim.x) {
+    const int h = item % a.c.heads;
+    const KvUnit u = units[item / a.c.heads];
+    const int q0 = a.q_start[u.req], q_len = a.q_start[u.req + 1] - q0, kv_len = a.kv_len[u.req];
+    const int rows = min(q_len * a.group - u.row, kRows);
+    const int r = wave * 32 + col, row = u.row + r, tok = row / a.group;
+    const bool in = r < rows && q0 + tok < a.total;
+    const int limit = in ? kv_len - q_len + tok + 1 : 0x7FFFFFFF;  // keys that the row sees
+
+    half8_t q[KS];
+    float rowf = a.scale_log2;
+    {
+      const uint16_t* src = a.q + (long long)(q0 + tok) * a.q_row + (long long)(h * a.group + row % a.group) * a.q_head;
+      uint4 raw[KS];
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+        raw[s] = in ? *reinterpret_cast<const uint4*>(src + 16 * ((s & ~1) + half) + 8 * (s & 1)) : uint4{0, 0, 0, 0};
+      if constexpr (kBf16) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top = max(top, max(word(raw[s], i) & 0x7FFFu, (word(raw[s], i) >> 16) & 0x7FFFu));
+        top = max(top, (uint32_t)__shfl_xor((int)top, 32, kWave));
+        const int e = row_exponent(top);
+        rowf *= ldexpf(1.0f, e);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) q[s] = as_h8(bf16_to_f16(raw[s], e));
+      } else {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) q[s] = as_h8(raw[s]);
+      }
+    }
+    // keys below `plain` need no mask in this wave, keys from `most` on do not matter to it
+    const int first_row = u.row + min(wave * 32, rows), end_row = u.row + min((wave + 1) * 32, rows);
+    const int plain = kv_len - q_len + first_row / a.group + 1;
+    const int most = end_row > first_row ? kv_len - q_len + (end_row - 1) / a.group + 1 : 0;
+    const int last = max(0, (u.kv_end - 1) >> a.c.b_shift);
+
+    float m = kLowest, l = 0.0f, x = 0.0f;
+    float16_t acc[ND];
+#pragma unroll
+    for (int n = 0; n < ND; ++n)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[n][e] = 0.0f;
+
+    unsigned long long bad_seen = 0;
+    Pages pages = load_pages(a, u.req, h, u.kv_begin >> a.c.b_shift, last, lane);
+    if (u.kv_begin < u.kv_end) bad_seen = pages.bad;
+
+    uint4 kr[NJ], vr[2];
+    const auto load = [&](int pos, const Pages& p) {
+      const int at = pos + 16 * part;
+      const int id = __builtin_amdgcn_readlane(p.id, min(at >> a.c.b_shift, last) - p.first);
+      const uint8_t* kb = a.c.data + ((long long)id * a.c.heads + h) * 2 * (a.c.B * D) + ((at & (a.c.B - 1)) >> 4) * (16 * D);
+      const uint8_t* vb = kb + a.c.B * D;
+      if (does_k) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) kr[j] = *reinterpret_cast<const uint4*>(kb + j * 1024 + lane * 16);
+      }
+      if (does_v) {
+        // (head size 64: the upper lanes repeat the lower ones)
+        const uint8_t* p0 = D == 128 ? vb + ((lane >> 4) & 1) * 1024 + half * 256 + (lane & 15) * 16
+                                     : vb + ((lane >> 4) & 1) * 256 + (lane & 15) * 16;
+        vr[0] = *reinterpret_cast<const uint4*>(p0);
+        vr[1] = *reinterpret_cast<const uint4*>(p0 + 512);
+      }
+    };
+    const auto store = [&](int pos, const Pages& p, char* buf) {
+      const int at = pos + 16 * part, pg = min(at >> a.c.b_shift, last) - p.first;
+      const bool bad = (p.bad >> pg) & 1;
+      if (does_k) {
+        // chunk c = 4 j + lane / 16 of token lane % 16
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          const int c = 4 * j + (lane >> 4);
+          char* dst = buf + ((((part >> 1) * KS + (c & ~1)) * 64) + (c & 1) * 32 + (part & 1) * 16 + (lane & 15)) * 16;
+          const uint2 w0 = kv_half4<kFmt>(kr[j].x), w1 = kv_half4<kFmt>(kr[j].y), w2 = kv_half4<kFmt>(kr[j].z),
+                      w3 = kv_half4<kFmt>(kr[j].w);
+          *reinterpret_cast<uint4*>(dst) = uint4{w0.x, w0.y, w1.x, w1.y};
+          *reinterpret_cast<uint4*>(dst + 1024) = uint4{w2.x, w2.y, w3.x, w3.y};
+        }
+        if (lane == pg) {
+          TileMeta* t = reinterpret_cast<TileMeta*>(buf + kKBytes + kVBytes);
+          reinterpret_cast<float*>(&t->ks)[part] = p.ks;
+          reinterpret_cast<float*>(&t->lv)[part] = p.lv;
+          reinterpret_cast<float*>(&t->iv)[part] = p.iv;
+          t->bad[part] = bad;
+        }
+      }
+      if (does_v) {
+        uint32_t keep[2] = {~0u, ~0u};
+        if (kFmt == NSMLP_KV_E4M3 && (at + 16 > kv_len || bad)) {
+          // codes past the end may be NaNs: a zero weight does not hide them
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int left = bad ? 0 : kv_len - (at + 8 * i + 4 * (D == 128 ? half : (lane >> 4) & 1));
+            keep[i] = left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+          }
+        }
+        char* vbuf = buf + kKBytes + part * ND * 1024;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint2 lo = kv_half4<kFmt>(word(vr[0], i) & keep[0]), hi = kv_half4<kFmt>(word(vr[1], i) & keep[1]);
+          const uint4 f = uint4{lo.x, lo.y, hi.x, hi.y};
+          if constexpr (D == 128) {
+            *reinterpret_cast<uint4*>(vbuf + (i * 64 + lane) * 16) = f;
+          } else {
+            if (lane < 32)
+              *reinterpret_cast<uint4*>(vbuf + ((i >> 1) * 64 + ((lane >> 4) & 1) * 32 + (lane & 15) + 16 * (i & 1)) * 16) = f;
+          }
+        }
+      }
+    };
+
+    // One tile's products.  kMasked: some rows do not see all of its keys.
+    const auto tile = [&](auto masked, int pos, const char* buf) {
+      constexpr bool kMasked = decltype(masked)::value;
+      const half8_t* kf = reinterpret_cast<const half8_t*>(buf) + lane;
+      const half8_t* vf = reinterpret_cast<const half8_t*>(buf + kKBytes) + lane;
+      const TileMeta* t = reinterpret_cast<const TileMeta*>(buf + kKBytes + kVBytes);
+      const float4_t ks = t->ks, lv = t->lv, iv = t->iv;
+      float16_t s[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[i][e] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) s[i] = mfma32(kf[(i * KS + k) * 64], q[k], s[i]);
+      }
+      // bit 8 i + e: whether the row sees key e of the lane's 8 among the tile's i-th 16
+      uint32_t see = ~0u;
+      if constexpr (kMasked) {
+        see = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int n = min(max(limit - pos - 8 * i - 4 * half, 0), 4);
+          see |= ((1u << n) - 1u) << (4 * i);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) see = t->bad[i] != 0 ? see & ~(0xFFu << (8 * i)) : see;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[i][e] = (see >> (16 * i + e)) & 1 ? s[i][e] : -INFINITY;
+      }
+      uint4 w[4];
+      float dl, dx;
+      const auto weights = [&]() {
+        dl = dx = 0.0f;
+        float most_sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float g = ks[i] * rowf, c = lv[i] - m;
+          float p[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) p[e] = exp2_fast(__builtin_fmaf(s[i >> 1][8 * (i & 1) + e], g, c));
+          float share = iv[i];
+          if constexpr (kMasked) {
+            // a hidden key's weight is zero whatever its block's scales are
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p[e] = (see >> (8 * i + e)) & 1 ? p[e] : 0.0f;
+            share = (see >> (8 * i)) & 0xFF ? share : 0.0f;
+          }
+          w[i] = uint4{pack_f16(p[0], p[1]), pack_f16(p[2], p[3]), pack_f16(p[4], p[5]), pack_f16(p[6], p[7])};
+          const half2_t one = {(_Float16)1.0f, (_Float16)1.0f};
+          float sum = __builtin_amdgcn_fdot2(as_half2(w[i].x), one, 0.0f, false);
+          sum = __builtin_amdgcn_fdot2(as_half2(w[i].y), one, sum, false);
+          sum = __builtin_amdgcn_fdot2(as_half2(w[i].z), one, sum, false);
+          sum = __builtin_amdgcn_fdot2(as_half2(w[i].w), one, sum, false);
+          most_sum = i == 0 ? sum : fmaxf(most_sum, sum);
+          dl = __builtin_fmaf(sum, share, dl);
+          if constexpr (kLse) dx = __builtin_fmaf(((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])), share, dx);
+        }
+        return most_sum;
+      };
+      sched_fence();  // the products' operands are not fetched further ahead than registers last
+      const float sum = weights();
+      if (__builtin_expect_with_probability(__any(sum > kSumLimit), 0, 0.999)) {
+        float top = kLowest;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, __builtin_fmaf(max16(s[i >> 1], 8 * (i & 1)), ks[i] * rowf, lv[i]));
+        top = fmaxf(top, __shfl_xor(top, 32, kWave));
+        top = ceilf(fmaxf(top, m));
+        const float scale = exp2_fast(m - top);
+        m = top;
+        l *= scale, x *= scale;
+#pragma unroll
+        for (int n = 0; n < ND; ++n) acc[n] *= scale;
+        (void)weights();
+      }
+      l += dl;
+      if constexpr (kLse) x += dx;
+      sched_fence();
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int n = 0; n < ND; ++n) acc[n] = mfma32(vf[(i * ND + n) * 64], as_h8(w[i]), acc[n]);
+      sched_fence();
+    };
+
+    char* cur = lds;
+    char* nxt = lds + kBuf;
+    if (u.kv_begin < u.kv_end) {
+      load(u.kv_begin, pages);
+      store(u.kv_begin, pages, cur);
+    }
+    __syncthreads();
+    int pos = u.kv_begin;
+    const auto ahead = [&]() {  // the next tile's codes, before this one's products
+      if (pos + kTileKeys < u.kv_end) {
+        const int hi = min((pos + 2 * kTileKeys - 1) >> a.c.b_shift, last);
+        if (hi - pages.first >= kWave) {
+          pages = load_pages(a, u.req, h, (pos + kTileKeys) >> a.c.b_shift, last, lane);
+          bad_seen |= pages.bad;
+        }
+        load(pos + kTileKeys, pages);
+      }
+    };
+    const auto next = [&]() {
+      if (pos + kTileKeys < u.kv_end) store(pos + kTileKeys, pages, nxt);
+      __syncthreads();
+      char* t = cur;
+      cur = nxt, nxt = t;
+      pos += kTileKeys;
+    };
+    // three loops, so that the accumulators stay where they are in each:
+    // tiles that all rows see, tiles with hidden keys (or, from the first block
+    // that is none, all that follow), tiles that only other waves need
+    while (pos < u.kv_end && pos + kTileKeys <= plain && bad_seen == 0) {
+      ahead();
+      tile(std::false_type{}, pos, cur);
+      next();
+    }
+    while (pos < u.kv_end && pos < most) {
+      ahead();
+      tile(std::true_type{}, pos, cur);
+      next();
+    }
+    while (pos < u.kv_end) {
+      ahead();
+      next();
+    }
+    if (bad_seen != 0 && lane == 0) atomicOr(a.status, NSMLP_STATUS_BLOCK_UNAVAILABLE);
+
+    // a lane's results: D / 32 runs of 16 dims, in pieces of 4
+    const auto dim_of = [&](int g) { return (g >> 1) * 64 + (g & 1) * 32 + 16 * half; };
+    const auto piece = [&](int g, int i, float f) {
+      if constexpr (D == 128) return float4_t{acc[0][4 * g + i], acc[1][4 * g + i], acc[2][4 * g + i], acc[3][4 * g + i]} * f;
+      else return float4_t{acc[0][4 * g + i], acc[0][8 + 4 * g + i], acc[1][4 * g + i], acc[1][8 + 4 * g + i]} * f;
+    };
+    l += __shfl_xor(l, 32, kWave), x += __shfl_xor(x, 32, kWave);
+    if (in) {
+      if (u.part >= 0) {
+        const long long at = ((long long)u.part * a.c.heads + h) * kRows + r;
+#pragma unroll
+        for (int g = 0; g < D / 32; ++g)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) *reinterpret_cast<float4_t*>(acc_out + at * D + dim_of(g) + 4 * i) = piece(g, i, 1.0f);
+        if (half == 0) *reinterpret_cast<float4_t*>(ml_out + 4 * at) = float4_t{m, l, x, 0.0f};
+      } else {
+        const long long at = (long long)(q0 + tok) * a.c.heads * a.group + h * a.group + row % a.group;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int g = 0; g < D / 32; ++g) {
+          uint32_t o[8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float4_t p = piece(g, i, inv);
+            o[2 * i] = to_out<kBf16>(p[0]) | (uint32_t)to_out<kBf16>(p[1]) << 16;
+            o[2 * i + 1] = to_out<kBf16>(p[2]) | (uint32_t)to_out<kBf16>(p[3]) << 16;
+          }
+          uint4* dst = reinterpret_cast<uint4*>(a.out + at * D + dim_of(g));
+          dst[0] = uint4{o[0], o[1], o[2], o[3]};
+          dst[1] = uint4{o[4], o[5], o[6], o[7]};
+        }
+        if (kLse && half == 0) a.lse[at] = x == 0.0f ? -INFINITY : (m + log2f(x)) * 0.6931471805599453f;
+      }
+    }
+  }
+}
+
 // ------------------------------------------------------------------ join --
 // One wave per row whose keys were shared out: weights 2^(m_p - max m), in the
 // order of the parts, so that the result does not depend on the schedule of
@@ -399,6 +725,19 @@ __global__ void __launch_bounds__(256) k_attn_join(KvAttnArgs a, const KvSplit* 
   }
 }
 
+template <int D, int kFmt, bool kBf16, int NW, bool kLse>
+void launch_tile(const KvAttnArgs& a, const KvUnit* units, hipStream_t s) {
+  constexpr int kLds = 2 * ((D / 16 * 2 + D / 32 * 4) * 1024 + 64);
+  static std::once_flag once;
+  std::call_once(once, [] {
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k_attn_tile<D, kFmt, kBf16, NW, kLse>),
+                              hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+  });
+  const unsigned grid = (unsigned)min((long long)a.s.max_units_b * a.c.heads, 65536LL);
+  k_attn_tile<D, kFmt, kBf16, NW, kLse><<<dim3(grid), dim3(NW * kWave), kLds, s>>>(a, units, a.sched + 2, a.s.max_units_b,
+                                                                                 a.acc_b, a.ml_b);
+}
+
 template <int D, int kFmt, bool kBf16>
 void attention_typed(const KvAttnArgs& a, hipStream_t s) {
   const KvUnit* ua = reinterpret_cast<const KvUnit*>(a.sched + a.s.off_units_a);
@@ -413,8 +752,8 @@ void attention_typed(const KvAttnArgs& a, hipStream_t s) {
     k_attn_join<D, kBf16><<<join_grid(a.s.max_splits_a, a.s.rows_a), dim3(256), 0, s>>>(a, sa, a.sched + 1, a.s.rows_a,
                                                                                        a.acc_a, a.ml_a);
   if (a.list_b) {
-    k_attn_stream<D, kFmt, kBf16, 1><<<grid(a.s.max_units_b), dim3(kStreamThreads), 0, s>>>(a, ub, a.sched + 2, a.s.max_units_b, a.s.rows_b,
-                                                                                           a.acc_b, a.ml_b);
+    if (a.s.rows_b == 256) a.lse != nullptr ? launch_tile<D, kFmt, kBf16, 8, true>(a, ub, s) : launch_tile<D, kFmt, kBf16, 8, false>(a, ub, s);
+    else a.lse != nullptr ? launch_tile<D, kFmt, kBf16, 4, true>(a, ub, s) : launch_tile<D, kFmt, kBf16, 4, false>(a, ub, s);
     if (a.s.max_splits_b > 0)
       k_attn_join<D, kBf16><<<join_grid(a.s.max_splits_b, a.s.rows_b), dim3(256), 0, s>>>(a, sb, a.sched + 3, a.s.rows_b,
                                                                                          a.acc_b, a.ml_b);

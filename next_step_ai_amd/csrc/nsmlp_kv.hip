@@ -576,13 +576,12 @@ void launch_kv_append(const KvAppendArgs& a, bool bf16, hipStream_t s) { NSMLP_K
 void launch_kv_read(const KvReadArgs& a, bool bf16, hipStream_t s) { NSMLP_KV_BY_TYPE(read_typed, a, bf16, s); }
 
 KvSchedule kv_schedule(int requests, int total, int max_new, int group, int kv_heads) {
-  (void)max_new;
   KvSchedule s;
   s.rows_a = 16;
-  s.rows_b = 16;
+  s.rows_b = (long long)max_new * group > 128 ? 256 : 128;
   const long long tiles_b = ((long long)total * group + s.rows_b - 1) / s.rows_b + requests;
   s.target_a = (1024 + kv_heads - 1) / kv_heads;
-  s.target_b = tiles_b * kv_heads >= 2048 ? 0 : (1024 + kv_heads - 1) / kv_heads;
+  s.target_b = tiles_b * kv_heads >= 512 ? 0 : (512 + kv_heads - 1) / kv_heads;
   s.min_a = 256;
   s.min_b = 512;
   // parts > 1 only where a request's keys exceed a part, so split units are at
