@@ -98,29 +98,34 @@ void launch_kv_read(const KvReadArgs& a, bool bf16, hipStream_t s);
 
 // Work of an attention call, listed by the step's plan.  A unit is up to
 // `rows` query rows of a request (row = token * group + head of the group)
-// against keys [kv_begin, kv_end) of every K/V head; rows whose keys are
-// shared out over several units leave partial results in the workspace
-// (part >= 0), joined afterwards, one KvSplit per such tile of rows.
-// Two lists: short requests (all rows fit one tile of `rows_a`), whose keys
-// are streamed, and the others, in tiles of `rows_b`.
+// against keys [kv_begin, kv_end) of every K/V head.  Two lists:
+//   a  requests whose rows fit one tile of 16: their keys are streamed.  All
+//      these requests' keys, one after the other in pieces of 64, are cut into
+//      equal shares, one per workgroup and K/V head; a unit is what a share
+//      holds of a request.  A request's units meet in the last to end.
+//   b  the others, in tiles of `rows_b` rows, their keys cut into equal parts
+//      where there are few tiles; parts are joined by a second launch, one
+//      KvSplit per tile.
 struct KvUnit {
-  int32_t req, row, kv_begin, kv_end, part, pad[3];
+  int32_t req, row, kv_begin, kv_end;
+  int32_t part, first, parts, split;  // this unit's partial (-1: none), the first of its rows', how many, which split
 };
 struct KvSplit {
   int32_t req, row, first, parts;
 };
 
 constexpr int kKvMaxRequests = 4096;
-constexpr int kKvHeaderInts = 16;  // units_a, splits_a, units_b, splits_b
+constexpr int kKvRowsA = 16;
+constexpr int kKvHeaderInts = 16;  // units a, shares, units b, splits b
 
 struct KvSchedule {  // sizes, from the host's knowledge of a step (kv_schedule)
-  int rows_a, rows_b;                    // rows of a tile of either list
-  int target_a, target_b;                // units wanted per K/V head (0: never split)
-  int min_a, min_b;                      // fewest keys worth a unit of its own
-  int max_units_a, max_units_b;          // list capacities
-  int max_parts_a, max_parts_b;          // partials
-  int max_splits_a, max_splits_b;
-  long long off_units_a, off_units_b, off_splits_a, off_splits_b, ints;  // in ints
+  int rows_b;                        // rows of a tile of list b
+  int shares;                        // of list a's keys, at most
+  int target_b;                      // units wanted per K/V head (0: never split)
+  int max_units_a, max_units_b;      // list capacities
+  int max_parts_a, max_parts_b, max_splits_b;
+  bool list_b;                       // whether a request can be long enough for list b
+  long long off_shares, off_units_a, off_units_b, off_splits_b, ints;  // in ints
 };
 KvSchedule kv_schedule(int requests, int total, int max_new, int group, int kv_heads);
 
@@ -147,8 +152,7 @@ struct KvAttnArgs {
   int max_blocks, R, total, group;
   float scale_log2;  // softmax scale times log2(e)
   float *acc_a, *ml_a, *acc_b, *ml_b;  // partial results of either list: [parts][kv_heads][rows][D], [..][4] (m, l, x)
-  int* status;
-  bool list_b;  // whether a request can be long enough for the second list
+  int *status, *count;                 // status word, arrival counters [parts_a][kv_heads] (zero, left zero)
   KvSchedule s;
 };
 // floats of the partial results, and where acc_a, ml_a, acc_b, ml_b start

@@ -63,14 +63,20 @@ __device__ __forceinline__ void block_scan(int (&v)[N], int (&total)[N], int (*w
 __device__ __forceinline__ int clip_len(int v) { return min(max(v, 0), 1 << 29); }
 
 // keys per part, so that about `target` units share the list's `work` keys
-__device__ __forceinline__ int part_keys(long long work, int target, int least) {
+__device__ __forceinline__ int part_keys(long long work, int target) {
   if (target <= 0) return 1 << 30;  // more than any request's
   const double each = ceil((double)work / target);  // exact: below 2^53, and a quotient's ceiling does not round down
   const double up = ceil(each * (1.0 / 128)) * 128;
-  return up < least ? least : up > (double)(1 << 30) ? 1 << 30 : (int)up;
+  return up < 512 ? 512 : up > (double)(1 << 30) ? 1 << 30 : (int)up;
 }
 
-constexpr int kPlanSums = 7;
+// list a counts keys in pieces of 64; a request without any takes one piece,
+// so that its rows are somebody's
+constexpr int kLeastShare = 4;  // pieces: 256 keys are worth a workgroup
+
+__device__ __forceinline__ int pieces_of(int keys) { return max(1, (keys + 63) >> 6); }
+
+constexpr int kPlanSums = 6;
 
 template <int kThreads, int kPer>
 __global__ void __launch_bounds__(kThreads) k_kv_plan(KvPlanArgs a) {
@@ -79,7 +85,7 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(KvPlanArgs a) {
   int* q_start = lds;             // [R + 1]
   int* base = q_start + a.R + 1;  // [R] blocks granted before the request; -1: refused
   int* first = base + a.R;        // [R] first unit of its list
-  int* split = first + a.R;       // [R] first split tile of its list
+  int* split = first + a.R;       // [R] list b: first split tile; list a: pieces before the request
   int* partial = split + a.R;     // [R] first partial
   int* len_s = partial + a.R;     // [R] cached tokens
   kernarg_warm<sizeof(KvPlanArgs)>();
@@ -106,12 +112,12 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(KvPlanArgs a) {
     sum[1] += max(need[i], 0);
   }
   block_scan<2, kThreads>(sum, total, wsum, tid);
-  // granted requests, and the work (tiles of rows times keys) of either list,
-  // summed exactly in three pieces of 20 bits (1024 of them stay in 30)
-  int at = sum[0], used = sum[1], kv[kPer], tiles[kPer];  // tiles < 0: list a
-  long long work[2] = {0, 0};
-  int cnt[kPlanSums] = {};  // units a, units b, split tiles a, b, partials a, b, blocks granted
-  int refused = 0;
+  // granted requests; list a's pieces, and list b's work (tiles of rows times
+  // keys) in three summands of 20 bits (1024 of them stay in 30)
+  int at = sum[0], used = sum[1], kv[kPer], tiles[kPer];  // tiles -1: list a
+  long long work = 0;
+  int cnt[kPlanSums] = {};  // units a, units b, splits b, partials a, partials b, blocks granted
+  int sums[5] = {}, sums_total[5];  // pieces of list a, work of list b, refused
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int r = r0 + i;
@@ -129,37 +135,39 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(KvPlanArgs a) {
         a.next[r] = ok ? cached[i] + fresh[i] : cached[i];
       }
     }
-    refused += in && !ok && fresh[i] > 0;
-    cnt[6] += in && ok ? n : 0;
+    sums[4] += in && !ok && fresh[i] > 0;
+    cnt[5] += in && ok ? n : 0;
     used += n;
     at += fresh[i];
     const int rows = min(fresh[i], a.row_limit) * a.group;
-    const bool b = rows > a.s.rows_a;
+    const bool b = rows > kKvRowsA;
     tiles[i] = b ? (rows + a.s.rows_b - 1) / a.s.rows_b : rows > 0 ? -1 : 0;
-    work[b ? 1 : 0] += (long long)kv[i] * abs(tiles[i]);
+    if (b) work += (long long)kv[i] * tiles[i];
+    else if (rows > 0) sums[0] += pieces_of(kv[i]);
   }
-  long long all[2];
-  {
-    int piece[kPlanSums] = {(int)(work[0] & 0xFFFFF), (int)((work[0] >> 20) & 0xFFFFF), (int)(work[0] >> 40),
-                            (int)(work[1] & 0xFFFFF), (int)((work[1] >> 20) & 0xFFFFF), (int)(work[1] >> 40), refused};
-    int sums[kPlanSums];
-    block_scan<kPlanSums, kThreads>(piece, sums, wsum, tid);
-    all[0] = sums[0] + ((long long)sums[1] << 20) + ((long long)sums[2] << 40);
-    all[1] = sums[3] + ((long long)sums[4] << 20) + ((long long)sums[5] << 40);
-    refused = sums[6];
-  }
-  const int keys_a = part_keys(all[0], a.s.target_a, a.s.min_a), keys_b = part_keys(all[1], a.s.target_b, a.s.min_b);
-  // units of each request: tiles of rows times parts of its keys
-  int parts[kPer];
+  sums[1] = (int)(work & 0xFFFFF), sums[2] = (int)((work >> 20) & 0xFFFFF), sums[3] = (int)(work >> 40);
+  block_scan<5, kThreads>(sums, sums_total, wsum, tid);
+  work = sums_total[1] + ((long long)sums_total[2] << 20) + ((long long)sums_total[3] << 40);
+  const int refused = sums_total[4];
+  const int share = max(kLeastShare, (sums_total[0] + a.s.shares - 1) / a.s.shares);  // pieces
+  const int keys_b = part_keys(work, a.s.target_b);
+  // units of each request: the shares that its pieces touch, or tiles of rows times parts of its keys
+  int parts[kPer], piece0[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const bool b = tiles[i] > 0;
-    const int n = abs(tiles[i]), keys = b ? keys_b : keys_a;
-    parts[i] = max(1, (int)(((unsigned)kv[i] + (unsigned)keys - 1) / (unsigned)keys));
-    const int u = n * parts[i], s = parts[i] > 1 ? n : 0, p = parts[i] > 1 ? u : 0;
-    cnt[0] += b ? 0 : u, cnt[1] += b ? u : 0;
-    cnt[2] += b ? 0 : s, cnt[3] += b ? s : 0;
-    cnt[4] += b ? 0 : p, cnt[5] += b ? p : 0;
+    piece0[i] = sums[0];
+    if (tiles[i] < 0) {
+      const int end = sums[0] + pieces_of(kv[i]);
+      parts[i] = (int)((unsigned)(end - 1) / (unsigned)share - (unsigned)sums[0] / (unsigned)share) + 1;
+      sums[0] = end;
+      cnt[0] += parts[i];
+      cnt[3] += parts[i] > 1 ? parts[i] : 0;
+    } else {
+      parts[i] = max(1, (int)(((unsigned)kv[i] + (unsigned)keys_b - 1) / (unsigned)keys_b));
+      cnt[1] += tiles[i] * parts[i];
+      cnt[2] += parts[i] > 1 ? tiles[i] : 0;
+      cnt[4] += parts[i] > 1 ? tiles[i] * parts[i] : 0;
+    }
   }
   int cnt_total[kPlanSums];
   block_scan<kPlanSums, kThreads>(cnt, cnt_total, wsum, tid);
@@ -167,23 +175,27 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(KvPlanArgs a) {
   for (int i = 0; i < kPer; ++i) {
     const int r = r0 + i;
     if (i >= per || r >= a.R) continue;
-    const bool b = tiles[i] > 0;
-    const int n = abs(tiles[i]), u = n * parts[i];
-    first[r] = b ? cnt[1] : cnt[0], split[r] = b ? cnt[3] : cnt[2], partial[r] = b ? cnt[5] : cnt[4];
-    cnt[b ? 1 : 0] += u;
-    if (parts[i] > 1) cnt[b ? 3 : 2] += n, cnt[b ? 5 : 4] += u;
+    if (tiles[i] < 0) {
+      first[r] = cnt[0], split[r] = piece0[i], partial[r] = cnt[3];
+      cnt[0] += parts[i];
+      if (parts[i] > 1) cnt[3] += parts[i];
+    } else {
+      first[r] = cnt[1], split[r] = cnt[2], partial[r] = cnt[4];
+      cnt[1] += tiles[i] * parts[i];
+      if (parts[i] > 1) cnt[2] += tiles[i], cnt[4] += tiles[i] * parts[i];
+    }
   }
   if (tid == 0) q_start[a.R] = total[0];
   if (blockIdx.x == 0 && tid == 0) {
     a.q_start[a.R] = total[0];
-    a.info[0] = (int)(((unsigned)head + (unsigned)cnt_total[6]) % N);
-    a.info[1] = count - cnt_total[6];
+    a.info[0] = (int)(((unsigned)head + (unsigned)cnt_total[5]) % N);
+    a.info[1] = count - cnt_total[5];
     a.info[2] = refused;
     a.info[3] = total[0];
     a.sched[0] = min(cnt_total[0], a.s.max_units_a);
-    a.sched[1] = min(cnt_total[2], a.s.max_splits_a);
+    a.sched[1] = min((sums_total[0] + share - 1) / share, a.s.shares);
     a.sched[2] = min(cnt_total[1], a.s.max_units_b);
-    a.sched[3] = min(cnt_total[3], a.s.max_splits_b);
+    a.sched[3] = min(cnt_total[2], a.s.max_splits_b);
   }
   __syncthreads();
   // slots: one thread per token; a block's first token also writes its entry
@@ -211,41 +223,54 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(KvPlanArgs a) {
     a.slots[t] = slot;
   }
   // work lists: one wave per request
+  int32_t* shares = a.sched + a.s.off_shares;
   KvUnit* units_a = reinterpret_cast<KvUnit*>(a.sched + a.s.off_units_a);
   KvUnit* units_b = reinterpret_cast<KvUnit*>(a.sched + a.s.off_units_b);
-  KvSplit* splits_a = reinterpret_cast<KvSplit*>(a.sched + a.s.off_splits_a);
   KvSplit* splits_b = reinterpret_cast<KvSplit*>(a.sched + a.s.off_splits_b);
-  auto write = [&](int r, int i, int q, int len, bool b, int tiles_r, int parts_r) {
-    const int per_tile = b ? a.s.rows_b : a.s.rows_a;
-    const int max_units = b ? a.s.max_units_b : a.s.max_units_a, max_splits = b ? a.s.max_splits_b : a.s.max_splits_a,
-              max_parts = b ? a.s.max_parts_b : a.s.max_parts_a;
-    // the last tile sees the most keys: it goes first
-    const int nth = parts_r == 1 ? i : (int)((unsigned)i / (unsigned)parts_r), part = i - nth * parts_r;
-    const int tile = tiles_r - 1 - nth;
-    const int last = min(q, (int)(((unsigned)(tile + 1) * (unsigned)per_tile + a.group - 1) / (unsigned)a.group));
-    const int keys_seen = max(0, len - q + last);  // of the tile's last row
-    const int each = parts_r == 1 ? keys_seen : ((int)((unsigned)(keys_seen + parts_r - 1) / (unsigned)parts_r) + 63) & ~63;
-    KvUnit u;
-    u.req = r;
-    u.row = tile * per_tile;
-    u.kv_begin = min(part * each, keys_seen);
-    u.kv_end = min((part + 1) * each, keys_seen);
-    u.part = parts_r > 1 ? partial[r] + i : -1;
-    u.pad[0] = u.pad[1] = u.pad[2] = 0;
-    if (first[r] + i < max_units && u.part < max_parts) (b ? units_b : units_a)[first[r] + i] = u;
-    if (parts_r > 1 && part == 0 && split[r] + nth < max_splits)
-      (b ? splits_b : splits_a)[split[r] + nth] = KvSplit{r, u.row, u.part, parts_r};
-  };
   constexpr int kWaves = kThreads / kWave;
   for (int r = (int)blockIdx.x * kWaves + wave; r < a.R; r += (int)gridDim.x * kWaves) {
     const int q = q_start[r + 1] - q_start[r];
     if (q == 0) continue;
     const int len = base[r] >= 0 ? len_s[r] + q : 0;
     const int rows = min(q, a.row_limit) * a.group;
-    const bool b = rows > a.s.rows_a;
-    const int n = b ? (rows + a.s.rows_b - 1) / a.s.rows_b : 1, keys = b ? keys_b : keys_a;
-    const int parts_r = max(1, (int)(((unsigned)len + (unsigned)keys - 1) / (unsigned)keys));
-    for (int i = lane; i < n * parts_r; i += kWave) write(r, i, q, len, b, n, parts_r);
+    KvUnit u;
+    u.req = r;
+    if (rows <= kKvRowsA) {
+      const int p0 = split[r], p1 = p0 + pieces_of(len), s0 = (int)((unsigned)p0 / (unsigned)share);
+      const int n = (int)((unsigned)(p1 - 1) / (unsigned)share) - s0 + 1;
+      for (int i = lane; i < n; i += kWave) {
+        const int begin = max(p0, (s0 + i) * share), end = min(p1, (s0 + i + 1) * share), at = first[r] + i;
+        u.row = 0;
+        u.kv_begin = min((begin - p0) * 64, len);
+        u.kv_end = min((end - p0) * 64, len);
+        u.part = n > 1 ? partial[r] + i : -1;
+        u.first = partial[r];
+        u.parts = n;
+        u.split = partial[r];
+        if (at < a.s.max_units_a && u.part < a.s.max_parts_a) units_a[at] = u;
+        // every share starts with a unit of its own
+        if (begin == (s0 + i) * share && s0 + i < a.s.shares) shares[s0 + i] = at;
+      }
+    } else {
+      const int tiles_r = (rows + a.s.rows_b - 1) / a.s.rows_b;
+      const int n = max(1, (int)(((unsigned)len + (unsigned)keys_b - 1) / (unsigned)keys_b));
+      for (int i = lane; i < tiles_r * n; i += kWave) {
+        // the last tile sees the most keys: it goes first
+        const int nth = n == 1 ? i : (int)((unsigned)i / (unsigned)n), p = i - nth * n, tile = tiles_r - 1 - nth;
+        const int last = min(q, (int)(((unsigned)(tile + 1) * (unsigned)a.s.rows_b + a.group - 1) / (unsigned)a.group));
+        const int seen = max(0, len - q + last);  // keys that the tile's last row sees
+        const int each = n == 1 ? seen : ((int)((unsigned)(seen + n - 1) / (unsigned)n) + 63) & ~63;
+        u.row = tile * a.s.rows_b;
+        u.kv_begin = min(p * each, seen);
+        u.kv_end = min((p + 1) * each, seen);
+        u.part = n > 1 ? partial[r] + i : -1;
+        u.first = partial[r] + nth * n;
+        u.parts = n;
+        u.split = split[r] + nth;
+        if (first[r] + i < a.s.max_units_b && u.part < a.s.max_parts_b) units_b[first[r] + i] = u;
+        if (n > 1 && p == 0 && u.split < a.s.max_splits_b) splits_b[u.split] = KvSplit{r, u.row, u.first, n};
+      }
+    }
   }
 }
 
@@ -577,24 +602,27 @@ void launch_kv_read(const KvReadArgs& a, bool bf16, hipStream_t s) { NSMLP_KV_BY
 
 KvSchedule kv_schedule(int requests, int total, int max_new, int group, int kv_heads) {
   KvSchedule s;
-  s.rows_a = 16;
+  s.list_b = (long long)(max_new < total ? max_new : total) * group > kKvRowsA;
   s.rows_b = (long long)max_new * group > 128 ? 256 : 128;
-  const long long tiles_b = ((long long)total * group + s.rows_b - 1) / s.rows_b + requests;
-  s.target_a = (1024 + kv_heads - 1) / kv_heads;
-  s.target_b = tiles_b * kv_heads >= 512 ? 0 : (512 + kv_heads - 1) / kv_heads;
-  s.min_a = 256;
-  s.min_b = 512;
-  // parts > 1 only where a request's keys exceed a part, so split units are at
-  // most twice the work over the keys of a part, and split tiles at most it
-  s.max_parts_a = 2 * s.target_a, s.max_parts_b = 2 * s.target_b;
-  s.max_splits_a = s.target_a, s.max_splits_b = s.target_b;
-  s.max_units_a = requests + s.max_parts_a;
+  // list a: two workgroups of 4 waves on every CU, or one of 8 beside list b's
+  s.shares = ((s.list_b ? 256 : 512) + kv_heads - 1) / kv_heads;
+  const long long tiles_b = s.list_b ? ((long long)total * group + s.rows_b - 1) / s.rows_b + requests : 0;
+  s.target_b = !s.list_b || tiles_b * kv_heads >= 512 ? 0 : (512 + kv_heads - 1) / kv_heads;
+  // list a: every share ends at most one unit that its request does not end,
+  // so units are at most requests + shares, and those of a request with several
+  // units at most twice the shares
+  s.max_units_a = requests + s.shares;
+  s.max_parts_a = 2 * s.shares;
+  // list b: parts > 1 only where a request's keys exceed a part, so split units
+  // are at most twice the work over the keys of a part, and split tiles at most it
+  s.max_parts_b = 2 * s.target_b;
+  s.max_splits_b = s.target_b;
   s.max_units_b = (int)tiles_b + s.max_parts_b;
   const long long unit = sizeof(KvUnit) / 4, split = sizeof(KvSplit) / 4;
-  s.off_units_a = kKvHeaderInts;
+  s.off_shares = kKvHeaderInts;
+  s.off_units_a = s.off_shares + (s.shares + 3) / 4 * 4;
   s.off_units_b = s.off_units_a + unit * s.max_units_a;
-  s.off_splits_a = s.off_units_b + unit * s.max_units_b;
-  s.off_splits_b = s.off_splits_a + split * s.max_splits_a;
+  s.off_splits_b = s.off_units_b + unit * s.max_units_b;
   s.ints = s.off_splits_b + split * s.max_splits_b;
   return s;
 }

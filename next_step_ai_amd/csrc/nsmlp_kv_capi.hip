@@ -83,6 +83,8 @@ int batch_schedule(const nsmlp_kv_batch* b, int total, int max_new, KvSchedule& 
   if (max_new < 0) return set_error(NSMLP_EINVAL, "max_new %d must not be negative", max_new);
   const int group = group_of(b);
   if ((long long)total * group > (1LL << 28)) return set_error(NSMLP_EINVAL, "%d tokens of %d heads: too many rows", total, group);
+  if ((long long)b->requests * b->max_blocks > (1LL << 30))
+    return set_error(NSMLP_EINVAL, "%d requests of %d blocks: at most 2^30 table entries", b->requests, b->max_blocks);
   s = kv_schedule(b->requests, total, max_new == 0 ? total : max_new, group, b->kv_heads);
   return NSMLP_OK;
 }
@@ -240,6 +242,7 @@ int nsmlp_paged_attention(const nsmlp_kv_cache* cache, const nsmlp_kv_batch* bat
   float* part = (float*)((char*)ws + align_up(kCounterBytes));
   a.acc_a = part + off[0], a.ml_a = part + off[1], a.acc_b = part + off[2], a.ml_b = part + off[3];
   a.status = (int*)((char*)ws + kStatusOff);
+  a.count = (int*)((char*)ws + kBlkCountOff);
   a.q = (const uint16_t*)q;
   a.q_row = q_row_stride, a.q_head = q_head_stride;
   a.out = (uint16_t*)out;
@@ -253,9 +256,6 @@ int nsmlp_paged_attention(const nsmlp_kv_cache* cache, const nsmlp_kv_batch* bat
   a.total = step->total;
   a.group = group_of(batch);
   a.scale_log2 = (float)((double)scale * 1.4426950408889634);
-  // requests of few rows are on one list, the others on the second: empty where no request can be that long
-  const int longest = step->max_new == 0 || step->max_new > step->total ? step->total : step->max_new;
-  a.list_b = (long long)longest * a.group > a.s.rows_a;
   launch_kv_attention(a, dtype == NSMLP_DTYPE_BF16, (hipStream_t)stream);
   return check_launch("nsmlp_paged_attention");
 }
