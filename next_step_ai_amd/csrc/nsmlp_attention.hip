@@ -28,6 +28,8 @@ constexpr float kLowest = -3.402823466e38f;
 // inside fp16: none is above 2^12.
 constexpr float kSumLimit = 4096.0f;
 
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float log2_fast(float x) { return __builtin_amdgcn_logf(x); }
 
@@ -64,7 +66,7 @@ __device__ __forceinline__ uint4 bf16_to_f16(const uint4& raw, int e) {
 
 // Pages of a range of keys, held one per lane: 64 pages from page `first`.
 struct Pages {
-  int id;          // block id (0 where the entry is not a block)
+  uint32_t lo, hi;   // where the (block, head)'s codes start (block 0's where the entry is not a block)
   float ks, lv, iv;  // K scale, log2 and reciprocal of the V scale
   unsigned long long bad;
   int first;
@@ -76,8 +78,10 @@ __device__ __forceinline__ Pages load_pages(const KvAttnArgs& a, int req, int h,
   const int pg = min(min(first + lane, last), a.max_blocks - 1);
   const int id = a.table[(long long)req * a.max_blocks + pg];
   const bool ok = id >= 0 && id < a.c.num_blocks;
-  p.id = ok ? id : 0;
-  const float2 s = *reinterpret_cast<const float2*>(a.c.scale + ((long long)p.id * a.c.heads + h) * 2);
+  const long long bh = (long long)(ok ? id : 0) * a.c.heads + h;
+  const long long off = bh * (2 * a.c.B * a.c.D);
+  p.lo = (uint32_t)off, p.hi = (uint32_t)(off >> 32);
+  const float2 s = *reinterpret_cast<const float2*>(a.c.scale + bh * 2);
   const float sv = s.y == 0.0f ? kKvScaleMin : s.y;  // a block that nothing was stored in
   p.bad = __ballot(!ok);
   p.ks = s.x;
@@ -86,8 +90,21 @@ __device__ __forceinline__ Pages load_pages(const KvAttnArgs& a, int req, int h,
   return p;
 }
 
+__device__ __forceinline__ const uint8_t* page_data(const KvAttnArgs& a, const Pages& p, int i) {
+  return a.c.data + ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)p.lo, i) |
+                     (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)p.hi, i) << 32);
+}
+
 __device__ __forceinline__ float lane_of(float v, int i) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i));
+}
+
+// A unit in scalar registers (left in memory it would be read again after
+// every barrier).
+__device__ __forceinline__ KvUnit load_unit(const KvUnit* p) {
+  const KvUnit v = *p;
+  return KvUnit{uniform(v.req),  uniform(v.row),   uniform(v.kv_begin), uniform(v.kv_end),
+                uniform(v.part), uniform(v.first), uniform(v.parts),    uniform(v.split)};
 }
 
 // ---------------------------------------------------------------- stream --
@@ -119,12 +136,12 @@ __device__ __forceinline__ float2 ld_coherent2(const float* p) {
 }
 
 template <int D, int kFmt, bool kBf16, int NW>
-__device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit& u, int h, StreamLds<D, NW>& lds) {
+__device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u, int h, StreamLds<D, NW>& lds) {
   constexpr int NJ = D / 64, KS = D / 32, ND = D / 16;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
   const bool want_lse = a.lse != nullptr;
-  const int q0 = a.q_start[u.req], q_len = a.q_start[u.req + 1] - q0, kv_len = a.kv_len[u.req];
+  const int q0 = uniform(a.q_start[u.req]), q_len = uniform(a.q_start[u.req + 1]) - q0, kv_len = uniform(a.kv_len[u.req]);
   const int rows = min(q_len * a.group, kKvRowsA);
 
   // this wave's keys
@@ -140,10 +157,9 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit& u
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int at = pos + 16 * s, pg = min(at >> a.c.b_shift, last) - pages.first;
-      const int id = __builtin_amdgcn_readlane(pages.id, pg);
       t.ks[s] = lane_of(pages.ks, pg), t.lv[s] = lane_of(pages.lv, pg), t.iv[s] = lane_of(pages.iv, pg);
       t.bad |= ((int)(pages.bad >> pg) & 1) << s;
-      const uint8_t* kb = a.c.data + ((long long)id * a.c.heads + h) * 2 * (a.c.B * D) + ((at & (a.c.B - 1)) >> 4) * (16 * D);
+      const uint8_t* kb = page_data(a, pages, pg) + ((at & (a.c.B - 1)) >> 4) * (16 * D);
       const uint8_t* vb = kb + a.c.B * D;
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
@@ -415,7 +431,7 @@ __device__ __forceinline__ void stream_share(const KvAttnArgs& a, int block, Str
   const int end = share + 1 < shares ? min(start[share + 1], units) : units;
   const KvUnit* list = reinterpret_cast<const KvUnit*>(a.sched + a.s.off_units_a);
   for (int i = start[share]; i < end; ++i) {
-    stream_unit<D, kFmt, kBf16, NW>(a, list[i], h, lds);
+    stream_unit<D, kFmt, kBf16, NW>(a, load_unit(list + i), h, lds);
     __syncthreads();
   }
 }
@@ -430,77 +446,168 @@ __global__ void __launch_bounds__(4 * kWave) k_attn_stream(KvAttnArgs a) {
 // ----------------------------------------------------------------- tiles --
 // Prompts and chunks: NW waves of 32 query rows each against tiles of 64 keys
 // that the workgroup decodes to fp16 once, in LDS, as the operands of
-// v_mfma_f32_32x32x16_f16 (A rows: keys or dims, B columns: queries):
-//   K fragment (32 keys, 16 dims): lane l: key l % 32, dims 16 (2 a + l / 32) + 8 u + 0..7
+// v_mfma_f32_32x32x16_f16 (A rows: keys or dims, B columns: queries).  Codes
+// are taken 16 bytes at a time from two places, a dword of each makes a lane's
+// 8 operands, of K and of V alike:
+//   K fragment (32 keys, 16 dims): lane l: key l % 32, dims 16 g + 4 i + 0..3 and D / 2 + the same
 //   V fragment (32 dims, 16 keys): lane l: keys 4 h + 0..3 and 8 + 4 h + 0..3, h = l / 32
-// so that the scores of a query stay in its two lanes, in the order in which
-// the second product wants the weights.
+// The scores of a query stay in its two lanes, in the order in which the
+// second product wants the weights.
 //
-// A tile's weights are taken under the reference as it stands; their sums, kept
-// anyway, tell whether one was too large for it (the first tile, and seldom
-// after), and only then is the maximum looked for.  References are integers,
-// so that rescaling is exact.
+// Weights are taken under the reference as it stands; their sums, kept anyway,
+// tell whether one was too large for it (the first tile, and seldom after), and
+// only then is the maximum looked for.  References are integers, so that
+// rescaling is exact.
 constexpr int kTileKeys = 64;
 
-__device__ __forceinline__ float max16(const float16_t& s, int at) {
+__device__ __forceinline__ float max8(const float16_t& s, int at) {
   return fmaxf(fmaxf(fmaxf(s[at], s[at + 1]), fmaxf(s[at + 2], s[at + 3])),
                fmaxf(fmaxf(s[at + 4], s[at + 5]), fmaxf(s[at + 6], s[at + 7])));
 }
 
-// What the products of a tile need to know of its blocks, per 16 keys.
-struct TileMeta {
-  float4_t ks, lv, iv;
-  int bad[4];
-};
+// What the weights of 16 keys need to know of their block: K scale, log2 and
+// reciprocal of the V scale, and (as bits) whether it is no block.
+typedef float4_t TileMeta;
 
-template <int D, int NW>
-constexpr int kTileLds = 2 * ((D / 16 * 2 + D / 32 * 4) * 1024 + 64);
+template <int D>
+constexpr int kTileBytes = (D / 16 * 2 + D / 32 * 4) * 1024;  // fragments of a tile, 1 KB each
+template <int D>
+constexpr int kTileLds = 2 * kTileBytes<D> + 4 * 4 * (int)sizeof(TileMeta);
 
 template <int D, int kFmt, bool kBf16, int NW, bool kLse>
-__device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit& u, int h, char* lds) {
-  constexpr int KS = D / 16, ND = D / 32, NJ = D / 64, kRows = 32 * NW;
-  constexpr int kKBytes = 2 * KS * 1024, kVBytes = 4 * ND * 1024;  // fragments of a tile: 1 KB each
-  constexpr int kBuf = kKBytes + kVBytes + 64;  // [2][K fragments, V fragments, TileMeta]
+__device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, int h, char* lds) {
+  constexpr int KS = D / 16, ND = D / 32, kRows = 32 * NW;
+  constexpr int kKBytes = 2 * KS * 1024, kVBytes = 4 * ND * 1024;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
-  // the 16 keys of a tile that this wave decodes: K, V or (4 waves) both
-  const int part = wave & 3;
-  const bool does_k = NW == 4 || wave < 4, does_v = NW == 4 || wave >= 4;
-  const int q0 = a.q_start[u.req], q_len = a.q_start[u.req + 1] - q0, kv_len = a.kv_len[u.req];
+  TileMeta* const metas = reinterpret_cast<TileMeta*>(lds + 2 * kTileBytes<D>);
+  const int q0 = uniform(a.q_start[u.req]), q_len = uniform(a.q_start[u.req + 1]) - q0, kv_len = uniform(a.kv_len[u.req]);
   const int rows = min(q_len * a.group - u.row, kRows);
   const int r = wave * 32 + col, row = u.row + r, tok = row / a.group;
   const bool in = r < rows && q0 + tok < a.total;
   const int limit = in ? kv_len - q_len + tok + 1 : 0x7FFFFFFF;  // keys that the row sees
+  const int last = max(0, (u.kv_end - 1) >> a.c.b_shift);
+  const int tiles = (u.kv_end - u.kv_begin + kTileKeys - 1) / kTileKeys;
+
+  // The 16 keys of a tile that this wave decodes: with 8 waves K (lower four)
+  // or V, with 4 both.  Where its lane reads in a (block, head)'s 16 keys, and
+  // where it writes.
+  constexpr int kRoles = NW == 8 ? 1 : 2;
+  const int part = wave & 3;
+  const bool upper = NW == 8 && wave >= 4;
+  uint32_t src[kRoles], src2[kRoles];
+  int dst[kRoles], dst_step[kRoles];
+#pragma unroll
+  for (int o = 0; o < kRoles; ++o) {
+    const bool v = kRoles == 2 ? o == 1 : upper;
+    if constexpr (D == 128) {
+      const int g = lane >> 4, t = lane & 15;
+      src[o] = v ? a.c.B * D + (g & 1) * 1024 + half * 256 + t * 16 : lane * 16;
+      src2[o] = src[o] + (v ? 512 : 1024);
+      dst[o] = v ? kKBytes + (part * ND * 64 + lane) * 16
+                 : ((((part >> 1) * KS + (g >> 1)) * 64) + (g & 1) * 32 + (part & 1) * 16 + t) * 16;
+      dst_step[o] = v ? 1024 : 2048;
+    } else {  // (the upper lanes repeat the lower ones)
+      const int g = (lane >> 4) & 1, t = lane & 15;
+      src[o] = (v ? a.c.B * D : 0) + g * 256 + t * 16;
+      src2[o] = src[o] + 512;
+      dst[o] = v ? kKBytes + (part * ND * 64 + g * 32 + t) * 16 : (((part >> 1) * KS * 64) + g * 32 + (part & 1) * 16 + t) * 16;
+      dst_step[o] = 1024;
+    }
+  }
+  unsigned long long bad_seen = 0;
+  Pages pages = load_pages(a, u.req, h, u.kv_begin >> a.c.b_shift, last, lane);
+  if (tiles > 0) bad_seen = pages.bad;
+  // this wave's page in tile i, as a lane of `pages`; past the last tile again the last
+  const auto at_of = [&](int i) { return u.kv_begin + min(i, tiles - 1) * kTileKeys + 16 * part; };
+  const auto page_of = [&](int i) { return min(at_of(i) >> a.c.b_shift, last) - pages.first; };
+  uint4 raw[kRoles][2];
+  const auto fetch = [&](int o, int i) {
+    const int at = at_of(i);
+    const uint8_t* base = page_data(a, pages, page_of(i)) + ((at & (a.c.B - 1)) >> 4) * (16 * D);
+    raw[o][0] = *reinterpret_cast<const uint4*>(base + src[o]);
+    raw[o][1] = *reinterpret_cast<const uint4*>(base + src2[o]);
+  };
+  // one of the 8 dwords at a time: decoded (half 0, 1 of piece j), and written with its pair
+  uint2 lo_piece;
+  const auto decode = [&](int o, int i, char* buf, int step) {
+    const int j = step >> 1;
+    uint32_t w = word(raw[o][step & 1], j);
+    if (kFmt == NSMLP_KV_E4M3 && (kRoles == 2 ? o == 1 : true)) {
+      // V codes past the end may be NaNs: a zero weight does not hide them
+      // (with 8 waves the lower four, which have K, keep all)
+      const int left = kv_len - (at_of(i) + 8 * (step & 1) + 4 * (D == 128 ? half : (lane >> 4) & 1));
+      const bool bad = (pages.bad >> page_of(i)) & 1;
+      const uint32_t mask = bad || left <= 0 ? 0u : left >= 4 ? ~0u : (1u << (8 * left)) - 1u;
+      w &= kRoles == 2 || upper ? mask : ~0u;
+    }
+    const uint2 v = kv_half4<kFmt>(w);
+    if (!(step & 1)) {
+      lo_piece = v;
+    } else {
+      int to = dst[o] + j * dst_step[o];
+      if constexpr (D == 64) {
+        // V: dims 4 t + j are rows t + 16 (j % 2) of fragment j / 2
+        if (kRoles == 2 ? o == 1 : upper) to = dst[o] + (j >> 1) * 1024 + (j & 1) * 256;
+      }
+      *reinterpret_cast<uint4*>(buf + to) = uint4{lo_piece.x, lo_piece.y, v.x, v.y};
+    }
+  };
+  const auto store_meta = [&](int i) {  // (every lane the same, and both waves of a part)
+    const int pg = page_of(i);
+    metas[(i & 3) * 4 + part] = TileMeta{lane_of(pages.ks, pg), lane_of(pages.lv, pg), lane_of(pages.iv, pg),
+                                         __int_as_float((int)((pages.bad >> pg) & 1))};
+  };
+  // the window of pages moves before the first tile that is not all in it is
+  // fetched, and keeps tiles from `from` on
+  const auto window_end = [&]() {  // that tile
+    const int keys = ((pages.first + kWave) << a.c.b_shift) - u.kv_begin;
+    return pages.first + kWave > last ? 0x7FFFFFFF : keys / kTileKeys;
+  };
+  int turn_at = window_end();
+  const auto turn_pages = [&](int from, int need) {
+    if (__builtin_expect_with_probability(need >= turn_at, 0, 0.95)) {
+      pages = load_pages(a, u.req, h, (u.kv_begin + min(from, tiles - 1) * kTileKeys) >> a.c.b_shift, last, lane);
+      bad_seen |= pages.bad;
+      turn_at = window_end();
+    }
+  };
+  if (tiles > 0) {
+#pragma unroll
+    for (int o = 0; o < kRoles; ++o) fetch(o, 0);
+  }
 
   half8_t q[KS];
   float rowf = a.scale_log2;
   {
-    const uint16_t* src = a.q + (long long)(q0 + tok) * a.q_row + (long long)(h * a.group + row % a.group) * a.q_head;
-    uint4 raw[KS];
+    const uint16_t* from = a.q + (long long)(q0 + tok) * a.q_row + (long long)(h * a.group + row % a.group) * a.q_head;
+    uint4 part_q[KS];
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
-      raw[s] = in ? *reinterpret_cast<const uint4*>(src + 16 * ((s & ~1) + half) + 8 * (s & 1)) : uint4{0, 0, 0, 0};
+    for (int s = 0; s < KS; ++s) {
+      // dims of K fragment s in this half of the wave
+      const int d = D == 128 ? 16 * (2 * (s & 1) + half) + 4 * (s >> 1) : 16 * half + 4 * s;
+      uint2 lo = {0, 0}, hi = {0, 0};
+      if (in) lo = *reinterpret_cast<const uint2*>(from + d), hi = *reinterpret_cast<const uint2*>(from + d + D / 2);
+      part_q[s] = uint4{lo.x, lo.y, hi.x, hi.y};
+    }
     if constexpr (kBf16) {
       uint32_t top = 0;
 #pragma unroll
       for (int s = 0; s < KS; ++s)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) top = max(top, max(word(raw[s], i) & 0x7FFFu, (word(raw[s], i) >> 16) & 0x7FFFu));
+        for (int i = 0; i < 4; ++i) top = max(top, max(word(part_q[s], i) & 0x7FFFu, (word(part_q[s], i) >> 16) & 0x7FFFu));
       top = max(top, (uint32_t)__shfl_xor((int)top, 32, kWave));
       const int e = row_exponent(top);
       rowf *= ldexpf(1.0f, e);
 #pragma unroll
-      for (int s = 0; s < KS; ++s) q[s] = as_h8(bf16_to_f16(raw[s], e));
+      for (int s = 0; s < KS; ++s) q[s] = as_h8(bf16_to_f16(part_q[s], e));
     } else {
 #pragma unroll
-      for (int s = 0; s < KS; ++s) q[s] = as_h8(raw[s]);
+      for (int s = 0; s < KS; ++s) q[s] = as_h8(part_q[s]);
     }
   }
-  // keys below `plain` need no mask in this wave, keys from `most` on do not matter to it
-  const int first_row = u.row + min(wave * 32, rows), end_row = u.row + min((wave + 1) * 32, rows);
-  const int plain = kv_len - q_len + first_row / a.group + 1;
-  const int most = end_row > first_row ? kv_len - q_len + (end_row - 1) / a.group + 1 : 0;
-  const int last = max(0, (u.kv_end - 1) >> a.c.b_shift);
+  // keys below this need no mask in this wave
+  const int plain = kv_len - q_len + (u.row + min(wave * 32, rows)) / a.group + 1;
 
   float m = kLowest, l = 0.0f, x = 0.0f;
   float16_t acc[ND];
@@ -509,124 +616,81 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit& u, 
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[n][e] = 0.0f;
 
-  unsigned long long bad_seen = 0;
-  Pages pages = load_pages(a, u.req, h, u.kv_begin >> a.c.b_shift, last, lane);
-  if (u.kv_begin < u.kv_end) bad_seen = pages.bad;
-
-  uint4 kr[NJ], vr[2];
-  const auto load = [&](int pos, const Pages& p) {
-    const int at = pos + 16 * part;
-    const int id = __builtin_amdgcn_readlane(p.id, min(at >> a.c.b_shift, last) - p.first);
-    const uint8_t* kb = a.c.data + ((long long)id * a.c.heads + h) * 2 * (a.c.B * D) + ((at & (a.c.B - 1)) >> 4) * (16 * D);
-    const uint8_t* vb = kb + a.c.B * D;
-    if (does_k) {
+  // Matrix half of a step: the product of the weights before with their
+  // values, and the scores of a tile, one product after the other.  Operands
+  // are fetched 6 products ahead, as an LDS read takes as long as several of
+  // them, and `side(k)` goes behind the k-th product: a wave issues in order,
+  // and a product keeps the matrix core for 32 cycles in which the wave can
+  // issue 7 other instructions.
+  constexpr int kValues = 4 * ND, kAll = kValues + 2 * KS, kAhead = 6;
+  float16_t s[2];
+  uint4 w[4];
+  const auto matrix = [&](const char* vbuf, const char* kbuf, auto both, auto&& side) {
+    constexpr int kSteps = decltype(both)::value ? kAll : kValues;
+    const half8_t* vf = reinterpret_cast<const half8_t*>(vbuf + kKBytes) + lane;
+    const half8_t* kf = reinterpret_cast<const half8_t*>(kbuf) + lane;
+    half8_t ring[8];
+    const auto get = [&](int k) {  // values: 16 keys' weights times all dims; scores: a fragment of either 32 keys
+      ring[k & 7] = k < kValues ? vf[k * 64] : kf[((k & 1) * KS + ((k - kValues) >> 1)) * 64];
+    };
+    sched_fence();
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) kr[j] = *reinterpret_cast<const uint4*>(kb + j * 1024 + lane * 16);
-    }
-    if (does_v) {
-      // (head size 64: the upper lanes repeat the lower ones)
-      const uint8_t* p0 = D == 128 ? vb + ((lane >> 4) & 1) * 1024 + half * 256 + (lane & 15) * 16
-                                   : vb + ((lane >> 4) & 1) * 256 + (lane & 15) * 16;
-      vr[0] = *reinterpret_cast<const uint4*>(p0);
-      vr[1] = *reinterpret_cast<const uint4*>(p0 + 512);
-    }
-  };
-  const auto store = [&](int pos, const Pages& p, char* buf) {
-    const int at = pos + 16 * part, pg = min(at >> a.c.b_shift, last) - p.first;
-    const bool bad = (p.bad >> pg) & 1;
-    if (does_k) {
-      // chunk c = 4 j + lane / 16 of token lane % 16
+    for (int k = 0; k < kAhead; ++k) get(k);
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const int c = 4 * j + (lane >> 4);
-        char* dst = buf + ((((part >> 1) * KS + (c & ~1)) * 64) + (c & 1) * 32 + (part & 1) * 16 + (lane & 15)) * 16;
-        const uint2 w0 = kv_half4<kFmt>(kr[j].x), w1 = kv_half4<kFmt>(kr[j].y), w2 = kv_half4<kFmt>(kr[j].z),
-                    w3 = kv_half4<kFmt>(kr[j].w);
-        *reinterpret_cast<uint4*>(dst) = uint4{w0.x, w0.y, w1.x, w1.y};
-        *reinterpret_cast<uint4*>(dst + 1024) = uint4{w2.x, w2.y, w3.x, w3.y};
-      }
-      if (lane == pg) {
-        TileMeta* t = reinterpret_cast<TileMeta*>(buf + kKBytes + kVBytes);
-        reinterpret_cast<float*>(&t->ks)[part] = p.ks;
-        reinterpret_cast<float*>(&t->lv)[part] = p.lv;
-        reinterpret_cast<float*>(&t->iv)[part] = p.iv;
-        t->bad[part] = bad;
-      }
-    }
-    if (does_v) {
-      uint32_t keep[2] = {~0u, ~0u};
-      if (kFmt == NSMLP_KV_E4M3 && (at + 16 > kv_len || bad)) {
-        // codes past the end may be NaNs: a zero weight does not hide them
+    for (int k = 0; k < kSteps; ++k) {
+      sched_fence();
+      if (k + kAhead < kSteps) get(k + kAhead);
+      if (k < kValues) {
+        acc[k % ND] = mfma32(ring[k & 7], as_h8(w[k / ND]), acc[k % ND]);
+      } else {
+        const int i = k & 1, f = (k - kValues) >> 1;
+        if (f == 0) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int left = bad ? 0 : kv_len - (at + 8 * i + 4 * (D == 128 ? half : (lane >> 4) & 1));
-          keep[i] = left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+          for (int e = 0; e < 16; ++e) s[i][e] = 0.0f;
         }
+        s[i] = mfma32(ring[k & 7], q[f], s[i]);
       }
-      char* vbuf = buf + kKBytes + part * ND * 1024;
+      side(k);
+    }
+    sched_fence();
+  };
+  // Vector half: the weights of the scores.
+  TileMeta meta[4];
+  const auto weigh = [&](int i_tile) {
+    const int pos = u.kv_begin + i_tile * kTileKeys;
+    float g[4], lv[4], iv[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) g[i] = meta[i][0] * rowf, lv[i] = meta[i][1], iv[i] = meta[i][2];
+    if (__builtin_expect_with_probability(pos + kTileKeys > plain || bad_seen != 0, 0, 0.99)) {
+      // some rows do not see all of the tile's keys: a hidden key's score is
+      // -inf, and where a lane sees none of 8 keys their block's scales, which
+      // may be anything, do not count
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint2 lo = kv_half4<kFmt>(word(vr[0], i) & keep[0]), hi = kv_half4<kFmt>(word(vr[1], i) & keep[1]);
-        const uint4 f = uint4{lo.x, lo.y, hi.x, hi.y};
-        if constexpr (D == 128) {
-          *reinterpret_cast<uint4*>(vbuf + (i * 64 + lane) * 16) = f;
-        } else {
-          if (lane < 32)
-            *reinterpret_cast<uint4*>(vbuf + ((i >> 1) * 64 + ((lane >> 4) & 1) * 32 + (lane & 15) + 16 * (i & 1)) * 16) = f;
+        uint32_t see = 0;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int n = min(max(limit - pos - 16 * i - 8 * j - 4 * half, 0), 4);
+          see |= ((1u << n) - 1u) << (4 * j);
         }
+        see = __float_as_int(meta[i][3]) != 0 ? 0 : see;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[i >> 1][8 * (i & 1) + e] = (see >> e) & 1 ? s[i >> 1][8 * (i & 1) + e] : -INFINITY;
+        g[i] = see == 0 ? 1.0f : g[i] < 1.1754944e-38f ? 1.1754944e-38f : g[i];  // (-inf times zero is no -inf)
+        lv[i] = see == 0 ? kLowest : lv[i];
+        iv[i] = see == 0 ? 0.0f : iv[i];
       }
     }
-  };
-
-  // One tile's products.  kMasked: some rows do not see all of its keys.
-  const auto tile = [&](auto masked, int pos, const char* buf) {
-    constexpr bool kMasked = decltype(masked)::value;
-    const half8_t* kf = reinterpret_cast<const half8_t*>(buf) + lane;
-    const half8_t* vf = reinterpret_cast<const half8_t*>(buf + kKBytes) + lane;
-    const TileMeta* t = reinterpret_cast<const TileMeta*>(buf + kKBytes + kVBytes);
-    const float4_t ks = t->ks, lv = t->lv, iv = t->iv;
-    float16_t s[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[i][e] = 0.0f;
-#pragma unroll
-      for (int k = 0; k < KS; ++k) s[i] = mfma32(kf[(i * KS + k) * 64], q[k], s[i]);
-    }
-    // bit 8 i + e: whether the row sees key e of the lane's 8 among the tile's i-th 16
-    uint32_t see = ~0u;
-    if constexpr (kMasked) {
-      see = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int n = min(max(limit - pos - 8 * i - 4 * half, 0), 4);
-        see |= ((1u << n) - 1u) << (4 * i);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) see = t->bad[i] != 0 ? see & ~(0xFFu << (8 * i)) : see;
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[i][e] = (see >> (16 * i + e)) & 1 ? s[i][e] : -INFINITY;
-    }
-    uint4 w[4];
     float dl, dx;
     const auto weights = [&]() {
       dl = dx = 0.0f;
       float most_sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float g = ks[i] * rowf, c = lv[i] - m;
+        const float c = lv[i] - m;
         float p[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) p[e] = exp2_fast(__builtin_fmaf(s[i >> 1][8 * (i & 1) + e], g, c));
-        float share = iv[i];
-        if constexpr (kMasked) {
-          // a hidden key's weight is zero whatever its block's scales are
-#pragma unroll
-          for (int e = 0; e < 8; ++e) p[e] = (see >> (8 * i + e)) & 1 ? p[e] : 0.0f;
-          share = (see >> (8 * i)) & 0xFF ? share : 0.0f;
-        }
+        for (int e = 0; e < 8; ++e) p[e] = exp2_fast(__builtin_fmaf(s[i >> 1][8 * (i & 1) + e], g[i], c));
         w[i] = uint4{pack_f16(p[0], p[1]), pack_f16(p[2], p[3]), pack_f16(p[4], p[5]), pack_f16(p[6], p[7])};
         const half2_t one = {(_Float16)1.0f, (_Float16)1.0f};
         float sum = __builtin_amdgcn_fdot2(as_half2(w[i].x), one, 0.0f, false);
@@ -634,19 +698,17 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit& u, 
         sum = __builtin_amdgcn_fdot2(as_half2(w[i].z), one, sum, false);
         sum = __builtin_amdgcn_fdot2(as_half2(w[i].w), one, sum, false);
         most_sum = i == 0 ? sum : fmaxf(most_sum, sum);
-        dl = __builtin_fmaf(sum, share, dl);
-        if constexpr (kLse) dx = __builtin_fmaf(((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])), share, dx);
+        dl = __builtin_fmaf(sum, iv[i], dl);
+        if constexpr (kLse) dx = __builtin_fmaf(((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])), iv[i], dx);
       }
       return most_sum;
     };
-    sched_fence();  // the products' operands are not fetched further ahead than registers last
     const float sum = weights();
     if (__builtin_expect_with_probability(__any(sum > kSumLimit), 0, 0.999)) {
-      float top = kLowest;
+      float top = m;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) top = fmaxf(top, __builtin_fmaf(max16(s[i >> 1], 8 * (i & 1)), ks[i] * rowf, lv[i]));
-      top = fmaxf(top, __shfl_xor(top, 32, kWave));
-      top = ceilf(fmaxf(top, m));
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, __builtin_fmaf(max8(s[i >> 1], 8 * (i & 1)), g[i], lv[i]));
+      top = ceilf(fmaxf(top, __shfl_xor(top, 32, kWave)));
       const float scale = exp2_fast(m - top);
       m = top;
       l *= scale, x *= scale;
@@ -656,55 +718,65 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit& u, 
     }
     l += dl;
     if constexpr (kLse) x += dx;
-    sched_fence();
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int n = 0; n < ND; ++n) acc[n] = mfma32(vf[(i * ND + n) * 64], as_h8(w[i]), acc[n]);
-    sched_fence();
   };
 
-  char* cur = lds;
-  char* nxt = lds + kBuf;
-  if (u.kv_begin < u.kv_end) {
-    load(u.kv_begin, pages);
-    store(u.kv_begin, pages, cur);
-  }
-  __syncthreads();
-  int pos = u.kv_begin;
-  const auto ahead = [&]() {  // the next tile's codes, before this one's products
-    if (pos + kTileKeys < u.kv_end) {
-      const int hi = min((pos + 2 * kTileKeys - 1) >> a.c.b_shift, last);
-      if (hi - pages.first >= kWave) {
-        pages = load_pages(a, u.req, h, (pos + kTileKeys) >> a.c.b_shift, last, lane);
-        bad_seen |= pages.bad;
-      }
-      load(pos + kTileKeys, pages);
+  // Steps.  A tile takes two, matrix and vector half; the first also decodes
+  // this wave's codes of another tile, in the shadow of the products.  With 8
+  // waves the upper four are one step behind, so that on every SIMD one wave has
+  // the matrix cores while the other has the vector unit.  Steps of the lower
+  // waves (the upper's are one later):
+  //   2 i      values of V(i - 1), scores of K(i); K(i + 1) written; V(i) written (by the upper, in 2 i + 1)
+  //   2 i + 1  weights of tile i
+  // K(i + 1) takes the place of K(i - 1), last read in step 2 i - 1, and V(i)
+  // that of V(i - 2), last read in step 2 i - 1.  The tile's scales are written
+  // in the vector half before, four tiles' in turn.
+  if (tiles > 0) {
+    char* const buf0 = lds;
+    char* const buf1 = lds + kTileBytes<D>;
+    // before the first step: K(0), its scales, and no values for no weights
+    if (!upper) {
+#pragma unroll
+      for (int t = 0; t < 8; ++t) decode(0, 0, buf0, t);
     }
-  };
-  const auto next = [&]() {
-    if (pos + kTileKeys < u.kv_end) store(pos + kTileKeys, pages, nxt);
+    store_meta(0);
+    for (int i = tid; i < kVBytes / 16; i += NW * kWave) reinterpret_cast<uint4*>(buf1 + kKBytes)[i] = uint4{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = uint4{0, 0, 0, 0};
+    turn_pages(0, 2);
+    if (!upper) fetch(0, 1);
     __syncthreads();
-    char* t = cur;
-    cur = nxt, nxt = t;
-    pos += kTileKeys;
-  };
-  // three loops, so that the accumulators stay where they are in each:
-  // tiles that all rows see, tiles with hidden keys (or, from the first block
-  // that is none, all that follow), tiles that only other waves need
-  while (pos < u.kv_end && pos + kTileKeys <= plain && bad_seen == 0) {
-    ahead();
-    tile(std::false_type{}, pos, cur);
-    next();
-  }
-  while (pos < u.kv_end && pos < most) {
-    ahead();
-    tile(std::true_type{}, pos, cur);
-    next();
-  }
-  while (pos < u.kv_end) {
-    ahead();
-    next();
+    if (upper) __syncthreads();
+    for (int i = 0; i < tiles; ++i) {
+      char* const cur = i & 1 ? buf1 : buf0;
+      char* const other = i & 1 ? buf0 : buf1;
+      // K(i + 1) or V(i) decoded and the next codes fetched, the next tile's
+      // scales written, this one's read
+      constexpr int kTasks = kRoles * 9 + 2;
+      __builtin_amdgcn_s_setprio(1);  // the products go first: the other wave's vector work fills what they leave
+      matrix(other, cur, std::true_type{}, [&](int k) {
+#pragma unroll
+        for (int t = k * kTasks / kAll; t < (k + 1) * kTasks / kAll; ++t) {
+          if (t == kTasks - 1) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) meta[j] = metas[(i & 3) * 4 + j];
+          } else if (t == kTasks - 2) {
+            store_meta(i + 1);
+          } else {
+            const int o = t / 9, part_t = t % 9;
+            const bool v = kRoles == 2 ? o == 1 : upper;
+            if (part_t < 8) decode(o, v ? i : i + 1, v ? cur : other, part_t);
+            else fetch(o, v ? i + 1 : i + 2);
+          }
+        }
+      });
+      __builtin_amdgcn_s_setprio(0);
+      __syncthreads();
+      weigh(i);
+      turn_pages(i + 1, i + 3);
+      if (NW == 8) __syncthreads();
+    }
+    matrix((tiles - 1) & 1 ? buf1 : buf0, nullptr, std::false_type{}, [](int) {});
+    if (NW == 8 && !upper) __syncthreads();
   }
   if (bad_seen != 0 && lane == 0) atomicOr(a.status, NSMLP_STATUS_BLOCK_UNAVAILABLE);
 
@@ -735,9 +807,9 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit& u, 
           o[2 * i] = to_out<kBf16>(p[0]) | (uint32_t)to_out<kBf16>(p[1]) << 16;
           o[2 * i + 1] = to_out<kBf16>(p[2]) | (uint32_t)to_out<kBf16>(p[3]) << 16;
         }
-        uint4* dst = reinterpret_cast<uint4*>(a.out + at * D + dim_of(g));
-        dst[0] = uint4{o[0], o[1], o[2], o[3]};
-        dst[1] = uint4{o[4], o[5], o[6], o[7]};
+        uint4* to = reinterpret_cast<uint4*>(a.out + at * D + dim_of(g));
+        to[0] = uint4{o[0], o[1], o[2], o[3]};
+        to[1] = uint4{o[4], o[5], o[6], o[7]};
       }
       if (kLse && half == 0) a.lse[at] = x == 0.0f ? -INFINITY : (m + log2f(x)) * 0.6931471805599453f;
     }
@@ -754,7 +826,7 @@ __global__ void __launch_bounds__(NW* kWave, 2) k_attn_both(KvAttnArgs a, int bl
     const int items = min(a.sched[2], a.s.max_units_b) * a.c.heads;
     const KvUnit* units = reinterpret_cast<const KvUnit*>(a.sched + a.s.off_units_b);
     for (int item = block; item < items; item += blocks_b) {
-      tile_unit<D, kFmt, kBf16, NW, kLse>(a, units[item / a.c.heads], item % a.c.heads, lds);
+      tile_unit<D, kFmt, kBf16, NW, kLse>(a, load_unit(units + item / a.c.heads), item % a.c.heads, lds);
       __syncthreads();
     }
   } else {
@@ -805,7 +877,7 @@ __global__ void __launch_bounds__(256) k_attn_join(KvAttnArgs a) {
 
 template <int D, int kFmt, bool kBf16, int NW, bool kLse>
 void launch_both(const KvAttnArgs& a, int stream_blocks, hipStream_t s) {
-  constexpr int kStream = (int)sizeof(StreamLds<D, NW>), kLds = kStream > kTileLds<D, NW> ? kStream : kTileLds<D, NW>;
+  constexpr int kStream = (int)sizeof(StreamLds<D, NW>), kLds = kStream > kTileLds<D> ? kStream : kTileLds<D>;
   static std::once_flag once;
   std::call_once(once, [] {
     (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k_attn_both<D, kFmt, kBf16, NW, kLse>),
