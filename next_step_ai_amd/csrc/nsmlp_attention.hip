@@ -113,10 +113,9 @@ __device__ __forceinline__ KvUnit load_unit(const KvUnit* p) {
 // dims) as rows and the queries as columns.
 template <int D, int NW>
 struct StreamLds {
-  float sum[NW][16][D + 4];  // the waves' results; then (m, l, x) of the rows of partials, kBatch at a time
+  float sum[NW][16][D + 4];  // the waves' results
   float ml[NW][3][16];
   int last;
-  static constexpr int kBatch = (int)(sizeof(float) * NW * (D + 4) / sizeof(float4_t));
 };
 
 template <int D>
@@ -353,56 +352,60 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
     for (int d = 0; d < kDims; ++d) o[d] += lds.sum[w][row][d0 + d];
   }
   if (u.part >= 0) {
-    // one of several units of these rows: the last one to end adds them up, in
-    // the order of the parts, so that the result does not depend on which it is
-    const long long at = ((long long)u.part * a.c.heads + h) * kKvRowsA + row;
-    if (row < rows) {
+    // One of several units of these rows: eight at a time are added up by the
+    // last of them to end, their sums again eight at a time, and so on, each
+    // sum in the order of the parts, so that the result does not depend on who
+    // is last.  A level costs one write, one atomic and one read that all
+    // threads have in flight at once (4 us; one workgroup reading 64 partials
+    // of 8 KB took 20 us).
+    int idx = u.part - u.first, n = u.parts, stride = 1;
+    int* count = a.count;
+    while (n > 1) {
+      const int group = idx >> 3, size = min(8, n - 8 * group);
+      if (size > 1) {
+        const long long step = (long long)stride * a.c.heads * kKvRowsA;
+        const long long at = ((long long)u.first * a.c.heads + h) * kKvRowsA + row + idx * step;
+        if (row < rows) {
 #pragma unroll
-      for (int d = 0; d < kDims; d += 2) st_coherent2(a.acc_a + at * D + d0 + d, o[d], o[d + 1]);
-      if (d0 == 0) st_coherent2(a.ml_a + 4 * at, mr, lr), st_coherent2(a.ml_a + 4 * at + 2, xr, 0.0f);
-    }
-    wait_stores();
-    __syncthreads();
-    int* count = a.count + u.split * a.c.heads + h;
-    if (tid == 0) lds.last = atomicAdd(count, 1) == u.parts - 1;
-    __syncthreads();
-    if (!lds.last) return;
-    if (tid == 0) atomicExch(count, 0);
-    float4_t* ml = reinterpret_cast<float4_t*>(&lds.sum[0][0][0]);
-    constexpr int kBatch = StreamLds<D, NW>::kBatch;
-    const long long step = (long long)a.c.heads * kKvRowsA, first = ((long long)u.first * a.c.heads + h) * kKvRowsA;
-    mr = kLowest, lr = xr = 0.0f;
+          for (int d = 0; d < kDims; d += 2) st_coherent2(a.acc_a + at * D + d0 + d, o[d], o[d + 1]);
+          if (d0 == 0) st_coherent2(a.ml_a + 4 * at, mr, lr), st_coherent2(a.ml_a + 4 * at + 2, xr, 0.0f);
+        }
+        wait_stores();
+        __syncthreads();
+        int* arrived = count + (u.first + group * 8 * stride) * a.c.heads + h;
+        if (tid == 0) lds.last = atomicAdd(arrived, 1) == size - 1;
+        __syncthreads();
+        if (!lds.last) return;
+        if (tid == 0) atomicExch(arrived, 0);
+        if (row < rows) {
+          const long long from = at + (group * 8 - idx) * step;
+          float2 ml[8][2], y[8][kDims / 2];
 #pragma unroll
-    for (int d = 0; d < kDims; ++d) o[d] = 0.0f;
-    for (int base = 0; base < u.parts; base += kBatch) {
-      const int n = min(kBatch, u.parts - base);
-      __syncthreads();
-      for (int i = tid; i < n * 16; i += NW * kWave) {
-        const float* src = a.ml_a + 4 * (first + (base + i / 16) * step + i % 16);
-        const float2 v0 = ld_coherent2(src), v1 = ld_coherent2(src + 2);
-        ml[i] = float4_t{v0.x, v0.y, v1.x, 0.0f};
-      }
-      __syncthreads();
-      if (row < rows) {
-        float top = mr;
-        for (int p = 0; p < n; ++p) top = fmaxf(top, ml[p * 16 + row][0]);
-        const float f = exp2_fast(mr - top);
-        mr = top, lr *= f, xr *= f;
+          for (int p = 0; p < 8; ++p) {
+            const long long q_at = from + min(p, size - 1) * step;  // (the last again: no branch between the reads)
+            ml[p][0] = ld_coherent2(a.ml_a + 4 * q_at), ml[p][1] = ld_coherent2(a.ml_a + 4 * q_at + 2);
 #pragma unroll
-        for (int d = 0; d < kDims; ++d) o[d] *= f;
-        const float* src = a.acc_a + (first + base * step + row) * D + d0;
-#pragma unroll 8
-        for (int p = 0; p < n; ++p) {
-          const float4_t v = ml[p * 16 + row];
-          const float w = exp2_fast(v[0] - mr);
-          lr += v[1] * w, xr += v[2] * w;
+            for (int d = 0; d < kDims / 2; ++d) y[p][d] = ld_coherent2(a.acc_a + q_at * D + d0 + 2 * d);
+          }
+          mr = ml[0][0].x;
 #pragma unroll
-          for (int d = 0; d < kDims; d += 2) {
-            const float2 y = ld_coherent2(src + p * step * D + d);
-            o[d] += y.x * w, o[d + 1] += y.y * w;
+          for (int p = 1; p < 8; ++p) mr = fmaxf(mr, ml[p][0].x);
+          lr = xr = 0.0f;
+#pragma unroll
+          for (int d = 0; d < kDims; ++d) o[d] = 0.0f;
+#pragma unroll
+          for (int p = 0; p < 8; ++p) {
+            const float f = exp2_fast(ml[p][0].x - mr);
+            if (p < size) {
+              lr += ml[p][0].y * f, xr += ml[p][1].x * f;
+#pragma unroll
+              for (int d = 0; d < kDims / 2; ++d) o[2 * d] += y[p][d].x * f, o[2 * d + 1] += y[p][d].y * f;
+            }
           }
         }
       }
+      idx = group, n = (n + 7) >> 3, stride *= 8;
+      count += kKvCounters;  // each level has counters of its own
     }
   }
   if (row < rows) {

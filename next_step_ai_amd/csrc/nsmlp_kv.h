@@ -116,6 +116,11 @@ struct KvSplit {
 
 constexpr int kKvMaxRequests = 4096;
 constexpr int kKvRowsA = 16;
+// arrival counters of a level of list a's joins, one per (partial, K/V head):
+// at most 2 shares, and shares times heads is below 512 + heads (<= 1024); 4
+// levels of 8 join 4096 parts, and there are at most 512
+constexpr int kKvCounters = 8192;
+static_assert(4 * kKvCounters <= kMaxK && 2 * (512 + 1024) <= kKvCounters, "the workspace's block counters");
 constexpr int kKvHeaderInts = 16;  // units a, shares, units b, splits b
 
 struct KvSchedule {  // sizes, from the host's knowledge of a step (kv_schedule)
@@ -152,7 +157,7 @@ struct KvAttnArgs {
   int max_blocks, R, total, group;
   float scale_log2;  // softmax scale times log2(e)
   float *acc_a, *ml_a, *acc_b, *ml_b;  // partial results of either list: [parts][kv_heads][rows][D], [..][4] (m, l, x)
-  int *status, *count;                 // status word, arrival counters [parts_a][kv_heads] (zero, left zero)
+  int *status, *count;  // status word, arrival counters [levels][kKvCounters] (zero, left zero)
   KvSchedule s;
 };
 // floats of the partial results, and where acc_a, ml_a, acc_b, ml_b start
