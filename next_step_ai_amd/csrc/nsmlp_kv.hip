@@ -605,7 +605,7 @@ KvSchedule kv_schedule(int requests, int total, int max_new, int group, int kv_h
   s.list_b = (long long)(max_new < total ? max_new : total) * group > kKvRowsA;
   s.rows_b = (long long)max_new * group > 128 ? 256 : 128;
   // list a: two workgroups of 4 waves on every CU, or one of 8 beside list b's
-  s.shares = ((s.list_b ? 256 : 512) + kv_heads - 1) / kv_heads;
+  s.shares = (256 + kv_heads - 1) / kv_heads;
   const long long tiles_b = s.list_b ? ((long long)total * group + s.rows_b - 1) / s.rows_b + requests : 0;
   s.target_b = !s.list_b || tiles_b * kv_heads >= 512 ? 0 : (512 + kv_heads - 1) / kv_heads;
   // list a: every share ends at most one unit that its request does not end,
