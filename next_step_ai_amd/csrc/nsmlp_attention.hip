@@ -838,35 +838,50 @@ __global__ void __launch_bounds__(NW* kWave, 2) k_attn_both(KvAttnArgs a, int bl
 }
 
 // ------------------------------------------------------------------ join --
-// One wave per row whose keys were shared out: weights 2^(m_p - max m), in the
-// order of the parts, so that the result does not depend on the schedule of
-// the device.
+// One wave per row of list b whose keys were shared out: weights 2^(m_p - m)
+// in the order of the parts, eight parts' results in flight at a time.
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(256) k_attn_join(KvAttnArgs a) {
+  kernarg_warm<sizeof(KvAttnArgs)>();
   constexpr int E = D / kWave;
-  const int lane = threadIdx.x & (kWave - 1), rows_b = a.s.rows_b;
+  const int lane = threadIdx.x & (kWave - 1), wave = uniform(threadIdx.x >> 6), rows_b = a.s.rows_b;
   const KvSplit* splits = reinterpret_cast<const KvSplit*>(a.sched + a.s.off_splits_b);
   const int items = min(a.sched[3], a.s.max_splits_b) * a.c.heads * rows_b;
-  for (int item = (int)blockIdx.x * 4 + (threadIdx.x >> 6); item < items; item += (int)gridDim.x * 4) {
+  for (int item = (int)blockIdx.x * 4 + wave; item < items; item += (int)gridDim.x * 4) {
     const int r = item % rows_b, h = item / rows_b % a.c.heads;
     const KvSplit sp = splits[item / rows_b / a.c.heads];
-    const int q0 = a.q_start[sp.req], q_len = a.q_start[sp.req + 1] - q0;
-    const int full = sp.row + r, tok = q0 + full / a.group;
-    if (full >= q_len * a.group || tok >= a.total) continue;
+    const int q0 = a.q_start[sp.req], rows = (a.q_start[sp.req + 1] - q0) * a.group;
     const long long first = ((long long)sp.first * a.c.heads + h) * rows_b + r, step = (long long)a.c.heads * rows_b;
-    float top = kLowest;
-    for (int p = lane; p < sp.parts; p += kWave) top = fmaxf(top, a.ml_b[4 * (first + p * step)]);
-    top = wave_max(top);
-    float l = 0.0f, x = 0.0f, o[E] = {};
-#pragma unroll 8
-    for (int p = 0; p < sp.parts; ++p) {
-      const long long at = first + p * step;
-      const float4_t ml = *reinterpret_cast<const float4_t*>(a.ml_b + 4 * at);
-      const float w = exp2_fast(ml[0] - top);
-      l += ml[1] * w, x += ml[2] * w;
+    float m = kLowest, l = 0.0f, x = 0.0f, o[E] = {};
+    for (int base = 0; base < sp.parts; base += 8) {
+      float4_t ml[8];
+      float y[8][E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] += a.acc_b[at * D + lane * E + e] * w;
+      for (int p = 0; p < 8; ++p) {
+        const long long at = first + min(base + p, sp.parts - 1) * step;  // (the last again: no branch between the reads)
+        ml[p] = *reinterpret_cast<const float4_t*>(a.ml_b + 4 * at);
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[p][e] = a.acc_b[at * D + lane * E + e];
+      }
+      float top = m;
+#pragma unroll
+      for (int p = 0; p < 8; ++p) top = fmaxf(top, ml[p][0]);
+      const float old = exp2_fast(m - top);
+      m = top, l *= old, x *= old;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] *= old;
+#pragma unroll
+      for (int p = 0; p < 8; ++p) {
+        const float w = exp2_fast(ml[p][0] - m);
+        if (base + p < sp.parts) {
+          l += ml[p][1] * w, x += ml[p][2] * w;
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[e] += y[p][e] * w;
+        }
+      }
     }
+    const int full = sp.row + r, tok = q0 + full / a.group;
+    if (full >= rows || tok >= a.total) continue;  // (rows that the tile does not have are read, and dropped)
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const long long at = (long long)tok * a.c.heads * a.group + h * a.group + full % a.group;
     if constexpr (E == 2)
@@ -874,7 +889,7 @@ __global__ void __launch_bounds__(256) k_attn_join(KvAttnArgs a) {
           to_out<kBf16>(o[0] * inv) | (uint32_t)to_out<kBf16>(o[1] * inv) << 16;
     else
       a.out[at * D + lane] = to_out<kBf16>(o[0] * inv);
-    if (a.lse != nullptr && lane == 0) a.lse[at] = x == 0.0f ? -INFINITY : (top + log2f(x)) * 0.6931471805599453f;
+    if (a.lse != nullptr && lane == 0) a.lse[at] = x == 0.0f ? -INFINITY : (m + log2f(x)) * 0.6931471805599453f;
   }
 }
 

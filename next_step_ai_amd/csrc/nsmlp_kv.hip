@@ -62,17 +62,18 @@ __device__ __forceinline__ void block_scan(int (&v)[N], int (&total)[N], int (*w
 
 __device__ __forceinline__ int clip_len(int v) { return min(max(v, 0), 1 << 29); }
 
+// list a counts keys in pieces of 64; a request without any takes one piece,
+// so that its rows are somebody's
+constexpr int kLeastShare = 4;     // pieces: 256 keys are worth a workgroup
+constexpr int kLeastPart = 1024;   // keys of list b that are worth a join
+
 // keys per part, so that about `target` units share the list's `work` keys
 __device__ __forceinline__ int part_keys(long long work, int target) {
   if (target <= 0) return 1 << 30;  // more than any request's
   const double each = ceil((double)work / target);  // exact: below 2^53, and a quotient's ceiling does not round down
   const double up = ceil(each * (1.0 / 128)) * 128;
-  return up < 512 ? 512 : up > (double)(1 << 30) ? 1 << 30 : (int)up;
+  return up < kLeastPart ? kLeastPart : up > (double)(1 << 30) ? 1 << 30 : (int)up;
 }
-
-// list a counts keys in pieces of 64; a request without any takes one piece,
-// so that its rows are somebody's
-constexpr int kLeastShare = 4;  // pieces: 256 keys are worth a workgroup
 
 __device__ __forceinline__ int pieces_of(int keys) { return max(1, (keys + 63) >> 6); }
 
@@ -603,10 +604,14 @@ void launch_kv_read(const KvReadArgs& a, bool bf16, hipStream_t s) { NSMLP_KV_BY
 KvSchedule kv_schedule(int requests, int total, int max_new, int group, int kv_heads) {
   KvSchedule s;
   s.list_b = (long long)(max_new < total ? max_new : total) * group > kKvRowsA;
-  s.rows_b = (long long)max_new * group > 128 ? 256 : 128;
-  // list a: two workgroups of 4 waves on every CU, or one of 8 beside list b's
+  // list a: one workgroup of 4 waves per CU has as many reads in flight as the
+  // memory takes (two: 131000 keys 50 -> 55 us, for the joins)
   s.shares = (256 + kv_heads - 1) / kv_heads;
-  const long long tiles_b = s.list_b ? ((long long)total * group + s.rows_b - 1) / s.rows_b + requests : 0;
+  // list b: 256 rows per workgroup where that still makes two for every CU
+  // (chunk of 2048 over 14336, 128 heads: 1.84 ms, with 128 rows 1.92), else 128
+  const long long rows = (long long)total * group;
+  s.rows_b = rows / 256 * kv_heads >= 512 ? 256 : 128;
+  const long long tiles_b = s.list_b ? (rows + s.rows_b - 1) / s.rows_b + requests : 0;
   s.target_b = !s.list_b || tiles_b * kv_heads >= 512 ? 0 : (512 + kv_heads - 1) / kv_heads;
   // list a: every share ends at most one unit that its request does not end,
   // so units are at most requests + shares, and those of a request with several
