@@ -508,7 +508,7 @@ int nsmlp_host_device_pointer(const void* host, void** device_ptr);
  * blocks out, and the attention that reads it.  No reference counterpart (the
  * reference's attention and its K/V cache are torch code, RT:5927-7142).
  *
- * Formats: NSMLP_KV_INT8: code in -127..127, scale = largest magnitude / 127.
+ * Formats: NSMLP_KV_INT8: code in -127..127, scale = largest magnitude times fp32(1 / 127).
  * NSMLP_KV_E4M3: OCP e4m3, scale = the smallest power of two that keeps the
  * largest magnitude within 448.  value = code * scale.  A (block, head)'s scale
  * never shrinks while the block is filled and is 2^-100 at least; where a call

@@ -9,11 +9,15 @@
 //   acc = sum_j 2^(e_j - m) v_j,   l = sum_j 2^(e_j - m) / vs_j,   o = acc / l
 // so a weight costs one fused multiply-add and one exp2, the weights fit fp16
 // whatever the scales of the blocks are, and the codes enter the products
-// exactly.  m follows the running maximum lazily: it moves only where a tile
-// exceeds it by more than 2^8, so most tiles neither rescale acc nor exchange
-// maxima between lanes; a weight is then at most 2^8, far inside fp16.
-// acc, l, m and the scores are fp32; a weight is rounded to fp16 once, as the
-// products' operand (relative 2^-12, averaged over the keys).
+// exactly.  m follows the running maximum lazily: when it is set, the largest
+// weight is about 2^10, and it is set again only where the weights' sums (of 4
+// or 8, kept anyway) pass 2^15.  So most tiles neither look for a maximum nor
+// rescale acc, no weight leaves fp16, and weights down to 2^-24 of the largest
+// keep their 11 bits (with the largest at 1 those below 2^-14 lost some, and
+// outputs over thousands of keys half a rounding).  m is an integer, so that
+// rescaling is exact.  acc, l, m and the scores are fp32; a weight is rounded to
+// fp16 once, as the products' operand, and l takes it as rounded: where few
+// keys carry a row its rounding cancels.
 #include <mutex>
 #include <type_traits>
 
@@ -24,9 +28,8 @@ namespace nsmlp {
 namespace {
 
 constexpr float kLowest = -3.402823466e38f;
-// A lane's weights of a tile (8 at a time) whose sum stays below this are far
-// inside fp16: none is above 2^12.
-constexpr float kSumLimit = 4096.0f;
+constexpr float kSumLimit = 32768.0f;
+constexpr float kLift = 10.0f;
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
@@ -137,6 +140,11 @@ __device__ __forceinline__ float2 ld_coherent2(const float* p) {
 template <int D, int kFmt, bool kBf16, int NW>
 __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u, int h, StreamLds<D, NW>& lds) {
   constexpr int NJ = D / 64, KS = D / 32, ND = D / 16;
+  // fp16 outputs: weights in two fp16 parts, so that their rounding does not
+  // add to the output's own (error against 64 bits 2.9e-4 -> 2.1e-4 of the norm,
+  // where 2.1e-4 is one rounding); the products have the time, as the codes'
+  // way from memory takes longer.  bf16 outputs round 8 times coarser.
+  constexpr bool kSplit = !kBf16;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
   const bool want_lse = a.lse != nullptr;
@@ -240,7 +248,7 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
         see |= ((1u << n) - 1u) << (4 * s);
       }
     }
-    uint2 w[2];
+    uint2 w[2], rest[2];  // weights, and (kSplit) what their rounding left
     float dl, dx;
     const auto weights = [&]() {
       float sums[2];
@@ -257,19 +265,22 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
           for (int i = 0; i < 4; ++i) p[i] = (see >> (4 * s + i)) & 1 ? p[i] : 0.0f;
           share = (see >> (4 * s)) & 0xF ? share : 0.0f;
         }
-        // the sum takes the weights as the products see them, rounded to fp16:
-        // where few keys carry the row, their rounding cancels
         w[s] = uint2{pack_f16(p[0], p[1]), pack_f16(p[2], p[3])};
         const half2_t one = {(_Float16)1.0f, (_Float16)1.0f};
         sums[s] = __builtin_amdgcn_fdot2(as_half2(w[s].y), one, __builtin_amdgcn_fdot2(as_half2(w[s].x), one, 0.0f, false), false);
-        dl = __builtin_fmaf(sums[s], share, dl);
-        if (want_lse) dx = __builtin_fmaf((p[0] + p[1]) + (p[2] + p[3]), share, dx);
+        if constexpr (kSplit) {
+          const half2_t a0 = as_half2(w[s].x), a1 = as_half2(w[s].y);
+          rest[s] = uint2{pack_f16(p[0] - (float)a0.x, p[1] - (float)a0.y), pack_f16(p[2] - (float)a1.x, p[3] - (float)a1.y)};
+        }
+        const float whole = (p[0] + p[1]) + (p[2] + p[3]);
+        dl = __builtin_fmaf(kSplit ? whole : sums[s], share, dl);
+        if (!kSplit && want_lse) dx = __builtin_fmaf(whole, share, dx);
       }
       return fmaxf(sums[0], sums[1]);
     };
     const float sum = weights();
     if (__builtin_expect_with_probability(__any(sum > kSumLimit), 0, 0.999)) {
-      float top = m;
+      float top = kLowest;
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -278,7 +289,7 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
           top = fmaxf(top, (see >> (4 * s + i)) & 1 ? e : kLowest);
         }
       top = fmaxf(top, __shfl_xor(top, 16, kWave));
-      top = ceilf(fmaxf(top, __shfl_xor(top, 32, kWave)));
+      top = fmaxf(m, ceilf(fmaxf(top, __shfl_xor(top, 32, kWave))) - kLift);  // (never down: other rows may have asked)
       const float scale = exp2_fast(m - top);
       m = top;
       l *= scale, x *= scale;
@@ -287,7 +298,7 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
       (void)weights();
     }
     l += dl;
-    if (want_lse) x += dx;
+    if (!kSplit && want_lse) x += dx;
     uint32_t keep[2] = {~0u, ~0u};
     if (kFmt == NSMLP_KV_E4M3 && kMasked) {
       // codes past the end may be NaNs: a zero weight does not hide them
@@ -297,11 +308,13 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
         keep[s] = left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
       }
     }
-    const half8_t wh = join4(w[0], w[1]);
+    const half8_t wh = join4(w[0], w[1]), wr = kSplit ? join4(rest[0], rest[1]) : wh;
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
-      acc[d] = mfma16(join4(kv_half4<kFmt>(word(t.v[0][d >> 2], d & 3) & keep[0]), kv_half4<kFmt>(word(t.v[1][d >> 2], d & 3) & keep[1])),
-                      wh, acc[d]);
+    for (int d = 0; d < ND; ++d) {
+      const half8_t v = join4(kv_half4<kFmt>(word(t.v[0][d >> 2], d & 3) & keep[0]), kv_half4<kFmt>(word(t.v[1][d >> 2], d & 3) & keep[1]));
+      acc[d] = mfma16(v, wh, acc[d]);
+      if constexpr (kSplit) acc[d] = mfma16(v, wr, acc[d]);
+    }
   };
   if (begin < end) {
     int pos = begin;
@@ -321,6 +334,7 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
   }
   if (bad_seen != 0 && lane == 0) atomicOr(a.status, NSMLP_STATUS_BLOCK_UNAVAILABLE);
 
+  if constexpr (kSplit) x = l;
   // join the waves: each result under the largest reference
   l += __shfl_xor(l, 16, kWave), x += __shfl_xor(x, 16, kWave);
   l += __shfl_xor(l, 32, kWave), x += __shfl_xor(x, 32, kWave);
@@ -457,10 +471,6 @@ __global__ void __launch_bounds__(4 * kWave) k_attn_stream(KvAttnArgs a) {
 // The scores of a query stay in its two lanes, in the order in which the
 // second product wants the weights.
 //
-// Weights are taken under the reference as it stands; their sums, kept anyway,
-// tell whether one was too large for it (the first tile, and seldom after), and
-// only then is the maximum looked for.  References are integers, so that
-// rescaling is exact.
 constexpr int kTileKeys = 64;
 
 __device__ __forceinline__ float max8(const float16_t& s, int at) {
@@ -708,10 +718,10 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
     };
     const float sum = weights();
     if (__builtin_expect_with_probability(__any(sum > kSumLimit), 0, 0.999)) {
-      float top = m;
+      float top = kLowest;
 #pragma unroll
       for (int i = 0; i < 4; ++i) top = fmaxf(top, __builtin_fmaf(max8(s[i >> 1], 8 * (i & 1)), g[i], lv[i]));
-      top = ceilf(fmaxf(top, __shfl_xor(top, 32, kWave)));
+      top = fmaxf(m, ceilf(fmaxf(top, __shfl_xor(top, 32, kWave))) - kLift);  // (never down: other rows may have asked)
       const float scale = exp2_fast(m - top);
       m = top;
       l *= scale, x *= scale;

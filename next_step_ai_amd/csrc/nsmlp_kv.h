@@ -60,7 +60,7 @@ __device__ __forceinline__ uint2 kv_half4(uint32_t w) {
   }
 }
 
-// The scale that a largest magnitude asks for.  int8: a / 127.  e4m3: the
+// The scale that a largest magnitude asks for.  int8: a times fp32(1 / 127).  e4m3: the
 // smallest power of two that keeps a within 448, so that recoding a block
 // under a larger scale moves exponents and rounds subnormals only.  Never
 // below 2^-100; NaN where a is not finite.
@@ -69,7 +69,7 @@ __device__ __forceinline__ float kv_scale_of(float a) {
   if (!(a < INFINITY)) return __uint_as_float(0x7FC00000u);
   float s;
   if constexpr (kFmt == NSMLP_KV_INT8) {
-    s = a / 127.0f;
+    s = a * (1.0f / 127.0f);
   } else {
     int e = 0;
     const float m = frexpf(a, &e);  // a = m 2^e, m in [0.5, 1)

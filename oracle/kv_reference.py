@@ -71,7 +71,7 @@ def scale_of(amax: np.float32, fmt: str) -> np.float32:
     if not np.isfinite(amax):
         return np.float32(np.nan)
     if fmt == "int8":
-        s = np.float32(amax) / np.float32(127)
+        s = np.float32(amax) * (np.float32(1) / np.float32(127))
     elif amax == 0:
         s = np.float32(0)
     else:
