@@ -107,7 +107,7 @@ __device__ __forceinline__ float lane_of(float v, int i) {
 __device__ __forceinline__ KvUnit load_unit(const KvUnit* p) {
   const KvUnit v = *p;
   return KvUnit{uniform(v.req),  uniform(v.row),   uniform(v.kv_begin), uniform(v.kv_end),
-                uniform(v.part), uniform(v.first), uniform(v.parts),    uniform(v.split)};
+                uniform(v.part), uniform(v.first), uniform(v.parts),    0};
 }
 
 // ---------------------------------------------------------------- stream --
@@ -470,7 +470,6 @@ __global__ void __launch_bounds__(4 * kWave) k_attn_stream(KvAttnArgs a) {
 //   V fragment (32 dims, 16 keys): lane l: keys 4 h + 0..3 and 8 + 4 h + 0..3, h = l / 32
 // The scores of a query stay in its two lanes, in the order in which the
 // second product wants the weights.
-//
 constexpr int kTileKeys = 64;
 
 __device__ __forceinline__ float max8(const float16_t& s, int at) {

@@ -108,7 +108,7 @@ void launch_kv_read(const KvReadArgs& a, bool bf16, hipStream_t s);
 //      KvSplit per tile.
 struct KvUnit {
   int32_t req, row, kv_begin, kv_end;
-  int32_t part, first, parts, split;  // this unit's partial (-1: none), the first of its rows', how many, which split
+  int32_t part, first, parts, pad;  // this unit's partial (-1: none), the first of its rows', how many
 };
 struct KvSplit {
   int32_t req, row, first, parts;

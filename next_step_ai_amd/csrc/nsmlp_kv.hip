@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(KvPlanArgs a) {
     if (q == 0) continue;
     const int len = base[r] >= 0 ? len_s[r] + q : 0;
     const int rows = min(q, a.row_limit) * a.group;
-    KvUnit u;
+    KvUnit u = {};
     u.req = r;
     if (rows <= kKvRowsA) {
       const int p0 = split[r], p1 = p0 + pieces_of(len), s0 = (int)((unsigned)p0 / (unsigned)share);
@@ -247,7 +247,6 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(KvPlanArgs a) {
         u.part = n > 1 ? partial[r] + i : -1;
         u.first = partial[r];
         u.parts = n;
-        u.split = partial[r];
         if (at < a.s.max_units_a && u.part < a.s.max_parts_a) units_a[at] = u;
         // every share starts with a unit of its own
         if (begin == (s0 + i) * share && s0 + i < a.s.shares) shares[s0 + i] = at;
@@ -267,9 +266,9 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(KvPlanArgs a) {
         u.part = n > 1 ? partial[r] + i : -1;
         u.first = partial[r] + nth * n;
         u.parts = n;
-        u.split = split[r] + nth;
+        const int join = split[r] + nth;
         if (first[r] + i < a.s.max_units_b && u.part < a.s.max_parts_b) units_b[first[r] + i] = u;
-        if (n > 1 && p == 0 && u.split < a.s.max_splits_b) splits_b[u.split] = KvSplit{r, u.row, u.first, n};
+        if (n > 1 && p == 0 && join < a.s.max_splits_b) splits_b[join] = KvSplit{r, u.row, u.first, n};
       }
     }
   }
@@ -279,41 +278,45 @@ constexpr int kPlanThreads = 1024;
 
 // Lengths, ring state and (for finished requests) the table after a step.  A
 // finished request's blocks return to the ring's end in the order of requests
-// and of their tables; one workgroup, as the order is a running sum.
+// and of their tables.  One workgroup, as lengths and state are read and
+// written in place; a running sum of the finished requests' blocks in LDS gives
+// every entry a thread of its own (with a thread per request the end of one of
+// 8192 blocks took 1100 us, now 10).
 __global__ void __launch_bounds__(kPlanThreads) k_kv_commit(KvCommitArgs a) {
   __shared__ int wsum[1][16];
+  __shared__ int before[kKvMaxRequests];  // entries of finished requests before this one
   const int tid = threadIdx.x;
   const int per = (a.R + kPlanThreads - 1) / kPlanThreads, r0 = tid * per;
   const unsigned N = (unsigned)a.num_blocks;
   const int* from = a.info != nullptr ? a.info : a.state;
   const int head = (int)((unsigned)from[0] % N), count = min(max(from[1], 0), a.num_blocks);
-  int mine[1] = {0}, total[1];
-  for (int i = 0; i < per; ++i) {
-    const int r = r0 + i;
-    if (r >= a.R) break;
-    const int len = a.next != nullptr ? a.next[r] : a.cached[r];
-    if (a.finished != nullptr && a.finished[r] != 0)
-      mine[0] += min((max(len, 0) + a.B - 1) >> a.b_shift, a.max_blocks);
-  }
-  block_scan<1, kPlanThreads>(mine, total, wsum, tid);
-  int at = mine[0];
-  for (int i = 0; i < per; ++i) {
-    const int r = r0 + i;
-    if (r >= a.R) break;
-    const int len = a.next != nullptr ? a.next[r] : a.cached[r];
-    if (a.finished != nullptr && a.finished[r] != 0) {
-      const int n = min((max(len, 0) + a.B - 1) >> a.b_shift, a.max_blocks);
-      for (int j = 0; j < n; ++j) {
-        // never more than the ring holds: a table with an id twice cannot push the ring past its size
-        if (count + at + j < a.num_blocks)
-          a.ring[((unsigned)head + (unsigned)(count + at + j)) % N] = a.table[(long long)r * a.max_blocks + j];
-        a.table[(long long)r * a.max_blocks + j] = -1;
-      }
-      at += n;
-      a.cached[r] = 0;
-    } else {
-      a.cached[r] = len;
+  const auto length = [&](int r) { return clip_len(a.next != nullptr ? a.next[r] : a.cached[r]); };
+  int mine[1] = {0}, total[1] = {0};
+  if (a.finished != nullptr) {
+    for (int i = 0; i < per && r0 + i < a.R; ++i) {
+      before[r0 + i] = mine[0];
+      if (a.finished[r0 + i] != 0) mine[0] += min((length(r0 + i) + a.B - 1) >> a.b_shift, a.max_blocks);
     }
+    block_scan<1, kPlanThreads>(mine, total, wsum, tid);
+    for (int i = 0; i < per && r0 + i < a.R; ++i) before[r0 + i] += mine[0];
+  }
+  __syncthreads();
+  for (int e = tid; e < total[0]; e += kPlanThreads) {
+    int lo = 0, hi = a.R;  // the last request with before <= e
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (before[mid] <= e) lo = mid;
+      else hi = mid;
+    }
+    int32_t* entry = a.table + (long long)lo * a.max_blocks + (e - before[lo]);
+    // never more than the ring holds: a table with an id twice cannot push the ring past its size
+    if (count + e < a.num_blocks) a.ring[((unsigned)head + (unsigned)(count + e)) % N] = *entry;
+    *entry = -1;
+  }
+  for (int i = 0; i < per && r0 + i < a.R; ++i) {
+    const int r = r0 + i;
+    if (a.finished != nullptr && a.finished[r] != 0) a.cached[r] = 0;
+    else if (a.next != nullptr) a.cached[r] = a.next[r];
   }
   if (tid == 0) {
     a.state[0] = head;
