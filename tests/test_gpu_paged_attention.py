@@ -281,3 +281,110 @@ def test_refusals(gpu):
     other = KvBatch(s.cache.num_blocks, 16, max_requests=1, max_blocks=4, q_heads=4, kv_heads=2)
     with pytest.raises(RuntimeError, match="another batch"):
         other.plan(torch.ones(1, dtype=torch.int32, device=gpu), 2, step=s.step)
+
+
+def check_wide(s, out, lse):
+    """`Served.check` with whole matrices, in 64 bits on the GPU."""
+    scale, G = s.D ** -0.5, s.q.shape[1] // s.plain.scale.shape[1]
+    u, t0 = (2.0 ** -11 if s.dtype == torch.float16 else 2.0 ** -8), 0
+    for r, (c, n) in enumerate(s.lengths):
+        k, v = (torch.from_numpy(s.plain.values(s.slots_of(r, c + n), w)).to(s.dev).double() for w in (0, 1))
+        hidden = torch.arange(c + n, device=s.dev)[None] > c + torch.arange(n, device=s.dev)[:, None]
+        most = float(v.abs().max())
+        for h in range(s.q.shape[1]):
+            kh, vh = k[:, h // G].contiguous(), v[:, h // G].contiguous()
+            e = (s.q[t0: t0 + n, h].double() @ kh.t().contiguous() * scale).masked_fill(hidden, -np.inf)
+            p = torch.softmax(e, 1)
+            want, wl, spread = p @ vh, torch.logsumexp(e, 1), p @ vh.abs()
+            got, gl = out[t0: t0 + n, h].double(), lse[t0: t0 + n, h].double()
+            bound = u * want.abs() + (2.0 ** -11 + 2.0 ** -15) * spread + (c + n) * 2.0 ** -25 * most + 2.0 ** -24
+            worst = ((got - want).abs() / bound).max().item()
+            assert worst <= 1.0, (r, h, worst)
+            assert ((gl - wl).abs() <= 2.0 ** -14 + 2.0 ** -20 * wl.abs()).all()
+        t0 += n
+
+
+@pytest.mark.parametrize("fmt,dtype,Hq,H,D,block,lengths", [
+    ("int8", torch.float16, 128, 128, 128, 16, [(1500, 700), (0, 333), (90, 1)]),
+    ("e4m3", torch.bfloat16, 128, 128, 128, 32, [(0, 257), (2301, 766), (7, 1), (1, 2)]),
+    ("e4m3", torch.float16, 256, 128, 64, 16, [(1100, 450), (5, 70)]),
+    ("int8", torch.bfloat16, 512, 512, 64, 64, [(100, 300)]),
+])
+def test_many_tokens_and_heads(gpu, fmt, dtype, Hq, H, D, block, lengths):
+    """Rows for two tiles of 256 per CU: more than 64 blocks of keys, ragged last tiles and rows, single tokens
+    next to them; then garbage past the ends, and a table entry that is no block."""
+    s = Served(gpu, lengths, Hq, H, D, block, fmt, dtype, seed=Hq + H + D)
+    out, lse = s.run()
+    check_wide(s, out, lse)
+    used = {x for r, (c, n) in enumerate(lengths) for x in s.slots_of(r, c + n)}
+    for x in set(range(s.cache.num_blocks * block)) - used:
+        tile = s.cache.data[x // block].view(H, 2, block // 16, 16 * D)[:, :, x % block // 16]
+        tile[:, 0].view(H, D // 16, 16, 16)[:, :, x % 16] = 0x7F
+        tile[:, 1].view(H, D // 64, 4, 64, 4)[:, :, x % 16 // 4, :, x % 4] = 0xFF
+    again, lse2 = s.run()
+    assert torch.equal(again, out) and torch.equal(lse2, lse)
+    # without its first block a request's rows see a cache whose first block is not there
+    s.batch.table[0, 0] = -1
+    got, _ = s.run()
+    first = lengths[0][1]
+    assert torch.equal(got[first:], out[first:])
+    c, n = lengths[0]
+    k, v = (torch.from_numpy(s.plain.values(s.slots_of(0, c + n)[block:], w)).to(gpu).double() for w in (0, 1))
+    for h in (0, Hq - 1):
+        kh, vh = k[:, h * H // Hq].contiguous(), v[:, h * H // Hq].contiguous()
+        want = torch.softmax(s.q[n - 1: n, h].double() @ kh.t().contiguous() * D ** -0.5, 1)
+        spread, want = want @ vh.abs(), want @ vh
+        u = 2.0 ** -11 if dtype == torch.float16 else 2.0 ** -8
+        bound = u * want.abs() + (2.0 ** -11 + 2.0 ** -15) * spread + (c + n) * 2.0 ** -25 * float(vh.abs().max()) + 2.0 ** -24
+        assert ((got[n - 1: n, h].double() - want).abs() <= bound).all()
+    from next_step_ai_amd._runtime import StatusWord, workspace
+
+    StatusWord(gpu, "paged attention").clear(workspace(1 << 20, gpu))
+
+
+def test_step_in_a_graph(gpu):
+    """plan, append, attention and commit captured once and replayed with other lengths, against the same steps
+    called one by one; eager work in between."""
+    from next_step_ai_amd.kv_cache import KvBatch, KvCache, paged_attention
+
+    R, total, Hq, H, D = 5, 24, 8, 2, 128
+    g = torch.Generator(device=gpu).manual_seed(5)
+
+    def fresh():
+        return KvBatch(60, 16, max_requests=R, max_blocks=12, q_heads=Hq, kv_heads=H, head_dim=D), KvCache(60, H, D, fmt="e4m3")
+
+    (b0, c0), (b1, c1) = fresh(), fresh()
+    new, ended = torch.zeros(R, dtype=torch.int32, device=gpu), torch.zeros(R, dtype=torch.int32, device=gpu)
+    k, v, q = (torch.zeros(total, h, D, dtype=torch.float16, device=gpu) for h in (H, H, Hq))
+    out = torch.zeros_like(q)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step = b1.plan(new, total)
+        paged_attention(q, c1, step, out=out)  # the stream's workspace
+        b1.commit()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        b1.plan(new, total, step=step)
+        c1.append(k, v, step.slots)
+        paged_attention(q, c1, step, out=out)
+        b1.commit(ended)
+    for lengths, end in (([10, 1, 0, 4, 9], []), ([1, 1, 1, 1, 1], [3]), ([3, 0, 17, 2, 2], []), ([1, 5, 1, 1, 16], [0, 2]),
+                         ([20, 1, 1, 1, 1], []), ([0, 0, 0, 0, 0], []), ([1, 1, 1, 1, 1], [])):
+        for t in (k, v, q):
+            t.normal_(generator=g)
+        new.copy_(torch.tensor(lengths, dtype=torch.int32))
+        ended.zero_()
+        for r in end:
+            ended[r] = 1
+        st = b0.plan(new, total)
+        c0.append(k, v, st.slots)
+        want = paged_attention(q, c0, st)
+        b0.commit(ended)
+        graph.replay()
+        torch.cuda.synchronize()
+        n = sum(lengths)
+        assert torch.equal(out[:n], want[:n])
+        assert torch.equal(c0.data, c1.data) and torch.equal(c0.scale, c1.scale)
+        assert torch.equal(b0.cached, b1.cached) and torch.equal(b0.state, b1.state) and torch.equal(b0.table, b1.table)
+        assert torch.equal(b0.ring, b1.ring)
