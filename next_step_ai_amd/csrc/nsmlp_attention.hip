@@ -847,58 +847,95 @@ __global__ void __launch_bounds__(NW* kWave, 2) k_attn_both(KvAttnArgs a, int bl
 }
 
 // ------------------------------------------------------------------ join --
-// One wave per row of list b whose keys were shared out: weights 2^(m_p - m)
-// in the order of the parts, eight parts' results in flight at a time.
+// Rows of list b whose keys were shared out: weights 2^(m_p - m), eight parts'
+// results in flight at a time.  Where there are many rows a wave has one;
+// where there are few, which then have many parts, a workgroup has one, every
+// wave takes a quarter of the parts, and their sums meet in LDS (24 rows of 43655
+// keys: the call 36 -> 31 us).
+template <int E>
+struct JoinSum {
+  float m, l, x, o[E];
+};
+
+template <int E>
+__device__ __forceinline__ JoinSum<E> join_parts(const KvAttnArgs& a, long long first, long long step, int begin, int end, int lane) {
+  JoinSum<E> s = {kLowest, 0.0f, 0.0f, {}};
+  for (int base = begin; base < end; base += 8) {
+    float4_t ml[8];
+    float y[8][E];
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      const long long at = first + min(base + p, end - 1) * step;  // (the last again: no branch between the reads)
+      ml[p] = *reinterpret_cast<const float4_t*>(a.ml_b + 4 * at);
+#pragma unroll
+      for (int e = 0; e < E; ++e) y[p][e] = a.acc_b[(at * kWave + lane) * E + e];
+    }
+    float top = s.m;
+#pragma unroll
+    for (int p = 0; p < 8; ++p) top = fmaxf(top, ml[p][0]);
+    const float old = exp2_fast(s.m - top);
+    s.m = top, s.l *= old, s.x *= old;
+#pragma unroll
+    for (int e = 0; e < E; ++e) s.o[e] *= old;
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      const float w = exp2_fast(ml[p][0] - s.m);
+      if (base + p < end) {
+        s.l += ml[p][1] * w, s.x += ml[p][2] * w;
+#pragma unroll
+        for (int e = 0; e < E; ++e) s.o[e] += y[p][e] * w;
+      }
+    }
+  }
+  return s;
+}
+
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(256) k_attn_join(KvAttnArgs a) {
   kernarg_warm<sizeof(KvAttnArgs)>();
   constexpr int E = D / kWave;
-  const int lane = threadIdx.x & (kWave - 1), wave = uniform(threadIdx.x >> 6), rows_b = a.s.rows_b;
+  __shared__ float part_o[4][D], part_m[4][3];
+  const int lane = threadIdx.x & (kWave - 1), wave = uniform(threadIdx.x >> 6), rows_b = a.s.rows_b, rows_j = a.s.join_rows;
   const KvSplit* splits = reinterpret_cast<const KvSplit*>(a.sched + a.s.off_splits_b);
-  const int items = min(a.sched[3], a.s.max_splits_b) * a.c.heads * rows_b;
-  for (int item = (int)blockIdx.x * 4 + wave; item < items; item += (int)gridDim.x * 4) {
-    const int r = item % rows_b, h = item / rows_b % a.c.heads;
-    const KvSplit sp = splits[item / rows_b / a.c.heads];
+  const int items = min(a.sched[3], a.s.max_splits_b) * a.c.heads * rows_j;
+  const bool wide = items <= 2 * (int)gridDim.x;
+  const int at_once = wide ? (int)gridDim.x : (int)gridDim.x * 4;
+  for (int item = wide ? (int)blockIdx.x : (int)blockIdx.x * 4 + wave; item < items; item += at_once) {
+    const int r = item % rows_j, h = item / rows_j % a.c.heads;
+    const KvSplit sp = splits[item / rows_j / a.c.heads];
     const int q0 = a.q_start[sp.req], rows = (a.q_start[sp.req + 1] - q0) * a.group;
+    const int full = sp.row + r, tok = q0 + full / a.group;
+    if (full >= rows || tok >= a.total) continue;  // (the same for all waves of a wide row)
     const long long first = ((long long)sp.first * a.c.heads + h) * rows_b + r, step = (long long)a.c.heads * rows_b;
-    float m = kLowest, l = 0.0f, x = 0.0f, o[E] = {};
-    for (int base = 0; base < sp.parts; base += 8) {
-      float4_t ml[8];
-      float y[8][E];
+    const int each = wide ? (sp.parts + 3) >> 2 : sp.parts, begin = wide ? min(wave * each, sp.parts) : 0;
+    JoinSum<E> s = join_parts<E>(a, first, step, begin, min(begin + each, sp.parts), lane);
+    if (wide) {
+      __syncthreads();  // (the row before has been read)
+      if (lane == 0) part_m[wave][0] = s.m, part_m[wave][1] = s.l, part_m[wave][2] = s.x;
 #pragma unroll
-      for (int p = 0; p < 8; ++p) {
-        const long long at = first + min(base + p, sp.parts - 1) * step;  // (the last again: no branch between the reads)
-        ml[p] = *reinterpret_cast<const float4_t*>(a.ml_b + 4 * at);
+      for (int e = 0; e < E; ++e) part_o[wave][lane * E + e] = s.o[e];
+      __syncthreads();
+      if (wave != 0) continue;
+      float top = kLowest;
 #pragma unroll
-        for (int e = 0; e < E; ++e) y[p][e] = a.acc_b[at * D + lane * E + e];
-      }
-      float top = m;
+      for (int w = 0; w < 4; ++w) top = fmaxf(top, part_m[w][0]);
+      s = {top, 0.0f, 0.0f, {}};
 #pragma unroll
-      for (int p = 0; p < 8; ++p) top = fmaxf(top, ml[p][0]);
-      const float old = exp2_fast(m - top);
-      m = top, l *= old, x *= old;
+      for (int w = 0; w < 4; ++w) {
+        const float f = exp2_fast(part_m[w][0] - top);
+        s.l += part_m[w][1] * f, s.x += part_m[w][2] * f;
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] *= old;
-#pragma unroll
-      for (int p = 0; p < 8; ++p) {
-        const float w = exp2_fast(ml[p][0] - m);
-        if (base + p < sp.parts) {
-          l += ml[p][1] * w, x += ml[p][2] * w;
-#pragma unroll
-          for (int e = 0; e < E; ++e) o[e] += y[p][e] * w;
-        }
+        for (int e = 0; e < E; ++e) s.o[e] += part_o[w][lane * E + e] * f;
       }
     }
-    const int full = sp.row + r, tok = q0 + full / a.group;
-    if (full >= rows || tok >= a.total) continue;  // (rows that the tile does not have are read, and dropped)
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float inv = s.l == 0.0f ? 0.0f : 1.0f / s.l;
     const long long at = (long long)tok * a.c.heads * a.group + h * a.group + full % a.group;
     if constexpr (E == 2)
       *reinterpret_cast<uint32_t*>(a.out + at * D + lane * 2) =
-          to_out<kBf16>(o[0] * inv) | (uint32_t)to_out<kBf16>(o[1] * inv) << 16;
+          to_out<kBf16>(s.o[0] * inv) | (uint32_t)to_out<kBf16>(s.o[1] * inv) << 16;
     else
-      a.out[at * D + lane] = to_out<kBf16>(o[0] * inv);
-    if (a.lse != nullptr && lane == 0) a.lse[at] = x == 0.0f ? -INFINITY : (m + log2f(x)) * 0.6931471805599453f;
+      a.out[at * D + lane] = to_out<kBf16>(s.o[0] * inv);
+    if (a.lse != nullptr && lane == 0) a.lse[at] = s.x == 0.0f ? -INFINITY : (s.m + log2f(s.x)) * 0.6931471805599453f;
   }
 }
 
@@ -925,7 +962,7 @@ void attention_typed(const KvAttnArgs& a, hipStream_t s) {
   if (a.s.rows_b == 256) lse ? launch_both<D, kFmt, kBf16, 8, true>(a, stream_blocks, s) : launch_both<D, kFmt, kBf16, 8, false>(a, stream_blocks, s);
   else lse ? launch_both<D, kFmt, kBf16, 4, true>(a, stream_blocks, s) : launch_both<D, kFmt, kBf16, 4, false>(a, stream_blocks, s);
   if (a.s.max_splits_b > 0) {
-    const long long waves = (long long)a.s.max_splits_b * a.c.heads * a.s.rows_b;
+    const long long waves = (long long)a.s.max_splits_b * a.c.heads * a.s.join_rows;
     k_attn_join<D, kBf16><<<dim3((unsigned)min((waves + 3) / 4, 2048LL)), dim3(256), 0, s>>>(a);
   }
 }

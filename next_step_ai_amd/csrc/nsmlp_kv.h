@@ -103,12 +103,12 @@ void launch_kv_read(const KvReadArgs& a, bool bf16, hipStream_t s);
 //      these requests' keys, one after the other in pieces of 64, are cut into
 //      equal shares, one per workgroup and K/V head; a unit is what a share
 //      holds of a request.  A request's units meet in the last to end.
-//   b  the others, in tiles of `rows_b` rows, their keys cut into equal parts
-//      where there are few tiles; parts are joined by a second launch, one
-//      KvSplit per tile.
+//   b  the others, in tiles of `rows_b` rows.  Where there are few tiles, a
+//      tile's keys are cut into parts, which a second launch joins, one KvSplit
+//      per tile.
 struct KvUnit {
   int32_t req, row, kv_begin, kv_end;
-  int32_t part, first, parts, pad;  // this unit's partial (-1: none), the first of its rows', how many
+  int32_t part, first, parts, pad;  // this unit's partial (-1: none); list a: the first of its rows', how many
 };
 struct KvSplit {
   int32_t req, row, first, parts;
@@ -124,9 +124,9 @@ static_assert(4 * kKvCounters <= kMaxK && 2 * (512 + 1024) <= kKvCounters, "the 
 constexpr int kKvHeaderInts = 16;  // units a, shares, units b, splits b
 
 struct KvSchedule {  // sizes, from the host's knowledge of a step (kv_schedule)
-  int rows_b;                        // rows of a tile of list b
+  int rows_b, join_rows;             // rows of a tile of list b, and how many of them a request can fill
   int shares;                        // of list a's keys, at most
-  int target_b;                      // units wanted per K/V head (0: never split)
+  int target_b;                      // CUs per K/V head that list b's keys are shared out to (0: they are not)
   int max_units_a, max_units_b;      // list capacities
   int max_parts_a, max_parts_b, max_splits_b;
   bool list_b;                       // whether a request can be long enough for list b

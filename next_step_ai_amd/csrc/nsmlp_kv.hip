@@ -65,15 +65,40 @@ __device__ __forceinline__ int clip_len(int v) { return min(max(v, 0), 1 << 29);
 // list a counts keys in pieces of 64; a request without any takes one piece,
 // so that its rows are somebody's
 constexpr int kLeastShare = 4;     // pieces: 256 keys are worth a workgroup
-constexpr int kLeastPart = 1024;   // keys of list b that are worth a join
+// Keys per part of list b, L.  A part costs its rows' fp32 sums written and read
+// back, about what kPartCost keys' products cost where the tile is full of rows.
+// With w keys of work per CU in all, the CUs take w (1 + cost / L) and the longest
+// part L; the two meet at `meet`.  Tiles with few rows are those of many short
+// requests: their parts cost little, and as nobody sorts them by length, the
+// last to end is what a smaller L shortens: w cost / L + L / 4 is least at `even`.
+// List a's keys count half, as the parts run next to them on the same CUs (a
+// prompt's 387 tokens next to 20 decodes: 37 us without, 31 with).
+// (Against equal parts of 1024 keys or more for all tiles of a request, over 150
+// drawn prompts, drafts and mixed steps: those above 18 us 37 -> 33 us on
+// average; a prompt of 1148 tokens and 40 heads 77 -> 41 us, 6 drafts of 44
+// uneven requests 111 -> 98 us.  Costs of 128 and 512 were up to 3% slower.)
+constexpr float kPartCost = 256.0f, kLeastPart = 192.0f;
 
-// keys per part, so that about `target` units share the list's `work` keys
-__device__ __forceinline__ int part_keys(long long work, int target) {
-  if (target <= 0) return 1 << 30;  // more than any request's
-  const double each = ceil((double)work / target);  // exact: below 2^53, and a quotient's ceiling does not round down
-  const double up = ceil(each * (1.0 / 128)) * 128;
-  return up < kLeastPart ? kLeastPart : up > (double)(1 << 30) ? 1 << 30 : (int)up;
+// 1 / L of a request with `rows` rows in `tiles` tiles
+__device__ __forceinline__ float parts_per_key(float w, int rows, int tiles, int rows_b) {
+  const float fill = (float)rows / (float)(tiles * rows_b), cost = kPartCost * fill;
+  const float meet = 0.5f * (w + sqrtf(w * (w + 4.0f * cost)));
+  const float even = 2.0f * sqrtf(w * cost) / fmaxf(1.0f - fill, 1e-3f);
+  return 1.0f / fmaxf(fmaxf(0.5f * w, kLeastPart), fminf(meet, even));
 }
+
+// keys that the last row of a tile of list b sees, of a request with q new tokens and len keys
+__device__ __forceinline__ int tile_keys(int tile, int q, int len, int rows_b, int group) {
+  const int last = min(q, (int)(((unsigned)(tile + 1) * (unsigned)rows_b + group - 1) / (unsigned)group));
+  return max(0, len - q + last);
+}
+// and the sum of that over the request's tiles, or a little more
+__device__ __forceinline__ long long work_of(int tiles, int q, int len, int rows_b, int group) {
+  if (len <= 0) return 0;
+  return (long long)tiles * (len - q) + (long long)(tiles - 1) * tiles / 2 * rows_b / group + tiles + q;
+}
+// parts of a tile: 1 below 1.35 L keys, at most 1.5 keys / L else
+__device__ __forceinline__ int parts_of(int seen, float per_key) { return max(1, (int)((float)seen * per_key + 0.65f)); }
 
 __device__ __forceinline__ int pieces_of(int keys) { return max(1, (keys + 63) >> 6); }
 
@@ -143,7 +168,7 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(KvPlanArgs a) {
     const int rows = min(fresh[i], a.row_limit) * a.group;
     const bool b = rows > kKvRowsA;
     tiles[i] = b ? (rows + a.s.rows_b - 1) / a.s.rows_b : rows > 0 ? -1 : 0;
-    if (b) work += (long long)kv[i] * tiles[i];
+    if (b) work += work_of(tiles[i], fresh[i], kv[i], a.s.rows_b, a.group);
     else if (rows > 0) sums[0] += pieces_of(kv[i]);
   }
   sums[1] = (int)(work & 0xFFFFF), sums[2] = (int)((work >> 20) & 0xFFFFF), sums[3] = (int)(work >> 40);
@@ -151,9 +176,10 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(KvPlanArgs a) {
   work = sums_total[1] + ((long long)sums_total[2] << 20) + ((long long)sums_total[3] << 40);
   const int refused = sums_total[4];
   const int share = max(kLeastShare, (sums_total[0] + a.s.shares - 1) / a.s.shares);  // pieces
-  const int keys_b = part_keys(work, a.s.target_b);
+  // keys of work per CU: list b's tiles times keys, and half of list a's keys
+  const float cu_keys = (float)(work + 32LL * sums_total[0]) / (float)max(a.s.target_b, 1);
   // units of each request: the shares that its pieces touch, or tiles of rows times parts of its keys
-  int parts[kPer], piece0[kPer];
+  int parts[kPer], split_tiles[kPer] = {}, split_parts[kPer] = {}, piece0[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     piece0[i] = sums[0];
@@ -164,10 +190,16 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(KvPlanArgs a) {
       cnt[0] += parts[i];
       cnt[3] += parts[i] > 1 ? parts[i] : 0;
     } else {
-      parts[i] = max(1, (int)(((unsigned)kv[i] + (unsigned)keys_b - 1) / (unsigned)keys_b));
-      cnt[1] += tiles[i] * parts[i];
-      cnt[2] += parts[i] > 1 ? tiles[i] : 0;
-      cnt[4] += parts[i] > 1 ? tiles[i] * parts[i] : 0;
+      if (a.s.target_b > 0 && tiles[i] > 0) {  // (there are fewer than 384 tiles then)
+        const float per_key = parts_per_key(cu_keys, min(fresh[i], a.row_limit) * a.group, tiles[i], a.s.rows_b);
+        for (int t = tiles[i] - 1; t >= 0; --t) {
+          const int n = parts_of(tile_keys(t, fresh[i], kv[i], a.s.rows_b, a.group), per_key);
+          if (n == 1) break;  // nor has a tile before it more
+          ++split_tiles[i], split_parts[i] += n;
+        }
+      }
+      parts[i] = tiles[i] - split_tiles[i] + split_parts[i];
+      cnt[1] += parts[i], cnt[2] += split_tiles[i], cnt[4] += split_parts[i];
     }
   }
   int cnt_total[kPlanSums];
@@ -182,8 +214,7 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(KvPlanArgs a) {
       if (parts[i] > 1) cnt[3] += parts[i];
     } else {
       first[r] = cnt[1], split[r] = cnt[2], partial[r] = cnt[4];
-      cnt[1] += tiles[i] * parts[i];
-      if (parts[i] > 1) cnt[2] += tiles[i], cnt[4] += tiles[i] * parts[i];
+      cnt[1] += parts[i], cnt[2] += split_tiles[i], cnt[4] += split_parts[i];
     }
   }
   if (tid == 0) q_start[a.R] = total[0];
@@ -252,23 +283,39 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(KvPlanArgs a) {
         if (begin == (s0 + i) * share && s0 + i < a.s.shares) shares[s0 + i] = at;
       }
     } else {
+      // a lane per tile; the last tile sees the most keys: it goes first
       const int tiles_r = (rows + a.s.rows_b - 1) / a.s.rows_b;
-      const int n = max(1, (int)(((unsigned)len + (unsigned)keys_b - 1) / (unsigned)keys_b));
-      for (int i = lane; i < tiles_r * n; i += kWave) {
-        // the last tile sees the most keys: it goes first
-        const int nth = n == 1 ? i : (int)((unsigned)i / (unsigned)n), p = i - nth * n, tile = tiles_r - 1 - nth;
-        const int last = min(q, (int)(((unsigned)(tile + 1) * (unsigned)a.s.rows_b + a.group - 1) / (unsigned)a.group));
-        const int seen = max(0, len - q + last);  // keys that the tile's last row sees
-        const int each = n == 1 ? seen : ((int)((unsigned)(seen + n - 1) / (unsigned)n) + 63) & ~63;
+      int at = first[r], part = partial[r], join = split[r];
+      if (a.s.target_b == 0) {  // no tile is split
+        u.part = -1;
+        for (int i = lane; i < tiles_r; i += kWave) {
+          const int tile = tiles_r - 1 - i;
+          u.row = tile * a.s.rows_b;
+          u.kv_end = tile_keys(tile, q, len, a.s.rows_b, a.group);
+          if (at + i < a.s.max_units_b) units_b[at + i] = u;
+        }
+        continue;
+      }
+      const float per_key = parts_per_key(cu_keys, rows, tiles_r, a.s.rows_b);
+      for (int i0 = 0; i0 < tiles_r; i0 += kWave) {
+        const int tile = tiles_r - 1 - i0 - lane;
+        const int seen = tile >= 0 ? tile_keys(tile, q, len, a.s.rows_b, a.group) : 0;
+        const int n = tile < 0 ? 0 : parts_of(seen, per_key), m = n > 1 ? n : 0;
+        const int n_sum = wave_scan(n), m_sum = wave_scan(m);
+        const unsigned long long splits = __ballot(m > 0);
+        const int my_at = at + n_sum - n, my_part = part + m_sum - m;
+        const int each = n <= 1 ? seen : ((int)((unsigned)(seen + n - 1) / (unsigned)n) + 63) & ~63;
         u.row = tile * a.s.rows_b;
-        u.kv_begin = min(p * each, seen);
-        u.kv_end = min((p + 1) * each, seen);
-        u.part = n > 1 ? partial[r] + i : -1;
-        u.first = partial[r] + nth * n;
-        u.parts = n;
-        const int join = split[r] + nth;
-        if (first[r] + i < a.s.max_units_b && u.part < a.s.max_parts_b) units_b[first[r] + i] = u;
-        if (n > 1 && p == 0 && join < a.s.max_splits_b) splits_b[join] = KvSplit{r, u.row, u.first, n};
+        for (int p = 0; p < n; ++p) {
+          u.kv_begin = min(p * each, seen);
+          u.kv_end = min((p + 1) * each, seen);
+          u.part = n > 1 ? my_part + p : -1;
+          if (my_at + p < a.s.max_units_b && u.part < a.s.max_parts_b) units_b[my_at + p] = u;
+        }
+        const int my_join = join + __popcll(splits & ((1ull << lane) - 1));
+        if (m > 0 && my_join < a.s.max_splits_b) splits_b[my_join] = KvSplit{r, u.row, my_part, n};
+        at += __builtin_amdgcn_readlane(n_sum, kWave - 1), part += __builtin_amdgcn_readlane(m_sum, kWave - 1);
+        join += __popcll(splits);
       }
     }
   }
@@ -606,7 +653,6 @@ void launch_kv_read(const KvReadArgs& a, bool bf16, hipStream_t s) { NSMLP_KV_BY
 
 KvSchedule kv_schedule(int requests, int total, int max_new, int group, int kv_heads) {
   KvSchedule s;
-  s.list_b = (long long)(max_new < total ? max_new : total) * group > kKvRowsA;
   // list a: one workgroup of 4 waves per CU has as many reads in flight as the
   // memory takes (two: 131000 keys 50 -> 55 us, for the joins)
   s.shares = (256 + kv_heads - 1) / kv_heads;
@@ -614,17 +660,21 @@ KvSchedule kv_schedule(int requests, int total, int max_new, int group, int kv_h
   // (chunk of 2048 over 14336, 128 heads: 1.84 ms, with 128 rows 1.92), else 128
   const long long rows = (long long)total * group;
   s.rows_b = rows / 256 * kv_heads >= 512 ? 256 : 128;
+  const long long most = (long long)(max_new < total ? max_new : total) * group;
+  s.list_b = most > kKvRowsA;
+  s.join_rows = most < s.rows_b ? (int)most : s.rows_b;
   const long long tiles_b = s.list_b ? (rows + s.rows_b - 1) / s.rows_b + requests : 0;
-  s.target_b = !s.list_b || tiles_b * kv_heads >= 512 ? 0 : (512 + kv_heads - 1) / kv_heads;
+  // its keys are shared out where the tiles do not make one and a half for every CU
+  s.target_b = !s.list_b || tiles_b * kv_heads >= 384 ? 0 : (256 + kv_heads - 1) / kv_heads;
   // list a: every share ends at most one unit that its request does not end,
   // so units are at most requests + shares, and those of a request with several
   // units at most twice the shares
   s.max_units_a = requests + s.shares;
   s.max_parts_a = 2 * s.shares;
-  // list b: parts > 1 only where a request's keys exceed a part, so split units
-  // are at most twice the work over the keys of a part, and split tiles at most it
-  s.max_parts_b = 2 * s.target_b;
-  s.max_splits_b = s.target_b;
+  // list b: a tile has two parts or more only past 1.35 L keys, and L is at least
+  // half the work over the target: split tiles are below 1.5 targets, their parts below 3
+  s.max_parts_b = 3 * s.target_b;
+  s.max_splits_b = 2 * s.target_b;
   s.max_units_b = (int)tiles_b + s.max_parts_b;
   const long long unit = sizeof(KvUnit) / 4, split = sizeof(KvSplit) / 4;
   s.off_shares = kKvHeaderInts;

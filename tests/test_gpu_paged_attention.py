@@ -388,3 +388,19 @@ def test_step_in_a_graph(gpu):
         assert torch.equal(c0.data, c1.data) and torch.equal(c0.scale, c1.scale)
         assert torch.equal(b0.cached, b1.cached) and torch.equal(b0.state, b1.state) and torch.equal(b0.table, b1.table)
         assert torch.equal(b0.ring, b1.ring)
+
+
+@pytest.mark.parametrize("fmt,dtype,Hq,H,D,block,lengths", [
+    ("e4m3", torch.float16, 8, 8, 128, 16, [(4, 1100)]),
+    ("int8", torch.bfloat16, 3, 1, 128, 32, [(0, 1500)]),
+    ("int8", torch.float16, 12, 4, 64, 16, [(2019, 37), (900, 1), (1300, 180)]),
+    ("e4m3", torch.bfloat16, 15, 5, 128, 64, [(37 * (i * i % 83), 6) for i in range(20)]),
+    ("int8", torch.float16, 4, 1, 128, 16, [(9001, 6), (5, 6), (2500, 6)]),
+])
+def test_parts_of_few_tiles(gpu, fmt, dtype, Hq, H, D, block, lengths):
+    """Tiles of one request with different numbers of parts, many rows and few, one tile with dozens of parts."""
+    s = Served(gpu, lengths, Hq, H, D, block, fmt, dtype, seed=Hq * len(lengths))
+    check_wide(s, *s.run())
+    again = s.run()
+    for x, y in zip(s.run(), again):
+        assert torch.equal(x, y)
