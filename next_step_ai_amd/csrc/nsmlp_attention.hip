@@ -113,7 +113,16 @@ __device__ __forceinline__ KvUnit load_unit(const KvUnit* p) {
 // ---------------------------------------------------------------- stream --
 // Up to 16 query rows against a range of keys.  The workgroup's waves share a
 // unit's keys out and their results meet in LDS; products with the keys (or
-// dims) as rows and the queries as columns.
+// dims) as rows and the queries as columns, so that a column's weights leave the
+// first product where the second wants them.
+//
+// What bounds it: the codes' way from HBM, read once.  All K/V heads' requests
+// together are cut into one equal share per CU, so that uneven lengths cost
+// nothing, and a wave has the next 32 keys' codes in flight while it works on
+// 32: 64 uneven requests (429 MB) 81 us, 5.3 TB/s; one token over 131000 keys
+// (269 MB, 31 partial results per row to join) 57 us, 4.7 TB/s.  A short chat (777
+// keys) takes 9.5 us, most of it the chain launch, schedule, lengths, block
+// table, scales, codes, join.
 template <int D, int NW>
 struct StreamLds {
   float sum[NW][16][D + 4];  // the waves' results
@@ -238,6 +247,7 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
       for (int s = 0; s < 2; ++s)
         sc[s] = mfma16(join4(kv_half4<kFmt>(word(t.k[s][i >> 1], 2 * (i & 1))), kv_half4<kFmt>(word(t.k[s][i >> 1], 2 * (i & 1) + 1))),
                        q[i], sc[s]);
+    mfma_drain();
     // bit 4 s + i: whether the row sees the lane's key i of the s-th 16
     uint32_t see = 0xFF;
     if constexpr (kMasked) {
@@ -334,6 +344,7 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
   }
   if (bad_seen != 0 && lane == 0) atomicOr(a.status, NSMLP_STATUS_BLOCK_UNAVAILABLE);
 
+  mfma_drain();
   if constexpr (kSplit) x = l;
   // join the waves: each result under the largest reference
   l += __shfl_xor(l, 16, kWave), x += __shfl_xor(x, 16, kWave);
@@ -470,6 +481,15 @@ __global__ void __launch_bounds__(4 * kWave) k_attn_stream(KvAttnArgs a) {
 //   V fragment (32 dims, 16 keys): lane l: keys 4 h + 0..3 and 8 + 4 h + 0..3, h = l / 32
 // The scores of a query stay in its two lanes, in the order in which the
 // second product wants the weights.
+//
+// What bounds it: the matrix cores, and the vector work that does not hide
+// behind them (an exp2, a multiply-add and a conversion per weight, and the
+// decoding, shared by 128 or 256 rows).  A product follows another after about
+// 47 cycles instead of 32, half of a step with 8 waves is the wave's own vector
+// half, in which the SIMD's other wave has its products: 2048 tokens over 14336
+// cached, 128 heads of 128, 1.98 ms, 1.04 PFLOP/s, matrix cores busy 54%; a
+// prompt of 4000 tokens and 32 heads 165-180 us (0.73-0.79 PFLOP/s: 1000 tiles
+// of uneven length on 512 places).
 constexpr int kTileKeys = 64;
 
 __device__ __forceinline__ float max8(const float16_t& s, int at) {
@@ -664,7 +684,7 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
       }
       side(k);
     }
-    sched_fence();
+    mfma_drain();
   };
   // Vector half: the weights of the scores.
   TileMeta meta[4];

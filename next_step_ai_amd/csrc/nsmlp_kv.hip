@@ -17,7 +17,8 @@ namespace {
 // (no slots, kv_len 0, lengths unchanged) where its blocks exceed the table's
 // width or the running sum the free count.
 //
-// What bounds it: latency.  8 requests write 224 bytes, 4096 requests 0.7 MB; a
+// What bounds it: latency (8 requests 6.5 us, 300 with 6513 tokens 11 us, 4096
+// with 73470 tokens 17 us).  8 requests write 224 bytes, 4096 requests 0.7 MB; a
 // step is a chain of one load of the lengths, two scans, one load of the
 // ring's entries and the stores.  Sums within a wave go through DPP adds (a
 // few cycles each; exchanges through LDS took most of the time before), the
@@ -79,8 +80,10 @@ constexpr int kLeastShare = 4;     // pieces: 256 keys are worth a workgroup
 // uneven requests 111 -> 98 us.  Costs of 128 and 512 were up to 3% slower.)
 constexpr float kPartCost = 256.0f, kLeastPart = 192.0f;
 
-// 1 / L of a request with `rows` rows in `tiles` tiles
+// 1 / L of a request with `rows` rows in `tiles` tiles.  (Parts are counted in
+// one place and listed in another: no contraction, so that both get the same.)
 __device__ __forceinline__ float parts_per_key(float w, int rows, int tiles, int rows_b) {
+#pragma clang fp contract(off)
   const float fill = (float)rows / (float)(tiles * rows_b), cost = kPartCost * fill;
   const float meet = 0.5f * (w + sqrtf(w * (w + 4.0f * cost)));
   const float even = 2.0f * sqrtf(w * cost) / fmaxf(1.0f - fill, 1e-3f);
@@ -98,7 +101,10 @@ __device__ __forceinline__ long long work_of(int tiles, int q, int len, int rows
   return (long long)tiles * (len - q) + (long long)(tiles - 1) * tiles / 2 * rows_b / group + tiles + q;
 }
 // parts of a tile: 1 below 1.35 L keys, at most 1.5 keys / L else
-__device__ __forceinline__ int parts_of(int seen, float per_key) { return max(1, (int)((float)seen * per_key + 0.65f)); }
+__device__ __forceinline__ int parts_of(int seen, float per_key) {
+#pragma clang fp contract(off)
+  return max(1, (int)((float)seen * per_key + 0.65f));
+}
 
 __device__ __forceinline__ int pieces_of(int keys) { return max(1, (keys + 63) >> 6); }
 
@@ -381,6 +387,10 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_commit(KvCommitArgs a) {
 // K: a lane holds 16 dims of a token (16 code bytes).  V: a lane holds 4 dims
 // of 4 tokens, which is how V's codes lie; the wave owns the block's V, so
 // bytes of other tokens in a piece of 16 are read and written back.
+//
+// What bounds it: memory latency.  A run is slots, rows, scale, codes one after
+// the other: 64 single tokens of 8 heads 4.1 us, next to an empty launch's 2.4;
+// 11420 tokens of prompts (70 MB) 21 us, 3.3 TB/s.
 constexpr int kAppendThreads = 256;
 
 template <bool kBf16>
@@ -578,7 +588,8 @@ __global__ void __launch_bounds__(kAppendThreads, B == 64 ? 2 : 4) k_kv_append(K
 // ------------------------------------------------------------------ read --
 // One thread per 16 dims of a (slot, head): values code * scale, rounded once.
 // The token's V bytes lie one in each dword of 4 pieces of 16; the threads of
-// the group's other tokens find the same pieces in the caches.
+// the group's other tokens find the same pieces in the caches.  11532 tokens of
+// 8 heads (71 MB) 17-18 us, 4 TB/s, three quarters of what a copy reaches.
 template <bool kBf16>
 __device__ __forceinline__ uint32_t pack_out(float a, float b) {
   if constexpr (kBf16) return __builtin_bit_cast(uint16_t, (__bf16)a) | (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)b) << 16;
