@@ -116,13 +116,15 @@ class KvCache:
 class _StepLayout:
     """Sizes of a step's buffers, which depend on its total and max_new alone."""
 
-    __slots__ = ("ints", "schedule_bytes", "ws_bytes")
+    __slots__ = ("ints", "sizes", "schedule_bytes", "ws_bytes")
 
     def __init__(self, batch: "KvBatch", total: int, max_new: int):
         self.schedule_bytes = int(_lib.lib().nsmlp_kv_schedule_bytes(batch._ref, total, max_new))
         if self.schedule_bytes == 0:
             raise RuntimeError(f"nsmlp_kv_schedule_bytes: {_lib.last_error()}")
-        self.ints = (3 * batch.requests + 5 + 3) // 4 * 4
+        R = batch.requests
+        self.ints = (3 * R + 5 + 3) // 4 * 4
+        self.sizes = [R + 1, R, R, 4, self.ints - 3 * R - 5 + self.schedule_bytes // 4]
         self.ws_bytes: dict[int, int] = {}
 
 
@@ -133,7 +135,7 @@ class KvStep:
     block table.  ``info`` and the others are device tensors: reading them
     waits for the stream."""
 
-    __slots__ = ("batch", "total", "max_new", "slots", "_buf", "_layout", "_view", "_ref")
+    __slots__ = ("batch", "total", "max_new", "slots", "_buf", "_layout", "_view", "_ref", "_split")
 
     def __init__(self, batch: "KvBatch", total: int, max_new: int):
         lay = batch._layout(total, max_new)
@@ -145,18 +147,24 @@ class KvStep:
         self._view = _lib.KvStepView(total, max_new, self.slots.data_ptr(), base, base + 4 * (R + 1), base + 4 * (2 * R + 1),
                                      base + 4 * (3 * R + 1), base + 4 * lay.ints, lay.schedule_bytes)
         self._ref = ctypes.byref(self._view)
+        self._split = None
+
+    def _part(self, i: int) -> torch.Tensor:
+        if self._split is None:  # one split takes half as long as three views
+            self._split = self._buf.split_with_sizes(self._layout.sizes)
+        return self._split[i]
 
     @property
     def q_start(self) -> torch.Tensor:
-        return self._buf.narrow(0, 0, self.batch.requests + 1)
+        return self._part(0)
 
     @property
     def kv_len(self) -> torch.Tensor:
-        return self._buf.narrow(0, self.batch.requests + 1, self.batch.requests)
+        return self._part(1)
 
     @property
     def info(self) -> torch.Tensor:
-        return self._buf.narrow(0, 3 * self.batch.requests + 1, 4)
+        return self._part(3)
 
     @property
     def table(self) -> torch.Tensor:
