@@ -17,8 +17,8 @@ namespace {
 // (no slots, kv_len 0, lengths unchanged) where its blocks exceed the table's
 // width or the running sum the free count.
 //
-// What bounds it: latency (8 requests 6.5 us, 300 with 6513 tokens 11 us, 4096
-// with 73470 tokens 17 us).  8 requests write 224 bytes, 4096 requests 0.7 MB; a
+// What bounds it: latency (8 requests 6.5 us, 300 with 6513 tokens 10 us, 4096
+// with 73470 tokens 14 us).  8 requests write 224 bytes, 4096 requests 0.7 MB; a
 // step is a chain of one load of the lengths, two scans, one load of the
 // ring's entries and the stores.  Sums within a wave go through DPP adds (a
 // few cycles each; exchanges through LDS took most of the time before), the
@@ -704,8 +704,9 @@ static void launch_plan(const KvPlanArgs& a, hipStream_t s) {
     (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k_kv_plan<kThreads, kPer>),
                               hipFuncAttributeMaxDynamicSharedMemorySize, kMost);
   });
-  // two tokens per thread, and at most 128 workgroups scan the lengths
-  const int groups = min(max((a.total + 2 * kThreads - 1) / (2 * kThreads), (a.R + 63) / 64), 128);
+  // two tokens per thread and 16 requests' lists per workgroup, but one workgroup per
+  // CU at most (64 requests' lists and 128 workgroups: 4096 requests 17 us, now 14)
+  const int groups = min(max((a.total + 2 * kThreads - 1) / (2 * kThreads), (a.R + 15) / 16), 256);
   k_kv_plan<kThreads, kPer><<<dim3(max(groups, 1)), dim3(kThreads), (6 * a.R + 1) * sizeof(int), s>>>(a);
 }
 
