@@ -102,6 +102,10 @@ __device__ __forceinline__ float lane_of(float v, int i) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i));
 }
 
+// Whether token i of the step is there.  (Lengths whose sum passes 32 bits leave
+// requests' first tokens below zero.)
+__device__ __forceinline__ bool in_step(const KvAttnArgs& a, int i) { return (unsigned)i < (unsigned)a.total; }
+
 // A unit in scalar registers (left in memory it would be read again after
 // every barrier).
 __device__ __forceinline__ KvUnit load_unit(const KvUnit* p) {
@@ -205,7 +209,7 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
   half8_t q[KS];
   float rowf = a.scale_log2;
   const int tok = col / a.group;
-  const bool in = col < rows && q0 + tok < a.total;
+  const bool in = col < rows && in_step(a, q0 + tok);
   const int limit = in ? kv_len - q_len + tok + 1 : 0x7FFFFFFF;  // keys that the row sees
   {
     const uint16_t* src = a.q + (long long)(q0 + tok) * a.q_row + (long long)(h * a.group + col % a.group) * a.q_head;
@@ -435,7 +439,7 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
   }
   if (row < rows) {
     const int tok_r = q0 + row / a.group, head = h * a.group + row % a.group;
-    if (tok_r < a.total) {
+    if (in_step(a, tok_r)) {
       const float inv = lr == 0.0f ? 0.0f : 1.0f / lr;
       const long long at = (long long)tok_r * a.c.heads * a.group + head;
 #pragma unroll
@@ -516,7 +520,7 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
   const int q0 = uniform(a.q_start[u.req]), q_len = uniform(a.q_start[u.req + 1]) - q0, kv_len = uniform(a.kv_len[u.req]);
   const int rows = min(q_len * a.group - u.row, kRows);
   const int r = wave * 32 + col, row = u.row + r, tok = row / a.group;
-  const bool in = r < rows && q0 + tok < a.total;
+  const bool in = r < rows && in_step(a, q0 + tok);
   const int limit = in ? kv_len - q_len + tok + 1 : 0x7FFFFFFF;  // keys that the row sees
   const int last = max(0, (u.kv_end - 1) >> a.c.b_shift);
   const int tiles = (u.kv_end - u.kv_begin + kTileKeys - 1) / kTileKeys;
@@ -925,7 +929,7 @@ __global__ void __launch_bounds__(256) k_attn_join(KvAttnArgs a) {
     const KvSplit sp = splits[item / rows_j / a.c.heads];
     const int q0 = a.q_start[sp.req], rows = (a.q_start[sp.req + 1] - q0) * a.group;
     const int full = sp.row + r, tok = q0 + full / a.group;
-    if (full >= rows || tok >= a.total) continue;  // (the same for all waves of a wide row)
+    if (full >= rows || !in_step(a, tok)) continue;  // (the same for all waves of a wide row)
     const long long first = ((long long)sp.first * a.c.heads + h) * rows_b + r, step = (long long)a.c.heads * rows_b;
     const int each = wide ? (sp.parts + 3) >> 2 : sp.parts, begin = wide ? min(wave * each, sp.parts) : 0;
     JoinSum<E> s = join_parts<E>(a, first, step, begin, min(begin + each, sp.parts), lane);

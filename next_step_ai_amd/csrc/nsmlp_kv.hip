@@ -245,7 +245,9 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(KvPlanArgs a) {
       else hi = mid;
     }
     long long slot = -1;
-    if (t < q_start[a.R] && base[lo] >= 0) {
+    // (lengths whose sum passes 32 bits leave q_start out of order: a token has a
+    // slot only inside its request, whose blocks the table holds)
+    if (t < q_start[a.R] && base[lo] >= 0 && (unsigned)t - (unsigned)q_start[lo] < (unsigned)q_start[lo + 1] - (unsigned)q_start[lo]) {
       const int c = len_s[lo];
       const int have = (c + a.B - 1) >> a.b_shift, p = c + t - q_start[lo], j = p >> a.b_shift;
       int32_t* entry = a.table + (long long)lo * a.max_blocks + j;
@@ -284,7 +286,7 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(KvPlanArgs a) {
         u.part = n > 1 ? partial[r] + i : -1;
         u.first = partial[r];
         u.parts = n;
-        if (at < a.s.max_units_a && u.part < a.s.max_parts_a) units_a[at] = u;
+        if ((unsigned)at < (unsigned)a.s.max_units_a && u.part < a.s.max_parts_a) units_a[at] = u;
         // every share starts with a unit of its own
         if (begin == (s0 + i) * share && s0 + i < a.s.shares) shares[s0 + i] = at;
       }
@@ -298,7 +300,7 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(KvPlanArgs a) {
           const int tile = tiles_r - 1 - i;
           u.row = tile * a.s.rows_b;
           u.kv_end = tile_keys(tile, q, len, a.s.rows_b, a.group);
-          if (at + i < a.s.max_units_b) units_b[at + i] = u;
+          if ((unsigned)(at + i) < (unsigned)a.s.max_units_b) units_b[at + i] = u;
         }
         continue;
       }
@@ -316,10 +318,10 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(KvPlanArgs a) {
           u.kv_begin = min(p * each, seen);
           u.kv_end = min((p + 1) * each, seen);
           u.part = n > 1 ? my_part + p : -1;
-          if (my_at + p < a.s.max_units_b && u.part < a.s.max_parts_b) units_b[my_at + p] = u;
+          if ((unsigned)(my_at + p) < (unsigned)a.s.max_units_b && u.part < a.s.max_parts_b) units_b[my_at + p] = u;
         }
         const int my_join = join + __popcll(splits & ((1ull << lane) - 1));
-        if (m > 0 && my_join < a.s.max_splits_b) splits_b[my_join] = KvSplit{r, u.row, my_part, n};
+        if (m > 0 && (unsigned)my_join < (unsigned)a.s.max_splits_b) splits_b[my_join] = KvSplit{r, u.row, my_part, n};
         at += __builtin_amdgcn_readlane(n_sum, kWave - 1), part += __builtin_amdgcn_readlane(m_sum, kWave - 1);
         join += __popcll(splits);
       }

@@ -404,3 +404,25 @@ def test_parts_of_few_tiles(gpu, fmt, dtype, Hq, H, D, block, lengths):
     again = s.run()
     for x, y in zip(s.run(), again):
         assert torch.equal(x, y)
+
+
+def test_lengths_whose_sum_passes_32_bits(gpu):
+    """New tokens far beyond the step's, whose sum is below zero in 32 bits: their requests are refused, no token gets a
+    slot outside its request, and the attention writes no row outside the step."""
+    from next_step_ai_amd.kv_cache import KvBatch, KvCache, paged_attention
+
+    for new in ([3] + [1 << 28] * 8 + [5], [3] + [1 << 28] * 16 + [5], [0x7FFFFFFF] * 40, [2] * 40 + [1 << 28] * 30 + [1] * 9):
+        batch = KvBatch(200, 16, max_requests=len(new), max_blocks=4, q_heads=8, kv_heads=2)
+        cache = KvCache(200, 2, 128)
+        for most in (0, 1):
+            step = batch.plan(torch.tensor(new, dtype=torch.int32, device=gpu), 9, max_new=most)
+            slots = step.slots.tolist()
+            assert all(-1 <= x < 200 * 16 for x in slots)
+            x = torch.ones(9, 2, 128, dtype=torch.float16, device=gpu)
+            cache.append(x, x, step.slots)
+            room = torch.full((27, 8, 128), 7.0, dtype=torch.float16, device=gpu)
+            paged_attention(torch.ones(9, 8, 128, dtype=torch.float16, device=gpu), cache, step, out=room[9:18])
+            assert (room[:9] == 7).all() and (room[18:] == 7).all()
+            with pytest.raises(RuntimeError, match="requests were refused"):
+                step.check()
+            assert int(step.info[1]) >= 0
