@@ -17,7 +17,10 @@
 // outputs over thousands of keys half a rounding).  m is an integer, so that
 // rescaling is exact.  acc, l, m and the scores are fp32; a weight is rounded to
 // fp16 once, as the products' operand, and l takes it as rounded: where few
-// keys carry a row its rounding cancels.
+// keys carry a row its rounding cancels.  A block whose V scale is far below
+// the others' (its V are zeros, say) has weights that fp16 rounds to nothing,
+// though its keys' share of l is as large as any: weights whose sum is small
+// enter l as they are.
 #include <mutex>
 #include <type_traits>
 
@@ -30,6 +33,9 @@ namespace {
 constexpr float kLowest = -3.402823466e38f;
 constexpr float kSumLimit = 32768.0f;
 constexpr float kLift = 10.0f;
+// Sums of weights below this may hold subnormal ones, which lose bits: above, what
+// 8 weights lose is below 2^-16 of the sum.
+constexpr float kSmallSum = 0.015625f;
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
@@ -287,7 +293,7 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
           rest[s] = uint2{pack_f16(p[0] - (float)a0.x, p[1] - (float)a0.y), pack_f16(p[2] - (float)a1.x, p[3] - (float)a1.y)};
         }
         const float whole = (p[0] + p[1]) + (p[2] + p[3]);
-        dl = __builtin_fmaf(kSplit ? whole : sums[s], share, dl);
+        dl = __builtin_fmaf(kSplit || sums[s] < kSmallSum ? whole : sums[s], share, dl);
         if (!kSplit && want_lse) dx = __builtin_fmaf(whole, share, dx);
       }
       return fmaxf(sums[0], sums[1]);
@@ -554,6 +560,12 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
   unsigned long long bad_seen = 0;
   Pages pages = load_pages(a, u.req, h, u.kv_begin >> a.c.b_shift, last, lane);
   if (tiles > 0) bad_seen = pages.bad;
+  // whether V scales so far lie more than a factor of 2^4 from the first one: only
+  // then can a weight that matters to l be too small for fp16 (the largest is
+  // 2^10, and weights below 2^-27 of it are lost at most)
+  const float lv_first = lane_of(pages.lv, 0);
+  const auto apart = [&]() { return __ballot(!(fabsf(pages.lv - lv_first) <= 4.0f)); };
+  unsigned long long uneven = apart();
   // this wave's page in tile i, as a lane of `pages`; past the last tile again the last
   const auto at_of = [&](int i) { return u.kv_begin + min(i, tiles - 1) * kTileKeys + 16 * part; };
   const auto page_of = [&](int i) { return min(at_of(i) >> a.c.b_shift, last) - pages.first; };
@@ -605,6 +617,7 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
     if (__builtin_expect_with_probability(need >= turn_at, 0, 0.95)) {
       pages = load_pages(a, u.req, h, (u.kv_begin + min(from, tiles - 1) * kTileKeys) >> a.c.b_shift, last, lane);
       bad_seen |= pages.bad;
+      uneven |= apart();
       turn_at = window_end();
     }
   };
@@ -751,6 +764,19 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
 #pragma unroll
       for (int n = 0; n < ND; ++n) acc[n] *= scale;
       (void)weights();
+    }
+    if (__builtin_expect_with_probability(uneven != 0, 0, 0.99)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float c = lv[i] - m;
+        float rounded = 0.0f, whole = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float p = exp2_fast(__builtin_fmaf(s[i >> 1][8 * (i & 1) + e], g[i], c));
+          whole += p, rounded += (float)(_Float16)p;
+        }
+        if (rounded < kSmallSum) dl = __builtin_fmaf(whole - rounded, iv[i], dl);
+      }
     }
     l += dl;
     if constexpr (kLse) x += dx;

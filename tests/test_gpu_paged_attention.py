@@ -426,3 +426,28 @@ def test_lengths_whose_sum_passes_32_bits(gpu):
             with pytest.raises(RuntimeError, match="requests were refused"):
                 step.check()
             assert int(step.info[1]) >= 0
+
+
+@pytest.mark.parametrize("fmt,dtype,Hq,H,D,block,lengths", [
+    ("int8", torch.float16, 8, 2, 128, 16, [(700, 1), (90, 3)]),
+    ("e4m3", torch.bfloat16, 4, 4, 64, 32, [(700, 1), (1500, 1)]),
+    ("int8", torch.bfloat16, 16, 1, 128, 16, [(5000, 1)]),
+    ("int8", torch.float16, 8, 2, 128, 16, [(1400, 70), (0, 300)]),
+    ("e4m3", torch.bfloat16, 4, 1, 64, 16, [(900, 150), (33, 1)]),
+    ("int8", torch.bfloat16, 128, 128, 128, 16, [(1500, 700), (0, 333)]),
+])
+@pytest.mark.parametrize("tiny", [0.0, 2.0 ** -20])
+def test_blocks_of_tiny_values(gpu, fmt, dtype, Hq, H, D, block, lengths, tiny):
+    """Blocks whose V are zeros, or far smaller than the others', keep their keys' share of the softmax: the first
+    block, single ones, and all of one request's but the last few."""
+    s = Served(gpu, lengths, Hq, H, D, block, fmt, dtype, seed=Hq + D)
+    for r, (c, n) in enumerate(lengths):
+        slots = s.slots_of(r, c + n)
+        k, v = (torch.from_numpy(s.rng.standard_normal((c + n, H, D))) for _ in range(2))
+        b = torch.arange(c + n) // block
+        few = (b % 3 == 0) if r == 0 else (b < (c + n) // block - 1)
+        v = torch.where(few[:, None, None], v * tiny, v).to(dtype)
+        k = k.to(dtype)
+        s.cache.append(k.to(gpu), v.to(gpu), torch.tensor(slots, device=gpu))
+        s.plain.append(k.float().numpy(), v.float().numpy(), slots)
+    check_wide(s, *s.run())
