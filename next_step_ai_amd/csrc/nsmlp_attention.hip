@@ -901,7 +901,11 @@ __global__ void __launch_bounds__(NW* kWave, 2) k_attn_both(KvAttnArgs a, int bl
 // results in flight at a time.  Where there are many rows a wave has one;
 // where there are few, which then have many parts, a workgroup has one, every
 // wave takes a quarter of the parts, and their sums meet in LDS (24 rows of 43655
-// keys: the call 36 -> 31 us).
+// keys: the call 36 -> 31 us).  Up to 8 parts are one batch of reads for one wave
+// too, and a workgroup per row then pays only where the workgroups are a few
+// per CU (between 1024 and 4096 rows: calls of 16 to 22 us 1.5 to 3 us longer with
+// it; below 1024: calls of 14 us 1 us shorter).  1024 workgroups: with 2048 the
+// launch that finds nothing to join takes 0.3 us longer, and no call is faster.
 template <int E>
 struct JoinSum {
   float m, l, x, o[E];
@@ -947,8 +951,8 @@ __global__ void __launch_bounds__(256) k_attn_join(KvAttnArgs a) {
   __shared__ float part_o[4][D], part_m[4][3];
   const int lane = threadIdx.x & (kWave - 1), wave = uniform(threadIdx.x >> 6), rows_b = a.s.rows_b, rows_j = a.s.join_rows;
   const KvSplit* splits = reinterpret_cast<const KvSplit*>(a.sched + a.s.off_splits_b);
-  const int items = min(a.sched[3], a.s.max_splits_b) * a.c.heads * rows_j;
-  const bool wide = items <= 2 * (int)gridDim.x;
+  const int tiles = min(a.sched[3], a.s.max_splits_b), items = tiles * a.c.heads * rows_j;
+  const bool wide = items <= (a.sched[4] > 8 * tiles ? 4096 : 1024);
   const int at_once = wide ? (int)gridDim.x : (int)gridDim.x * 4;
   for (int item = wide ? (int)blockIdx.x : (int)blockIdx.x * 4 + wave; item < items; item += at_once) {
     const int r = item % rows_j, h = item / rows_j % a.c.heads;
@@ -1013,7 +1017,7 @@ void attention_typed(const KvAttnArgs& a, hipStream_t s) {
   else lse ? launch_both<D, kFmt, kBf16, 4, true>(a, stream_blocks, s) : launch_both<D, kFmt, kBf16, 4, false>(a, stream_blocks, s);
   if (a.s.max_splits_b > 0) {
     const long long waves = (long long)a.s.max_splits_b * a.c.heads * a.s.join_rows;
-    k_attn_join<D, kBf16><<<dim3((unsigned)min((waves + 3) / 4, 2048LL)), dim3(256), 0, s>>>(a);
+    k_attn_join<D, kBf16><<<dim3((unsigned)min((waves + 3) / 4, 1024LL)), dim3(256), 0, s>>>(a);
   }
 }
 
