@@ -905,7 +905,7 @@ __global__ void __launch_bounds__(NW* kWave, 2) k_attn_both(KvAttnArgs a, int bl
 // too, and a workgroup per row then pays only where the workgroups are a few
 // per CU (between 1024 and 4096 rows: calls of 16 to 22 us 1.5 to 3 us longer with
 // it; below 1024: calls of 14 us 1 us shorter).  1024 workgroups: with 2048 the
-// launch that finds nothing to join takes 0.3 us longer, and no call is faster.
+// call that finds nothing to join takes 0.2 us longer, and no call is faster.
 template <int E>
 struct JoinSum {
   float m, l, x, o[E];
