@@ -581,7 +581,8 @@ size_t nsmlp_kv_schedule_bytes(const nsmlp_kv_batch* batch, int total, int max_n
  * slots: the step's tokens, request by request; q_start: where each request's
  * tokens start; kv_len: cached + new.  A request is refused (slots -1, kv_len
  * 0, nothing taken) where its blocks would exceed max_blocks, its new tokens
- * max_new, or the blocks asked for up to and with it the free ones.  info:
+ * max_new, or the blocks asked for up to and with it the free ones (requests
+ * refused for the first two ask for none).  info:
  * the ring's (head, count) after the step, requests refused, the sum of
  * new_tokens.  Tokens of the step past that sum get slot -1.  The batch's
  * lengths and ring stay as they are until nsmlp_kv_commit, so that a plan can

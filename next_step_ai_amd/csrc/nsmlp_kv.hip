@@ -15,7 +15,9 @@ namespace {
 //   need = ceil((cached + fresh) / B) - ceil(cached / B)
 // blocks, the ring's entries head + (sum of need before r) ...; it is refused
 // (no slots, kv_len 0, lengths unchanged) where its blocks exceed the table's
-// width or the running sum the free count.
+// width, its new tokens max_new, or the running sum the free count.  The ring
+// moves on by the blocks granted, so what the first two refuse is in no sum;
+// past the free count every later request that needs a block is refused too.
 //
 // What bounds it: latency (8 requests 6.5 us, 300 with 6513 tokens 10 us, 4096
 // with 73470 tokens 14 us).  8 requests write 224 bytes, 4096 requests 0.7 MB; a
@@ -139,7 +141,7 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(KvPlanArgs a) {
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int have = (cached[i] + a.B - 1) >> a.b_shift, tot = (cached[i] + fresh[i] + a.B - 1) >> a.b_shift;
-    need[i] = tot <= a.max_blocks ? tot - have : -1;  // -1: longer than the table
+    need[i] = tot <= a.max_blocks && fresh[i] <= a.max_new ? tot - have : -1;  // -1: longer than the table or max_new
     sum[0] += fresh[i];
     sum[1] += max(need[i], 0);
   }
@@ -155,7 +157,7 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(KvPlanArgs a) {
     const int r = r0 + i;
     const bool in = i < per && r < a.R;
     const int n = max(need[i], 0);
-    const bool ok = need[i] >= 0 && (n == 0 || used + n <= count) && fresh[i] <= a.max_new;
+    const bool ok = need[i] >= 0 && (n == 0 || used + n <= count);
     kv[i] = in && ok ? cached[i] + fresh[i] : 0;
     if (in) {
       q_start[r] = at;

@@ -27,7 +27,7 @@ class PlainBatch:
         for r, n in enumerate(new):
             have, tot = -(-self.cached[r] // B), -(-(self.cached[r] + n) // B)
             ok = tot <= self.max_blocks and (max_new == 0 or n <= max_new)
-            need = tot - have if tot <= self.max_blocks else 0
+            need = tot - have if ok else 0  # what is refused for its length asks for nothing
             if need:
                 ok = ok and asked + need <= len(self.free)
                 asked += need
