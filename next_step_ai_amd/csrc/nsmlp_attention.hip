@@ -156,6 +156,20 @@ __device__ __forceinline__ float2 ld_coherent2(const float* p) {
   return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
 }
 
+// Zeros and -inf in the rows of a request without keys (a refused one), which
+// may be more than a unit's 16.
+template <int D>
+__device__ __forceinline__ void fill_unseen(const KvAttnArgs& a, int req, int h) {
+  const int q0 = uniform(a.q_start[req]), q_len = uniform(a.q_start[req + 1]) - q0;
+  const long long first = max(q0, 0), tokens = min((long long)q0 + q_len, (long long)a.total) - first;
+  const int pieces = a.group * D / 8;  // of a token, 16 bytes each
+  for (long long i = threadIdx.x; i < tokens * pieces; i += blockDim.x)
+    reinterpret_cast<uint4*>(a.out + ((first + i / pieces) * a.c.heads + h) * a.group * D)[i % pieces] = uint4{0, 0, 0, 0};
+  if (a.lse == nullptr) return;
+  for (long long i = threadIdx.x; i < tokens * a.group; i += blockDim.x)
+    a.lse[((first + i / a.group) * a.c.heads + h) * a.group + i % a.group] = -INFINITY;
+}
+
 template <int D, int kFmt, bool kBf16, int NW>
 __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u, int h, StreamLds<D, NW>& lds) {
   constexpr int NJ = D / 64, KS = D / 32, ND = D / 16;
@@ -168,7 +182,7 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
   const int col = lane & 15, grp = lane >> 4;
   const bool want_lse = a.lse != nullptr;
   const int q0 = uniform(a.q_start[u.req]), q_len = uniform(a.q_start[u.req + 1]) - q0, kv_len = uniform(a.kv_len[u.req]);
-  const int rows = min(q_len * a.group, kKvRowsA);
+  const int rows = q_len > kKvRowsA ? kKvRowsA : min(q_len * a.group, kKvRowsA);
 
   // this wave's keys
   const int each = ((u.kv_end - u.kv_begin + NW - 1) / NW + 31) & ~31;
@@ -469,7 +483,9 @@ __device__ __forceinline__ void stream_share(const KvAttnArgs& a, int block, Str
   const int end = share + 1 < shares ? min(start[share + 1], units) : units;
   const KvUnit* list = reinterpret_cast<const KvUnit*>(a.sched + a.s.off_units_a);
   for (int i = start[share]; i < end; ++i) {
-    stream_unit<D, kFmt, kBf16, NW>(a, load_unit(list + i), h, lds);
+    const KvUnit u = load_unit(list + i);
+    if (u.kv_end == 0) fill_unseen<D>(a, u.req, h);
+    else stream_unit<D, kFmt, kBf16, NW>(a, u, h, lds);
     __syncthreads();
   }
 }

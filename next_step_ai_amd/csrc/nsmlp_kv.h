@@ -99,7 +99,8 @@ void launch_kv_read(const KvReadArgs& a, bool bf16, hipStream_t s);
 // Work of an attention call, listed by the step's plan.  A unit is up to
 // `rows` query rows of a request (row = token * group + head of the group)
 // against keys [kv_begin, kv_end) of every K/V head.  Two lists:
-//   a  requests whose rows fit one tile of 16: their keys are streamed.  All
+//   a  requests whose rows fit one tile of 16 (or any that a step without list b
+//      refuses for their length): their keys are streamed.  All
 //      these requests' keys, one after the other in pieces of 64, are cut into
 //      equal shares, one per workgroup and K/V head; a unit is what a share
 //      holds of a request.  A request's units meet in the last to end.

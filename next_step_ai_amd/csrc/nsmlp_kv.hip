@@ -108,6 +108,11 @@ __device__ __forceinline__ int parts_of(int seen, float per_key) {
   return max(1, (int)((float)seen * per_key + 0.65f));
 }
 
+// Which list a request is in.  Without a list b its rows are list a's however
+// many they are: then it is longer than max_new, refused, and its rows are only
+// to be filled (or the step's total is less than the requests' sum).
+__device__ __forceinline__ bool in_list_b(const KvPlanArgs& a, int rows) { return a.s.list_b && rows > kKvRowsA; }
+
 __device__ __forceinline__ int pieces_of(int keys) { return max(1, (keys + 63) >> 6); }
 
 constexpr int kPlanSums = 6;
@@ -174,7 +179,7 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(KvPlanArgs a) {
     used += n;
     at += fresh[i];
     const int rows = min(fresh[i], a.row_limit) * a.group;
-    const bool b = rows > kKvRowsA;
+    const bool b = in_list_b(a, rows);
     tiles[i] = b ? (rows + a.s.rows_b - 1) / a.s.rows_b : rows > 0 ? -1 : 0;
     if (b) work += work_of(tiles[i], fresh[i], kv[i], a.s.rows_b, a.group);
     else if (rows > 0) sums[0] += pieces_of(kv[i]);
@@ -278,7 +283,7 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(KvPlanArgs a) {
     const int rows = min(q, a.row_limit) * a.group;
     KvUnit u = {};
     u.req = r;
-    if (rows <= kKvRowsA) {
+    if (!in_list_b(a, rows)) {
       const int p0 = split[r], p1 = p0 + pieces_of(len), s0 = (int)((unsigned)p0 / (unsigned)share);
       const int n = (int)((unsigned)(p1 - 1) / (unsigned)share) - s0 + 1;
       for (int i = lane; i < n; i += kWave) {

@@ -61,3 +61,36 @@ def test_blocks_over_steps_with_every_refusal(gpu, requests, block, seed):
         plain.commit(ended)
         batch.commit(ints([int(r in ended) for r in range(requests)], gpu))
         assert batch.cached.tolist() == plain.cached and owned(batch, pool) == plain.blocks
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.float16, 128), (torch.bfloat16, 64)])
+@pytest.mark.parametrize("group,most", [(8, 1), (2, 6), (16, 1), (1, 16), (40, 1)])
+def test_rows_of_a_request_longer_than_max_new(gpu, dtype, D, group, most):
+    """Zeros and -inf in all of them, next to requests that are served, also where no request of max_new tokens fills
+    more than one tile of 16 rows."""
+    from next_step_ai_amd.kv_cache import KvBatch, KvCache, paged_attention
+
+    H, new = 2, [1, 40, 0, most, most + 1, 1]
+    total = sum(new)
+    b = KvBatch(20, 16, max_requests=len(new), max_blocks=4, q_heads=H * group, kv_heads=H)
+    c = KvCache(20, H, D)
+    g = torch.Generator(device=gpu).manual_seed(group)
+    st = b.plan(ints(new, gpu), total + 1, max_new=most)
+    assert st.kv_len.tolist() == [1, 0, 0, most, 0, 1]
+    k, v, q = (torch.randn(total + 1, h, D, device=gpu, generator=g).to(dtype) for h in (H, H, H * group))
+    c.append(k, v, st.slots)
+    for with_lse in (True, False):
+        out = torch.full_like(q, 3.0)
+        lse = torch.full(q.shape[:2], 3.0, device=gpu) if with_lse else None
+        paged_attention(q, c, st, out=out, lse=lse)
+        t0 = 0
+        for n in new:
+            refused = n > most
+            rows = out[t0: t0 + n]
+            assert bool((rows == 0).all()) if refused else bool((rows.abs().amax(-1) > 0).all())
+            if with_lse:
+                assert ((lse[t0: t0 + n] == -np.inf) == refused).all()
+            t0 += n
+        assert (out[total:] == 3).all() and (lse is None or (lse[total:] == 3).all())
+        # one key: the row is its value, read back
+        assert torch.equal(out[0].view(H, group, D), c.read(st.slots[:1], dtype)["v"][0][:, None].expand(H, group, D))
