@@ -515,7 +515,7 @@ int nsmlp_host_device_pointer(const void* host, void** device_ptr);
  * raises it, the stored codes are rewritten as code'(code * old / new), rounded
  * to nearest even like new values.  A call that writes a block's first token
  * starts its scale anew.  A value that is not finite makes the (block, head)'s
- * scale NaN until then.
+ * scale NaN until then (e4m3: and its codes zero, so that no code is a NaN).
  * data: [num_blocks][kv_heads][2][block_tokens * head_dim] bytes in an order of
  * the library's own; scale: [num_blocks][kv_heads][2] (K, V).  Both are zeroed
  * once by the caller.  head_dim 64 or 128; 16-byte aligned. */

@@ -421,7 +421,9 @@ __device__ __forceinline__ float in_hi(uint32_t w) {
 // correctly rounded r makes the corrected product the correctly rounded
 // quotient); adding 1.5 2^23 + 128 rounds it to an integer, to even, and leaves
 // code + 128 in the low byte (|x / s| < 127.5, as s is at least the largest
-// magnitude / 127).  An e4m3 scale is a power of two: x r is exact.
+// magnitude / 127).  An e4m3 scale is a power of two: x r is exact.  Under a NaN
+// scale e4m3 codes are zero: the scale makes their values NaN, and a NaN code
+// would also reach rows of the attention that give it a weight of zero.
 template <int kFmt>
 __device__ __forceinline__ uint32_t kv_encode4(const float (&x)[4], float s, float r) {
   if constexpr (kFmt == NSMLP_KV_INT8) {
@@ -435,9 +437,9 @@ __device__ __forceinline__ uint32_t kv_encode4(const float (&x)[4], float s, flo
     const uint32_t lo = __builtin_amdgcn_perm(c[1], c[0], 0x0C0C0400u), hi = __builtin_amdgcn_perm(c[3], c[2], 0x04000C0Cu);
     return lo | hi;
   } else {
-    (void)s;
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * r, x[1] * r, 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2] * r, x[3] * r, w, true);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(x[2] * r, x[3] * r, w, true);
+    return s == s ? (uint32_t)w : 0u;
   }
 }
 

@@ -94,3 +94,72 @@ def test_rows_of_a_request_longer_than_max_new(gpu, dtype, D, group, most):
         assert (out[total:] == 3).all() and (lse is None or (lse[total:] == 3).all())
         # one key: the row is its value, read back
         assert torch.equal(out[0].view(H, group, D), c.read(st.slots[:1], dtype)["v"][0][:, None].expand(H, group, D))
+
+
+# --------------------------------------------- values that are not finite --
+def rows_against_formula(q, keys, values, out, first, u, group):
+    """Rows i < len(q), which see keys 0 .. first + i, against the formula in 64 bits; the tolerance of an output's
+    rounding u, the weights' to fp16 (2^-11 each, 2^-25 of the largest value where one is subnormal) and fp32 scores."""
+    D = q.shape[-1]
+    k, v = keys.double(), values.double()
+    n = k.shape[0]
+    hidden = torch.arange(n, device=q.device)[None] > first + torch.arange(q.shape[0], device=q.device)[:, None]
+    for h in range(q.shape[1]):
+        kh, vh = k[:, h // group].contiguous(), v[:, h // group].contiguous()
+        e = (q[:, h].double() @ kh.t().contiguous() * D ** -0.5).masked_fill(hidden, -np.inf)
+        p = torch.softmax(e, 1)
+        want, spread = p @ vh, p @ vh.abs()
+        bound = u * want.abs() + (2.0 ** -11 + 2.0 ** -15) * spread + n * 2.0 ** -25 * float(vh.abs().max()) + 2.0 ** -24
+        assert ((out[:, h].double() - want).abs() <= bound).all(), h
+
+
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("Hq,H,D,block,cached,new,bad", [
+    (4, 2, 64, 16, 13, 6, 5),         # a draft: 16 rows streamed, the block begins inside it
+    (8, 8, 128, 16, 30, 9, 4),
+    (4, 2, 64, 16, 20, 40, 30),       # a chunk: a tile of 128 rows
+    (6, 1, 128, 32, 0, 100, 70),
+    (256, 128, 64, 16, 100, 520, 333),  # tiles of 256 rows
+])
+def test_a_value_that_is_not_finite_reaches_only_rows_that_see_its_block(gpu, which, value, fmt, Hq, H, D, block, cached, new, bad):
+    """Appended in a step's later token: rows that end before its block are as the formula says, rows that see the
+    block are NaN, and so is what is read back, in its head alone."""
+    from next_step_ai_amd.kv_cache import KvBatch, KvCache, paged_attention
+
+    dtype = torch.bfloat16
+    pool = (cached + new) // block + 2
+    b = KvBatch(pool, block, max_requests=1, max_blocks=pool, q_heads=Hq, kv_heads=H, head_dim=D)
+    c = KvCache(pool, H, D, block_tokens=block, fmt=fmt)
+    g = torch.Generator(device=gpu).manual_seed(new)
+
+    def rows(n, h):
+        return torch.randn(n, h, D, device=gpu, generator=g).to(dtype)
+
+    if cached:
+        st = b.plan(ints([cached], gpu), cached)
+        c.append(rows(cached, H), rows(cached, H), st.slots)
+        b.commit()
+    st = b.plan(ints([new], gpu), new, max_new=new)
+    kv, head, G = {"k": rows(new, H), "v": rows(new, H)}, H - 1, Hq // H
+    kv[which][bad, head, 3] = value
+    q = rows(new, Hq)
+    c.append(kv["k"], kv["v"], st.slots)
+    lse = torch.empty(new, Hq, device=gpu)
+    out = paged_attention(q, c, st, lse=lse)
+    start = (cached + bad) // block * block  # the block's first token
+    clean = start - cached                   # rows that end before it
+    assert 0 < clean < new
+    at = torch.arange(cached + new, device=gpu)
+    stored = c.read(st.table[0][at // block].long() * block + at % block, dtype)
+    poisoned = torch.zeros(cached + new, H, dtype=torch.bool, device=gpu)
+    poisoned[start: start + block, head] = True
+    assert torch.equal(stored[which].isnan().all(-1), poisoned) and torch.equal(stored[which].isnan().any(-1), poisoned)
+    assert not stored["v" if which == "k" else "k"].isnan().any()
+    mine = slice(head * G, (head + 1) * G)
+    assert out[clean:, mine].isnan().all() and lse[clean:, mine].isnan().all()
+    assert not out[:clean].isnan().any() and not out[:, : head * G].isnan().any()
+    assert lse[:clean].isfinite().all() and lse[:, : head * G].isfinite().all()
+    if fmt == "e4m3":  # rounded to bf16 without loss: 4 bits and a power of two
+        rows_against_formula(q[:clean], stored["k"][:start], stored["v"][:start], out[:clean], cached, 2.0 ** -8, G)
