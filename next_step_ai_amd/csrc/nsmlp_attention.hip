@@ -354,6 +354,7 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
     int pos = begin;
     while (pos + 64 <= min(end, plain) && bad_seen == 0) {  // two tiles, the next two's codes behind them
       fetch(t1, pos + 32);
+      if (bad_seen != 0) break;  // (of a new window of pages, which may be t1's)
       use(std::false_type{}, t0, pos);
       fetch(t0, pos + 64);
       use(std::false_type{}, t1, pos + 32);

@@ -163,3 +163,49 @@ def test_a_value_that_is_not_finite_reaches_only_rows_that_see_its_block(gpu, wh
     assert lse[:clean].isfinite().all() and lse[:, : head * G].isfinite().all()
     if fmt == "e4m3":  # rounded to bf16 without loss: 4 bits and a power of two
         rows_against_formula(q[:clean], stored["k"][:start], stored["v"][:start], out[:clean], cached, 2.0 ** -8, G)
+
+
+# ------------------------------------------------------- far into a request --
+def test_a_table_entry_that_is_no_block_in_a_later_window_of_pages(gpu):
+    """A wave that starts 32 tokens into a block of 64 takes its second window of 64 pages between the two tiles of a
+    pair: a bad entry there hides its keys as one in the first window does, whatever block 0 holds."""
+    from next_step_ai_amd._runtime import StatusWord, workspace
+    from next_step_ai_amd.kv_cache import KvBatch, KvCache, paged_attention
+
+    H, D, B, n = 256, 64, 64, 16500  # one share for all keys, a quarter (4128, rounded up to 32) for each wave
+    blocks = -(-n // B)
+    b = KvBatch(blocks + 1, B, max_requests=1, max_blocks=blocks, q_heads=H, kv_heads=H, head_dim=D,
+                free_blocks=torch.arange(1, blocks + 1))
+    c = KvCache(blocks + 1, H, D, block_tokens=B)
+    g = torch.Generator(device=gpu).manual_seed(1)
+    q = torch.randn(1, H, D, device=gpu, generator=g).half()
+    big = (4 * q).expand(B, H, D)  # block 0: keys that a softmax would not overlook, with large values
+    c.append(big, torch.full_like(big, 100.0), torch.arange(B, device=gpu))
+    st = b.plan(ints([n - 1], gpu), n - 1)
+    for at in range(0, n - 1, 4 * 1024):  # (blocks whole in every call)
+        to = min(at + 4 * 1024, n - 1)
+        k, v = (torch.randn(to - at, H, D, device=gpu, generator=g).half() for _ in range(2))
+        c.append(k, v, st.slots[at:to])
+    b.commit()
+    st = b.plan(ints([1], gpu), 1, max_new=1)
+    c.append(q, q, st.slots)
+    slots = (st.table[0][torch.arange(n, device=gpu) // B].long() * B + torch.arange(n, device=gpu) % B)
+    heads = (0, 1, 100, 255)
+    stored = c.read(slots)
+    scale = c.scale[slots // B]  # (tokens, heads, 2)
+    for page in (64, 127, 128, 129, blocks - 1):
+        was = b.table[0, page].clone()
+        b.table[0, page] = -1
+        out = paged_attention(q, c, st)
+        b.table[0, page] = was
+        keep = torch.arange(n, device=gpu) // B != page
+        for h in heads:
+            # the codes' values exactly: what is read back, rounded to fp16, over the scale is a whole number
+            k, v = (torch.round(stored[x][:, h].double() / scale[:, h, i, None].double()) * scale[:, h, i, None].double()
+                    for i, x in ((0, "k"), (1, "v")))
+            e = (k[keep] @ q[0, h].double()) * D ** -0.5
+            p = torch.softmax(e, 0)
+            want, spread = p @ v[keep], p @ v[keep].abs()
+            bound = 2.0 ** -11 * want.abs() + (2.0 ** -11 + 2.0 ** -15) * spread + n * 2.0 ** -25 * float(v.abs().max()) + 2.0 ** -24
+            assert ((out[0, h].double() - want).abs() <= bound).all(), (page, h)
+    StatusWord(gpu, "paged attention").clear(workspace(1 << 20, gpu))
