@@ -18,6 +18,7 @@ NF4_CODE = (
 
 _ws_lock = threading.Lock()
 _workspaces: dict[tuple[int, int], torch.Tensor] = {}
+_outgrown: list[torch.Tensor] = []
 _codes: dict[int, torch.Tensor] = {}
 _supported: dict[int, bool] = {}
 
@@ -49,7 +50,10 @@ def require_device(t: torch.Tensor, what: str = "input") -> torch.device:
 
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     """Workspace for the current stream of `device`, grown on demand.  Its
-    counter region is zeroed once at allocation; kernels keep it zero."""
+    counter region is zeroed once at allocation; kernels keep it zero.  One
+    that has been outgrown is kept, as a captured graph may hold its address
+    (each is at least twice the one before: all of them are no larger than
+    the one in use)."""
     key = (device.index, stream_handle(device))
     with _ws_lock:
         ws = _workspaces.get(key)
@@ -61,6 +65,8 @@ def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
             off = (-ws.data_ptr()) % 256
             ws = ws[off: off + size]
             _lib.call("nsmlp_workspace_init", ptr(ws), ws.numel(), key[1])
+            if key in _workspaces:
+                _outgrown.append(_workspaces[key])
             _workspaces[key] = ws
         return ws
 

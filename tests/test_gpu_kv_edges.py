@@ -209,3 +209,51 @@ def test_a_table_entry_that_is_no_block_in_a_later_window_of_pages(gpu):
             bound = 2.0 ** -11 * want.abs() + (2.0 ** -11 + 2.0 ** -15) * spread + n * 2.0 ** -25 * float(v.abs().max()) + 2.0 ** -24
             assert ((out[0, h].double() - want).abs() <= bound).all(), (page, h)
     StatusWord(gpu, "paged attention").clear(workspace(1 << 20, gpu))
+
+
+def test_a_captured_step_after_a_larger_call_on_its_stream(gpu, monkeypatch):
+    """The graph's workspace is its own still when a later call has made the stream's larger: partial results and
+    arrival counters of every replay, next to memory that others have filled since."""
+    from next_step_ai_amd import _runtime
+    from next_step_ai_amd._runtime import workspace
+    from next_step_ai_amd.kv_cache import KvBatch, KvCache, paged_attention
+
+    monkeypatch.setattr(_runtime, "_workspaces", {})  # streams that no test has used
+    lengths, Hq, H, D = [5000, 700, 3100], 8, 2, 128
+    g = torch.Generator(device=gpu).manual_seed(6)
+    b = KvBatch(600, 16, max_requests=3, max_blocks=400, q_heads=Hq, kv_heads=H, head_dim=D)
+    c = KvCache(600, H, D)
+    st = b.plan(ints(lengths, gpu), sum(lengths))
+    k, v = (torch.randn(sum(lengths), H, D, device=gpu, generator=g).half() for _ in range(2))
+    c.append(k, v, st.slots)
+    b.commit()
+    st = b.plan(ints([1, 1, 1], gpu), 3, max_new=1)
+    c.append(k[:3], v[:3], st.slots)
+    q, out = (torch.randn(3, Hq, D, device=gpu, generator=g).half() for _ in range(2))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        paged_attention(q, c, st, out=out)
+        small = workspace(1, gpu).numel()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        paged_attention(q, c, st, out=out)
+    big = KvBatch(600, 16, max_requests=1, max_blocks=400, q_heads=4 * Hq, kv_heads=4 * H, head_dim=D)
+    wide = KvCache(600, 4 * H, D)
+    with torch.cuda.stream(side):
+        long = big.plan(ints([300], gpu), 300)
+        x = torch.randn(300, 4 * H, D, device=gpu, generator=g).half()
+        wide.append(x, x, long.slots)
+        paged_attention(x.repeat(1, 4, 1), wide, long)
+        assert workspace(1, gpu).numel() > small
+        fill = [torch.full((small + 256,), 0x7F, dtype=torch.uint8, device=gpu) for _ in range(8)]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        q.normal_(generator=g)
+        out.fill_(3.0)
+        want = paged_attention(q, c, st)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        assert all((f == 0x7F).all() for f in fill)
