@@ -53,7 +53,9 @@ def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     counter region is zeroed once at allocation; kernels keep it zero.  One
     that has been outgrown is kept, as a captured graph may hold its address
     (each is at least twice the one before: all of them are no larger than
-    the one in use)."""
+    the one in use).  Inside a graph capture a stream's own workspace is used
+    where it is large enough; one that is made there is the call's alone, as
+    the node that zeroes its counters runs with the graph only."""
     key = (device.index, stream_handle(device))
     with _ws_lock:
         ws = _workspaces.get(key)
@@ -65,6 +67,8 @@ def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
             off = (-ws.data_ptr()) % 256
             ws = ws[off: off + size]
             _lib.call("nsmlp_workspace_init", ptr(ws), ws.numel(), key[1])
+            if torch.cuda.is_current_stream_capturing():
+                return ws
             if key in _workspaces:
                 _outgrown.append(_workspaces[key])
             _workspaces[key] = ws

@@ -257,3 +257,44 @@ def test_a_captured_step_after_a_larger_call_on_its_stream(gpu, monkeypatch):
         torch.cuda.synchronize()
         assert torch.equal(out, want)
         assert all((f == 0x7F).all() for f in fill)
+
+
+def test_a_step_captured_without_a_call_before_it(gpu, monkeypatch):
+    """Its workspace is made inside the capture: eager calls on that stream before the first replay have one of their
+    own, and replays give what eager calls give."""
+    from next_step_ai_amd import _runtime
+    from next_step_ai_amd.kv_cache import KvBatch, KvCache, paged_attention
+
+    monkeypatch.setattr(_runtime, "_workspaces", {})
+    n, Hq, H, D = 4000, 8, 2, 128
+    g = torch.Generator(device=gpu).manual_seed(7)
+    b = KvBatch(300, 16, max_requests=1, max_blocks=300, q_heads=Hq, kv_heads=H, head_dim=D)
+    caches = [KvCache(300, H, D) for _ in range(2)]
+    st = b.plan(ints([n], gpu), n)
+    for c in caches:
+        c.append(*(torch.randn(n, H, D, device=gpu, generator=g).half() for _ in range(2)), st.slots)
+    b.commit()
+    st = b.plan(ints([1], gpu), 1, max_new=1)
+    q, *outs = (torch.randn(1, Hq, D, device=gpu, generator=g).half() for _ in range(3))
+    for c in caches:
+        c.append(q[:, :H], q[:, :H], st.slots)
+    want = [paged_attention(q, c, st) for c in caches]  # (and the kernels are loaded)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        for c, out in zip(caches, outs):
+            paged_attention(q, c, st, out=out)
+    with torch.cuda.stream(side):
+        eager = [paged_attention(q, c, st) for c in caches]
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(eager, want))
+    for _ in range(4):
+        for out in outs:
+            out.fill_(3.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(outs, want))
+        with torch.cuda.stream(side):
+            assert torch.equal(paged_attention(q, caches[0], st), want[0])
+        torch.cuda.synchronize()

@@ -40,3 +40,20 @@ def test_a_workspace_that_has_grown_keeps_the_old_memory(streams):
     assert [c[0] for c in streams.calls] == ["nsmlp_workspace_init"] * 2
     streams.handle = 8
     assert _runtime.workspace(1, cpu) is not second
+
+
+def test_a_workspace_made_inside_a_capture_is_the_graphs_alone(streams):
+    """Its counters are cleared by a node of the graph, so nobody else may use it before the graph has run."""
+    cpu = torch.device("cpu")
+    streams.capturing = True
+    captured = _runtime.workspace(100, cpu)
+    again = _runtime.workspace(100, cpu)  # the next call of the same capture
+    assert again is not captured and [c[0] for c in streams.calls] == ["nsmlp_workspace_init"] * 2
+    streams.capturing = False
+    eager = _runtime.workspace(100, cpu)
+    assert eager is not captured and len(streams.calls) == 3 and streams.calls[2][1] == eager.data_ptr()
+    streams.capturing = True
+    assert _runtime.workspace(100, cpu) is eager  # one that the stream had before is used as it is
+    larger = _runtime.workspace(eager.numel() + 1, cpu)
+    streams.capturing = False
+    assert larger is not eager and _runtime.workspace(100, cpu) is eager
