@@ -268,7 +268,9 @@ def paged_attention(q: torch.Tensor, cache: KvCache, step: KvStep, *, scale: flo
     bf16) over the cache, causal at the end of each request (its new tokens'
     K and V are appended before the call).  ``scale`` defaults to
     1/sqrt(head_dim).  Returns ``out`` [total, q_heads, head_dim]; ``lse``
-    ([total, q_heads] fp32) receives the log of the softmax sums."""
+    ([total, q_heads] fp32) receives the log of the softmax sums.  ``ws``: a
+    uint8 workspace of ``step.workspace_bytes(head_dim)`` that
+    ``nsmlp_workspace_init`` has cleared, in place of the stream's own."""
     b, device, dim = step.batch, cache.device, cache.head_dim
     if b.device != device:
         raise RuntimeError(f"the cache is on {device} and the batch on {b.device}")
@@ -287,6 +289,8 @@ def paged_attention(q: torch.Tensor, cache: KvCache, step: KvStep, *, scale: flo
         raise RuntimeError(f"lse must be a contiguous fp32 tensor {(total, heads)} on {device}")
     if ws is None:
         ws = workspace(step.workspace_bytes(dim), device)
+    elif ws.device != device or not ws.is_contiguous():
+        raise RuntimeError(f"ws must be a contiguous tensor on {device}, got one on {ws.device} with strides {ws.stride()}")
     _lib.call("nsmlp_paged_attention", cache._ref, b._ref, step._ref, qp, q_row, q_head, _DTYPES[dtype],
               dim ** -0.5 if scale is None else float(scale), out.data_ptr(), None if lse is None else lse.data_ptr(),
               ws.data_ptr(), ws.numel(), stream_handle(device))

@@ -298,3 +298,18 @@ def test_a_step_captured_without_a_call_before_it(gpu, monkeypatch):
         with torch.cuda.stream(side):
             assert torch.equal(paged_attention(q, caches[0], st), want[0])
         torch.cuda.synchronize()
+
+
+# ------------------------------------------------------------- arguments --
+def test_workspaces_that_the_kernels_cannot_use(gpu):
+    """One in host memory, and one that is larger than its memory."""
+    from next_step_ai_amd.kv_cache import KvBatch, KvCache, paged_attention
+
+    b, c = KvBatch(8, 16, max_requests=2, max_blocks=4, q_heads=4, kv_heads=2, head_dim=64), KvCache(8, 2, 64)
+    st = b.plan(ints([20, 3], gpu), 23)
+    x = torch.ones(23, 4, 64, dtype=torch.float16, device=gpu)
+    c.append(x[:, :2], x[:, :2], st.slots)
+    for ws in (torch.zeros(1 << 25, dtype=torch.uint8), torch.zeros(256, dtype=torch.uint8, device=gpu).expand(1 << 17, 256)):
+        with pytest.raises(RuntimeError, match="ws must be"):
+            paged_attention(x, c, st, ws=ws)
+    assert torch.equal(paged_attention(x, c, st), x)
