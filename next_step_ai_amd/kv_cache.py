@@ -135,7 +135,7 @@ class KvStep:
     block table.  ``info`` and the others are device tensors: reading them
     waits for the stream."""
 
-    __slots__ = ("batch", "total", "max_new", "slots", "_buf", "_layout", "_view", "_ref", "_split")
+    __slots__ = ("batch", "total", "max_new", "slots", "planned", "_buf", "_layout", "_view", "_ref", "_split")
 
     def __init__(self, batch: "KvBatch", total: int, max_new: int):
         lay = batch._layout(total, max_new)
@@ -148,6 +148,7 @@ class KvStep:
                                      base + 4 * (3 * R + 1), base + 4 * lay.ints, lay.schedule_bytes)
         self._ref = ctypes.byref(self._view)
         self._split = None
+        self.planned = False
 
     def _part(self, i: int) -> torch.Tensor:
         if self._split is None:  # one split takes half as long as three views
@@ -248,6 +249,7 @@ class KvBatch:
         elif step.batch is not self or step.total != total or step.max_new != max_new:
             raise RuntimeError("the step to plan into belongs to another batch, total or max_new")
         _lib.call("nsmlp_kv_plan", self._ref, new_tokens.data_ptr(), step._ref, stream_handle(self.device))
+        step.planned = True
         self._step = step
         return step
 
@@ -274,6 +276,8 @@ def paged_attention(q: torch.Tensor, cache: KvCache, step: KvStep, *, scale: flo
     b, device, dim = step.batch, cache.device, cache.head_dim
     if b.device != device:
         raise RuntimeError(f"the cache is on {device} and the batch on {b.device}")
+    if not step.planned:  # its lists are what the memory held
+        raise RuntimeError("the step has not been planned (KvBatch.plan)")
     total, heads = step.total, b.q_heads
     q, qp, q_row, q_head = _rows(q, "q", heads, dim, device)
     if q.shape[0] != total:

@@ -313,3 +313,23 @@ def test_workspaces_that_the_kernels_cannot_use(gpu):
         with pytest.raises(RuntimeError, match="ws must be"):
             paged_attention(x, c, st, ws=ws)
     assert torch.equal(paged_attention(x, c, st), x)
+
+
+def test_a_step_that_no_plan_has_written(gpu):
+    """Its work lists hold anything: the attention refuses it until a plan has been made into it."""
+    from next_step_ai_amd import _lib
+    from next_step_ai_amd.kv_cache import KvBatch, KvCache, KvStep, paged_attention
+
+    b, c = KvBatch(8, 16, max_requests=2, max_blocks=4, q_heads=4, kv_heads=2, head_dim=64), KvCache(8, 2, 64)
+    x = torch.ones(23, 4, 64, dtype=torch.float16, device=gpu)
+    st = KvStep(b, 23, 0)
+    with pytest.raises(RuntimeError, match="not been planned"):
+        paged_attention(x, c, st)
+    with _lib.injected_faults("kv_plan=hip:1"):
+        with pytest.raises(RuntimeError, match="injected fault"):
+            b.plan(ints([20, 3], gpu), 23, step=st)
+    with pytest.raises(RuntimeError, match="not been planned"):
+        paged_attention(x, c, st)
+    assert b.plan(ints([20, 3], gpu), 23, step=st) is st
+    c.append(x[:, :2], x[:, :2], st.slots)
+    assert torch.equal(paged_attention(x, c, st), x)
