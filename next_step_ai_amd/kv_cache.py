@@ -259,8 +259,9 @@ class KvBatch:
         if finished is not None and (finished.dtype != torch.int32 or finished.device != self.device
                                      or int(finished.numel()) != self.requests or not finished.is_contiguous()):
             raise RuntimeError(f"finished must be a contiguous int32 [{self.requests}] tensor on {self.device}")
-        st, self._step = self._step, None
+        st = self._step
         _lib.call("nsmlp_kv_commit", self._ref, None if st is None else st._ref, ptr(finished), stream_handle(self.device))
+        self._step = None  # (a commit that fails can be made again)
 
 
 def paged_attention(q: torch.Tensor, cache: KvCache, step: KvStep, *, scale: float | None = None,

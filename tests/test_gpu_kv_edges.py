@@ -333,3 +333,20 @@ def test_a_step_that_no_plan_has_written(gpu):
     assert b.plan(ints([20, 3], gpu), 23, step=st) is st
     c.append(x[:, :2], x[:, :2], st.slots)
     assert torch.equal(paged_attention(x, c, st), x)
+
+
+def test_commit_that_fails_can_be_made_again(gpu):
+    """A commit that raises has done nothing: the plan is still the one to commit."""
+    from next_step_ai_amd import _lib
+    from next_step_ai_amd.kv_cache import KvBatch
+
+    b = KvBatch(8, 16, max_requests=2, max_blocks=4, q_heads=4, kv_heads=2)
+    b.plan(ints([20, 3], gpu), 23)
+    with _lib.injected_faults("kv_commit=hip:1"):
+        with pytest.raises(RuntimeError, match="injected fault"):
+            b.commit()
+    assert b.cached.tolist() == [0, 0]
+    b.commit()
+    assert b.cached.tolist() == [20, 3]
+    b.commit()
+    assert b.cached.tolist() == [20, 3]
