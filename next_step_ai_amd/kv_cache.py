@@ -45,11 +45,16 @@ def _rows(t: torch.Tensor, what: str, heads: int, dim: int, device: torch.device
     if t.device != device:
         raise RuntimeError(f"{what} must be a GPU tensor on {device}, got {t.device}")
     row, head, one = t.stride()
+    # (a dimension of one element may have any stride, and a copy keeps it)
+    if t.shape[0] <= 1:
+        row = heads * dim
+    if heads == 1:
+        head = dim
     p = t.data_ptr()
     if one != 1 or row % 8 or head % 8 or p % 16:
         t = t.contiguous()
         t = t if t.data_ptr() % 16 == 0 else t.clone()
-        row, head, _ = t.stride()
+        row, head = heads * dim, dim
         p = t.data_ptr()
     return t, p, row, head
 

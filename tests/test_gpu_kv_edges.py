@@ -350,3 +350,22 @@ def test_commit_that_fails_can_be_made_again(gpu):
     assert b.cached.tolist() == [20, 3]
     b.commit()
     assert b.cached.tolist() == [20, 3]
+
+
+def test_one_token_or_one_head_of_any_stride(gpu):
+    """A decode step's rows where they lie in a fused projection of odd width, and one K/V head of any stride."""
+    from next_step_ai_amd.kv_cache import KvBatch, KvCache, paged_attention
+
+    g = torch.Generator(device=gpu).manual_seed(8)
+    for H in (1, 2):
+        b, c, same = (KvBatch(8, 16, max_requests=1, max_blocks=4, q_heads=2 * H, kv_heads=H, head_dim=64),
+                      KvCache(8, H, 64), KvCache(8, H, 64))
+        st = b.plan(ints([1], gpu), 1, max_new=1)
+        wide = torch.randn(4 * H * 64 + 3, device=gpu, generator=g).half()
+        q = wide.as_strided((1, 2 * H, 64), (4 * H * 64 + 3, 64, 1))
+        k = wide.as_strided((1, H, 64), (4 * H * 64 + 3, 64 if H > 1 else 77, 1), 2 * H * 64)
+        v = wide.as_strided((1, H, 64), (4 * H * 64 + 3, 64 if H > 1 else 77, 1), 3 * H * 64)
+        c.append(k, v, st.slots)
+        same.append(k.reshape(-1).view(1, H, 64), v.reshape(-1).view(1, H, 64), st.slots)
+        assert torch.equal(c.data, same.data) and torch.equal(c.scale, same.scale)
+        assert torch.equal(paged_attention(q, c, st), paged_attention(q.reshape(-1).view(1, 2 * H, 64), c, st))
