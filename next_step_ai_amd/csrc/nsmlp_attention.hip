@@ -33,6 +33,8 @@ namespace {
 constexpr float kLowest = -3.402823466e38f;
 constexpr float kSumLimit = 32768.0f;
 constexpr float kLift = 10.0f;
+constexpr int kUnitLog2 = 15;
+constexpr float kUnit = 1.0f / (1 << kUnitLog2);
 // Sums of weights below this may hold subnormal ones, which lose bits: above, what
 // 8 weights lose is below 2^-16 of the sum.
 constexpr float kSmallSum = 0.015625f;
@@ -76,7 +78,7 @@ __device__ __forceinline__ uint4 bf16_to_f16(const uint4& raw, int e) {
 // Pages of a range of keys, held one per lane: 64 pages from page `first`.
 struct Pages {
   uint32_t lo, hi;   // where the (block, head)'s codes start (block 0's where the entry is not a block)
-  float ks, lv, iv;  // K scale, log2 and reciprocal of the V scale
+  float ks, lv, iv;  // K scale, log2 of the V scale, kUnit over it
   unsigned long long bad;
   int first;
 };
@@ -95,7 +97,7 @@ __device__ __forceinline__ Pages load_pages(const KvAttnArgs& a, int req, int h,
   p.bad = __ballot(!ok);
   p.ks = s.x;
   p.lv = log2_fast(sv);
-  p.iv = 1.0f / sv;
+  p.iv = kUnit / sv;
   return p;
 }
 
@@ -106,6 +108,12 @@ __device__ __forceinline__ const uint8_t* page_data(const KvAttnArgs& a, const P
 
 __device__ __forceinline__ float lane_of(float v, int i) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i));
+}
+
+// What a row's acc is multiplied by, and its lse, at the end.
+__device__ __forceinline__ float inverse_of(float l) { return l == 0.0f ? 0.0f : kUnit / l; }
+__device__ __forceinline__ float lse_of(float m, float x) {
+  return x == 0.0f ? -INFINITY : (m + (float)kUnitLog2 + log2f(x)) * 0.6931471805599453f;
 }
 
 // Whether token i of the step is there.  (Lengths whose sum passes 32 bits leave
@@ -461,13 +469,13 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
   if (row < rows) {
     const int tok_r = q0 + row / a.group, head = h * a.group + row % a.group;
     if (in_step(a, tok_r)) {
-      const float inv = lr == 0.0f ? 0.0f : 1.0f / lr;
+      const float inv = inverse_of(lr);
       const long long at = (long long)tok_r * a.c.heads * a.group + head;
 #pragma unroll
       for (int d = 0; d < kDims; d += 2)
         *reinterpret_cast<uint32_t*>(a.out + at * D + d0 + d) =
             to_out<kBf16>(o[d] * inv) | (uint32_t)to_out<kBf16>(o[d + 1] * inv) << 16;
-      if (want_lse && d0 == 0) a.lse[at] = xr == 0.0f ? -INFINITY : (mr + log2f(xr)) * 0.6931471805599453f;
+      if (want_lse && d0 == 0) a.lse[at] = lse_of(mr, xr);
     }
   }
 }
@@ -524,8 +532,8 @@ __device__ __forceinline__ float max8(const float16_t& s, int at) {
                fmaxf(fmaxf(s[at + 4], s[at + 5]), fmaxf(s[at + 6], s[at + 7])));
 }
 
-// What the weights of 16 keys need to know of their block: K scale, log2 and
-// reciprocal of the V scale, and (as bits) whether it is no block.
+// What the weights of 16 keys need to know of their block: K scale, log2 of
+// the V scale, kUnit over it, and (as bits) whether it is no block.
 typedef float4_t TileMeta;
 
 template <int D>
@@ -876,7 +884,7 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
       if (half == 0) *reinterpret_cast<float4_t*>(a.ml_b + 4 * at) = float4_t{m, l, x, 0.0f};
     } else {
       const long long at = (long long)(q0 + tok) * a.c.heads * a.group + h * a.group + row % a.group;
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const float inv = inverse_of(l);
 #pragma unroll
       for (int g = 0; g < D / 32; ++g) {
         uint32_t o[8];
@@ -890,7 +898,7 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
         to[0] = uint4{o[0], o[1], o[2], o[3]};
         to[1] = uint4{o[4], o[5], o[6], o[7]};
       }
-      if (kLse && half == 0) a.lse[at] = x == 0.0f ? -INFINITY : (m + log2f(x)) * 0.6931471805599453f;
+      if (kLse && half == 0) a.lse[at] = lse_of(m, x);
     }
   }
 }
@@ -999,14 +1007,14 @@ __global__ void __launch_bounds__(256) k_attn_join(KvAttnArgs a) {
         for (int e = 0; e < E; ++e) s.o[e] += part_o[w][lane * E + e] * f;
       }
     }
-    const float inv = s.l == 0.0f ? 0.0f : 1.0f / s.l;
+    const float inv = inverse_of(s.l);
     const long long at = (long long)tok * a.c.heads * a.group + h * a.group + full % a.group;
     if constexpr (E == 2)
       *reinterpret_cast<uint32_t*>(a.out + at * D + lane * 2) =
           to_out<kBf16>(s.o[0] * inv) | (uint32_t)to_out<kBf16>(s.o[1] * inv) << 16;
     else
       a.out[at * D + lane] = to_out<kBf16>(s.o[0] * inv);
-    if (a.lse != nullptr && lane == 0) a.lse[at] = s.x == 0.0f ? -INFINITY : (s.m + log2f(s.x)) * 0.6931471805599453f;
+    if (a.lse != nullptr && lane == 0) a.lse[at] = lse_of(s.m, s.x);
   }
 }
 

@@ -369,3 +369,42 @@ def test_one_token_or_one_head_of_any_stride(gpu):
         same.append(k.reshape(-1).view(1, H, 64), v.reshape(-1).view(1, H, 64), st.slots)
         assert torch.equal(c.data, same.data) and torch.equal(c.scale, same.scale)
         assert torch.equal(paged_attention(q, c, st), paged_attention(q.reshape(-1).view(1, 2 * H, 64), c, st))
+
+
+@pytest.mark.parametrize("value", [0.0, 2.0 ** -95])
+@pytest.mark.parametrize("Hq,H,D,block,n,new", [
+    (4, 1, 64, 64, 1200000, 1),      # streamed
+    (4, 1, 64, 64, 1200000, 33),     # a tile of 128 rows, its keys in parts
+    (128, 128, 64, 64, 1200000, 1100),  # tiles of 256 rows, whole requests
+])
+def test_many_keys_at_the_least_scale(gpu, value, Hq, H, D, block, n, new):
+    """V scales of 2^-100 (values of zero among them) for all of a long request: the sums of the weights over the scales
+    stay within fp32, so lse is finite and outputs keep their share."""
+    from next_step_ai_amd.kv_cache import KvBatch, KvCache, paged_attention
+
+    blocks = -(-n // block)
+    b = KvBatch(blocks, block, max_requests=1, max_blocks=blocks, q_heads=Hq, kv_heads=H, head_dim=D)
+    c = KvCache(blocks, H, D, block_tokens=block, fmt="e4m3")
+    g = torch.Generator(device=gpu).manual_seed(2)
+    k = torch.randn(block, H, D, device=gpu, generator=g).bfloat16()  # every block holds the same keys
+    v = torch.full((block, H, D), value, dtype=torch.bfloat16, device=gpu)
+    st = b.plan(ints([n - new], gpu), n - new)
+    b.commit()
+    st = b.plan(ints([new], gpu), new, max_new=new)
+    c.append(k, v, torch.arange(block, device=gpu))
+    c.data[1:], c.scale[1:] = c.data[0], c.scale[0]
+    assert (c.scale[:, :, 1] == 2.0 ** -100).all()
+    q = (torch.randn(new, Hq, D, device=gpu, generator=g) * 0.25).bfloat16()
+    lse = torch.empty(new, Hq, device=gpu)
+    out = paged_attention(q, c, st, lse=lse)
+    kept = c.read(torch.arange(block, device=gpu), torch.bfloat16)["k"].double()  # (exact: 4 bits and a power of two)
+    seen = n - new + 1 + torch.arange(new, device=gpu)
+    times = (seen[:, None] - torch.arange(block, device=gpu) + block - 1) // block  # how often a row sees each of the keys
+    for h in range(0, Hq, max(1, Hq // 4)):
+        e = q[:, h].double() @ kept[:, h * H // Hq].t().contiguous() * D ** -0.5
+        want = torch.logsumexp(e + times.double().log(), 1)
+        # fp32 sums of n / 64 tiles one after the other, each rounded (the same way, as the keys repeat): 2^-24 per tile
+        sums = n / 64 * 2.0 ** -24
+        assert ((lse[:, h].double() - want).abs() <= 2.0 ** -14 + sums + 2.0 ** -20 * want.abs()).all()
+        # all values are the same: a row is that value, but for its own rounding (2^-9), the weights' (2^-11) and two sums
+        assert ((out[:, h].double() - value).abs() <= (2.0 ** -9 + 2.0 ** -11 + 2.0 ** -15 + 2 * sums) * value).all()
