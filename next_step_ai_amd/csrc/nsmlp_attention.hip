@@ -75,6 +75,28 @@ __device__ __forceinline__ uint4 bf16_to_f16(const uint4& raw, int e) {
   return uint4{o[0], o[1], o[2], o[3]};
 }
 
+// Scores beyond 2^12 (in powers of two).  s + lv - m in one fused operation needs
+// lv - m rounded first, which costs the weight 2^-24 |m|, and past 2^27 the
+// difference of two roundings of a score leaves exp2's range.  So where m is that
+// far, a score is rounded, m subtracted from it, which is exact where the two
+// are close, and lv added then.  Such an m is the largest s + lv, rounded; what
+// that rounding leaves above it is 2^4 for scores below 2^28, and more only where
+// lv, too, is beyond the score's last bit: such weights count as 2^15.
+constexpr float kFar = 4096.0f;
+
+__device__ __forceinline__ bool is_far(float m) { return fabsf(m) >= kFar && m != kLowest; }
+
+// the reference that a row whose largest s + lv is `top` wants: a whole number
+__device__ __forceinline__ float reference_of(float top) {
+  const float c = ceilf(top);
+  return is_far(c) ? c : c - kLift;
+}
+__device__ __forceinline__ float far_exponent(float s, float g, float lv, float m) {
+#pragma clang fp contract(off)
+  const float t = s * g;
+  return is_far(m) ? fminf((t - m) + lv, 15.0f) : (t - m) + lv;
+}
+
 // Pages of a range of keys, held one per lane: 64 pages from page `first`.
 struct Pages {
   uint32_t lo, hi;   // where the (block, head)'s codes start (block 0's where the entry is not a block)
@@ -266,6 +288,7 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
   const int plain = kv_len - q_len + 1;
 
   float m = kLowest, l = 0.0f, x = 0.0f;  // reference, sum of the rounded weights, sum of the weights
+  float sum_limit = kSumLimit;            // (below any sum where m is far)
   float4_t acc[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) acc[d] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
@@ -292,12 +315,13 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
     }
     uint2 w[2], rest[2];  // weights, and (kSplit) what their rounding left
     float dl, dx;
+    float gs[2] = {t.ks[0] * rowf, t.ks[1] * rowf}, lvs[2] = {t.lv[0], t.lv[1]};
     const auto weights = [&]() {
       float sums[2];
       dl = dx = 0.0f;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const float g = t.ks[s] * rowf, c = t.lv[s] - m;
+        const float g = gs[s], c = lvs[s] - m;
         float p[4], share = t.iv[s];
 #pragma unroll
         for (int i = 0; i < 4; ++i) p[i] = exp2_fast(__builtin_fmaf(sc[s][i], g, c));
@@ -321,22 +345,29 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
       return fmaxf(sums[0], sums[1]);
     };
     const float sum = weights();
-    if (__builtin_expect_with_probability(__any(sum > kSumLimit), 0, 0.999)) {
+    if (__builtin_expect_with_probability(__any(sum > sum_limit), 0, 0.999)) {
       float top = kLowest;
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float e = __builtin_fmaf(sc[s][i], t.ks[s] * rowf, t.lv[s]);
-          top = fmaxf(top, (see >> (4 * s + i)) & 1 ? e : kLowest);
-        }
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, (see >> (4 * s + i)) & 1 ? __builtin_fmaf(sc[s][i], gs[s], lvs[s]) : kLowest);
       top = fmaxf(top, __shfl_xor(top, 16, kWave));
-      top = fmaxf(m, ceilf(fmaxf(top, __shfl_xor(top, 32, kWave))) - kLift);  // (never down: other rows may have asked)
+      top = reference_of(fmaxf(top, __shfl_xor(top, 32, kWave)));
+      top = fmaxf(m, top);  // (never down: other rows may have asked)
       const float scale = exp2_fast(m - top);
       m = top;
+      sum_limit = is_far(m) ? -1.0f : kSumLimit;
       l *= scale, x *= scale;
 #pragma unroll
       for (int d = 0; d < ND; ++d) acc[d] *= scale;
+      if (__builtin_expect_with_probability(__any(is_far(m)), 0, 0.999)) {  // the scores become their weights' exponents
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sc[s][i] = far_exponent(sc[s][i], gs[s], lvs[s], m);
+          gs[s] = 1.0f, lvs[s] = m;
+        }
+      }
       (void)weights();
     }
     l += dl;
@@ -684,6 +715,7 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
   const int plain = kv_len - q_len + (u.row + min(wave * 32, rows)) / a.group + 1;
 
   float m = kLowest, l = 0.0f, x = 0.0f;
+  float sum_limit = kSumLimit;  // (below any sum where m is far)
   float16_t acc[ND];
 #pragma unroll
   for (int n = 0; n < ND; ++n)
@@ -778,16 +810,26 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
       return most_sum;
     };
     const float sum = weights();
-    if (__builtin_expect_with_probability(__any(sum > kSumLimit), 0, 0.999)) {
+    if (__builtin_expect_with_probability(__any(sum > sum_limit), 0, 0.999)) {
       float top = kLowest;
 #pragma unroll
       for (int i = 0; i < 4; ++i) top = fmaxf(top, __builtin_fmaf(max8(s[i >> 1], 8 * (i & 1)), g[i], lv[i]));
-      top = fmaxf(m, ceilf(fmaxf(top, __shfl_xor(top, 32, kWave))) - kLift);  // (never down: other rows may have asked)
+      top = reference_of(fmaxf(top, __shfl_xor(top, 32, kWave)));
+      top = fmaxf(m, top);  // (never down: other rows may have asked)
       const float scale = exp2_fast(m - top);
       m = top;
+      sum_limit = is_far(m) ? -1.0f : kSumLimit;
       l *= scale, x *= scale;
 #pragma unroll
       for (int n = 0; n < ND; ++n) acc[n] *= scale;
+      if (__builtin_expect_with_probability(__any(is_far(m)), 0, 0.999)) {  // the scores become their weights' exponents
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) s[i >> 1][8 * (i & 1) + e] = far_exponent(s[i >> 1][8 * (i & 1) + e], g[i], lv[i], m);
+          g[i] = 1.0f, lv[i] = m;
+        }
+      }
       (void)weights();
     }
     if (__builtin_expect_with_probability(uneven != 0, 0, 0.99)) {
