@@ -966,13 +966,11 @@ __global__ void __launch_bounds__(NW* kWave, 2) k_attn_both(KvAttnArgs a, int bl
 // ------------------------------------------------------------------ join --
 // Rows of list b whose keys were shared out: weights 2^(m_p - m), eight parts'
 // results in flight at a time.  Where there are many rows a wave has one;
-// where there are few, which then have many parts, a workgroup has one, every
-// wave takes a quarter of the parts, and their sums meet in LDS (24 rows of 43655
-// keys: the call 36 -> 31 us).  Up to 8 parts are one batch of reads for one wave
-// too, and a workgroup per row then pays only where the workgroups are a few
-// per CU (between 1024 and 4096 rows: calls of 16 to 22 us 1.5 to 3 us longer with
-// it; below 1024: calls of 14 us 1 us shorter).  1024 workgroups: with 2048 the
-// call that finds nothing to join takes 0.2 us longer, and no call is faster.
+// up to 1024 (four per CU) a workgroup has one, every wave takes a quarter of the
+// parts, and their sums meet in LDS.  Whole calls, a wave per row against a
+// workgroup: 12 tokens of 24 heads over 15692 keys 17.8 us, 16.0; 6 of 12 heads
+// over 102424 keys 52.5, 40.8.  With the bound at 4096: 32 tokens of 64 heads over
+// 10000 keys (2048 rows) 36.9 us, 40.4; 64 of 32 heads over 40000 59.7, 63.0.
 template <int E>
 struct JoinSum {
   float m, l, x, o[E];
@@ -1019,7 +1017,7 @@ __global__ void __launch_bounds__(256) k_attn_join(KvAttnArgs a) {
   const int lane = threadIdx.x & (kWave - 1), wave = uniform(threadIdx.x >> 6), rows_b = a.s.rows_b, rows_j = a.s.join_rows;
   const KvSplit* splits = reinterpret_cast<const KvSplit*>(a.sched + a.s.off_splits_b);
   const int tiles = min(a.sched[3], a.s.max_splits_b), items = tiles * a.c.heads * rows_j;
-  const bool wide = items <= (a.sched[4] > 8 * tiles ? 4096 : 1024);
+  const bool wide = items <= 1024;
   const int at_once = wide ? (int)gridDim.x : (int)gridDim.x * 4;
   for (int item = wide ? (int)blockIdx.x : (int)blockIdx.x * 4 + wave; item < items; item += at_once) {
     const int r = item % rows_j, h = item / rows_j % a.c.heads;

@@ -122,7 +122,7 @@ constexpr int kKvRowsA = 16;
 // levels of 8 join 4096 parts, and there are at most 512
 constexpr int kKvCounters = 8192;
 static_assert(4 * kKvCounters <= kMaxK && 2 * (512 + 1024) <= kKvCounters, "the workspace's block counters");
-constexpr int kKvHeaderInts = 16;  // units a, shares, units b, splits b, their parts
+constexpr int kKvHeaderInts = 16;  // units a, shares, units b, splits b
 
 struct KvSchedule {  // sizes, from the host's knowledge of a step (kv_schedule)
   int rows_b, join_rows;             // rows of a tile of list b, and how many of them a request can fill

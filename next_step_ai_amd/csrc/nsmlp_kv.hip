@@ -241,7 +241,6 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(KvPlanArgs a) {
     a.sched[1] = min((sums_total[0] + share - 1) / share, a.s.shares);
     a.sched[2] = min(cnt_total[1], a.s.max_units_b);
     a.sched[3] = min(cnt_total[2], a.s.max_splits_b);
-    a.sched[4] = cnt_total[4];
   }
   __syncthreads();
   // slots: one thread per token; a block's first token also writes its entry

@@ -505,3 +505,26 @@ def test_equal_scores_of_any_size(gpu, fmt, size, Hq, H, D, block, cached, new):
     # roundings of the row, the weights and the values read back, 2^-11 each; the log of a scale next to a score below
     # 2^12 in powers of two, 2^-12
     assert ((out.double() - want).abs() <= 2.0 ** -11 * want.abs() + (2.0 ** -10 + 2.0 ** -12 + 2.0 ** -15) * spread + 2.0 ** -24).all()
+
+
+# ------------------------------------------------ variants, by their sizes --
+@pytest.mark.parametrize("Hq,H,D,new", [
+    (64, 8, 128, 32),  # 2048 rows to join: a wave for each
+    (32, 4, 64, 8),    # 256: a workgroup for each
+])
+def test_rows_joined_from_many_parts(gpu, Hq, H, D, new):
+    from next_step_ai_amd.kv_cache import KvBatch, KvCache, paged_attention
+
+    n, dtype = 9000 + new, torch.bfloat16
+    b = KvBatch(600, 16, max_requests=1, max_blocks=600, q_heads=Hq, kv_heads=H, head_dim=D)
+    c = KvCache(600, H, D, fmt="e4m3")
+    g = torch.Generator(device=gpu).manual_seed(9)
+    st = b.plan(ints([9000], gpu), 9000)
+    c.append(*(torch.randn(9000, H, D, device=gpu, generator=g).to(dtype) for _ in range(2)), st.slots)
+    b.commit()
+    st = b.plan(ints([new], gpu), new, max_new=new)
+    c.append(*(torch.randn(new, H, D, device=gpu, generator=g).to(dtype) for _ in range(2)), st.slots)
+    q = torch.randn(new, Hq, D, device=gpu, generator=g).to(dtype)
+    at = torch.arange(n, device=gpu)
+    stored = c.read(st.table[0][at // 16].long() * 16 + at % 16, dtype)
+    rows_against_formula(q, stored["k"], stored["v"], paged_attention(q, c, st), 9000, 2.0 ** -8, Hq // H)
