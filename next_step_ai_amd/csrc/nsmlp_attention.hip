@@ -159,9 +159,9 @@ __device__ __forceinline__ KvUnit load_unit(const KvUnit* p) {
 // What bounds it: the codes' way from HBM, read once.  All K/V heads' requests
 // together are cut into one equal share per CU, so that uneven lengths cost
 // nothing, and a wave has the next 32 keys' codes in flight while it works on
-// 32: 64 uneven requests (429 MB) 81 us, 5.3 TB/s; one token over 131000 keys
-// (269 MB, 31 partial results per row to join) 57 us, 4.7 TB/s.  A short chat (777
-// keys) takes 9.5 us, most of it the chain launch, schedule, lengths, block
+// 32: 64 uneven requests (429 MB) 82 us, 5.2 TB/s; one token over 131000 keys
+// (269 MB, 31 partial results per row to join) 58 us, 4.7 TB/s.  A short chat (777
+// keys) takes 9.9 us, most of it the chain launch, schedule, lengths, block
 // table, scales, codes, join.
 template <int D, int NW>
 struct StreamLds {
@@ -206,7 +206,8 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
   // fp16 outputs: weights in two fp16 parts, so that their rounding does not
   // add to the output's own (error against 64 bits 2.9e-4 -> 2.1e-4 of the norm,
   // where 2.1e-4 is one rounding); the products have the time, as the codes'
-  // way from memory takes longer.  bf16 outputs round 8 times coarser.
+  // way from memory takes longer (131000 keys 57.8 us with one part and with two,
+  // 12 drafts 16.4 and 16.5).  bf16 outputs round 8 times coarser.
   constexpr bool kSplit = !kBf16;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;

@@ -75,11 +75,10 @@ constexpr int kLeastShare = 4;     // pieces: 256 keys are worth a workgroup
 // requests: their parts cost little, and as nobody sorts them by length, the
 // last to end is what a smaller L shortens: w cost / L + L / 4 is least at `even`.
 // List a's keys count half, as the parts run next to them on the same CUs (a
-// prompt's 387 tokens next to 20 decodes: 37 us without, 31 with).
-// (Against equal parts of 1024 keys or more for all tiles of a request, over 150
-// drawn prompts, drafts and mixed steps: those above 18 us 37 -> 33 us on
-// average; a prompt of 1148 tokens and 40 heads 77 -> 41 us, 6 drafts of 44
-// uneven requests 111 -> 98 us.  Costs of 128 and 512 were up to 3% slower.)
+// prompt's 387 tokens next to 20 decodes: 39 us without, 32 with).
+// Costs of 128 and 512 over 27 drawn prompts, drafts and mixed steps: 0.2% longer
+// and 0.9% shorter calls on average, single ones 9% shorter to 8% longer and 20%
+// shorter to 9% longer; least parts of 96 and 384: 0.7% longer on average.
 constexpr float kPartCost = 256.0f, kLeastPart = 192.0f;
 
 // 1 / L of a request with `rows` rows in `tiles` tiles.  (Parts are counted in
@@ -651,8 +650,11 @@ template <int D, int kFmt, bool kBf16>
 void append_typed(KvAppendArgs a, hipStream_t s) {
   // Most tokens of a long call are a prompt's, and the waves that find no first
   // token of a run cost a round trip each: several tokens per wave where even
-  // then every CU has a dozen waves.  More would leave single tokens that stand
-  // next to each other to one wave, one after the other.
+  // then every CU has a dozen waves.  Single tokens that stand next to each other
+  // are then one wave's, one after the other.  With 1, 8 and 16 tokens per wave,
+  // 8 heads: prompts of 4096 tokens (65536 pairs) 32.6, 10.5, 9.6 us, of 8192 62.5,
+  // 17.0, 13.9; single tokens, 1024 of them 16.0, 17.7, 28.2 us, 2048 29.0, 23.0, 32.1,
+  // 4096 53.9, 41.1, 41.7; 290 next to 7000 of prompts 46.9, 18.3, 30.2.
   const long long pairs = (long long)a.n * a.c.heads * 2;
   a.take = pairs >= 128 * 1024 ? 16 : pairs >= 32 * 1024 ? 8 : 1;
   const long long waves = (long long)((a.n + a.take - 1) / a.take) * a.c.heads * 2, per = kAppendThreads / kWave;
@@ -676,10 +678,10 @@ void launch_kv_read(const KvReadArgs& a, bool bf16, hipStream_t s) { NSMLP_KV_BY
 KvSchedule kv_schedule(int requests, int total, int max_new, int group, int kv_heads) {
   KvSchedule s;
   // list a: one workgroup of 4 waves per CU has as many reads in flight as the
-  // memory takes (two: 131000 keys 50 -> 55 us, for the joins)
+  // memory takes (two: 131000 keys 57.9 -> 62.5 us, for the joins)
   s.shares = (256 + kv_heads - 1) / kv_heads;
   // list b: 256 rows per workgroup where that still makes two for every CU
-  // (chunk of 2048 over 14336, 128 heads: 1.84 ms, with 128 rows 1.92), else 128
+  // (chunk of 2048 over 14336, 128 heads: 2.01 ms, with 128 rows 2.11), else 128
   const long long rows = (long long)total * group;
   s.rows_b = rows / 256 * kv_heads >= 512 ? 256 : 128;
   const long long most = (long long)(max_new < total ? max_new : total) * group;

@@ -528,3 +528,43 @@ def test_rows_joined_from_many_parts(gpu, Hq, H, D, new):
     at = torch.arange(n, device=gpu)
     stored = c.read(st.table[0][at // 16].long() * 16 + at % 16, dtype)
     rows_against_formula(q, stored["k"], stored["v"], paged_attention(q, c, st), 9000, 2.0 ** -8, Hq // H)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("block,D,lengths", [
+    (16, 64, [1] * 300),                                  # 38400 runs' heads: a wave looks at 8 tokens
+    (16, 128, [1] * 700 + [0, 333, 1, 2, 17] + [1] * 90),  # 146304: at 16
+    (64, 64, [500, 1, 1, 63, 65, 1, 900]),
+    (32, 64, [31, 33, 1] * 7),
+])
+def test_append_of_many_tokens(gpu, fmt, block, D, lengths):
+    """A long call, whose waves look at several tokens each, stores what the same rows store request by request."""
+    from next_step_ai_amd.kv_cache import KvBatch, KvCache
+
+    R, H, n = len(lengths), 64, sum(lengths)
+    cached = [(7 * r) % 40 for r in range(R)]
+    need = [-(-(a + b) // block) for a, b in zip(cached, lengths)]
+    pool = sum(need)
+    g = torch.Generator(device=gpu).manual_seed(10)
+    b = KvBatch(pool, block, max_requests=R, max_blocks=max(need), q_heads=H, kv_heads=H,
+                free_blocks=torch.randperm(pool, generator=torch.Generator().manual_seed(1)))
+    whole, single = KvCache(pool, H, D, block_tokens=block, fmt=fmt), KvCache(pool, H, D, block_tokens=block, fmt=fmt)
+    for new in (cached, lengths):
+        st = b.plan(ints(new, gpu), sum(new))
+        st.check()
+        k, v = (torch.randn(sum(new), H, D, device=gpu, generator=g) * torch.randn(sum(new), 1, 1, device=gpu, generator=g).exp2()
+                for _ in range(2))
+        k, v = k.half(), v.half()
+        whole.append(k, v, st.slots)
+        at = 0
+        for m in new:
+            to = at + m
+            first = at  # whole blocks at a time, at most 255 tokens in a call
+            while first < to:
+                room = 192 - int(st.slots[first]) % block
+                last = min(to, first + room)
+                single.append(k[first:last], v[first:last], st.slots[first:last])
+                first = last
+            at = to
+        b.commit()
+        assert torch.equal(whole.data, single.data) and torch.equal(whole.scale, single.scale)
