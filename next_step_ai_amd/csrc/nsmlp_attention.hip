@@ -15,12 +15,13 @@
 // rescale acc, no weight leaves fp16, and weights down to 2^-24 of the largest
 // keep their 11 bits (with the largest at 1 those below 2^-14 lost some, and
 // outputs over thousands of keys half a rounding).  m is an integer, so that
-// rescaling is exact.  acc, l, m and the scores are fp32; a weight is rounded to
-// fp16 once, as the products' operand, and l takes it as rounded: where few
-// keys carry a row its rounding cancels.  A block whose V scale is far below
-// the others' (its V are zeros, say) has weights that fp16 rounds to nothing,
-// though its keys' share of l is as large as any: weights whose sum is small
-// enter l as they are.
+// rescaling is exact.  acc, l, m and the scores are fp32.  A weight is an operand
+// of the products in two fp16 parts where rows are few, and rounded to fp16
+// once where they are many, as a second product would cost as much as the first.
+// There l takes it as rounded: where few keys carry a row its rounding cancels.
+// A block whose V scale is far below the others' (its V are zeros, say) has
+// weights that fp16 rounds to nothing, though its keys' share of l is as large as
+// any: weights whose sum is small enter l as they are.
 #include <mutex>
 #include <type_traits>
 
@@ -166,7 +167,7 @@ __device__ __forceinline__ KvUnit load_unit(const KvUnit* p) {
 template <int D, int NW>
 struct StreamLds {
   float sum[NW][16][D + 4];  // the waves' results
-  float ml[NW][3][16];
+  float ml[NW][2][16];
   int last;
 };
 
@@ -203,15 +204,13 @@ __device__ __forceinline__ void fill_unseen(const KvAttnArgs& a, int req, int h)
 template <int D, int kFmt, bool kBf16, int NW>
 __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u, int h, StreamLds<D, NW>& lds) {
   constexpr int NJ = D / 64, KS = D / 32, ND = D / 16;
-  // fp16 outputs: weights in two fp16 parts, so that their rounding does not
-  // add to the output's own (error against 64 bits 2.9e-4 -> 2.1e-4 of the norm,
-  // where 2.1e-4 is one rounding); the products have the time, as the codes'
-  // way from memory takes longer (131000 keys 57.8 us with one part and with two,
-  // 12 drafts 16.4 and 16.5).  bf16 outputs round 8 times coarser.
-  constexpr bool kSplit = !kBf16;
+  // Weights go in two fp16 parts, 22 bits, so that their rounding does not add to
+  // the output's own (fp16: error against 64 bits 2.9e-4 -> 2.1e-4 of the norm, one
+  // rounding; bf16: 64 requests' outputs 7.6e-4 -> 5e-5 from those of fp32 weights).
+  // The products have the time, as the codes' way from memory takes longer:
+  // 131000 keys 57.8 us with one part and with two, 64 requests 82.7 and 82.9.
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
-  const bool want_lse = a.lse != nullptr;
   const int q0 = uniform(a.q_start[u.req]), q_len = uniform(a.q_start[u.req + 1]) - q0, kv_len = uniform(a.kv_len[u.req]);
   const int rows = q_len > kKvRowsA ? kKvRowsA : min(q_len * a.group, kKvRowsA);
 
@@ -288,8 +287,8 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
   // keys below this need no mask: every row of the unit sees them
   const int plain = kv_len - q_len + 1;
 
-  float m = kLowest, l = 0.0f, x = 0.0f;  // reference, sum of the rounded weights, sum of the weights
-  float sum_limit = kSumLimit;            // (below any sum where m is far)
+  float m = kLowest, l = 0.0f;  // reference, sum of the weights
+  float sum_limit = kSumLimit;  // (below any sum where m is far)
   float4_t acc[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) acc[d] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
@@ -314,12 +313,12 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
         see |= ((1u << n) - 1u) << (4 * s);
       }
     }
-    uint2 w[2], rest[2];  // weights, and (kSplit) what their rounding left
-    float dl, dx;
+    uint2 w[2], rest[2];  // weights, and what their rounding left
+    float dl;
     float gs[2] = {t.ks[0] * rowf, t.ks[1] * rowf}, lvs[2] = {t.lv[0], t.lv[1]};
     const auto weights = [&]() {
       float sums[2];
-      dl = dx = 0.0f;
+      dl = 0.0f;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const float g = gs[s], c = lvs[s] - m;
@@ -333,15 +332,10 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
           share = (see >> (4 * s)) & 0xF ? share : 0.0f;
         }
         w[s] = uint2{pack_f16(p[0], p[1]), pack_f16(p[2], p[3])};
-        const half2_t one = {(_Float16)1.0f, (_Float16)1.0f};
-        sums[s] = __builtin_amdgcn_fdot2(as_half2(w[s].y), one, __builtin_amdgcn_fdot2(as_half2(w[s].x), one, 0.0f, false), false);
-        if constexpr (kSplit) {
-          const half2_t a0 = as_half2(w[s].x), a1 = as_half2(w[s].y);
-          rest[s] = uint2{pack_f16(p[0] - (float)a0.x, p[1] - (float)a0.y), pack_f16(p[2] - (float)a1.x, p[3] - (float)a1.y)};
-        }
-        const float whole = (p[0] + p[1]) + (p[2] + p[3]);
-        dl = __builtin_fmaf(kSplit || sums[s] < kSmallSum ? whole : sums[s], share, dl);
-        if (!kSplit && want_lse) dx = __builtin_fmaf(whole, share, dx);
+        const half2_t a0 = as_half2(w[s].x), a1 = as_half2(w[s].y);
+        rest[s] = uint2{pack_f16(p[0] - (float)a0.x, p[1] - (float)a0.y), pack_f16(p[2] - (float)a1.x, p[3] - (float)a1.y)};
+        sums[s] = (p[0] + p[1]) + (p[2] + p[3]);
+        dl = __builtin_fmaf(sums[s], share, dl);
       }
       return fmaxf(sums[0], sums[1]);
     };
@@ -358,7 +352,7 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
       const float scale = exp2_fast(m - top);
       m = top;
       sum_limit = is_far(m) ? -1.0f : kSumLimit;
-      l *= scale, x *= scale;
+      l *= scale;
 #pragma unroll
       for (int d = 0; d < ND; ++d) acc[d] *= scale;
       if (__builtin_expect_with_probability(__any(is_far(m)), 0, 0.999)) {  // the scores become their weights' exponents
@@ -372,7 +366,6 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
       (void)weights();
     }
     l += dl;
-    if (!kSplit && want_lse) x += dx;
     uint32_t keep[2] = {~0u, ~0u};
     if (kFmt == NSMLP_KV_E4M3 && kMasked) {
       // codes past the end may be NaNs: a zero weight does not hide them
@@ -382,12 +375,12 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
         keep[s] = left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
       }
     }
-    const half8_t wh = join4(w[0], w[1]), wr = kSplit ? join4(rest[0], rest[1]) : wh;
+    const half8_t wh = join4(w[0], w[1]), wr = join4(rest[0], rest[1]);
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
       const half8_t v = join4(kv_half4<kFmt>(word(t.v[0][d >> 2], d & 3) & keep[0]), kv_half4<kFmt>(word(t.v[1][d >> 2], d & 3) & keep[1]));
       acc[d] = mfma16(v, wh, acc[d]);
-      if constexpr (kSplit) acc[d] = mfma16(v, wr, acc[d]);
+      acc[d] = mfma16(v, wr, acc[d]);
     }
   };
   if (begin < end) {
@@ -410,11 +403,10 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
   if (bad_seen != 0 && lane == 0) atomicOr(a.status, NSMLP_STATUS_BLOCK_UNAVAILABLE);
 
   mfma_drain();
-  if constexpr (kSplit) x = l;
   // join the waves: each result under the largest reference
-  l += __shfl_xor(l, 16, kWave), x += __shfl_xor(x, 16, kWave);
-  l += __shfl_xor(l, 32, kWave), x += __shfl_xor(x, 32, kWave);
-  if (grp == 0) lds.ml[wave][0][col] = m, lds.ml[wave][1][col] = l, lds.ml[wave][2][col] = x;
+  l += __shfl_xor(l, 16, kWave);
+  l += __shfl_xor(l, 32, kWave);
+  if (grp == 0) lds.ml[wave][0][col] = m, lds.ml[wave][1][col] = l;
   __syncthreads();
   {
     float top = kLowest;
@@ -431,13 +423,13 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
   __syncthreads();
   constexpr int kPerRow = NW * kWave / 16, kDims = D / kPerRow;
   const int row = tid / kPerRow, d0 = tid % kPerRow * kDims;
-  float mr = kLowest, lr = 0.0f, xr = 0.0f, o[kDims] = {};
+  float mr = kLowest, lr = 0.0f, o[kDims] = {};
 #pragma unroll
   for (int w = 0; w < NW; ++w) mr = fmaxf(mr, lds.ml[w][0][row]);
 #pragma unroll
   for (int w = 0; w < NW; ++w) {
     const float f = exp2_fast(lds.ml[w][0][row] - mr);
-    lr += lds.ml[w][1][row] * f, xr += lds.ml[w][2][row] * f;
+    lr += lds.ml[w][1][row] * f;
 #pragma unroll
     for (int d = 0; d < kDims; ++d) o[d] += lds.sum[w][row][d0 + d];
   }
@@ -458,7 +450,7 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
         if (row < rows) {
 #pragma unroll
           for (int d = 0; d < kDims; d += 2) st_coherent2(a.acc_a + at * D + d0 + d, o[d], o[d + 1]);
-          if (d0 == 0) st_coherent2(a.ml_a + 4 * at, mr, lr), st_coherent2(a.ml_a + 4 * at + 2, xr, 0.0f);
+          if (d0 == 0) st_coherent2(a.ml_a + 2 * at, mr, lr);
         }
         wait_stores();
         __syncthreads();
@@ -469,25 +461,25 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
         if (tid == 0) atomicExch(arrived, 0);
         if (row < rows) {
           const long long from = at + (group * 8 - idx) * step;
-          float2 ml[8][2], y[8][kDims / 2];
+          float2 ml[8], y[8][kDims / 2];
 #pragma unroll
           for (int p = 0; p < 8; ++p) {
             const long long q_at = from + min(p, size - 1) * step;  // (the last again: no branch between the reads)
-            ml[p][0] = ld_coherent2(a.ml_a + 4 * q_at), ml[p][1] = ld_coherent2(a.ml_a + 4 * q_at + 2);
+            ml[p] = ld_coherent2(a.ml_a + 2 * q_at);
 #pragma unroll
             for (int d = 0; d < kDims / 2; ++d) y[p][d] = ld_coherent2(a.acc_a + q_at * D + d0 + 2 * d);
           }
-          mr = ml[0][0].x;
+          mr = ml[0].x;
 #pragma unroll
-          for (int p = 1; p < 8; ++p) mr = fmaxf(mr, ml[p][0].x);
-          lr = xr = 0.0f;
+          for (int p = 1; p < 8; ++p) mr = fmaxf(mr, ml[p].x);
+          lr = 0.0f;
 #pragma unroll
           for (int d = 0; d < kDims; ++d) o[d] = 0.0f;
 #pragma unroll
           for (int p = 0; p < 8; ++p) {
-            const float f = exp2_fast(ml[p][0].x - mr);
+            const float f = exp2_fast(ml[p].x - mr);
             if (p < size) {
-              lr += ml[p][0].y * f, xr += ml[p][1].x * f;
+              lr += ml[p].y * f;
 #pragma unroll
               for (int d = 0; d < kDims / 2; ++d) o[2 * d] += y[p][d].x * f, o[2 * d + 1] += y[p][d].y * f;
             }
@@ -507,7 +499,7 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
       for (int d = 0; d < kDims; d += 2)
         *reinterpret_cast<uint32_t*>(a.out + at * D + d0 + d) =
             to_out<kBf16>(o[d] * inv) | (uint32_t)to_out<kBf16>(o[d + 1] * inv) << 16;
-      if (want_lse && d0 == 0) a.lse[at] = lse_of(mr, xr);
+      if (a.lse != nullptr && d0 == 0) a.lse[at] = lse_of(mr, lr);
     }
   }
 }
@@ -1093,7 +1085,7 @@ size_t kv_attn_partial_floats(const KvSchedule& s, int kv_heads, int D, size_t (
   size_t at = 0;
   const size_t ra = (size_t)s.max_parts_a * kv_heads * kKvRowsA, rb = (size_t)s.max_parts_b * kv_heads * s.rows_b;
   off[0] = at, at += ra * D;
-  off[1] = at, at += ra * 4;
+  off[1] = at, at += ra * 2;
   off[2] = at, at += rb * D;
   off[3] = at, at += rb * 4;
   return at;

@@ -157,7 +157,7 @@ struct KvAttnArgs {
   const int32_t *table, *q_start, *kv_len, *sched;
   int max_blocks, R, total, group;
   float scale_log2;  // softmax scale times log2(e)
-  float *acc_a, *ml_a, *acc_b, *ml_b;  // partial results of either list: [parts][kv_heads][rows][D], [..][4] (m, l, x)
+  float *acc_a, *ml_a, *acc_b, *ml_b;  // partial results of either list: [parts][kv_heads][rows][D], [..][2] (m, l), [..][4] (m, l, x)
   int *status, *count;  // status word, arrival counters [levels][kKvCounters] (zero, left zero)
   KvSchedule s;
 };

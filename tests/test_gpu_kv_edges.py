@@ -568,3 +568,37 @@ def test_append_of_many_tokens(gpu, fmt, block, D, lengths):
             at = to
         b.commit()
         assert torch.equal(whole.data, single.data) and torch.equal(whole.scale, single.scale)
+
+
+@pytest.mark.parametrize("fmt,Hq,H,D", [("e4m3", 32, 8, 128), ("int8", 16, 1, 64)])
+def test_weights_of_single_tokens_are_not_rounded_in_bf16(gpu, fmt, Hq, H, D):
+    """Streamed rows are the bf16 roundings of numbers within 2^-14 of the weights (fp32 scores up to 64 and sums) of the
+    formula: one rounding, and where a weight's to fp16 would add 2^-11 none."""
+    from next_step_ai_amd.kv_cache import KvBatch, KvCache, paged_attention
+
+    lengths, dtype = [700, 61, 1, 2500], torch.bfloat16
+    b = KvBatch(300, 16, max_requests=4, max_blocks=200, q_heads=Hq, kv_heads=H, head_dim=D)
+    c = KvCache(300, H, D, fmt=fmt)
+    g = torch.Generator(device=gpu).manual_seed(11)
+    st = b.plan(ints(lengths, gpu), sum(lengths))
+    c.append(*(torch.randn(sum(lengths), H, D, device=gpu, generator=g).to(dtype) for _ in range(2)), st.slots)
+    b.commit()
+    st = b.plan(ints([1] * 4, gpu), 4, max_new=1)
+    c.append(*(torch.randn(4, H, D, device=gpu, generator=g).to(dtype) for _ in range(2)), st.slots)
+    q = torch.randn(4, Hq, D, device=gpu, generator=g).to(dtype)
+    out = paged_attention(q, c, st)
+    for r, n in enumerate(lengths):
+        at = torch.arange(n + 1, device=gpu)
+        slots = st.table[r][at // 16].long() * 16 + at % 16
+        scale = c.scale[slots // 16].double()
+        # values as the codes say: what is read back, rounded to fp16, over the scale is near a code of 4 bits or a whole number
+        back = c.read(slots)
+        exact = []
+        for i, x in ((0, "k"), (1, "v")):
+            y = back[x].double() / scale[:, :, i, None]
+            exact.append((torch.round(y) if fmt == "int8" else y.float().to(torch.float8_e4m3fn).double()) * scale[:, :, i, None])
+        for h in range(Hq):
+            k, v = (x[:, h * H // Hq].contiguous() for x in exact)
+            p = torch.softmax(k @ q[r, h].double() * D ** -0.5, 0)
+            want, near = p @ v, 2.0 ** -14 * (p @ v.abs()) + 2.0 ** -24
+            assert ((want - near).to(dtype) <= out[r, h]).all() and (out[r, h] <= (want + near).to(dtype)).all()
