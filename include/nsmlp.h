@@ -586,10 +586,12 @@ size_t nsmlp_kv_schedule_bytes(const nsmlp_kv_batch* batch, int total, int max_n
  * the ring's (head, count) after the step, requests refused, the sum of
  * new_tokens.  Tokens of the step past that sum get slot -1.  The batch's
  * lengths and ring stay as they are until nsmlp_kv_commit, so that a plan can
- * be made again.  The schedule lists the attention's work. */
+ * be made again (with other new_tokens, requests after the first whose need
+ * changes get other blocks: rows appended for them are lost).  The schedule lists
+ * the attention's work. */
 int nsmlp_kv_plan(const nsmlp_kv_batch* batch, const int32_t* new_tokens, const nsmlp_kv_step* step, void* stream);
 
-/* Makes a step's lengths and ring state the batch's (step NULL: they stay),
+/* Makes a step's lengths (all of its new tokens) and ring state the batch's (step NULL: they stay),
  * then ends the requests with finished[r] != 0 (NULL: none): their blocks go to
  * the ring's end in the order of requests and of their tables, their entries
  * become -1 and their lengths 0. */
@@ -604,9 +606,12 @@ int nsmlp_kv_commit(const nsmlp_kv_batch* batch, const nsmlp_kv_step* step, cons
  * A token that sees no key (a refused request's) gets zeros and -inf; rows past
  * the step's tokens are left as they are.  A table entry that is not a block
  * (or past max_blocks) hides its keys and sets
- * NSMLP_STATUS_BLOCK_UNAVAILABLE in the workspace's status word.  fp32 sums;
- * the result does not depend on how the work is scheduled, only on the batch's
- * lengths.  scale > 0. */
+ * NSMLP_STATUS_BLOCK_UNAVAILABLE in the workspace's status word.  fp32 scores
+ * and sums; a softmax weight is an fp16 operand of the products, or two (22 bits)
+ * where a request has up to 16 rows per K/V head; the result does not depend on
+ * how the work is scheduled, only on the batch's lengths.  scale > 0.  The step
+ * is one that nsmlp_kv_plan has written; ws is cleared once by
+ * nsmlp_workspace_init. */
 size_t nsmlp_paged_attention_workspace_bytes(const nsmlp_kv_batch* batch, int total, int max_new, int head_dim);
 int nsmlp_paged_attention(const nsmlp_kv_cache* cache, const nsmlp_kv_batch* batch, const nsmlp_kv_step* step, const void* q,
                           long long q_row_stride, long long q_head_stride, int dtype, float scale, void* out, float* lse,

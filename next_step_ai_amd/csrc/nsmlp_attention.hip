@@ -161,8 +161,8 @@ __device__ __forceinline__ KvUnit load_unit(const KvUnit* p) {
 // together are cut into one equal share per CU, so that uneven lengths cost
 // nothing, and a wave has the next 32 keys' codes in flight while it works on
 // 32: 64 uneven requests (429 MB) 82 us, 5.2 TB/s; one token over 131000 keys
-// (269 MB, 31 partial results per row to join) 58 us, 4.7 TB/s.  A short chat (777
-// keys) takes 9.9 us, most of it the chain launch, schedule, lengths, block
+// (269 MB, 31 partial results per row to join) 57.5 us, 4.7 TB/s.  A short chat (777
+// keys) takes 9.5 us, most of it the chain launch, schedule, lengths, block
 // table, scales, codes, join.
 template <int D, int NW>
 struct StreamLds {
@@ -546,7 +546,7 @@ __global__ void __launch_bounds__(4 * kWave) k_attn_stream(KvAttnArgs a) {
 // decoding, shared by 128 or 256 rows).  A product follows another after about
 // 47 cycles instead of 32, half of a step with 8 waves is the wave's own vector
 // half, in which the SIMD's other wave has its products: 2048 tokens over 14336
-// cached, 128 heads of 128, 1.98 ms, 1.04 PFLOP/s, matrix cores busy 54%; a
+// cached, 128 heads of 128, 2.0 ms, 1.03 PFLOP/s, matrix cores busy 54%; a
 // prompt of 4000 tokens and 32 heads 165-180 us (0.73-0.79 PFLOP/s: 1000 tiles
 // of uneven length on 512 places).
 constexpr int kTileKeys = 64;

@@ -76,9 +76,9 @@ constexpr int kLeastShare = 4;     // pieces: 256 keys are worth a workgroup
 // last to end is what a smaller L shortens: w cost / L + L / 4 is least at `even`.
 // List a's keys count half, as the parts run next to them on the same CUs (a
 // prompt's 387 tokens next to 20 decodes: 39 us without, 32 with).
-// Costs of 128 and 512 over 27 drawn prompts, drafts and mixed steps: 0.2% longer
-// and 0.9% shorter calls on average, single ones 9% shorter to 8% longer and 20%
-// shorter to 9% longer; least parts of 96 and 384: 0.7% longer on average.
+// Costs of 128 and 512 over 25 drawn prompts, drafts and mixed steps: 0.2% longer
+// and 1% shorter calls on average, single ones 9% shorter to 8% longer and 20%
+// shorter to 9% longer; least parts of 96 and 384: 0.7% and 0.8% longer on average.
 constexpr float kPartCost = 256.0f, kLeastPart = 192.0f;
 
 // 1 / L of a request with `rows` rows in `tiles` tiles.  (Parts are counted in

@@ -138,7 +138,7 @@ class KvStep:
     [requests + 1], ``kv_len`` [requests], ``info`` [4] = (ring head, free
     blocks, refused requests, sum of new tokens) after it, ``table`` the batch's
     block table.  ``info`` and the others are device tensors: reading them
-    waits for the stream."""
+    waits for the stream.  ``planned``: whether a plan has written them."""
 
     __slots__ = ("batch", "total", "max_new", "slots", "planned", "_buf", "_layout", "_view", "_ref", "_split")
 
@@ -243,7 +243,8 @@ class KvBatch:
         the most of one request where the caller knows it (it decides which
         kernels the attention launches).  Lengths and free blocks stay as they
         are until :meth:`commit`; a plan that is not committed can be made
-        again.  ``step``: an earlier step of the same ``total`` and ``max_new``
+        again (with other ``new_tokens``, requests after the first whose need
+        of blocks changes get other ones).  ``step``: an earlier step of the same ``total`` and ``max_new``
         whose buffers are written again (a captured graph's)."""
         total, max_new = int(total), int(max_new)
         if new_tokens.dtype != torch.int32 or new_tokens.device != self.device or new_tokens.numel() != self.requests \
@@ -259,7 +260,7 @@ class KvBatch:
         return step
 
     def commit(self, finished: torch.Tensor | None = None) -> None:
-        """Make the last plan's lengths the batch's, and end the requests with
+        """Make the last plan's lengths (all of its new tokens) the batch's, and end the requests with
         ``finished`` [requests] (int32, not 0): their blocks become free."""
         if finished is not None and (finished.dtype != torch.int32 or finished.device != self.device
                                      or int(finished.numel()) != self.requests or not finished.is_contiguous()):
