@@ -501,14 +501,15 @@ int nsmlp_absmax_dq_dequantize(const uint8_t* q, long long n, int dq_block, cons
  * pinned buffers and H2D copies, RT:3437-3493, safetensor_loader.py:172-201). */
 int nsmlp_host_device_pointer(const void* host, void** device_ptr);
 
-/* --------------------------------------------- paged K/V cache in 8 bits
+/* ---------------------------------------- paged K/V cache in 8 or 4 bits
  * The attention side of a decoder layer: a cache of K and V rows in blocks of
  * `block_tokens` tokens (16, 32 or 64), 8 bits per value with one fp32 scale
- * per (block, K/V head) for K and one for V, the bookkeeping that hands the
+ * per (block, K/V head) for K and one for V, or 4 bits per value with one
+ * power of two per 32 dims of a token's row, the bookkeeping that hands the
  * blocks out, and the attention that reads it.  No reference counterpart (the
  * reference's attention and its K/V cache are torch code, RT:5927-7142).
  *
- * Formats: NSMLP_KV_INT8: code in -127..127, scale = largest magnitude times fp32(1 / 127).
+ * 8-bit formats: NSMLP_KV_INT8: code in -127..127, scale = largest magnitude times fp32(1 / 127).
  * NSMLP_KV_E4M3: OCP e4m3, scale = the smallest power of two that keeps the
  * largest magnitude within 448.  value = code * scale.  A (block, head)'s scale
  * never shrinks while the block is filled and is 2^-100 at least; where a call
@@ -518,11 +519,23 @@ int nsmlp_host_device_pointer(const void* host, void** device_ptr);
  * scale NaN until then (e4m3: and its codes zero, so that no code is a NaN).
  * data: [num_blocks][kv_heads][2][block_tokens * head_dim] bytes in an order of
  * the library's own; scale: [num_blocks][kv_heads][2] (K, V).  Both are zeroed
- * once by the caller.  head_dim 64 or 128; 16-byte aligned. */
+ * once by the caller.  head_dim 64 or 128; 16-byte aligned.
+ *
+ * 4-bit format: NSMLP_KV_E2M1: OCP e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a
+ * sign), rounded to nearest, ties to the even code; scale = the smallest power
+ * of two, from 2^-23 to 2^13, that keeps the largest magnitude of 32
+ * neighbouring dims of a token's K or V within 6.  So every stored value is an
+ * fp16 number: magnitudes past 49152 become 49152, those up to 2^-25 zero.  Stored
+ * tokens are never rewritten.  A token whose K or V row (of a K/V head) holds a
+ * value that is not finite reads as NaN, in K and V, until its slot is written
+ * again.  data: [num_blocks][kv_heads][block_tokens * head_dim * 17 / 16] bytes
+ * (codes and scales) in an order of the library's own, zeroed once by the
+ * caller; scale is not used. */
 #define NSMLP_DTYPE_F16 0
 #define NSMLP_DTYPE_BF16 1
 #define NSMLP_KV_INT8 0
 #define NSMLP_KV_E4M3 1
+#define NSMLP_KV_E2M1 4
 
 typedef struct nsmlp_kv_cache {
   int num_blocks, kv_heads, head_dim, block_tokens, format;
@@ -533,11 +546,35 @@ typedef struct nsmlp_kv_cache {
 /* Stores K and V rows k, v [n][kv_heads][head_dim] (strides in elements,
  * multiples of 8; the last dimension contiguous) at slots[n] (block *
  * block_tokens + offset; a slot outside the cache, such as -1, stores nothing).
- * The tokens of one block stand next to each other in the call, in the order
- * of their offsets, as nsmlp_kv_plan lists them. */
+ * No slot stands twice in a call.  In 8 bits the tokens of one block stand next
+ * to each other in the call, in the order of their offsets, as nsmlp_kv_plan
+ * lists them. */
 int nsmlp_kv_append(const nsmlp_kv_cache* cache, const void* k, long long k_row_stride, long long k_head_stride,
                     const void* v, long long v_row_stride, long long v_head_stride, int dtype, const int64_t* slots, int n,
                     void* stream);
+
+/* Angles of a rotary position encoding: table [positions][head_dim / 2][2]
+ * fp32, cos and sin of position * frequency i, 16-byte aligned.  interleaved 0:
+ * frequency i turns dims i and i + head_dim / 2; 1: dims 2 i and 2 i + 1. */
+typedef struct nsmlp_rotary {
+  int positions, head_dim, interleaved;
+  const float* table;
+} nsmlp_rotary;
+
+/* nsmlp_kv_append with the rows of K turned by their positions on the way, and
+ * query rows turned next to them.  A pair (a, b) becomes a cos - b sin, b cos +
+ * a sin: the exact sum of the two products rounded to fp32 and then to dtype, so
+ * that what is stored is what nsmlp_kv_append stores of such rows.
+ * positions[n]: a row of K whose position is not in the table becomes NaN.
+ * q [n][q_heads][head_dim] (strides as k's; NULL: none) goes to q_out, which
+ * may be q itself with the same strides and must not overlap it otherwise; a
+ * row whose position is negative (a token of no request) is left as it was in
+ * q_out, one past the table becomes NaN.  k is not changed. */
+int nsmlp_kv_append_rotated(const nsmlp_kv_cache* cache, const nsmlp_rotary* rotary, const void* k, long long k_row_stride,
+                            long long k_head_stride, const void* v, long long v_row_stride, long long v_head_stride, int dtype,
+                            const int64_t* slots, const int32_t* positions, int n, const void* q, long long q_row_stride,
+                            long long q_head_stride, int q_heads, void* q_out, long long out_row_stride,
+                            long long out_head_stride, void* stream);
 
 /* The stored values at slots[n], rounded to dtype: k_out, v_out
  * [n][kv_heads][head_dim], contiguous; zeros for a slot outside the cache. */
@@ -560,8 +597,9 @@ typedef struct nsmlp_kv_batch {
 
 /* One step of a batch.  total: tokens of the step's tensors; max_new: the most
  * new tokens of a request (0: not known).  slots[total], q_start[requests + 1],
- * kv_len[requests], next[requests], info[4] and the schedule
- * (nsmlp_kv_schedule_bytes) are written by nsmlp_kv_plan. */
+ * kv_len[requests], next[requests], info[4], the schedule
+ * (nsmlp_kv_schedule_bytes) and, where it is not NULL, positions[total] are
+ * written by nsmlp_kv_plan. */
 typedef struct nsmlp_kv_step {
   int total, max_new;
   int64_t* slots;
@@ -571,6 +609,7 @@ typedef struct nsmlp_kv_step {
   int32_t* info;
   int32_t* schedule;
   size_t schedule_bytes;
+  int32_t* positions;
 } nsmlp_kv_step;
 
 size_t nsmlp_kv_schedule_bytes(const nsmlp_kv_batch* batch, int total, int max_new); /* 0: invalid arguments */
@@ -578,8 +617,9 @@ size_t nsmlp_kv_schedule_bytes(const nsmlp_kv_batch* batch, int total, int max_n
 /* Plans a step that adds new_tokens[requests] tokens: request r takes
  * ceil((cached + new) / block_tokens) - ceil(cached / block_tokens) blocks from
  * the ring's front, requests in order, and its table entries are written.
- * slots: the step's tokens, request by request; q_start: where each request's
- * tokens start; kv_len: cached + new.  A request is refused (slots -1, kv_len
+ * slots: the step's tokens, request by request; positions: how many of its
+ * request's tokens stand before each (-1 where the slot is); q_start: where each
+ * request's tokens start; kv_len: cached + new.  A request is refused (slots -1, kv_len
  * 0, nothing taken) where its blocks would exceed max_blocks, its new tokens
  * max_new, or the blocks asked for up to and with it the free ones (requests
  * refused for the first two ask for none).  info:

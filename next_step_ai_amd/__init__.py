@@ -5,7 +5,8 @@ Modules:
               entry points (same names and signatures)
   router      the learned-basis router on the GPU (route_sparse_mlp)
   slot_table  the HBM hot-block slot table and the one-call decode layer
-  kv_cache    paged K/V cache in 8 bits, its block tables and its attention
+  kv_cache    paged K/V cache in 8 or 4 bits, its block tables and its attention
+  rotary      angles of a rotary position encoding
   layout      block-bank layout contract and the active-block layout
   synth       seeded synthetic NF4 layers generated on the GPU
 """

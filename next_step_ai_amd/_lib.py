@@ -34,6 +34,7 @@ NSMLP_DTYPE_F16 = 0
 NSMLP_DTYPE_BF16 = 1
 NSMLP_KV_INT8 = 0
 NSMLP_KV_E4M3 = 1
+NSMLP_KV_E2M1 = 4
 
 
 class SlotTable(ctypes.Structure):
@@ -106,8 +107,14 @@ class KvStepView(ctypes.Structure):
 
     _fields_ = [
         ("total", I32), ("max_new", I32), ("slots", P), ("q_start", P), ("kv_len", P), ("next", P), ("info", P),
-        ("schedule", P), ("schedule_bytes", SZ),
+        ("schedule", P), ("schedule_bytes", SZ), ("positions", P),
     ]
+
+
+class RotaryView(ctypes.Structure):
+    """Mirror of ``nsmlp_rotary``."""
+
+    _fields_ = [("positions", I32), ("head_dim", I32), ("interleaved", I32), ("table", P)]
 
 
 # name -> (restype, argtypes)
@@ -156,6 +163,8 @@ SIGNATURES: dict[str, tuple] = {
     "nsmlp_cache_promote": (I32, [ctypes.POINTER(SlotTable), ctypes.POINTER(CacheState), P, I32, I32, P, P, SZ, P]),
     "nsmlp_cache_record_f32": (I32, [P, I32, P, I32, I32, P, P]),
     "nsmlp_kv_append": (I32, [ctypes.POINTER(KvCacheView), P, I64, I64, P, I64, I64, I32, P, I32, P]),
+    "nsmlp_kv_append_rotated": (I32, [ctypes.POINTER(KvCacheView), ctypes.POINTER(RotaryView), P, I64, I64, P, I64, I64, I32, P, P,
+                                      I32, P, I64, I64, I32, P, I64, I64, P]),
     "nsmlp_kv_read": (I32, [ctypes.POINTER(KvCacheView), P, I32, P, P, I32, P]),
     "nsmlp_kv_schedule_bytes": (SZ, [ctypes.POINTER(KvBatchView), I32, I32]),
     "nsmlp_kv_plan": (I32, [ctypes.POINTER(KvBatchView), P, ctypes.POINTER(KvStepView), P]),

@@ -1,4 +1,4 @@
-// Attention over the paged 8-bit K/V cache (layouts: nsmlp_kv.h).
+// Attention over the paged K/V cache in 8 or 4 bits (layouts: nsmlp_kv.h).
 //
 // For a query row and the keys j it sees, with codes k, v, scales ks, vs of
 // the key's (block, head) and c = softmax scale * log2(e):
@@ -22,6 +22,15 @@
 // A block whose V scale is far below the others' (its V are zeros, say) has
 // weights that fp16 rounds to nothing, though its keys' share of l is as large as
 // any: weights whose sum is small enter l as they are.
+//
+// In 4 bits a code's scale is its token's and its 32 dims', so it cannot leave the
+// products: codes are decoded to their values, which are fp16 numbers, by the
+// conversion that applies the scale, and vs = ks = 1 above.  A pair of V operands
+// is of two tokens, whose scales differ, while a conversion takes one scale for
+// the two codes of a byte: bytes hold two dims of one token, and a byte permute
+// per pair brings the tokens together.  (A token that is not finite has a NaN
+// for its K scale and zeros for V: its score is NaN where it is seen, and V is
+// finite in any place that a weight of zero hides.)
 #include <mutex>
 #include <type_traits>
 
@@ -98,7 +107,8 @@ __device__ __forceinline__ float far_exponent(float s, float g, float lv, float 
   return is_far(m) ? fminf((t - m) + lv, 15.0f) : (t - m) + lv;
 }
 
-// Pages of a range of keys, held one per lane: 64 pages from page `first`.
+// Pages of a range of keys, held one per lane: 64 pages from page `first`.  (In 4
+// bits the scales are read with the codes.)
 struct Pages {
   uint32_t lo, hi;   // where the (block, head)'s codes start (block 0's where the entry is not a block)
   float ks, lv, iv;  // K scale, log2 of the V scale, kUnit over it
@@ -106,6 +116,7 @@ struct Pages {
   int first;
 };
 
+template <int kFmt>
 __device__ __forceinline__ Pages load_pages(const KvAttnArgs& a, int req, int h, int first, int last, int lane) {
   Pages p;
   p.first = first;
@@ -113,11 +124,15 @@ __device__ __forceinline__ Pages load_pages(const KvAttnArgs& a, int req, int h,
   const int id = a.table[(long long)req * a.max_blocks + pg];
   const bool ok = id >= 0 && id < a.c.num_blocks;
   const long long bh = (long long)(ok ? id : 0) * a.c.heads + h;
-  const long long off = bh * (2 * a.c.B * a.c.D);
+  const long long off = bh * kv_block_bytes<kFmt>(a.c.B, a.c.D);
   p.lo = (uint32_t)off, p.hi = (uint32_t)(off >> 32);
+  p.bad = __ballot(!ok);
+  if constexpr (kFmt == NSMLP_KV_E2M1) {
+    p.ks = 1.0f, p.lv = 0.0f, p.iv = kUnit;
+    return p;
+  }
   const float2 s = *reinterpret_cast<const float2*>(a.c.scale + bh * 2);
   const float sv = s.y == 0.0f ? kKvScaleMin : s.y;  // a block that nothing was stored in
-  p.bad = __ballot(!ok);
   p.ks = s.x;
   p.lv = log2_fast(sv);
   p.iv = kUnit / sv;
@@ -131,6 +146,47 @@ __device__ __forceinline__ const uint8_t* page_data(const KvAttnArgs& a, const P
 
 __device__ __forceinline__ float lane_of(float v, int i) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i));
+}
+
+// What a lane holds of 16 tokens' K or V in 4 bits: D/32 dwords.
+template <int D>
+struct Codes4 {
+  uint32_t w[D / 32];
+};
+template <int D>
+__device__ __forceinline__ Codes4<D> load_codes4(const uint8_t* p) {
+  Codes4<D> o;
+  if constexpr (D == 128) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    o.w[0] = v.x, o.w[1] = v.y, o.w[2] = v.z, o.w[3] = v.w;
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    o.w[0] = v.x, o.w[1] = v.y;
+  }
+  return o;
+}
+__device__ __forceinline__ float scale4(uint32_t bytes, int i) { return __uint_as_float(((bytes >> (8 * i)) & 0xFFu) << 23); }
+
+// the two values of byte i (known when compiled) under a scale
+__device__ __forceinline__ uint32_t values4(uint32_t w, float scale, int i) {
+  half2_t v = i == 0   ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 0)
+              : i == 1 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 1)
+              : i == 2 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 2)
+                       : __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 3);
+  return __builtin_bit_cast(uint32_t, v);
+}
+// Of 4 tokens' values of two neighbouring dims: the lower dim's, the upper's.
+__device__ __forceinline__ uint2 lower4(const uint32_t (&v)[4]) {
+  return uint2{__builtin_amdgcn_perm(v[1], v[0], 0x05040100u), __builtin_amdgcn_perm(v[3], v[2], 0x05040100u)};
+}
+__device__ __forceinline__ uint2 upper4(const uint32_t (&v)[4]) {
+  return uint2{__builtin_amdgcn_perm(v[1], v[0], 0x07060302u), __builtin_amdgcn_perm(v[3], v[2], 0x07060302u)};
+}
+// Token j's two values of the m-th byte of its D/16 dims, j = 0..3.
+template <int D>
+__device__ __forceinline__ uint32_t token_values4(const Codes4<D>& c, uint32_t scales, int j, int m) {
+  if constexpr (D == 128) return values4(c.w[j], scale4(scales, j), m);
+  else return values4(c.w[j >> 1], scale4(scales, j), m + 2 * (j & 1));
 }
 
 // What a row's acc is multiplied by, and its lse, at the end.
@@ -171,10 +227,16 @@ struct StreamLds {
   int last;
 };
 
-template <int D>
+template <int D, int kFmt>
 struct StreamTile {  // 32 keys, two tiles of 16: codes, and their blocks' scales in scalar registers
   uint4 k[2][D / 64], v[2][D / 64];
   float ks[2], lv[2], iv[2];
+  int bad;
+};
+template <int D>
+struct StreamTile<D, NSMLP_KV_E2M1> {
+  Codes4<D> k[2], v[2];
+  uint32_t ks[2], vs[2];  // scale bytes: of the lane's K, of its 4 tokens of V
   int bad;
 };
 
@@ -204,6 +266,7 @@ __device__ __forceinline__ void fill_unseen(const KvAttnArgs& a, int req, int h)
 template <int D, int kFmt, bool kBf16, int NW>
 __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u, int h, StreamLds<D, NW>& lds) {
   constexpr int NJ = D / 64, KS = D / 32, ND = D / 16;
+  constexpr bool k4 = kFmt == NSMLP_KV_E2M1;
   // Weights go in two fp16 parts, 22 bits, so that their rounding does not add to
   // the output's own (fp16: error against 64 bits 2.9e-4 -> 2.1e-4 of the norm, one
   // rounding; bf16: 64 requests' outputs 7.6e-4 -> 5e-5 from those of fp32 weights).
@@ -222,37 +285,52 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
   // the first tiles' codes are on their way while the queries are made ready
   unsigned long long bad_seen = 0;
   Pages pages;
-  const auto load = [&](StreamTile<D>& t, int pos) {
+  // where the lane's scales of 16 tokens are, in 4 bits (K: D/4 dims of a token, V: D/16 dims of 4 tokens)
+  const int ks_at = a.c.B * D + (grp * (D / 4) >> 5) * 16 + col;
+  const int vs_at = a.c.B * D + a.c.B * D / 32 + (grp * (D / 32) + (col * (D / 16) >> 5)) * 4;
+  const auto load = [&](StreamTile<D, kFmt>& t, int pos) {
     t.bad = 0;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int at = pos + 16 * s, pg = min(at >> a.c.b_shift, last) - pages.first;
-      t.ks[s] = lane_of(pages.ks, pg), t.lv[s] = lane_of(pages.lv, pg), t.iv[s] = lane_of(pages.iv, pg);
-      t.bad |= ((int)(pages.bad >> pg) & 1) << s;
-      const uint8_t* kb = page_data(a, pages, pg) + ((at & (a.c.B - 1)) >> 4) * (16 * D);
-      const uint8_t* vb = kb + a.c.B * D;
+      if constexpr (k4) {
+        t.bad |= ((int)(pages.bad >> pg) & 1) << s;
+        const uint8_t* base = page_data(a, pages, pg);
+        const int tile = (at & (a.c.B - 1)) >> 4;
+        t.k[s] = load_codes4<D>(base + tile * (8 * D) + lane * (D / 8));
+        t.v[s] = load_codes4<D>(base + a.c.B * D / 2 + tile * (8 * D) + lane * (D / 8));
+        t.ks[s] = base[ks_at + tile * (D / 2)];
+        t.vs[s] = *reinterpret_cast<const uint32_t*>(base + vs_at + tile * (D / 2));
+        continue;
+      } else {
+        t.ks[s] = lane_of(pages.ks, pg), t.lv[s] = lane_of(pages.lv, pg), t.iv[s] = lane_of(pages.iv, pg);
+        t.bad |= ((int)(pages.bad >> pg) & 1) << s;
+        const uint8_t* kb = page_data(a, pages, pg) + ((at & (a.c.B - 1)) >> 4) * (16 * D);
+        const uint8_t* vb = kb + a.c.B * D;
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        t.k[s][j] = *reinterpret_cast<const uint4*>(kb + j * 1024 + lane * 16);
-        t.v[s][j] = *reinterpret_cast<const uint4*>(vb + j * 1024 + lane * 16);
+        for (int j = 0; j < NJ; ++j) {
+          t.k[s][j] = *reinterpret_cast<const uint4*>(kb + j * 1024 + lane * 16);
+          t.v[s][j] = *reinterpret_cast<const uint4*>(vb + j * 1024 + lane * 16);
+        }
       }
     }
   };
   // past the wave's keys its last tile is read again: no branch around a load
   const int last_tile = begin < end ? begin + ((end - 1 - begin) & ~31) : begin;
-  const auto fetch = [&](StreamTile<D>& t, int pos) {
+  const auto fetch = [&](StreamTile<D, kFmt>& t, int pos) {
     pos = min(pos, last_tile);
     if (min((pos + 31) >> a.c.b_shift, last) - pages.first >= kWave) {
-      pages = load_pages(a, u.req, h, pos >> a.c.b_shift, last, lane);
+      pages = load_pages<kFmt>(a, u.req, h, pos >> a.c.b_shift, last, lane);
       bad_seen |= pages.bad;
     }
     load(t, pos);
   };
-  StreamTile<D> t0, t1;
+  StreamTile<D, kFmt> t0, t1, t2, t3;  // (in 8 bits the last two are not used)
   if (begin < end) {
-    pages = load_pages(a, u.req, h, begin >> a.c.b_shift, last, lane);
+    pages = load_pages<kFmt>(a, u.req, h, begin >> a.c.b_shift, last, lane);
     bad_seen = pages.bad;
     load(t0, begin);
+    if constexpr (k4) fetch(t1, begin + 32), fetch(t2, begin + 64);
   }
 
   // queries: columns of the products, 8 dims per lane and step
@@ -266,7 +344,8 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
     uint4 raw[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s)
-      raw[s] = in ? *reinterpret_cast<const uint4*>(src + 64 * (s >> 1) + 16 * grp + 8 * (s & 1)) : uint4{0, 0, 0, 0};
+      raw[s] = in ? *reinterpret_cast<const uint4*>(src + (k4 ? (D / 4) * grp + 8 * s : 64 * (s >> 1) + 16 * grp + 8 * (s & 1)))
+                  : uint4{0, 0, 0, 0};
     if constexpr (kBf16) {
       uint32_t top = 0;
 #pragma unroll
@@ -293,15 +372,22 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
 #pragma unroll
   for (int d = 0; d < ND; ++d) acc[d] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
-  const auto use = [&](auto masked, const StreamTile<D>& t, int pos) {
+  const auto use = [&](auto masked, const StreamTile<D, kFmt>& t, int pos) {
     constexpr bool kMasked = decltype(masked)::value;
     float4_t sc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
     for (int i = 0; i < KS; ++i)
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-        sc[s] = mfma16(join4(kv_half4<kFmt>(word(t.k[s][i >> 1], 2 * (i & 1))), kv_half4<kFmt>(word(t.k[s][i >> 1], 2 * (i & 1) + 1))),
-                       q[i], sc[s]);
+      for (int s = 0; s < 2; ++s) {
+        if constexpr (k4) {
+          const float f = scale4(t.ks[s], 0);
+          const uint32_t c = t.k[s].w[i];
+          sc[s] = mfma16(as_h8(uint4{values4(c, f, 0), values4(c, f, 1), values4(c, f, 2), values4(c, f, 3)}), q[i], sc[s]);
+        } else {
+          sc[s] = mfma16(join4(kv_half4<kFmt>(word(t.k[s][i >> 1], 2 * (i & 1))), kv_half4<kFmt>(word(t.k[s][i >> 1], 2 * (i & 1) + 1))),
+                         q[i], sc[s]);
+        }
+      }
     mfma_drain();
     // bit 4 s + i: whether the row sees the lane's key i of the s-th 16
     uint32_t see = 0xFF;
@@ -315,14 +401,19 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
     }
     uint2 w[2], rest[2];  // weights, and what their rounding left
     float dl;
-    float gs[2] = {t.ks[0] * rowf, t.ks[1] * rowf}, lvs[2] = {t.lv[0], t.lv[1]};
+    float gs[2], lvs[2], ivs[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      if constexpr (k4) gs[s] = rowf, lvs[s] = 0.0f, ivs[s] = kUnit;
+      else gs[s] = t.ks[s] * rowf, lvs[s] = t.lv[s], ivs[s] = t.iv[s];
+    }
     const auto weights = [&]() {
       float sums[2];
       dl = 0.0f;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const float g = gs[s], c = lvs[s] - m;
-        float p[4], share = t.iv[s];
+        float p[4], share = ivs[s];
 #pragma unroll
         for (int i = 0; i < 4; ++i) p[i] = exp2_fast(__builtin_fmaf(sc[s][i], g, c));
         if constexpr (kMasked) {
@@ -376,14 +467,53 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
       }
     }
     const half8_t wh = join4(w[0], w[1]), wr = join4(rest[0], rest[1]);
+    if constexpr (k4) {
+#pragma unroll
+      for (int m2 = 0; m2 < ND / 2; ++m2) {
+        uint32_t c[2][4];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) c[s][j] = token_values4<D>(t.v[s], t.vs[s], j, m2);
+        const half8_t lo = join4(lower4(c[0]), lower4(c[1])), hi = join4(upper4(c[0]), upper4(c[1]));
+        acc[2 * m2] = mfma16(lo, wh, acc[2 * m2]);
+        acc[2 * m2] = mfma16(lo, wr, acc[2 * m2]);
+        acc[2 * m2 + 1] = mfma16(hi, wh, acc[2 * m2 + 1]);
+        acc[2 * m2 + 1] = mfma16(hi, wr, acc[2 * m2 + 1]);
+      }
+      return;
+    }
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
-      const half8_t v = join4(kv_half4<kFmt>(word(t.v[0][d >> 2], d & 3) & keep[0]), kv_half4<kFmt>(word(t.v[1][d >> 2], d & 3) & keep[1]));
-      acc[d] = mfma16(v, wh, acc[d]);
-      acc[d] = mfma16(v, wr, acc[d]);
+      if constexpr (!k4) {
+        const half8_t v = join4(kv_half4<kFmt>(word(t.v[0][d >> 2], d & 3) & keep[0]), kv_half4<kFmt>(word(t.v[1][d >> 2], d & 3) & keep[1]));
+        acc[d] = mfma16(v, wh, acc[d]);
+        acc[d] = mfma16(v, wr, acc[d]);
+      }
     }
   };
-  if (begin < end) {
+  if (k4 && begin < end) {
+    // half the bytes of a key: three tiles' codes on their way behind the one in use
+    int pos = begin;
+    while (pos + 128 <= min(end, plain) && bad_seen == 0) {
+      fetch(t3, pos + 96);
+      if (bad_seen != 0) break;  // (of a new window of pages, which may be t3's; t0 to t2 are older or looked at next time)
+      use(std::false_type{}, t0, pos);
+      fetch(t0, pos + 128);
+      use(std::false_type{}, t1, pos + 32);
+      fetch(t1, pos + 160);
+      use(std::false_type{}, t2, pos + 64);
+      fetch(t2, pos + 192);
+      use(std::false_type{}, t3, pos + 96);
+      pos += 128;
+    }
+    while (pos < end) {
+      fetch(t3, pos + 96);
+      use(std::true_type{}, t0, pos);
+      t0 = t1, t1 = t2, t2 = t3;
+      pos += 32;
+    }
+  } else if (begin < end) {
     int pos = begin;
     while (pos + 64 <= min(end, plain) && bad_seen == 0) {  // two tiles, the next two's codes behind them
       fetch(t1, pos + 32);
@@ -413,8 +543,16 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
 #pragma unroll
     for (int w = 0; w < NW; ++w) top = fmaxf(top, lds.ml[w][0][col]);
     const float scale = exp2_fast(m - top);
+    if constexpr (k4) {
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int n = 0; n < ND; n += 4)
+          *reinterpret_cast<float4_t*>(&lds.sum[wave][col][ND * (4 * grp + i) + n]) =
+              float4_t{acc[n][i], acc[n + 1][i], acc[n + 2][i], acc[n + 3][i]} * scale;
+    }
+#pragma unroll
+    for (int j = 0; !k4 && j < NJ; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         *reinterpret_cast<float4_t*>(&lds.sum[wave][col][64 * j + 16 * grp + 4 * i]) =
@@ -568,6 +706,7 @@ constexpr int kTileLds = 2 * kTileBytes<D> + 4 * 4 * (int)sizeof(TileMeta);
 template <int D, int kFmt, bool kBf16, int NW, bool kLse>
 __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, int h, char* lds) {
   constexpr int KS = D / 16, ND = D / 32, kRows = 32 * NW;
+  constexpr bool k4 = kFmt == NSMLP_KV_E2M1;
   constexpr int kKBytes = 2 * KS * 1024, kVBytes = 4 * ND * 1024;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
@@ -591,7 +730,15 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
 #pragma unroll
   for (int o = 0; o < kRoles; ++o) {
     const bool v = kRoles == 2 ? o == 1 : upper;
-    if constexpr (D == 128) {
+    if constexpr (k4) {
+      // K: D/4 dims of a token; V: 4 tokens of D/16 dims, and the 4 tokens 8 behind them, a half of the dims each lane
+      const int g = lane >> 4, t = lane & 15;
+      src[o] = v ? a.c.B * D / 2 + (half * 16 + t) * (D / 8) : lane * (D / 8);
+      src2[o] = src[o] + 4 * D;
+      dst[o] = v ? kKBytes + (part * ND * 64 + lane) * 16
+                 : ((((part >> 1) * KS + (g >> 1) * (D / 32)) * 64) + (g & 1) * 32 + (part & 1) * 16 + t) * 16;
+      dst_step[o] = 1024;
+    } else if constexpr (D == 128) {
       const int g = lane >> 4, t = lane & 15;
       src[o] = v ? a.c.B * D + (g & 1) * 1024 + half * 256 + t * 16 : lane * 16;
       src2[o] = src[o] + (v ? 512 : 1024);
@@ -607,18 +754,66 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
     }
   }
   unsigned long long bad_seen = 0;
-  Pages pages = load_pages(a, u.req, h, u.kv_begin >> a.c.b_shift, last, lane);
+  Pages pages = load_pages<kFmt>(a, u.req, h, u.kv_begin >> a.c.b_shift, last, lane);
   if (tiles > 0) bad_seen = pages.bad;
   // whether V scales so far lie more than a factor of 2^4 from the first one: only
   // then can a weight that matters to l be too small for fp16 (the largest is
   // 2^10, and weights below 2^-27 of it are lost at most)
   const float lv_first = lane_of(pages.lv, 0);
-  const auto apart = [&]() { return __ballot(!(fabsf(pages.lv - lv_first) <= 4.0f)); };
+  const auto apart = [&]() { return k4 ? 0ull : __ballot(!(fabsf(pages.lv - lv_first) <= 4.0f)); };
   unsigned long long uneven = apart();
   // this wave's page in tile i, as a lane of `pages`; past the last tile again the last
   const auto at_of = [&](int i) { return u.kv_begin + min(i, tiles - 1) * kTileKeys + 16 * part; };
   const auto page_of = [&](int i) { return min(at_of(i) >> a.c.b_shift, last) - pages.first; };
   uint4 raw[kRoles][2];
+  Codes4<D> raw4[kRoles][2];   // in 4 bits: codes, and scale bytes
+  uint32_t scales[kRoles][2];
+  // where the lane's scales of 16 tokens are (K: one byte; V: 4 tokens each)
+  const int ks_at = a.c.B * D + ((lane >> 4) * (D / 4) >> 5) * 16 + (lane & 15);
+  const int vs_at = a.c.B * D + a.c.B * D / 32 + (half * (D / 32) + ((lane & 15) * (D / 16) >> 5)) * 4;
+  const auto fetch4 = [&](auto is_v, int o, int i) {
+    const int at = at_of(i), tile = (at & (a.c.B - 1)) >> 4;
+    const uint8_t* base = page_data(a, pages, page_of(i));
+    raw4[o][0] = load_codes4<D>(base + tile * (8 * D) + src[o]);
+    if constexpr (decltype(is_v)::value) {
+      raw4[o][1] = load_codes4<D>(base + tile * (8 * D) + src2[o]);
+      scales[o][0] = *reinterpret_cast<const uint32_t*>(base + vs_at + tile * (D / 2));
+      scales[o][1] = *reinterpret_cast<const uint32_t*>(base + vs_at + tile * (D / 2) + D / 4);
+    } else {
+      scales[o][0] = base[ks_at + tile * (D / 2)];
+    }
+  };
+  // K: a dword's 8 values in two steps; V: two dims' 8 tokens in four
+  uint2 first4[2], second4[2];
+  const auto decode4 = [&](auto is_v, int o, char* buf, int step) {
+    if constexpr (decltype(is_v)::value) {
+      const int m = step >> 2;
+      if (m >= D / 64) return;
+      if ((step & 3) < 2) {
+        const int i = step & 1;
+        // the lane's half of a token's dims
+        const int shift = (lane >> 4 & 1) * (D / 8);
+        uint32_t v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t w = D == 128 ? raw4[o][i].w[j & (D / 32 - 1)] : raw4[o][i].w[j >> 1];
+          v[j] = values4(w >> shift, scale4(scales[o][i], j), D == 128 ? m : 2 * (j & 1));
+        }
+        (i == 0 ? first4 : second4)[0] = lower4(v), (i == 0 ? first4 : second4)[1] = upper4(v);
+      } else {
+        const int k = step & 1;
+        *reinterpret_cast<uint4*>(buf + dst[o] + (2 * m + k) * 1024) = uint4{first4[k].x, first4[k].y, second4[k].x, second4[k].y};
+      }
+    } else {
+      const int j = step >> 1;
+      if (j >= D / 32) return;
+      const float f = scale4(scales[o][0], 0);
+      const uint32_t w = raw4[o][0].w[j];
+      if (!(step & 1)) first4[0] = uint2{values4(w, f, 0), values4(w, f, 1)};
+      else
+        *reinterpret_cast<uint4*>(buf + dst[o] + j * 1024) = uint4{first4[0].x, first4[0].y, values4(w, f, 2), values4(w, f, 3)};
+    }
+  };
   const auto fetch = [&](int o, int i) {
     const int at = at_of(i);
     const uint8_t* base = page_data(a, pages, page_of(i)) + ((at & (a.c.B - 1)) >> 4) * (16 * D);
@@ -664,13 +859,16 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
   int turn_at = window_end();
   const auto turn_pages = [&](int from, int need) {
     if (__builtin_expect_with_probability(need >= turn_at, 0, 0.95)) {
-      pages = load_pages(a, u.req, h, (u.kv_begin + min(from, tiles - 1) * kTileKeys) >> a.c.b_shift, last, lane);
+      pages = load_pages<kFmt>(a, u.req, h, (u.kv_begin + min(from, tiles - 1) * kTileKeys) >> a.c.b_shift, last, lane);
       bad_seen |= pages.bad;
       uneven |= apart();
       turn_at = window_end();
     }
   };
-  if (tiles > 0) {
+  if (k4 && tiles > 0) {
+    if (!upper) fetch4(std::false_type{}, 0, 0);
+    if (upper || kRoles == 2) fetch4(std::true_type{}, kRoles - 1, 0);
+  } else if (tiles > 0) {
 #pragma unroll
     for (int o = 0; o < kRoles; ++o) fetch(o, 0);
   }
@@ -682,6 +880,11 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
     uint4 part_q[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
+      if constexpr (k4) {
+        const int at = (D / 4) * (2 * (s / (D / 32)) + half) + 8 * (s % (D / 32));
+        part_q[s] = in ? *reinterpret_cast<const uint4*>(from + at) : uint4{0, 0, 0, 0};
+        continue;
+      }
       // dims of K fragment s in this half of the wave
       const int d = D == 128 ? 16 * (2 * (s & 1) + half) + 4 * (s >> 1) : 16 * half + 4 * s;
       uint2 lo = {0, 0}, hi = {0, 0};
@@ -704,6 +907,7 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
       for (int s = 0; s < KS; ++s) q[s] = as_h8(part_q[s]);
     }
   }
+  if constexpr (k4) rowf = fmaxf(rowf, 1.1754944e-38f);  // (-inf times zero is no -inf)
   // keys below this need no mask in this wave
   const int plain = kv_len - q_len + (u.row + min(wave * 32, rows)) / a.group + 1;
 
@@ -759,7 +963,10 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
     const int pos = u.kv_begin + i_tile * kTileKeys;
     float g[4], lv[4], iv[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) g[i] = meta[i][0] * rowf, lv[i] = meta[i][1], iv[i] = meta[i][2];
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (k4) g[i] = rowf, lv[i] = 0.0f, iv[i] = kUnit;
+      else g[i] = meta[i][0] * rowf, lv[i] = meta[i][1], iv[i] = meta[i][2];
+    }
     if (__builtin_expect_with_probability(pos + kTileKeys > plain || bad_seen != 0, 0, 0.99)) {
       // some rows do not see all of the tile's keys: a hidden key's score is
       // -inf, and where a lane sees none of 8 keys their block's scales, which
@@ -772,9 +979,13 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
           const int n = min(max(limit - pos - 16 * i - 8 * j - 4 * half, 0), 4);
           see |= ((1u << n) - 1u) << (4 * j);
         }
-        see = __float_as_int(meta[i][3]) != 0 ? 0 : see;
+        bool no_block;
+        if constexpr (k4) no_block = (pages.bad >> (min((pos + 16 * i) >> a.c.b_shift, last) - pages.first)) & 1;
+        else no_block = __float_as_int(meta[i][3]) != 0;
+        see = no_block ? 0 : see;
 #pragma unroll
         for (int e = 0; e < 8; ++e) s[i >> 1][8 * (i & 1) + e] = (see >> e) & 1 ? s[i >> 1][8 * (i & 1) + e] : -INFINITY;
+        if constexpr (k4) continue;
         g[i] = see == 0 ? 1.0f : g[i] < 1.1754944e-38f ? 1.1754944e-38f : g[i];  // (-inf times zero is no -inf)
         lv[i] = see == 0 ? kLowest : lv[i];
         iv[i] = see == 0 ? 0.0f : iv[i];
@@ -858,14 +1069,20 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
     // before the first step: K(0), its scales, and no values for no weights
     if (!upper) {
 #pragma unroll
-      for (int t = 0; t < 8; ++t) decode(0, 0, buf0, t);
+      for (int t = 0; t < 8; ++t) {
+        if constexpr (k4) decode4(std::false_type{}, 0, buf0, t);
+        else decode(0, 0, buf0, t);
+      }
     }
-    store_meta(0);
+    if constexpr (!k4) store_meta(0);
     for (int i = tid; i < kVBytes / 16; i += NW * kWave) reinterpret_cast<uint4*>(buf1 + kKBytes)[i] = uint4{0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = uint4{0, 0, 0, 0};
     turn_pages(0, 2);
-    if (!upper) fetch(0, 1);
+    if (!upper) {
+      if constexpr (k4) fetch4(std::false_type{}, 0, 1);
+      else fetch(0, 1);
+    }
     __syncthreads();
     if (upper) __syncthreads();
     for (int i = 0; i < tiles; ++i) {
@@ -875,22 +1092,44 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
       // scales written, this one's read
       constexpr int kTasks = kRoles * 9 + 2;
       __builtin_amdgcn_s_setprio(1);  // the products go first: the other wave's vector work fills what they leave
-      matrix(other, cur, std::true_type{}, [&](int k) {
+      if constexpr (k4) {
+        // K's and V's codes are decoded differently: a copy of the products for either role
+        const auto tasks = [&](auto is_v, int o, int t) {
+          constexpr bool v = decltype(is_v)::value;
+          if (t < 8) decode4(is_v, o, v ? cur : other, t);
+          else fetch4(is_v, o, v ? i + 1 : i + 2);
+        };
+        const auto run = [&](auto is_v) {
+          matrix(other, cur, std::true_type{}, [&](int k) {
+            constexpr int kAll4 = kRoles * 9;
 #pragma unroll
-        for (int t = k * kTasks / kAll; t < (k + 1) * kTasks / kAll; ++t) {
-          if (t == kTasks - 1) {
+            for (int t = k * kAll4 / kAll; t < (k + 1) * kAll4 / kAll; ++t) {
+              if constexpr (kRoles == 1) tasks(is_v, 0, t);
+              else if (t < 9) tasks(std::false_type{}, 0, t);
+              else tasks(std::true_type{}, kRoles - 1, t - 9);
+            }
+          });
+        };
+        if (upper) run(std::true_type{});
+        else run(std::false_type{});
+      } else {
+        matrix(other, cur, std::true_type{}, [&](int k) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) meta[j] = metas[(i & 3) * 4 + j];
-          } else if (t == kTasks - 2) {
-            store_meta(i + 1);
-          } else {
-            const int o = t / 9, part_t = t % 9;
-            const bool v = kRoles == 2 ? o == 1 : upper;
-            if (part_t < 8) decode(o, v ? i : i + 1, v ? cur : other, part_t);
-            else fetch(o, v ? i + 1 : i + 2);
+          for (int t = k * kTasks / kAll; t < (k + 1) * kTasks / kAll; ++t) {
+            if (t == kTasks - 1) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) meta[j] = metas[(i & 3) * 4 + j];
+            } else if (t == kTasks - 2) {
+              store_meta(i + 1);
+            } else {
+              const int o = t / 9, part_t = t % 9;
+              const bool v = kRoles == 2 ? o == 1 : upper;
+              if (part_t < 8) decode(o, v ? i : i + 1, v ? cur : other, part_t);
+              else fetch(o, v ? i + 1 : i + 2);
+            }
           }
-        }
-      });
+        });
+      }
       __builtin_amdgcn_s_setprio(0);
       __syncthreads();
       weigh(i);
@@ -903,9 +1142,17 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
   if (bad_seen != 0 && lane == 0) atomicOr(a.status, NSMLP_STATUS_BLOCK_UNAVAILABLE);
 
   // a lane's results: D / 32 runs of 16 dims, in pieces of 4
-  const auto dim_of = [&](int g) { return (g >> 1) * 64 + (g & 1) * 32 + 16 * half; };
+  const auto dim_of = [&](int g) {
+    return k4 ? (D / 16) * (8 * (g >> 2) + 4 * half + (g & 3)) : (g >> 1) * 64 + (g & 1) * 32 + 16 * half;
+  };
+  constexpr int kRuns = k4 ? 8 : D / 32, kPieces = k4 ? D / 64 : 4;
   const auto piece = [&](int g, int i, float f) {
-    if constexpr (D == 128) return float4_t{acc[0][4 * g + i], acc[1][4 * g + i], acc[2][4 * g + i], acc[3][4 * g + i]} * f;
+    // (4 bits: 8 runs of D/16 dims, a run D/16 (8 (g / 4) + 4 half + g % 4), pieces of 4)
+    if constexpr (k4) {
+      const int e = 4 * (g >> 2) + (g & 3);
+      if constexpr (D == 128) return float4_t{acc[0][8 * i + e], acc[1][8 * i + e], acc[ND - 2][8 * i + e], acc[ND - 1][8 * i + e]} * f;
+      else return float4_t{acc[0][e], acc[1][e], acc[0][8 + e], acc[1][8 + e]} * f;
+    } else if constexpr (D == 128) return float4_t{acc[0][4 * g + i], acc[1][4 * g + i], acc[2][4 * g + i], acc[3][4 * g + i]} * f;
     else return float4_t{acc[0][4 * g + i], acc[0][8 + 4 * g + i], acc[1][4 * g + i], acc[1][8 + 4 * g + i]} * f;
   };
   l += __shfl_xor(l, 32, kWave), x += __shfl_xor(x, 32, kWave);
@@ -913,25 +1160,29 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
     if (u.part >= 0) {
       const long long at = ((long long)u.part * a.c.heads + h) * kRows + r;
 #pragma unroll
-      for (int g = 0; g < D / 32; ++g)
+      for (int g = 0; g < kRuns; ++g)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) *reinterpret_cast<float4_t*>(a.acc_b + at * D + dim_of(g) + 4 * i) = piece(g, i, 1.0f);
+        for (int i = 0; i < kPieces; ++i) *reinterpret_cast<float4_t*>(a.acc_b + at * D + dim_of(g) + 4 * i) = piece(g, i, 1.0f);
       if (half == 0) *reinterpret_cast<float4_t*>(a.ml_b + 4 * at) = float4_t{m, l, x, 0.0f};
     } else {
       const long long at = (long long)(q0 + tok) * a.c.heads * a.group + h * a.group + row % a.group;
       const float inv = inverse_of(l);
 #pragma unroll
-      for (int g = 0; g < D / 32; ++g) {
-        uint32_t o[8];
+      for (int g = 0; g < kRuns; ++g) {
+        uint32_t o[2 * kPieces];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kPieces; ++i) {
           const float4_t p = piece(g, i, inv);
           o[2 * i] = to_out<kBf16>(p[0]) | (uint32_t)to_out<kBf16>(p[1]) << 16;
           o[2 * i + 1] = to_out<kBf16>(p[2]) | (uint32_t)to_out<kBf16>(p[3]) << 16;
         }
-        uint4* to = reinterpret_cast<uint4*>(a.out + at * D + dim_of(g));
-        to[0] = uint4{o[0], o[1], o[2], o[3]};
-        to[1] = uint4{o[4], o[5], o[6], o[7]};
+        if constexpr (kPieces == 1) {
+          *reinterpret_cast<uint2*>(a.out + at * D + dim_of(g)) = uint2{o[0], o[1]};
+        } else {
+          uint4* to = reinterpret_cast<uint4*>(a.out + at * D + dim_of(g));
+          to[0] = uint4{o[0], o[1], o[2], o[3]};
+          if constexpr (kPieces == 4) to[1] = uint4{o[4], o[5], o[6], o[7]};
+        }
       }
       if (kLse && half == 0) a.lse[at] = lse_of(m, x);
     }
@@ -1092,7 +1343,13 @@ size_t kv_attn_partial_floats(const KvSchedule& s, int kv_heads, int D, size_t (
 }
 
 void launch_kv_attention(const KvAttnArgs& a, bool bf16, hipStream_t s) {
-  NSMLP_KV_BY_TYPE(attention_typed, a, bf16, s);
+  if (a.c.fmt != NSMLP_KV_E2M1) {
+    NSMLP_KV_BY_TYPE(attention_typed, a, bf16, s);
+  } else if (a.c.D == 128) {
+    bf16 ? attention_typed<128, NSMLP_KV_E2M1, true>(a, s) : attention_typed<128, NSMLP_KV_E2M1, false>(a, s);
+  } else {
+    bf16 ? attention_typed<64, NSMLP_KV_E2M1, true>(a, s) : attention_typed<64, NSMLP_KV_E2M1, false>(a, s);
+  }
 }
 
 }  // namespace nsmlp

@@ -547,7 +547,7 @@ extern "C" {
 
 const char* nsmlp_last_error(void) { return g_err; }
 
-int nsmlp_version(void) { return 107; }
+int nsmlp_version(void) { return 108; }
 
 int nsmlp_fault_inject(const char* spec) { return fault_set(spec); }
 

@@ -1,8 +1,8 @@
-// Paged K/V cache in 8 bits: layouts, argument blocks and device helpers
-// shared by the bookkeeping kernels (nsmlp_kv.hip) and the attention
-// (nsmlp_attention.hip).
+// Paged K/V cache in 8 or 4 bits: layouts, argument blocks and device helpers
+// shared by the bookkeeping kernels (nsmlp_kv.hip), those of the 4-bit format
+// and the rotation (nsmlp_kv4.hip) and the attention (nsmlp_attention.hip).
 //
-// Layout.  A block holds B tokens (16, 32 or 64) of every K/V head.  Its bytes
+// Layout in 8 bits.  A block holds B tokens (16, 32 or 64) of every K/V head.  Its bytes
 // are [kv_heads][2: K, V][B * D]; a (block, head)'s K and V are runs of B/16
 // tiles of 16 tokens, 16 D bytes each, ordered so that 64 lanes reading 16
 // bytes each at consecutive addresses hold an MFMA operand:
@@ -13,6 +13,19 @@
 // the product of V (rows: dims) with the weights wants them, so weights need
 // no exchange between lanes.
 // scale [blocks][kv_heads][2] fp32: value = code * scale.
+//
+// Layout in 4 bits (NSMLP_KV_E2M1).  A (block, head) is a run of K codes, V
+// codes, K scales and V scales, each a run of B/16 tiles of 16 tokens.  A code
+// is an e2m1 nibble, a byte two neighbouring dims of a token (the lower dim in
+// the low nibble), a scale byte a power of two, 2^(byte - 127), of 32 dims of a
+// token.  With r = 16th part of the dims (D/16 of them) and w = D/32 bytes:
+//   K tile  [4 quarters of the dims][16 tokens][D/4 dims]           8 D bytes
+//   V tile  [4 token groups][16 r][4 tokens][D/16 dims]             8 D bytes
+//   K scale [D/32][16 tokens], V scale [4 token groups][D/32][4 tokens]
+// so that a lane's 16 (or 8) bytes are its operand of the same products: K's
+// under one scale, V's 4 tokens under one scale each, which a conversion to fp16
+// applies on the way.  A token's bytes are its own in both, so that tokens are
+// stored without reading what stands next to them.
 #pragma once
 
 #include "nsmlp_internal.h"
@@ -25,8 +38,14 @@ constexpr float kKvScaleMin = 7.888609052210118e-31f;  // 2^-100
 struct KvView {
   uint8_t* data;
   float* scale;
-  int num_blocks, heads, D, B, b_shift, fmt;  // fmt: NSMLP_KV_INT8 / NSMLP_KV_E4M3
+  int num_blocks, heads, D, B, b_shift, fmt;  // fmt: NSMLP_KV_INT8 / NSMLP_KV_E4M3 / NSMLP_KV_E2M1
 };
+
+// bytes of a (block, head), K and V
+template <int kFmt>
+__host__ __device__ constexpr int kv_block_bytes(int B, int D) {
+  return kFmt == NSMLP_KV_E2M1 ? B * D + B * D / 16 : 2 * B * D;
+}
 
 // byte of (token t, dim d) inside a (block, head)'s K or V
 __host__ __device__ __forceinline__ int kv_k_off(int D, int t, int d) {
@@ -35,6 +54,23 @@ __host__ __device__ __forceinline__ int kv_k_off(int D, int t, int d) {
 __host__ __device__ __forceinline__ int kv_v_off(int D, int t, int d) {
   return (t >> 4) * 16 * D + (d >> 6) * 1024 + ((t & 15) >> 2) * 256 + (d & 63) * 4 + (t & 3);
 }
+
+// The same of the 4-bit format: where the D/16 dims from D/16 * r of token t
+// start in K and in V (codes), and the byte of its 32 dims' scale.
+__host__ __device__ __forceinline__ int kv4_k_off(int D, int t, int r) {
+  return (t >> 4) * 8 * D + ((r >> 2) * 16 + (t & 15)) * (D / 8) + (r & 3) * (D / 32);
+}
+__host__ __device__ __forceinline__ int kv4_v_off(int D, int t, int r) {
+  return (t >> 4) * 8 * D + (((t & 15) >> 2) * 16 + r) * (D / 8) + (t & 3) * (D / 32);
+}
+__host__ __device__ __forceinline__ int kv4_ks_off(int D, int t, int group) { return (t >> 4) * (D / 2) + group * 16 + (t & 15); }
+__host__ __device__ __forceinline__ int kv4_vs_off(int D, int t, int group) {
+  return (t >> 4) * (D / 2) + (((t & 15) >> 2) * (D / 32) + group) * 4 + (t & 3);
+}
+// The scales' exponents: a code times 2^-23 to 2^13 is an fp16 number, subnormal
+// ones among them.  255 in K's scales marks a token whose K or V is not finite.
+constexpr int kKv4Least = -23, kKv4Most = 13;
+constexpr uint32_t kKv4Bad = 255;
 
 // int8 codes are stored with 128 added, so that a byte next to 0x64 is the
 // fp16 value 1024 + 128 + code: two permutes and two packed subtractions turn
@@ -78,6 +114,18 @@ __device__ __forceinline__ float kv_scale_of(float a) {
   return fmaxf(s, kKvScaleMin);
 }
 
+// Angles by position, and the query rows that an append rotates on the way.
+struct KvRotateArgs {
+  const float* table;        // [reach][D / 2][2] cos, sin; NULL: no rotation
+  const int32_t* positions;  // [n]
+  int reach, interleaved;
+  const uint16_t* q;  // [n][q_heads][D] or NULL
+  uint16_t* q_out;
+  long long q_row, q_head, out_row, out_head;  // strides in elements
+  int q_heads;
+  unsigned first;  // workgroup of the first query rows (set by the launch)
+};
+
 struct KvAppendArgs {
   KvView c;
   const uint16_t *k, *v;
@@ -85,8 +133,10 @@ struct KvAppendArgs {
   const int64_t* slots;
   int n;
   int take;  // tokens that a wave looks at (set by the launch)
+  KvRotateArgs rot;
 };
-void launch_kv_append(const KvAppendArgs& a, bool bf16, hipStream_t s);
+void launch_kv_append(const KvAppendArgs& a, bool bf16, hipStream_t s);   // 8 bits
+void launch_kv_append4(const KvAppendArgs& a, bool bf16, hipStream_t s);  // 4 bits
 
 struct KvReadArgs {
   KvView c;
@@ -95,6 +145,7 @@ struct KvReadArgs {
   uint16_t *k, *v;  // [n][heads][D]
 };
 void launch_kv_read(const KvReadArgs& a, bool bf16, hipStream_t s);
+void launch_kv_read4(const KvReadArgs& a, bool bf16, hipStream_t s);
 
 // Work of an attention call, listed by the step's plan.  A unit is up to
 // `rows` query rows of a request (row = token * group + head of the group)
@@ -141,6 +192,7 @@ struct KvPlanArgs {
   int32_t* table;                    // [R][max_blocks]
   const int32_t *ring, *state;       // [num_blocks] free blocks, (head, count)
   int64_t* slots;                    // [total]
+  int32_t* positions;                // [total] or NULL
   int32_t *q_start, *kv_len, *next;  // [R + 1], [R], [R]
   int32_t* info;                     // [4] head, count, refused, tokens
   int32_t* sched;
@@ -173,7 +225,7 @@ struct KvCommitArgs {
 };
 void launch_kv_commit(const KvCommitArgs& a, hipStream_t s);
 
-// f<D, format, bf16>(args) for the cache's head size and format
+// f<D, format, bf16>(args) for the cache's head size and 8-bit format
 #define NSMLP_KV_BY_TYPE(f, a, bf16, s)                                                            \
   do {                                                                                             \
     const bool i8_ = (a).c.fmt == NSMLP_KV_INT8;                                                   \

@@ -1,6 +1,6 @@
-// Bookkeeping of the paged 8-bit K/V cache: a step's plan (block tables, slot
-// maps, the attention's work lists), commit, append and read.
-#include "nsmlp_kv.h"
+// Bookkeeping of the paged K/V cache: a step's plan (block tables, slot maps,
+// the attention's work lists) and commit; append and read in 8 bits.
+#include "nsmlp_rotate.h"
 
 #include <mutex>
 
@@ -267,6 +267,7 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(KvPlanArgs a) {
       if (id >= 0 && id < a.num_blocks) slot = ((long long)id << a.b_shift) + (p & (a.B - 1));
     }
     a.slots[t] = slot;
+    if (a.positions != nullptr) a.positions[t] = slot < 0 ? -1 : len_s[lo] + t - q_start[lo];
   }
   // work lists: one wave per request
   int32_t* shares = a.sched + a.s.off_shares;
@@ -401,19 +402,6 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_commit(KvCommitArgs a) {
 // 11420 tokens of prompts (70 MB) 21 us, 3.3 TB/s.
 constexpr int kAppendThreads = 256;
 
-template <bool kBf16>
-__device__ __forceinline__ float in_value(uint32_t h) {
-  if constexpr (kBf16) return __uint_as_float(h << 16);
-  else return h2f((uint16_t)h);
-}
-template <bool kBf16>
-__device__ __forceinline__ float in_lo(uint32_t w) { return in_value<kBf16>(w & 0xFFFFu); }
-template <bool kBf16>
-__device__ __forceinline__ float in_hi(uint32_t w) {
-  if constexpr (kBf16) return __uint_as_float(w & 0xFFFF0000u);
-  else return in_value<kBf16>(w >> 16);
-}
-
 // Codes of four values under scale s (r = 1 / s rounded), in byte order.  The
 // int8 quotient is rounded as a division: x r corrected by its residual (a
 // correctly rounded r makes the corrected product the correctly rounded
@@ -454,7 +442,7 @@ __device__ __forceinline__ uint32_t top16(uint32_t top, uint32_t w) {
   return max(top, max(w & 0x7FFFu, (w >> 16) & 0x7FFFu));
 }
 
-template <int D, int B, int kFmt, bool kBf16>
+template <int D, int B, int kFmt, bool kBf16, bool kRotate>
 __device__ __forceinline__ void append_run(const KvAppendArgs& a, int t, long long slot, int n, int h, bool is_v, int lane) {
   const long long blk = slot / B;
   const int o0 = (int)(slot & (B - 1));  // first new offset
@@ -487,6 +475,19 @@ __device__ __forceinline__ void append_run(const KvAppendArgs& a, int t, long lo
       if (i < n) {
         const uint4* q = reinterpret_cast<const uint4*>(x + i * a.k_row);
         u[p][0] = q[0], u[p][1] = q[1];
+      }
+      if constexpr (kRotate) {
+        // a row's other half is kChunks / 2 lanes away (of tokens past the run, zeros)
+        uint32_t w[8], other[8];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          w[4 * j] = u[p][j].x, w[4 * j + 1] = u[p][j].y, w[4 * j + 2] = u[p][j].z, w[4 * j + 3] = u[p][j].w;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) other[j] = (uint32_t)__shfl_xor((int)w[j], kChunks / 2, kWave);
+        if (i < n) {
+          rotate<16, kBf16>(w, other, angles_of<D, 16>(a.rot, a.rot.positions[t + i], c * 16), a.rot.interleaved);
+          u[p][0] = uint4{w[0], w[1], w[2], w[3]}, u[p][1] = uint4{w[4], w[5], w[6], w[7]};
+        }
       }
     }
 #pragma unroll
@@ -564,10 +565,14 @@ __device__ __forceinline__ void append_run(const KvAppendArgs& a, int t, long lo
   }
 }
 
-template <int D, int B, int kFmt, bool kBf16>
+template <int D, int B, int kFmt, bool kBf16, bool kRotate>
 __global__ void __launch_bounds__(kAppendThreads, B == 64 ? 2 : 4) k_kv_append(KvAppendArgs a) {
   kernarg_warm<sizeof(KvAppendArgs)>();
   const int lane = threadIdx.x & (kWave - 1);
+  if (kRotate && blockIdx.x >= a.rot.first) {
+    rotate_queries<D, kBf16>(a.rot, a.n, (long long)(blockIdx.x - a.rot.first) * (kAppendThreads / 16) + (threadIdx.x >> 4), lane);
+    return;
+  }
   const int item = (int)blockIdx.x * (kAppendThreads / kWave) + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int two_heads = 2 * a.c.heads;
   const int t0 = item / two_heads * a.take, hk = item % two_heads;
@@ -591,7 +596,7 @@ __global__ void __launch_bounds__(kAppendThreads, B == 64 ? 2 : 4) k_kv_append(K
     const int n = after == ~0ull ? kWave : 1 + __builtin_ctzll(~after);
     const long long slot = ((long long)__builtin_amdgcn_readlane((int)(s0 >> 32), i) << 32) |
                            (uint32_t)__builtin_amdgcn_readlane((int)s0, i);
-    append_run<D, B, kFmt, kBf16>(a, t0 + i, slot, min(n, B - (int)(slot & (B - 1))), hk >> 1, hk & 1, lane);
+    append_run<D, B, kFmt, kBf16, kRotate>(a, t0 + i, slot, min(n, B - (int)(slot & (B - 1))), hk >> 1, hk & 1, lane);
   }
 }
 
@@ -600,12 +605,6 @@ __global__ void __launch_bounds__(kAppendThreads, B == 64 ? 2 : 4) k_kv_append(K
 // The token's V bytes lie one in each dword of 4 pieces of 16; the threads of
 // the group's other tokens find the same pieces in the caches.  11532 tokens of
 // 8 heads (71 MB) 17-18 us, 4 TB/s, three quarters of what a copy reaches.
-template <bool kBf16>
-__device__ __forceinline__ uint32_t pack_out(float a, float b) {
-  if constexpr (kBf16) return __builtin_bit_cast(uint16_t, (__bf16)a) | (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)b) << 16;
-  else return f2h(a) | (uint32_t)f2h(b) << 16;
-}
-
 template <int D, int kFmt, bool kBf16>
 __global__ void __launch_bounds__(256) k_kv_read(KvReadArgs a) {
   kernarg_warm<sizeof(KvReadArgs)>();
@@ -646,6 +645,14 @@ __global__ void __launch_bounds__(256) k_kv_read(KvReadArgs a) {
   vp[0] = uint4{vo[0], vo[1], vo[2], vo[3]}, vp[1] = uint4{vo[4], vo[5], vo[6], vo[7]};
 }
 
+template <int D, int kFmt, bool kBf16, bool kRotate>
+void append_blocks(const KvAppendArgs& a, dim3 grid, hipStream_t s) {
+  const dim3 block(kAppendThreads);
+  if (a.c.B == 16) k_kv_append<D, 16, kFmt, kBf16, kRotate><<<grid, block, 0, s>>>(a);
+  else if (a.c.B == 32) k_kv_append<D, 32, kFmt, kBf16, kRotate><<<grid, block, 0, s>>>(a);
+  else k_kv_append<D, 64, kFmt, kBf16, kRotate><<<grid, block, 0, s>>>(a);
+}
+
 template <int D, int kFmt, bool kBf16>
 void append_typed(KvAppendArgs a, hipStream_t s) {
   // Most tokens of a long call are a prompt's, and the waves that find no first
@@ -658,10 +665,14 @@ void append_typed(KvAppendArgs a, hipStream_t s) {
   const long long pairs = (long long)a.n * a.c.heads * 2;
   a.take = pairs >= 128 * 1024 ? 16 : pairs >= 32 * 1024 ? 8 : 1;
   const long long waves = (long long)((a.n + a.take - 1) / a.take) * a.c.heads * 2, per = kAppendThreads / kWave;
-  const dim3 grid((unsigned)((waves + per - 1) / per)), block(kAppendThreads);
-  if (a.c.B == 16) k_kv_append<D, 16, kFmt, kBf16><<<grid, block, 0, s>>>(a);
-  else if (a.c.B == 32) k_kv_append<D, 32, kFmt, kBf16><<<grid, block, 0, s>>>(a);
-  else k_kv_append<D, 64, kFmt, kBf16><<<grid, block, 0, s>>>(a);
+  a.rot.first = (unsigned)((waves + per - 1) / per);
+  if (a.rot.table == nullptr) {
+    append_blocks<D, kFmt, kBf16, false>(a, dim3(a.rot.first), s);
+    return;
+  }
+  constexpr int kUnits = kAppendThreads / 16;
+  const long long queries = a.rot.q != nullptr ? query_units(a.rot, a.n) : 0;
+  append_blocks<D, kFmt, kBf16, true>(a, dim3(a.rot.first + (unsigned)((queries + kUnits - 1) / kUnits)), s);
 }
 
 template <int D, int kFmt, bool kBf16>

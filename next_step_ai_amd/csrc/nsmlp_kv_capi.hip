@@ -1,4 +1,4 @@
-// C ABI of the paged 8-bit K/V cache and its attention: argument validation
+// C ABI of the paged K/V cache and its attention: argument validation
 // and launches.  Declarations are in include/nsmlp.h.
 #include <math.h>
 #include <string.h>
@@ -23,13 +23,15 @@ int cache_view(const nsmlp_kv_cache* c, KvView& v) {
     return set_error(NSMLP_EINVAL, "head_dim %d must be 64 or 128", c->head_dim);
   if (block_shift(c->block_tokens) < 0)
     return set_error(NSMLP_EINVAL, "block_tokens %d must be 16, 32 or 64", c->block_tokens);
-  if (c->format != NSMLP_KV_INT8 && c->format != NSMLP_KV_E4M3)
+  if (c->format != NSMLP_KV_INT8 && c->format != NSMLP_KV_E4M3 && c->format != NSMLP_KV_E2M1)
     return set_error(NSMLP_EINVAL, "unknown cache format %d", c->format);
   if (c->kv_heads < 1 || c->kv_heads > 1024) return set_error(NSMLP_EINVAL, "kv_heads %d out of range [1, 1024]", c->kv_heads);
   if (c->num_blocks < 1 || c->num_blocks > (1 << 26))
     return set_error(NSMLP_EINVAL, "num_blocks %d out of range [1, 2^26]", c->num_blocks);
-  if (c->data == nullptr || c->scale == nullptr) return set_error(NSMLP_EINVAL, "cache data and scale must be non-NULL");
-  if (!aligned16(c->data) || !aligned16(c->scale)) return set_error(NSMLP_EINVAL, "cache data and scale must be 16-byte aligned");
+  const bool scales = c->format != NSMLP_KV_E2M1;  // (in 4 bits they stand among the codes)
+  if (c->data == nullptr || (scales && c->scale == nullptr)) return set_error(NSMLP_EINVAL, "cache data and scale must be non-NULL");
+  if (!aligned16(c->data) || (scales && !aligned16(c->scale)))
+    return set_error(NSMLP_EINVAL, "cache data and scale must be 16-byte aligned");
   v.data = c->data;
   v.scale = c->scale;
   v.num_blocks = c->num_blocks;
@@ -73,6 +75,28 @@ int check_batch(const nsmlp_kv_batch* b) {
 
 constexpr int kMaxTokens = 1 << 24;
 
+int append_args(const nsmlp_kv_cache* cache, const void* k, long long k_row, long long k_head, const void* v, long long v_row,
+                long long v_head, int dtype, const int64_t* slots, int n, KvAppendArgs& a) {
+  int rc = cache_view(cache, a.c);
+  if (rc || (rc = check_dtype(dtype))) return rc;
+  if (n < 0 || n > kMaxTokens || (long long)n * a.c.heads > (1 << 28))
+    return set_error(NSMLP_EINVAL, "n = %d rows of %d heads: at most 2^24 rows and 2^28 heads' rows", n, a.c.heads);
+  if (n == 0) return NSMLP_OK;
+  if (slots == nullptr) return set_error(NSMLP_EINVAL, "slots must be non-NULL");
+  if ((rc = check_rows("k", k, k_row, k_head)) || (rc = check_rows("v", v, v_row, v_head))) return rc;
+  a.k = (const uint16_t*)k;
+  a.v = (const uint16_t*)v;
+  a.k_row = k_row, a.k_head = k_head, a.v_row = v_row, a.v_head = v_head;
+  a.slots = slots;
+  a.n = n;
+  return NSMLP_OK;
+}
+
+void launch_append(const KvAppendArgs& a, bool bf16, hipStream_t s) {
+  if (a.c.fmt == NSMLP_KV_E2M1) launch_kv_append4(a, bf16, s);
+  else launch_kv_append(a, bf16, s);
+}
+
 // query rows per token and K/V head (the attention itself wants a whole number)
 int group_of(const nsmlp_kv_batch* b) { return (b->q_heads + b->kv_heads - 1) / b->kv_heads; }
 
@@ -114,22 +138,51 @@ int nsmlp_kv_append(const nsmlp_kv_cache* cache, const void* k, long long k_row_
                     const void* v, long long v_row_stride, long long v_head_stride, int dtype, const int64_t* slots, int n,
                     void* stream) {
   NSMLP_FAULT_POINT("kv_append");
-  KvAppendArgs a;
-  int rc = cache_view(cache, a.c);
-  if (rc || (rc = check_dtype(dtype))) return rc;
-  if (n < 0 || n > kMaxTokens || (long long)n * a.c.heads > (1 << 28))
-    return set_error(NSMLP_EINVAL, "n = %d rows of %d heads: at most 2^24 rows and 2^28 heads' rows", n, a.c.heads);
-  if (n == 0) return NSMLP_OK;
-  if (slots == nullptr) return set_error(NSMLP_EINVAL, "slots must be non-NULL");
-  if ((rc = check_rows("k", k, k_row_stride, k_head_stride)) || (rc = check_rows("v", v, v_row_stride, v_head_stride))) return rc;
+  KvAppendArgs a = {};
+  int rc = append_args(cache, k, k_row_stride, k_head_stride, v, v_row_stride, v_head_stride, dtype, slots, n, a);
+  if (rc || n == 0) return rc;
   if ((rc = check_device())) return rc;
-  a.k = (const uint16_t*)k;
-  a.v = (const uint16_t*)v;
-  a.k_row = k_row_stride, a.k_head = k_head_stride, a.v_row = v_row_stride, a.v_head = v_head_stride;
-  a.slots = slots;
-  a.n = n;
-  launch_kv_append(a, dtype == NSMLP_DTYPE_BF16, (hipStream_t)stream);
+  launch_append(a, dtype == NSMLP_DTYPE_BF16, (hipStream_t)stream);
   return check_launch("nsmlp_kv_append");
+}
+
+int nsmlp_kv_append_rotated(const nsmlp_kv_cache* cache, const nsmlp_rotary* rotary, const void* k, long long k_row_stride,
+                            long long k_head_stride, const void* v, long long v_row_stride, long long v_head_stride, int dtype,
+                            const int64_t* slots, const int32_t* positions, int n, const void* q, long long q_row_stride,
+                            long long q_head_stride, int q_heads, void* q_out, long long out_row_stride,
+                            long long out_head_stride, void* stream) {
+  NSMLP_FAULT_POINT("kv_append_rotated");
+  KvAppendArgs a = {};
+  int rc = append_args(cache, k, k_row_stride, k_head_stride, v, v_row_stride, v_head_stride, dtype, slots, n, a);
+  if (rc) return rc;
+  if (rotary == nullptr || rotary->table == nullptr) return set_error(NSMLP_EINVAL, "rotary and its table must be non-NULL");
+  if (!aligned16(rotary->table)) return set_error(NSMLP_EINVAL, "the rotary table must be 16-byte aligned");
+  if (rotary->head_dim != a.c.D)
+    return set_error(NSMLP_EINVAL, "the rotary table is for head_dim %d, the cache has %d", rotary->head_dim, a.c.D);
+  if (rotary->positions < 1) return set_error(NSMLP_EINVAL, "rotary positions %d must be at least 1", rotary->positions);
+  if (rotary->interleaved != 0 && rotary->interleaved != 1)
+    return set_error(NSMLP_EINVAL, "interleaved %d must be 0 or 1", rotary->interleaved);
+  if (n == 0) return NSMLP_OK;
+  if (positions == nullptr) return set_error(NSMLP_EINVAL, "positions must be non-NULL");
+  if (q != nullptr) {
+    if (q_heads < 1 || (long long)n * q_heads > (1LL << 28))
+      return set_error(NSMLP_EINVAL, "q_heads %d of %d tokens: at least 1 and at most 2^28 heads' rows", q_heads, n);
+    if ((rc = check_rows("q", q, q_row_stride, q_head_stride)) || (rc = check_rows("q_out", q_out, out_row_stride, out_head_stride)))
+      return rc;
+    if (q == q_out && (q_row_stride != out_row_stride || q_head_stride != out_head_stride))
+      return set_error(NSMLP_EINVAL, "queries that are rotated in place keep their strides");
+  }
+  if ((rc = check_device())) return rc;
+  a.rot.table = rotary->table;
+  a.rot.positions = positions;
+  a.rot.reach = rotary->positions;
+  a.rot.interleaved = rotary->interleaved;
+  a.rot.q = (const uint16_t*)q;
+  a.rot.q_out = (uint16_t*)q_out;
+  a.rot.q_row = q_row_stride, a.rot.q_head = q_head_stride, a.rot.out_row = out_row_stride, a.rot.out_head = out_head_stride;
+  a.rot.q_heads = q_heads;
+  launch_append(a, dtype == NSMLP_DTYPE_BF16, (hipStream_t)stream);
+  return check_launch("nsmlp_kv_append_rotated");
 }
 
 int nsmlp_kv_read(const nsmlp_kv_cache* cache, const int64_t* slots, int n, void* k_out, void* v_out, int dtype,
@@ -148,7 +201,8 @@ int nsmlp_kv_read(const nsmlp_kv_cache* cache, const int64_t* slots, int n, void
   a.n = n;
   a.k = (uint16_t*)k_out;
   a.v = (uint16_t*)v_out;
-  launch_kv_read(a, dtype == NSMLP_DTYPE_BF16, (hipStream_t)stream);
+  if (a.c.fmt == NSMLP_KV_E2M1) launch_kv_read4(a, dtype == NSMLP_DTYPE_BF16, (hipStream_t)stream);
+  else launch_kv_read(a, dtype == NSMLP_DTYPE_BF16, (hipStream_t)stream);
   return check_launch("nsmlp_kv_read");
 }
 
@@ -177,6 +231,7 @@ int nsmlp_kv_plan(const nsmlp_kv_batch* batch, const int32_t* new_tokens, const 
   a.ring = batch->ring;
   a.state = batch->state;
   a.slots = step->slots;
+  a.positions = step->positions;
   a.q_start = step->q_start;
   a.kv_len = step->kv_len;
   a.next = step->next;

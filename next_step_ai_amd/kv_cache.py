@@ -1,17 +1,19 @@
-"""Paged K/V cache in 8 bits and the attention that reads it: the attention
-side of the decoder layers whose MLPs the rest of the package runs.
+"""Paged K/V cache in 8 or 4 bits and the attention that reads it: the
+attention side of the decoder layers whose MLPs the rest of the package runs.
 
     cache = KvCache(num_blocks, kv_heads, head_dim)              # one per layer
     batch = KvBatch(num_blocks, 16, max_requests=R, max_blocks=W, q_heads=Hq, kv_heads=H, head_dim=D)
     step = batch.plan(new_tokens, total, max_new=n)              # once per step, for every layer
-    cache.append(k, v, step.slots)                               # per layer
+    cache.append(k, v, step.slots)                               # per layer, or with a rotary encoding:
+    q = cache.append_rotated(k, v, step.slots, step.positions, rotary, q=q)
     out = paged_attention(q, cache, step)                        # [total, Hq, D]
     batch.commit(finished)                                       # once per step
 
 ``KvBatch`` keeps the requests' lengths, block tables and free blocks on the
 device; a step's plan is one kernel, and no call synchronises.  ``KvCache``
-holds a layer's K and V codes with one scale per (block, head) for each; the
-formats are described in ``nsmlp.h``.  The reference has no such cache: its
+holds a layer's K and V codes with one scale per (block, head) for each in 8
+bits, one per 32 dims of a token in 4 bits; the formats are described in
+``nsmlp.h``.  The reference has no such cache: its
 attention and K/V cache are torch code in ``streaming_llama_runtime.py``
 (RT:5927-7142).  There is no CPU path.
 """
@@ -23,10 +25,11 @@ import torch
 
 from . import _lib
 from ._runtime import ptr, require_device, stream_handle, workspace
+from .rotary import Rotary
 
 __all__ = ["KvCache", "KvBatch", "KvStep", "paged_attention"]
 
-_FORMATS = {"int8": _lib.NSMLP_KV_INT8, "e4m3": _lib.NSMLP_KV_E4M3}
+_FORMATS = {"int8": _lib.NSMLP_KV_INT8, "e4m3": _lib.NSMLP_KV_E4M3, "e2m1": _lib.NSMLP_KV_E2M1}
 _DTYPES = {torch.float16: _lib.NSMLP_DTYPE_F16, torch.bfloat16: _lib.NSMLP_DTYPE_BF16}
 
 
@@ -59,6 +62,17 @@ def _rows(t: torch.Tensor, what: str, heads: int, dim: int, device: torch.device
     return t, p, row, head
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the memory between two tensors' first and last elements meets."""
+    def span(t: torch.Tensor) -> tuple[int, int]:
+        ends = [(n - 1) * s for n, s in zip(t.shape, t.stride())]
+        first = t.data_ptr() + t.element_size() * sum(e for e in ends if e < 0)
+        return first, t.data_ptr() + t.element_size() * (sum(e for e in ends if e > 0) + 1)
+
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
 def _slots(t: torch.Tensor, device: torch.device) -> torch.Tensor:
     if t.dtype != torch.int64 or t.dim() != 1 or t.device != device:
         raise RuntimeError(f"slots must be an int64 [tokens] tensor on {device}")
@@ -67,7 +81,9 @@ def _slots(t: torch.Tensor, device: torch.device) -> torch.Tensor:
 
 class KvCache:
     """A layer's K and V: ``num_blocks`` blocks of ``block_tokens`` (16, 32 or
-    64) tokens, ``fmt`` "int8" or "e4m3", ``head_dim`` 64 or 128."""
+    64) tokens, ``fmt`` "int8", "e4m3" or, in 4 bits, "e2m1", ``head_dim`` 64 or
+    128.  ``data`` holds the codes, ``scale`` the (block, head)s' scales (None in
+    4 bits, where they stand among the codes)."""
 
     def __init__(self, num_blocks: int, kv_heads: int, head_dim: int, *, block_tokens: int = 16, fmt: str = "int8",
                  device=None):
@@ -82,8 +98,12 @@ class KvCache:
         self.device = _device(device)
         self.num_blocks, self.kv_heads, self.head_dim = int(num_blocks), int(kv_heads), int(head_dim)
         self.block_tokens, self.fmt = int(block_tokens), fmt
-        self.data = torch.zeros(num_blocks, kv_heads, 2, block_tokens * head_dim, dtype=torch.uint8, device=self.device)
-        self.scale = torch.zeros(num_blocks, kv_heads, 2, dtype=torch.float32, device=self.device)
+        if fmt == "e2m1":
+            self.data = torch.zeros(num_blocks, kv_heads, block_tokens * head_dim * 17 // 16, dtype=torch.uint8, device=self.device)
+            self.scale = None
+        else:
+            self.data = torch.zeros(num_blocks, kv_heads, 2, block_tokens * head_dim, dtype=torch.uint8, device=self.device)
+            self.scale = torch.zeros(num_blocks, kv_heads, 2, dtype=torch.float32, device=self.device)
         self._view = _lib.KvCacheView(num_blocks=self.num_blocks, kv_heads=self.kv_heads, head_dim=self.head_dim,
                                       block_tokens=self.block_tokens, format=_FORMATS[fmt], data=ptr(self.data),
                                       scale=ptr(self.scale))
@@ -91,18 +111,68 @@ class KvCache:
 
     def append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         """Store the rows ``k``, ``v`` [tokens, kv_heads, head_dim] at ``slots``
-        (a plan's: a block's tokens stand next to each other, in order; a slot
-        of -1 stores nothing).  Where the new rows exceed a block's scale its
-        stored codes are rewritten under the larger one."""
+        (a plan's: a block's tokens stand next to each other, in order, none
+        twice; a slot of -1 stores nothing).  Where the new rows exceed a block's
+        scale in 8 bits its stored codes are rewritten under the larger one."""
         k, kp, k_row, k_head = _rows(k, "k", self.kv_heads, self.head_dim, self.device)
         v, vp, v_row, v_head = _rows(v, "v", self.kv_heads, self.head_dim, self.device)
         slots = _slots(slots, self.device)
         n = slots.shape[0]
+        self._same_length(k, v, n)
+        _lib.call("nsmlp_kv_append", self._ref, kp, k_row, k_head, vp, v_row, v_head, _DTYPES[k.dtype], slots.data_ptr(), n,
+                  stream_handle(self.device))
+
+    def _same_length(self, k: torch.Tensor, v: torch.Tensor, n: int) -> None:
         if k.dtype != v.dtype or k.shape[0] != n or v.shape[0] != n:
             raise RuntimeError(f"k, v and slots must be of the same length and k and v of one dtype: got {tuple(k.shape)} "
                                f"{k.dtype}, {tuple(v.shape)} {v.dtype} and {n} slots")
-        _lib.call("nsmlp_kv_append", self._ref, kp, k_row, k_head, vp, v_row, v_head, _DTYPES[k.dtype], slots.data_ptr(), n,
+
+    def append_rotated(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, positions: torch.Tensor, rotary: Rotary,
+                       *, q: torch.Tensor | None = None, q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+        """:meth:`append` with the rows of ``k`` turned by their ``positions``
+        [tokens] (int32, a plan's) on the way, and those of ``q`` [tokens, heads,
+        head_dim], which are returned in ``q_out`` (may be ``q`` itself).  What is
+        stored is what ``append`` stores of rows turned in 64 bits and rounded to
+        fp32 and to their type; ``k`` is not changed.  A position that is not in
+        the table makes its rows NaN; a query row at a negative one (a token of no
+        request) is left as it was in ``q_out``."""
+        k, kp, k_row, k_head = _rows(k, "k", self.kv_heads, self.head_dim, self.device)
+        v, vp, v_row, v_head = _rows(v, "v", self.kv_heads, self.head_dim, self.device)
+        slots = _slots(slots, self.device)
+        n = slots.shape[0]
+        self._same_length(k, v, n)
+        if rotary.device != self.device or rotary.head_dim != self.head_dim:
+            raise RuntimeError(f"the rotary table is for head_dim {rotary.head_dim} on {rotary.device}, the cache has "
+                               f"{self.head_dim} on {self.device}")
+        if positions.dtype != torch.int32 or positions.device != self.device or tuple(positions.shape) != (n,):
+            raise RuntimeError(f"positions must be an int32 [{n}] tensor on {self.device}")
+        positions = positions.contiguous()
+        if q is None:
+            if q_out is not None:
+                raise RuntimeError("q_out without q")
+            _lib.call("nsmlp_kv_append_rotated", self._ref, rotary._ref, kp, k_row, k_head, vp, v_row, v_head, _DTYPES[k.dtype],
+                      slots.data_ptr(), positions.data_ptr(), n, None, 0, 0, 0, None, 0, 0, stream_handle(self.device))
+            return None
+        heads = q.shape[1] if q.dim() == 3 else 0
+        rows, qp, q_row, q_head = _rows(q, "q", heads, self.head_dim, self.device)
+        if rows.shape[0] != n or rows.dtype != k.dtype or heads < 1:
+            raise RuntimeError(f"q must be [{n}, heads, {self.head_dim}] of k's dtype {k.dtype}, got {tuple(q.shape)} {q.dtype}")
+        if q_out is None:
+            q_out = torch.empty((n, heads, self.head_dim), dtype=rows.dtype, device=self.device)
+            op, o_row, o_head = q_out.data_ptr(), heads * self.head_dim, self.head_dim
+        else:
+            if q_out.dtype != rows.dtype or q_out.shape != q.shape:
+                raise RuntimeError(f"q_out must be {tuple(q.shape)} {q.dtype}, got {tuple(q_out.shape)} {q_out.dtype}")
+            out, op, o_row, o_head = _rows(q_out, "q_out", heads, self.head_dim, self.device)
+            if out is not q_out or (n > 1 and abs(o_row) < self.head_dim) or (heads > 1 and abs(o_head) < self.head_dim):
+                raise RuntimeError("q_out must be 16-byte aligned with strides of whole rows that are multiples of 8 elements")
+            same = op == qp and (q_row, q_head) == (o_row, o_head)
+            if n and not same and _overlap(rows, q_out):
+                raise RuntimeError("q_out overlaps q: it must be q itself or lie apart from it")
+        _lib.call("nsmlp_kv_append_rotated", self._ref, rotary._ref, kp, k_row, k_head, vp, v_row, v_head, _DTYPES[k.dtype],
+                  slots.data_ptr(), positions.data_ptr(), n, qp, q_row, q_head, heads, op, o_row, o_head,
                   stream_handle(self.device))
+        return q_out
 
     def read(self, slots: torch.Tensor, dtype: torch.dtype = torch.float16) -> dict[str, torch.Tensor]:
         """The stored rows at ``slots``: ``{"k": ..., "v": ...}`` of [tokens,
@@ -129,13 +199,14 @@ class _StepLayout:
             raise RuntimeError(f"nsmlp_kv_schedule_bytes: {_lib.last_error()}")
         R = batch.requests
         self.ints = (3 * R + 5 + 3) // 4 * 4
-        self.sizes = [R + 1, R, R, 4, self.ints - 3 * R - 5 + self.schedule_bytes // 4]
+        self.sizes = [R + 1, R, R, 4, self.ints - 3 * R - 5 + self.schedule_bytes // 4, total]
         self.ws_bytes: dict[int, int] = {}
 
 
 class KvStep:
-    """A planned step: ``slots`` [total] int64 (-1: none), ``q_start``
-    [requests + 1], ``kv_len`` [requests], ``info`` [4] = (ring head, free
+    """A planned step: ``slots`` [total] int64 (-1: none), ``positions``
+    [total] (how many of its request's tokens stand before each; -1: none),
+    ``q_start`` [requests + 1], ``kv_len`` [requests], ``info`` [4] = (ring head, free
     blocks, refused requests, sum of new tokens) after it, ``table`` the batch's
     block table.  ``info`` and the others are device tensors: reading them
     waits for the stream.  ``planned``: whether a plan has written them."""
@@ -146,11 +217,12 @@ class KvStep:
         lay = batch._layout(total, max_new)
         self.batch, self.total, self.max_new, self._layout = batch, total, max_new, lay
         self.slots = batch._slot.new_empty(total)  # (1.2 us; torch.empty with a dtype and a device takes 1.7)
-        # q_start, kv_len, next and info, then the schedule at the next 16 bytes
-        self._buf = batch.state.new_empty(lay.ints + lay.schedule_bytes // 4)
+        # q_start, kv_len, next and info, then the schedule at the next 16 bytes, then positions
+        self._buf = batch.state.new_empty(lay.ints + lay.schedule_bytes // 4 + total)
         base, R = self._buf.data_ptr(), batch.requests
         self._view = _lib.KvStepView(total, max_new, self.slots.data_ptr(), base, base + 4 * (R + 1), base + 4 * (2 * R + 1),
-                                     base + 4 * (3 * R + 1), base + 4 * lay.ints, lay.schedule_bytes)
+                                     base + 4 * (3 * R + 1), base + 4 * lay.ints, lay.schedule_bytes,
+                                     base + 4 * lay.ints + lay.schedule_bytes)
         self._ref = ctypes.byref(self._view)
         self._split = None
         self.planned = False
@@ -171,6 +243,10 @@ class KvStep:
     @property
     def info(self) -> torch.Tensor:
         return self._part(3)
+
+    @property
+    def positions(self) -> torch.Tensor:
+        return self._part(5)
 
     @property
     def table(self) -> torch.Tensor:

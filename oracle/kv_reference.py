@@ -1,5 +1,5 @@
-"""Plain restatements of the paged 8-bit K/V cache for the tests: a step's plan
-with loops, the codes in numpy (fp32 operations one by one, each rounded as
+"""Plain restatements of the paged K/V cache for the tests: a step's plan with
+loops, the codes in numpy (fp32 operations one by one, each rounded as
 IEEE says, so codes and scales can be compared bit for bit) and the attention
 in 64 bits with the masks written out."""
 from __future__ import annotations
@@ -82,16 +82,53 @@ def scale_of(amax: np.float32, fmt: str) -> np.float32:
     return max(np.float32(s), SCALE_MIN)
 
 
+GRID4 = np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
+
+
+def encode4(x: np.ndarray) -> tuple[np.ndarray, np.ndarray]:
+    """Rows [..., dim] -> (values of their e2m1 codes, scale of each 32 dims), by trying every exponent and every code."""
+    g = np.asarray(x, np.float64).reshape(*x.shape[:-1], -1, 32)
+    most = np.abs(g).max(-1)
+    scale = np.full(most.shape, 2.0 ** 13)
+    for e in range(12, -24, -1):
+        scale = np.where(most <= 6.0 * 2.0 ** e, 2.0 ** e, scale)
+    away = np.abs(np.minimum(np.abs(g / scale[..., None]), 8.0)[..., None] - GRID4)
+    # the nearest; of two as near the even one
+    code = np.argmin(away + np.where(np.arange(8) % 2, 2.0 ** -40, 0.0), -1)
+    return (np.sign(g) * GRID4[code]).reshape(x.shape).astype(np.float32), scale.astype(np.float32)
+
+
+def rotate(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, interleaved: bool) -> torch.Tensor:
+    """Rows [tokens, heads, dim] in fp16 or bf16 under cos, sin [tokens, dim / 2] in fp32: 64 bits, then fp32, then the type."""
+    d = x.double()
+    half = x.shape[-1] // 2
+    c, s = cos.double()[:, None], sin.double()[:, None]
+    out = torch.empty_like(d)
+    at = (slice(0, None, 2), slice(1, None, 2)) if interleaved else (slice(0, half), slice(half, None))
+    out[..., at[0]] = d[..., at[0]] * c - d[..., at[1]] * s
+    out[..., at[1]] = d[..., at[1]] * c + d[..., at[0]] * s
+    return out.float().to(x.dtype)
+
+
 class PlainCache:
-    """codes (as fp32 values) [blocks, heads, 2, block, dim], scale [blocks, heads, 2]."""
+    """codes (as fp32 values) [blocks, heads, 2, block, dim], scale [blocks, heads, 2] (e2m1: [blocks, heads, 2, block, dim / 32])."""
 
     def __init__(self, blocks, heads, dim, block, fmt):
         self.fmt, self.block = fmt, block
         self.codes = np.zeros((blocks, heads, 2, block, dim), np.float32)
-        self.scale = np.zeros((blocks, heads, 2), np.float32)
+        self.scale = np.zeros((blocks, heads, 2) + ((block, dim // 32) if fmt == "e2m1" else ()), np.float32)
 
     def append(self, k: np.ndarray, v: np.ndarray, slots) -> None:
         """k, v [tokens, heads, dim] fp32; a block's tokens one after the other."""
+        if self.fmt == "e2m1":
+            for i, s in enumerate(int(s) for s in slots):
+                for h in range(k.shape[1] if s >= 0 else 0):
+                    finite = np.isfinite(k[i, h]).all() and np.isfinite(v[i, h]).all()
+                    for which, x in ((0, k), (1, v)):
+                        codes, scale = encode4(x[i, h]) if finite else (0.0, np.nan)
+                        self.codes[s // self.block, h, which, s % self.block] = codes
+                        self.scale[s // self.block, h, which, s % self.block] = scale
+            return
         B, i, slots = self.block, 0, [int(s) for s in slots]
         while i < len(slots):
             if slots[i] < 0:
@@ -119,6 +156,11 @@ class PlainCache:
     def values(self, slots, which: int) -> np.ndarray:
         """fp32 values [tokens, heads, dim]: code * scale, rounded once."""
         s = np.asarray(slots, np.int64)
+        if self.fmt == "e2m1":
+            at = (s // self.block, slice(None), which, s % self.block)
+            out = self.codes[at] * np.repeat(self.scale[at], 32, -1)
+            out[s < 0] = 0
+            return out
         out = self.codes[s // self.block, :, which, s % self.block] * self.scale[s // self.block][:, :, which, None]
         out[s < 0] = 0
         return out
