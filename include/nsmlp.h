@@ -446,6 +446,27 @@ typedef struct nsmlp_nf4_matrix {
 int nsmlp_dense_linear_nf4_f16(const nsmlp_nf4_matrix* w, const void* x, int rows, void* out, float* out_f32,
                                void* stream);
 
+/* Log probabilities of given tokens, entropies and the most likely tokens, from
+ * logits [rows][vocab] (dtype NSMLP_DTYPE_*; rows row_stride elements apart, a
+ * row's elements next to each other, aligned to their own size only).  With p =
+ * softmax of a row:
+ *   logprob[r] = log p[tokens[r]]              (tokens and logprob NULL: none)
+ *   entropy[r] = -sum_j p_j log p_j            (nullable)
+ *   top_ids, top_logprobs [rows][top]: the `top` (at most 64) largest logits'
+ *   indices, largest first, the lower index first among equals (-0 equals +0),
+ *   and their log p.
+ * fp32 sums.  A logit of -inf has p = 0; where a row has nothing else, its log
+ * probabilities are -inf and its entropy is 0.  A NaN or +inf in a row makes all
+ * its numbers NaN; a NaN is below every number in the order of top_ids.  A token
+ * outside [0, vocab), such as -1 for a row without one, gives NaN.  No
+ * counterpart in the reference, whose samplers work on the logits in torch.  ws
+ * (needed where nsmlp_token_logprobs_workspace_bytes is not 0) is cleared once
+ * by nsmlp_workspace_init. */
+size_t nsmlp_token_logprobs_workspace_bytes(int rows, int vocab, int dtype, int top);
+int nsmlp_token_logprobs(const void* logits, long long row_stride, int dtype, int rows, int vocab, const int64_t* tokens, int top,
+                         float* logprob, float* entropy, int64_t* top_ids, float* top_logprobs, void* ws, size_t ws_bytes,
+                         void* stream);
+
 /* silu(gate) * up elementwise in fp32, rounded to fp16 (TSM:1577-1578). */
 int nsmlp_silu_mul_f16(const void* gate, const void* up, void* out, long long n, void* stream);
 
@@ -533,6 +554,7 @@ int nsmlp_host_device_pointer(const void* host, void** device_ptr);
  * caller; scale is not used. */
 #define NSMLP_DTYPE_F16 0
 #define NSMLP_DTYPE_BF16 1
+#define NSMLP_DTYPE_F32 2 /* nsmlp_token_logprobs only */
 #define NSMLP_KV_INT8 0
 #define NSMLP_KV_E4M3 1
 #define NSMLP_KV_E2M1 4

@@ -32,6 +32,7 @@ NSMLP_STATUS_BLOCK_UNAVAILABLE = 1
 NSMLP_STATUS_FIXED_RANGE = 2
 NSMLP_DTYPE_F16 = 0
 NSMLP_DTYPE_BF16 = 1
+NSMLP_DTYPE_F32 = 2
 NSMLP_KV_INT8 = 0
 NSMLP_KV_E4M3 = 1
 NSMLP_KV_E2M1 = 4
@@ -152,6 +153,8 @@ SIGNATURES: dict[str, tuple] = {
     "nsmlp_output_linear_nf4_f16": (I32, [P, I32, I32, P, I32, I32, P, P, P, P, I32, P, I32, P, P, SZ, P]),
     "nsmlp_input_linear_nf4_f16": (I32, [P, I32, I32, P, I32, P, P, P, I32, I32, P, I32, P, P]),
     "nsmlp_dense_linear_nf4_f16": (I32, [ctypes.POINTER(Nf4Matrix), P, I32, P, P, P]),
+    "nsmlp_token_logprobs_workspace_bytes": (SZ, [I32, I32, I32, I32]),
+    "nsmlp_token_logprobs": (I32, [P, I64, I32, I32, I32, P, I32, P, P, P, P, P, SZ, P]),
     "nsmlp_silu_mul_f16": (I32, [P, P, P, I64, P]),
     "nsmlp_gather_row_blocks": (I32, [P, P, I32, P, I32, I32, I32, P, P, P]),
     "nsmlp_gather_down_columns": (I32, [P, P, P, I32, I32, I32, I32, I32, P, P, P]),

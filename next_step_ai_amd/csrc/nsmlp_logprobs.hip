@@ -1,0 +1,423 @@
+// Log probabilities of given tokens, entropies and the most likely tokens from
+// the logits, in one pass over them.
+//
+// With m the largest logit of a row (finite), l = sum e^(z - m) and x = sum e^(z - m) (z - m):
+//   log p_t = (z_t - m) - log l          entropy = log l - x / l
+// Neither subtracts large numbers from each other, as z - log sum e^z would.
+// Every lane keeps its own m, l, x (fp32), raises m once per batch of
+// vectors, and lanes, waves and workgroups join theirs under the largest m.  A
+// NaN or +inf makes l NaN; -inf adds nothing to l, and to x neither, as the
+// factor z - m is held above -200, below which e^(z - m) is zero.
+//
+// The top n of a row are found as whole numbers (order of the logit, then the
+// lower index first): 64 bits, all different.  A wave keeps the candidates above
+// its n-th largest so far in LDS and drops all but n where they pass 64; the first
+// bound is the n-th largest of the lanes' own maxima of the first batch.  So nearly
+// all vectors cost one comparison.  A NaN counts as below every number.
+#include "nsmlp_internal.h"
+
+namespace nsmlp {
+
+namespace {
+
+constexpr int kLpThreads = 256, kLpWaves = kLpThreads / kWave;
+constexpr int kLpBatch = 4;          // vectors of 16 bytes that a lane has in flight
+constexpr int kLpMaxTop = 64;
+constexpr int kLpMaxSplits = 32;
+constexpr float kLog2e = 1.4426950408889634f, kLowest = -3.402823466e38f;
+
+struct LogprobArgs {
+  const uint8_t* logits;
+  long long row_bytes;
+  int rows, vocab, top, splits;
+  const int64_t* tokens;   // [rows] or NULL
+  float *logprob, *entropy;  // [rows], nullable
+  int64_t* top_ids;        // [rows][top]
+  float* top_logprobs;
+  float* part_sums;        // [rows][splits][4]: m, l, x
+  uint64_t* part_top;      // [rows][splits][top]
+  int* count;              // [rows] workgroups of a row that have ended (zero, left zero)
+};
+
+enum class Logit { kF16, kBf16, kF32 };
+template <Logit T>
+constexpr int kPerVector = T == Logit::kF32 ? 4 : 8;
+
+template <Logit T>
+__device__ __forceinline__ float value_at(const uint4& v, int i) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  if constexpr (T == Logit::kF32) return __uint_as_float(w[i]);
+  else if constexpr (T == Logit::kBf16) return __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
+  else return h2f((uint16_t)(w[i >> 1] >> (16 * (i & 1))));
+}
+template <Logit T>
+__device__ __forceinline__ float load_one(const uint8_t* row, long long i) {
+  if constexpr (T == Logit::kF32) return reinterpret_cast<const float*>(row)[i];
+  else if constexpr (T == Logit::kBf16) return __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(row)[i] << 16);
+  else return h2f(reinterpret_cast<const uint16_t*>(row)[i]);
+}
+
+// A logit's place in the order: larger for a larger one, -0 as +0, 0 for NaN.
+__device__ __forceinline__ uint32_t order_of(float z) {
+  const uint32_t b = __float_as_uint(z + 0.0f);
+  return z != z ? 0u : (int)b < 0 ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float logit_of(uint32_t order) {
+  return order == 0 ? __uint_as_float(0x7FC00000u) : __uint_as_float((int)order < 0 ? order & 0x7FFFFFFFu : ~order);
+}
+__device__ __forceinline__ uint64_t entry_of(float z, uint32_t index) { return (uint64_t)order_of(z) << 32 | (0xFFFFFFFFu - index); }
+__device__ __forceinline__ uint32_t index_of(uint64_t entry) { return 0xFFFFFFFFu - (uint32_t)entry; }
+
+// LDS writes of a wave are read by its other lanes: LDS keeps a wave's
+// operations in order, this keeps the compiler's.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// Candidates of a wave: up to 128 entries in LDS, of which the n largest count.
+struct WaveTop {
+  uint64_t* buf;   // [128]
+  int n, count;    // (both the same in all lanes)
+  uint64_t bound;  // entries at or below it are not among the n largest
+  float least;     // the bound's logit (-inf where every vector is to be looked at)
+  int lane;
+
+  __device__ __forceinline__ void start(uint64_t* b, int top, int l) {
+    buf = b, n = top, count = 0, bound = 0, least = -INFINITY, lane = l;
+  }
+
+  // The n largest, in order, and the bound that follows.  An entry's place is the
+  // number of larger ones; 0 stands for none.
+  __device__ __forceinline__ void settle() {
+    wave_sync();
+    const uint64_t a = lane < count ? buf[lane] : 0, b = lane + kWave < count ? buf[lane + kWave] : 0;
+    int above_a = 0, above_b = 0;
+    if (count > kWave) {
+      for (int j = 0; j < count; ++j) {
+        const uint64_t v = buf[j];
+        above_a += v > a, above_b += v > b;
+      }
+    } else {
+      for (int j = 0; j < count; ++j) above_a += buf[j] > a;
+    }
+    wave_sync();
+    if (a != 0 && above_a < n) buf[above_a] = a;
+    if (b != 0 && above_b < n) buf[above_b] = b;
+    wave_sync();
+    if (count >= n) {
+      count = n;
+      raise(buf[n - 1]);
+    }
+  }
+  __device__ __forceinline__ void raise(uint64_t to) {
+    bound = to;
+    const uint32_t order = (uint32_t)(to >> 32);
+    least = order < 0x00800000u ? -INFINITY : logit_of(order);  // (-inf and NaN)
+  }
+  // Every lane may bring an entry.
+  __device__ __forceinline__ void offer(bool mine, uint64_t entry) {
+    const bool in = mine && entry > bound;
+    const unsigned long long who = __ballot(in);
+    if (who == 0) return;
+    if (in) buf[count + __popcll(who & ((1ull << lane) - 1))] = entry;
+    count += __popcll(who);
+    if (count > kWave) settle();
+  }
+};
+
+// Sums under a largest logit m.
+struct Sums {
+  float m, l, x;
+};
+__device__ __forceinline__ void rebase(Sums& s, float m) {
+  const float d = s.m - m, f = __builtin_amdgcn_exp2f(d * kLog2e);
+  s.x = f * __builtin_fmaf(fmaxf(d, -200.0f), s.l, s.x);
+  s.l *= f;
+  s.m = m;
+}
+__device__ __forceinline__ Sums join_wave(Sums s) {
+  rebase(s, wave_max(s.m));
+  s.l = wave_sum(s.l), s.x = wave_sum(s.x);
+  return s;
+}
+
+__device__ __forceinline__ float log_prob(float z, const Sums& s, float log_l) {
+  return s.l == 0.0f ? -INFINITY : (z - s.m) - log_l;  // (nothing but -inf in the row)
+}
+
+// The row's results from its sums and, in `list`, its n largest.
+template <Logit T>
+__device__ __forceinline__ void write_row(const LogprobArgs& a, int row, const uint8_t* logits, const Sums& s, const uint64_t* list,
+                                          int tid) {
+  const float log_l = logf(s.l);
+  if (tid == 0) {
+    if (a.logprob != nullptr) {
+      const int64_t t = a.tokens[row];
+      a.logprob[row] = t >= 0 && t < a.vocab ? log_prob(load_one<T>(logits, t), s, log_l) : __uint_as_float(0x7FC00000u);
+    }
+    if (a.entropy != nullptr) a.entropy[row] = s.l == 0.0f ? 0.0f : log_l - s.x / s.l;
+  }
+  if (tid < a.top) {
+    const uint64_t e = list[tid];
+    a.top_ids[(long long)row * a.top + tid] = (int64_t)index_of(e);
+    a.top_logprobs[(long long)row * a.top + tid] = log_prob(logit_of((uint32_t)(e >> 32)), s, log_l);
+  }
+}
+
+template <Logit T, bool kTop>
+__global__ void __launch_bounds__(kLpThreads) k_token_logprobs(LogprobArgs a) {
+  kernarg_warm<sizeof(LogprobArgs)>();
+  constexpr int kPer = kPerVector<T>, kSize = T == Logit::kF32 ? 4 : 2;
+  __shared__ uint64_t bufs[kLpWaves][2 * kWave];
+  __shared__ uint64_t merged[kLpMaxTop];
+  __shared__ float sums[kLpWaves][3];
+  __shared__ int last;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int row = (int)(blockIdx.x / (unsigned)a.splits), split = (int)(blockIdx.x % (unsigned)a.splits);
+  const uint8_t* logits = a.logits + (long long)row * a.row_bytes;
+  // Vectors start at multiples of 16 bytes, the first one up to 15 bytes before
+  // the row: its elements that are not the row's are not loaded, nor the last one's.
+  const int lead = (int)((uintptr_t)logits & 15) / kSize;
+  const long long vectors = ((long long)lead + a.vocab + kPer - 1) / kPer;
+  const int steps = (int)((vectors + kWave - 1) / kWave);  // of a wave: 64 vectors
+  const int first = (int)((long long)steps * split / a.splits), end = (int)((long long)steps * (split + 1) / a.splits);
+
+  WaveTop top;
+  if constexpr (kTop) top.start(bufs[wave], a.top, lane);
+  Sums s = {kLowest, 0.0f, 0.0f};
+  for (int at = first + wave; at < end; at += kLpWaves * kLpBatch) {
+    uint4 raw[kLpBatch];
+#pragma unroll
+    for (int u = 0; u < kLpBatch; ++u) {
+      const int step = at + u * kLpWaves;
+      const long long v = (long long)step * kWave + lane, i0 = v * kPer - lead;
+      if (step < end && i0 >= 0 && i0 + kPer <= a.vocab) {
+        raw[u] = *reinterpret_cast<const uint4*>(logits + i0 * kSize);
+      } else {
+        // -inf where there is no logit
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = T == Logit::kF32 ? 0xFF800000u : T == Logit::kBf16 ? 0xFF80FF80u : 0xFC00FC00u;
+        if (step < end) {
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) {
+            if (i0 + j < 0 || i0 + j >= a.vocab) continue;
+            if constexpr (kSize == 4) w[j] = reinterpret_cast<const uint32_t*>(logits)[i0 + j];
+            else w[j >> 1] = (w[j >> 1] & (j & 1 ? 0xFFFFu : 0xFFFF0000u)) |
+                             (uint32_t)reinterpret_cast<const uint16_t*>(logits)[i0 + j] << (16 * (j & 1));
+          }
+        }
+        raw[u] = uint4{w[0], w[1], w[2], w[3]};
+      }
+    }
+    float most[kLpBatch], all = s.m;
+#pragma unroll
+    for (int u = 0; u < kLpBatch; ++u) {
+      most[u] = value_at<T>(raw[u], 0);
+#pragma unroll
+      for (int j = 1; j < kPer; ++j) most[u] = fmaxf(most[u], value_at<T>(raw[u], j));
+      all = fmaxf(all, most[u]);
+    }
+    rebase(s, all);
+#pragma unroll
+    for (int u = 0; u < kLpBatch; ++u)
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const float d = value_at<T>(raw[u], j) - s.m, p = __builtin_amdgcn_exp2f(d * kLog2e);
+        s.l += p;
+        s.x = __builtin_fmaf(p, fmaxf(d, -200.0f), s.x);
+      }
+    if constexpr (kTop) {
+      const auto entry = [&](int u, int j, bool& there) {
+        const int step = at + u * kLpWaves;
+        const long long i = ((long long)step * kWave + lane) * kPer - lead + j;
+        there = step < end && i >= 0 && i < a.vocab;
+        return entry_of(value_at<T>(raw[u], j), (uint32_t)i);
+      };
+      if (at == first + wave) {
+        // the first bound: the n-th largest of the lanes' maxima
+        uint64_t mine = 0;
+#pragma unroll
+        for (int u = 0; u < kLpBatch; ++u)
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) {
+            bool there;
+            const uint64_t e = entry(u, j, there);
+            mine = there && e > mine ? e : mine;
+          }
+        top.offer(true, mine);
+        top.settle();
+        if (top.bound != 0) top.raise(top.bound - 1);  // itself among those that pass
+        top.count = 0;
+      }
+#pragma unroll
+      for (int u = 0; u < kLpBatch; ++u) {
+        if (__ballot(!(most[u] < top.least)) == 0) continue;
+#pragma unroll 1  // (seldom reached: short rather than fast)
+        for (int j = 0; j < kPer; ++j) {
+          bool there;
+          const uint64_t e = entry(u, j, there);
+          top.offer(there, e);
+        }
+      }
+    }
+  }
+  if constexpr (kTop) {
+    top.settle();
+    for (int i = top.count + lane; i < a.top; i += kWave) bufs[wave][i] = 0;  // a wave with fewer logits
+  }
+  s = join_wave(s);
+  if (lane == 0) sums[wave][0] = s.m, sums[wave][1] = s.l, sums[wave][2] = s.x;
+  __syncthreads();
+  {
+    float m = sums[0][0];
+#pragma unroll
+    for (int w = 1; w < kLpWaves; ++w) m = fmaxf(m, sums[w][0]);
+    Sums r = {m, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < kLpWaves; ++w) {
+      Sums p = {sums[w][0], sums[w][1], sums[w][2]};
+      rebase(p, m);
+      r.l += p.l, r.x += p.x;
+    }
+    s = r;
+  }
+  if constexpr (kTop) {
+    // the waves' lists: an entry's place is the number of larger ones in all of them
+    if (lane < a.top) {
+      const uint64_t mine = bufs[wave][lane];
+      int above = lane;
+#pragma unroll
+      for (int w = 0; w < kLpWaves; ++w)
+        for (int j = 0; w != wave && j < a.top; ++j) above += bufs[w][j] > mine;
+      if (mine != 0 && above < a.top) merged[above] = mine;
+    }
+    // (a workgroup with fewer logits than n: none of them has the places behind)
+    if (tid < a.top) {
+      const long long here = min((long long)end * kWave * kPer - lead, (long long)a.vocab) - max((long long)first * kWave * kPer - lead, 0LL);
+      if (tid >= here) merged[tid] = 0;
+    }
+    __syncthreads();
+  }
+  if (a.splits == 1) {
+    write_row<T>(a, row, logits, s, merged, tid);
+    return;
+  }
+  // One of several workgroups of the row: the last to end joins them, in their order.
+  const long long at = (long long)row * a.splits + split;
+  if (tid == 0) {
+    st_coherent(a.part_sums + at * 4, s.m);
+    st_coherent(a.part_sums + at * 4 + 1, s.l);
+    st_coherent(a.part_sums + at * 4 + 2, s.x);
+  }
+  if (kTop && tid < a.top) __hip_atomic_store(a.part_top + at * a.top + tid, merged[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  wait_stores();
+  __syncthreads();
+  if (tid == 0) last = atomicAdd(a.count + row, 1) == a.splits - 1;
+  __syncthreads();
+  if (!last || wave != 0) return;
+  if (lane == 0) atomicExch(a.count + row, 0);
+  const long long row_at = (long long)row * a.splits;
+  Sums p = {kLowest, 0.0f, 0.0f};
+  if (lane < a.splits) {
+    const float* from = a.part_sums + (row_at + lane) * 4;
+    p = {ld_coherent(from), ld_coherent(from + 1), ld_coherent(from + 2)};
+  }
+  p = join_wave(p);
+  if constexpr (kTop) {
+    // a lane per workgroup: the lists' first entries, their second ones, and so on,
+    // until none is among the largest
+    top.start(bufs[0], a.top, lane);
+    const uint64_t* from = a.part_top + (row_at + min(lane, a.splits - 1)) * a.top;
+    for (int i = 0; i < a.top; ++i) {
+      const uint64_t e = __hip_atomic_load(const_cast<uint64_t*>(from + i), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (__ballot(lane < a.splits && e > top.bound) == 0) break;
+      top.offer(lane < a.splits && e != 0, e);
+    }
+    top.settle();
+    wave_sync();
+  }
+  write_row<T>(a, row, logits, p, bufs[0], lane);
+}
+
+// Workgroups of a row: about a thousand in all, none with less than a batch of vectors per wave.
+int splits_of(int rows, int vocab, int size) {
+  const long long steps = ((long long)vocab * size + 16 * kWave - 1) / (16 * kWave);
+  const long long most = (steps + kLpWaves * kLpBatch - 1) / (kLpWaves * kLpBatch), want = (1024 + rows - 1) / rows;
+  const long long s = most < want ? most : want;
+  return (int)(s < 1 ? 1 : s > kLpMaxSplits ? kLpMaxSplits : s);
+}
+constexpr int kLpMaxRows = 1 << 24;
+
+int check_shape(int rows, int vocab, int dtype, int top) {
+  if (rows < 0 || rows > kLpMaxRows) return set_error(NSMLP_EINVAL, "rows %d out of range [0, 2^24]", rows);
+  if (vocab < 1 || vocab > (1 << 30)) return set_error(NSMLP_EINVAL, "vocabulary %d out of range [1, 2^30]", vocab);
+  if (dtype != NSMLP_DTYPE_F16 && dtype != NSMLP_DTYPE_BF16 && dtype != NSMLP_DTYPE_F32)
+    return set_error(NSMLP_EINVAL, "unknown dtype %d", dtype);
+  if (top < 0 || top > kLpMaxTop || top > vocab)
+    return set_error(NSMLP_EINVAL, "top %d out of range [0, %d], or more than the vocabulary %d", top, kLpMaxTop, vocab);
+  return NSMLP_OK;
+}
+size_t workspace_of(int rows, int vocab, int dtype, int top) {
+  const int splits = rows == 0 ? 1 : splits_of(rows, vocab, dtype == NSMLP_DTYPE_F32 ? 4 : 2);
+  return splits == 1 ? 0 : align_up(kCounterBytes) + (size_t)rows * splits * (16 + 8 * (size_t)top);
+}
+
+template <Logit T>
+void launch(const LogprobArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)a.rows * (unsigned)a.splits), block(kLpThreads);
+  if (a.top > 0) k_token_logprobs<T, true><<<grid, block, 0, s>>>(a);
+  else k_token_logprobs<T, false><<<grid, block, 0, s>>>(a);
+}
+
+}  // namespace
+
+}  // namespace nsmlp
+
+using namespace nsmlp;
+
+extern "C" {
+
+size_t nsmlp_token_logprobs_workspace_bytes(int rows, int vocab, int dtype, int top) {
+  return check_shape(rows, vocab, dtype, top) ? 0 : workspace_of(rows, vocab, dtype, top);
+}
+
+int nsmlp_token_logprobs(const void* logits, long long row_stride, int dtype, int rows, int vocab, const int64_t* tokens, int top,
+                         float* logprob, float* entropy, int64_t* top_ids, float* top_logprobs, void* ws, size_t ws_bytes,
+                         void* stream) {
+  NSMLP_FAULT_POINT("token_logprobs");
+  int rc = check_shape(rows, vocab, dtype, top);
+  if (rc || rows == 0) return rc;
+  if ((tokens == nullptr) != (logprob == nullptr)) return set_error(NSMLP_EINVAL, "tokens and logprob go together");
+  if (top > 0 && (top_ids == nullptr || top_logprobs == nullptr))
+    return set_error(NSMLP_EINVAL, "top_ids and top_logprobs must be non-NULL");
+  const int size = dtype == NSMLP_DTYPE_F32 ? 4 : 2;
+  if (logits == nullptr || (uintptr_t)logits % size != 0)
+    return set_error(NSMLP_EINVAL, "logits must be non-NULL and aligned to their elements");
+  const size_t need = workspace_of(rows, vocab, dtype, top);
+  if (need > 0 && (ws == nullptr || ws_bytes < need))
+    return set_error(NSMLP_ENOSPC, "token_logprobs workspace needs %zu bytes, got %zu", need, ws == nullptr ? (size_t)0 : ws_bytes);
+  if (need > 0 && ((uintptr_t)ws & (kAlign - 1)) != 0) return set_error(NSMLP_EINVAL, "workspace must be 256-byte aligned");
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return set_error(NSMLP_ENODEV, "no HIP device");
+  LogprobArgs a = {};
+  a.logits = (const uint8_t*)logits;
+  a.row_bytes = row_stride * size;
+  a.rows = rows, a.vocab = vocab, a.top = top;
+  a.splits = splits_of(rows, vocab, size);
+  a.tokens = tokens;
+  a.logprob = logprob, a.entropy = entropy;
+  a.top_ids = top_ids, a.top_logprobs = top_logprobs;
+  if (need > 0) {
+    a.part_top = (uint64_t*)((char*)ws + align_up(kCounterBytes));
+    a.part_sums = (float*)(a.part_top + (size_t)rows * a.splits * top);
+    a.count = (int*)((char*)ws + kBlkCountOff);
+  }
+  if (dtype == NSMLP_DTYPE_F16) launch<Logit::kF16>(a, (hipStream_t)stream);
+  else if (dtype == NSMLP_DTYPE_BF16) launch<Logit::kBf16>(a, (hipStream_t)stream);
+  else launch<Logit::kF32>(a, (hipStream_t)stream);
+  return check_launch("nsmlp_token_logprobs");
+}
+
+}  // extern "C"

@@ -15,6 +15,9 @@ the loader hands over, lm_head.py:221-241, 292-303).
 come back in bf16 after an fp16 computation).  A meta whose ``active_idx``
 does not list every block once, in order, goes through
 ``triton_sparse_input_linear_4bit`` exactly as the reference does.
+
+``token_logprobs`` gives what a server answers with next to its tokens: their
+log probabilities, the entropies and the most likely alternatives.
 """
 from __future__ import annotations
 
@@ -23,10 +26,12 @@ import ctypes
 import torch
 
 from . import _lib
-from ._runtime import aligned16, as_f16, ptr, require_device, stream_handle
+from ._runtime import aligned16, as_f16, ptr, require_device, stream_handle, workspace
 from .nested_absmax import NestedAbsmax
 
-__all__ = ["resolve_lm_head_block_size", "lm_head_nf4_meta", "dense_linear_nf4", "lm_head_forward"]
+__all__ = ["resolve_lm_head_block_size", "lm_head_nf4_meta", "dense_linear_nf4", "lm_head_forward", "token_logprobs"]
+
+_LOGIT_DTYPES = {torch.float16: _lib.NSMLP_DTYPE_F16, torch.bfloat16: _lib.NSMLP_DTYPE_BF16, torch.float32: _lib.NSMLP_DTYPE_F32}
 
 
 def resolve_lm_head_block_size(in_features: int) -> int:
@@ -161,3 +166,49 @@ def lm_head_forward(hidden: torch.Tensor, meta: dict) -> torch.Tensor:
             quant_block_size=int(meta["quant_block_size"]), bias=None, block_size=int(meta["block_size"]))
     logits = logits if out_dtype == torch.float16 else logits.to(out_dtype)
     return logits.view(*hidden.shape[:-1], V)
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, top: int = 0,
+                   ws: torch.Tensor | None = None) -> dict[str, torch.Tensor]:
+    """What ``logits`` [..., V] (fp16, bf16 or fp32) say about ``tokens`` [...]
+    (int64): ``{"logprob": [...], "entropy": [...], "top_ids": [..., top],
+    "top_logprobs": [..., top]}``, ids int64, the others fp32; without
+    ``tokens`` no "logprob".  Alternatives (at most 64) stand from the largest
+    logit on, the lower id first among equals.  A logit of -inf has no
+    probability; a row of nothing else gives -inf and an entropy of 0, one with a
+    NaN or +inf gives NaN, and so does a token outside [0, V), such as -1 for a
+    row without one.  ``ws``: a uint8 workspace that ``nsmlp_workspace_init`` has
+    cleared, in place of the stream's own."""
+    device = require_device(logits, "logits")
+    dtype = _LOGIT_DTYPES.get(logits.dtype)
+    if dtype is None:
+        raise RuntimeError(f"logits must be fp16, bf16 or fp32, got {logits.dtype}")
+    if logits.dim() < 1:
+        raise RuntimeError("logits must have a last dimension, the vocabulary")
+    shape, V = logits.shape[:-1], int(logits.shape[-1])
+    z = logits if logits.dim() == 2 else logits.reshape(-1 if V else 0, V)
+    rows = int(z.shape[0])
+    if V > 1 and z.stride(1) != 1:
+        z = z.contiguous()
+    if tokens is not None and (tokens.dtype != torch.int64 or tokens.device != device or tokens.shape != shape):
+        raise RuntimeError(f"tokens must be an int64 {tuple(shape)} tensor on {device}, got {tuple(tokens.shape)} {tokens.dtype} on "
+                           f"{tokens.device}")
+    top = int(top)
+    need = int(_lib.lib().nsmlp_token_logprobs_workspace_bytes(rows, V, dtype, max(top, 0)))
+    t = None if tokens is None else tokens.reshape(-1).contiguous()
+    f32 = torch.empty((1 if t is None else 2) * rows + rows * max(top, 0), dtype=torch.float32, device=device)
+    ids = torch.empty(rows * max(top, 0), dtype=torch.int64, device=device)
+    entropy, at = f32[:rows], f32.data_ptr()
+    logprob = None if t is None else f32[rows: 2 * rows]
+    first = rows if t is None else 2 * rows
+    if need and ws is None:
+        ws = workspace(need, device)
+    elif ws is not None and (ws.device != device or not ws.is_contiguous()):
+        raise RuntimeError(f"ws must be a contiguous tensor on {device}, got one on {ws.device} with strides {ws.stride()}")
+    _lib.call("nsmlp_token_logprobs", z.data_ptr(), z.stride(0) if rows > 1 else V, dtype, rows, V, ptr(t), top,
+              None if t is None else at + 4 * rows, at, ids.data_ptr(), at + 4 * first, None if ws is None else ws.data_ptr(),
+              0 if ws is None else ws.numel() * ws.element_size(), stream_handle(device))
+    out = {} if t is None else {"logprob": logprob.view(shape)}
+    out["entropy"] = entropy.view(shape)
+    out["top_ids"], out["top_logprobs"] = ids.view(*shape, top), f32[first:].view(*shape, top)
+    return out

@@ -1,0 +1,72 @@
+"""Token log probabilities on the host: what the call refuses before any device work, its sizes, injected faults."""
+import ctypes
+import os
+
+import pytest
+import torch
+
+EINVAL, ENOSPC, ENODEV, EIO = -22, -28, -19, -5
+
+
+@pytest.fixture(scope="module")
+def L():
+    from next_step_ai_amd import _lib
+
+    if not os.path.exists(_lib.LIB_PATH):
+        from next_step_ai_amd import build_lib
+
+        build_lib.build()
+    yield _lib.lib()
+    _lib.fault_inject(None)
+
+
+KEEP = ctypes.create_string_buffer(1 << 16)
+MEM = (ctypes.addressof(KEEP) + 255) // 256 * 256
+
+
+def call(L, **kw):
+    x = dict(logits=MEM, stride=1000, dtype=0, rows=2, vocab=1000, tokens=MEM, top=3, logprob=MEM, entropy=MEM, top_ids=MEM,
+             top_logprobs=MEM, ws=MEM, ws_bytes=1 << 40)
+    x.update(kw)
+    return L.nsmlp_token_logprobs(x["logits"], x["stride"], x["dtype"], x["rows"], x["vocab"], x["tokens"], x["top"], x["logprob"],
+                                  x["entropy"], x["top_ids"], x["top_logprobs"], x["ws"], x["ws_bytes"], None)
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(rows=-1), EINVAL, b"rows"), (dict(rows=(1 << 24) + 1), EINVAL, b"rows"), (dict(vocab=0), EINVAL, b"vocabulary"),
+    (dict(vocab=(1 << 30) + 1), EINVAL, b"vocabulary"), (dict(dtype=3), EINVAL, b"dtype"), (dict(top=-1), EINVAL, b"top"),
+    (dict(top=65), EINVAL, b"top"), (dict(vocab=2), EINVAL, b"top"), (dict(tokens=None), EINVAL, b"go together"),
+    (dict(logprob=None), EINVAL, b"go together"), (dict(top_ids=None), EINVAL, b"top_ids"),
+    (dict(top_logprobs=None), EINVAL, b"top_ids"), (dict(logits=None), EINVAL, b"logits"), (dict(logits=MEM + 1), EINVAL, b"aligned"),
+    (dict(dtype=2, logits=MEM + 2), EINVAL, b"aligned"), (dict(vocab=100000, ws=None), ENOSPC, b"workspace"),
+    (dict(vocab=100000, ws_bytes=1000), ENOSPC, b"workspace"), (dict(vocab=100000, ws=MEM + 16), EINVAL, b"256-byte")])
+def test_refusals(L, kw, code, text):
+    assert call(L, **kw) == code and text in L.nsmlp_last_error(), L.nsmlp_last_error()
+
+
+def test_no_rows(L):
+    assert call(L, rows=0) == 0 and call(L, rows=0, logits=None, ws=None, ws_bytes=0) == 0
+
+
+def test_sizes(L):
+    """A workspace only where a row is shared out: few rows and many logits."""
+    size = L.nsmlp_token_logprobs_workspace_bytes
+    assert size(1, 1000, 0, 5) == 0 and size(4096, 128256, 1, 20) == 0 and size(0, 128256, 1, 20) == 0
+    assert 0 < size(1, 128256, 0, 20) < 1 << 20 and size(1, 128256, 2, 20) >= size(1, 128256, 2, 0) > 0
+    assert size(1, 128256, 0, 65) == 0 and size(1, 10, 0, 11) == 0 and size(1, 128256, 7, 1) == 0
+
+
+@pytest.mark.parametrize("kind,code", [("hip", EIO), ("nospc", ENOSPC), ("nodev", ENODEV)])
+def test_fault_point(L, kind, code):
+    from next_step_ai_amd import _lib
+
+    with _lib.injected_faults(f"token_logprobs={kind}:1"):
+        assert call(L, rows=0) == code and b"nsmlp_token_logprobs" in L.nsmlp_last_error()
+        assert call(L, rows=0) == 0
+
+
+def test_python_wants_a_gpu():
+    from next_step_ai_amd.lm_head import token_logprobs
+
+    with pytest.raises(RuntimeError, match="GPU"):
+        token_logprobs(torch.zeros(2, 5))
