@@ -730,15 +730,7 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
 #pragma unroll
   for (int o = 0; o < kRoles; ++o) {
     const bool v = kRoles == 2 ? o == 1 : upper;
-    if constexpr (k4) {
-      // K: D/4 dims of a token; V: 4 tokens of D/16 dims, and the 4 tokens 8 behind them, a half of the dims each lane
-      const int g = lane >> 4, t = lane & 15;
-      src[o] = v ? a.c.B * D / 2 + (half * 16 + t) * (D / 8) : lane * (D / 8);
-      src2[o] = src[o] + 4 * D;
-      dst[o] = v ? kKBytes + (part * ND * 64 + lane) * 16
-                 : ((((part >> 1) * KS + (g >> 1) * (D / 32)) * 64) + (g & 1) * 32 + (part & 1) * 16 + t) * 16;
-      dst_step[o] = 1024;
-    } else if constexpr (D == 128) {
+    if constexpr (D == 128) {
       const int g = lane >> 4, t = lane & 15;
       src[o] = v ? a.c.B * D + (g & 1) * 1024 + half * 256 + t * 16 : lane * 16;
       src2[o] = src[o] + (v ? 512 : 1024);
@@ -766,52 +758,60 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
   const auto at_of = [&](int i) { return u.kv_begin + min(i, tiles - 1) * kTileKeys + 16 * part; };
   const auto page_of = [&](int i) { return min(at_of(i) >> a.c.b_shift, last) - pages.first; };
   uint4 raw[kRoles][2];
-  Codes4<D> raw4[kRoles][2];   // in 4 bits: codes, and scale bytes
-  uint32_t scales[kRoles][2];
-  // where the lane's scales of 16 tokens are (K: one byte; V: 4 tokens each)
-  const int ks_at = a.c.B * D + ((lane >> 4) * (D / 4) >> 5) * 16 + (lane & 15);
-  const int vs_at = a.c.B * D + a.c.B * D / 32 + (half * (D / 32) + ((lane & 15) * (D / 16) >> 5)) * 4;
-  const auto fetch4 = [&](auto is_v, int o, int i) {
+  // In 4 bits every wave decodes K and V of its 16 keys, with 8 waves a half of
+  // either: K lane: token l % 16, dims D/4 (l / 16) + D/8 o + 0..D/8-1 (half o); V
+  // lane: tokens 8 o + 4 (l / 32) + 0..3, dims D/16 (l % 16) + D/32 (l / 16 % 2) +
+  // 0..D/32-1, which are its own places in the D/32 fragments of 32 dims.
+  constexpr int kWords = D / 64;
+  const int half_at = NW == 8 && upper ? 1 : 0;
+  uint32_t k_raw[kRoles][kWords], k_scale = 0, v_scale[kRoles];
+  Codes4<D> v_raw[kRoles];
+  const int k_src = lane * (D / 8) + half_at * (D / 16), v_src = a.c.B * D / 2 + (half * 16 + (lane & 15)) * (D / 8) + half_at * (4 * D);
+  const int ks_src = a.c.B * D + ((lane >> 4) * (D / 4) >> 5) * 16 + (lane & 15);
+  const int vs_src = a.c.B * D + a.c.B * D / 32 + (half * (D / 32) + ((lane & 15) * (D / 16) >> 5)) * 4 + half_at * (D / 4);
+  const int k_dst = (((part >> 1) * KS + (lane >> 5) * (D / 32) + half_at * kWords) * 64 + ((lane >> 4) & 1) * 32 + (part & 1) * 16 +
+                     (lane & 15)) * 16;
+  const int v_dst = kKBytes + (part * ND * 64 + lane) * 16 + half_at * 8;
+  const auto fetch_k4 = [&](int i) {
     const int at = at_of(i), tile = (at & (a.c.B - 1)) >> 4;
     const uint8_t* base = page_data(a, pages, page_of(i));
-    raw4[o][0] = load_codes4<D>(base + tile * (8 * D) + src[o]);
-    if constexpr (decltype(is_v)::value) {
-      raw4[o][1] = load_codes4<D>(base + tile * (8 * D) + src2[o]);
-      scales[o][0] = *reinterpret_cast<const uint32_t*>(base + vs_at + tile * (D / 2));
-      scales[o][1] = *reinterpret_cast<const uint32_t*>(base + vs_at + tile * (D / 2) + D / 4);
-    } else {
-      scales[o][0] = base[ks_at + tile * (D / 2)];
+    const uint32_t* p = reinterpret_cast<const uint32_t*>(base + tile * (8 * D) + k_src);
+#pragma unroll
+    for (int o = 0; o < kRoles; ++o)
+#pragma unroll
+      for (int j = 0; j < kWords; ++j) k_raw[o][j] = p[o * kWords + j];
+    k_scale = base[ks_src + tile * (D / 2)];
+  };
+  const auto fetch_v4 = [&](int i) {
+    const int at = at_of(i), tile = (at & (a.c.B - 1)) >> 4;
+    const uint8_t* base = page_data(a, pages, page_of(i));
+#pragma unroll
+    for (int o = 0; o < kRoles; ++o) {
+      v_raw[o] = load_codes4<D>(base + tile * (8 * D) + v_src + o * (4 * D));
+      v_scale[o] = *reinterpret_cast<const uint32_t*>(base + vs_src + tile * (D / 2) + o * (D / 4));
     }
   };
-  // K: a dword's 8 values in two steps; V: two dims' 8 tokens in four
-  uint2 first4[2], second4[2];
-  const auto decode4 = [&](auto is_v, int o, char* buf, int step) {
-    if constexpr (decltype(is_v)::value) {
-      const int m = step >> 2;
-      if (m >= D / 64) return;
-      if ((step & 3) < 2) {
-        const int i = step & 1;
-        // the lane's half of a token's dims
-        const int shift = (lane >> 4 & 1) * (D / 8);
-        uint32_t v[4];
+  // a dword of K in two steps, two dims of V's 4 tokens in two
+  uint2 k_piece;
+  uint32_t v_piece[4];
+  const auto decode_k4 = [&](int o, char* buf, int step) {
+    const int j = step >> 1;
+    const float f = scale4(k_scale, 0);
+    const uint32_t w = k_raw[o][j];
+    if (!(step & 1)) k_piece = uint2{values4(w, f, 0), values4(w, f, 1)};
+    else
+      *reinterpret_cast<uint4*>(buf + k_dst + (o * kWords + j) * 1024) = uint4{k_piece.x, k_piece.y, values4(w, f, 2), values4(w, f, 3)};
+  };
+  const auto decode_v4 = [&](int o, char* buf, int step) {
+    const int m = step >> 1;
+    if (!(step & 1)) {
+      const int shift = ((lane >> 4) & 1) * (D / 8);  // the lane's half of a token's dims
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t w = D == 128 ? raw4[o][i].w[j & (D / 32 - 1)] : raw4[o][i].w[j >> 1];
-          v[j] = values4(w >> shift, scale4(scales[o][i], j), D == 128 ? m : 2 * (j & 1));
-        }
-        (i == 0 ? first4 : second4)[0] = lower4(v), (i == 0 ? first4 : second4)[1] = upper4(v);
-      } else {
-        const int k = step & 1;
-        *reinterpret_cast<uint4*>(buf + dst[o] + (2 * m + k) * 1024) = uint4{first4[k].x, first4[k].y, second4[k].x, second4[k].y};
-      }
+      for (int j = 0; j < 4; ++j)
+        v_piece[j] = values4(v_raw[o].w[D == 128 ? j & (D / 32 - 1) : j >> 1] >> shift, scale4(v_scale[o], j), D == 128 ? m : 2 * (j & 1));
     } else {
-      const int j = step >> 1;
-      if (j >= D / 32) return;
-      const float f = scale4(scales[o][0], 0);
-      const uint32_t w = raw4[o][0].w[j];
-      if (!(step & 1)) first4[0] = uint2{values4(w, f, 0), values4(w, f, 1)};
-      else
-        *reinterpret_cast<uint4*>(buf + dst[o] + j * 1024) = uint4{first4[0].x, first4[0].y, values4(w, f, 2), values4(w, f, 3)};
+      *reinterpret_cast<uint2*>(buf + v_dst + 2 * m * 1024 + o * 8) = lower4(v_piece);
+      *reinterpret_cast<uint2*>(buf + v_dst + (2 * m + 1) * 1024 + o * 8) = upper4(v_piece);
     }
   };
   const auto fetch = [&](int o, int i) {
@@ -866,8 +866,8 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
     }
   };
   if (k4 && tiles > 0) {
-    if (!upper) fetch4(std::false_type{}, 0, 0);
-    if (upper || kRoles == 2) fetch4(std::true_type{}, kRoles - 1, 0);
+    fetch_k4(0);
+    fetch_v4(0);
   } else if (tiles > 0) {
 #pragma unroll
     for (int o = 0; o < kRoles; ++o) fetch(o, 0);
@@ -1067,22 +1067,20 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
     char* const buf0 = lds;
     char* const buf1 = lds + kTileBytes<D>;
     // before the first step: K(0), its scales, and no values for no weights
-    if (!upper) {
+    if constexpr (k4) {
 #pragma unroll
-      for (int t = 0; t < 8; ++t) {
-        if constexpr (k4) decode4(std::false_type{}, 0, buf0, t);
-        else decode(0, 0, buf0, t);
-      }
+      for (int t = 0; t < kRoles * 2 * kWords; ++t) decode_k4(t / (2 * kWords), buf0, t % (2 * kWords));
+    } else if (!upper) {
+#pragma unroll
+      for (int t = 0; t < 8; ++t) decode(0, 0, buf0, t);
     }
     if constexpr (!k4) store_meta(0);
     for (int i = tid; i < kVBytes / 16; i += NW * kWave) reinterpret_cast<uint4*>(buf1 + kKBytes)[i] = uint4{0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = uint4{0, 0, 0, 0};
     turn_pages(0, 2);
-    if (!upper) {
-      if constexpr (k4) fetch4(std::false_type{}, 0, 1);
-      else fetch(0, 1);
-    }
+    if constexpr (k4) fetch_k4(1);
+    else if (!upper) fetch(0, 1);
     __syncthreads();
     if (upper) __syncthreads();
     for (int i = 0; i < tiles; ++i) {
@@ -1092,28 +1090,19 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
       // scales written, this one's read
       constexpr int kTasks = kRoles * 9 + 2;
       __builtin_amdgcn_s_setprio(1);  // the products go first: the other wave's vector work fills what they leave
-      if constexpr (k4) {
-        // K's and V's codes are decoded differently: a copy of the products for either role
-        const auto tasks = [&](auto is_v, int o, int t) {
-          constexpr bool v = decltype(is_v)::value;
-          if (t < 8) decode4(is_v, o, v ? cur : other, t);
-          else fetch4(is_v, o, v ? i + 1 : i + 2);
-        };
-        const auto run = [&](auto is_v) {
-          matrix(other, cur, std::true_type{}, [&](int k) {
-            constexpr int kAll4 = kRoles * 9;
+      matrix(other, cur, std::true_type{}, [&](int k) {
+        if constexpr (k4) {
+          // K(i + 1) and V(i), this wave's share of both, and the next codes
+          constexpr int kSteps4 = 2 * kWords, kTasks4 = kRoles * 2 * kSteps4 + 2;
 #pragma unroll
-            for (int t = k * kAll4 / kAll; t < (k + 1) * kAll4 / kAll; ++t) {
-              if constexpr (kRoles == 1) tasks(is_v, 0, t);
-              else if (t < 9) tasks(std::false_type{}, 0, t);
-              else tasks(std::true_type{}, kRoles - 1, t - 9);
-            }
-          });
-        };
-        if (upper) run(std::true_type{});
-        else run(std::false_type{});
-      } else {
-        matrix(other, cur, std::true_type{}, [&](int k) {
+          for (int t = k * kTasks4 / kAll; t < (k + 1) * kTasks4 / kAll; ++t) {
+            constexpr int kK = kRoles * kSteps4;
+            if (t < kK) decode_k4(t / kSteps4, other, t % kSteps4);
+            else if (t == kK) fetch_k4(i + 2);
+            else if (t <= 2 * kK) decode_v4((t - kK - 1) / kSteps4, cur, (t - kK - 1) % kSteps4);
+            else fetch_v4(i + 1);
+          }
+        } else {
 #pragma unroll
           for (int t = k * kTasks / kAll; t < (k + 1) * kTasks / kAll; ++t) {
             if (t == kTasks - 1) {
@@ -1128,8 +1117,8 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
               else fetch(o, v ? i + 1 : i + 2);
             }
           }
-        });
-      }
+        }
+      });
       __builtin_amdgcn_s_setprio(0);
       __syncthreads();
       weigh(i);
