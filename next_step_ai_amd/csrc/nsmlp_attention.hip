@@ -75,6 +75,8 @@ __device__ __forceinline__ int row_exponent(uint32_t top) { return min(max((int)
 
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
+__device__ __forceinline__ uint32_t top_of(uint32_t top, uint32_t w) { return max(top, max(w & 0x7FFFu, (w >> 16) & 0x7FFFu)); }
+
 __device__ __forceinline__ uint4 bf16_to_f16(const uint4& raw, int e) {
   uint32_t o[4];
 #pragma unroll
@@ -116,12 +118,13 @@ struct Pages {
   int first;
 };
 
+__device__ __forceinline__ int load_entry(const KvAttnArgs& a, int req, int first, int last, int lane) {
+  return a.table[(long long)req * a.max_blocks + min(min(first + lane, last), a.max_blocks - 1)];
+}
 template <int kFmt>
-__device__ __forceinline__ Pages load_pages(const KvAttnArgs& a, int req, int h, int first, int last, int lane) {
+__device__ __forceinline__ Pages pages_of(const KvAttnArgs& a, int id, int h, int first) {
   Pages p;
   p.first = first;
-  const int pg = min(min(first + lane, last), a.max_blocks - 1);
-  const int id = a.table[(long long)req * a.max_blocks + pg];
   const bool ok = id >= 0 && id < a.c.num_blocks;
   const long long bh = (long long)(ok ? id : 0) * a.c.heads + h;
   const long long off = bh * kv_block_bytes<kFmt>(a.c.B, a.c.D);
@@ -137,6 +140,11 @@ __device__ __forceinline__ Pages load_pages(const KvAttnArgs& a, int req, int h,
   p.lv = log2_fast(sv);
   p.iv = kUnit / sv;
   return p;
+}
+
+template <int kFmt>
+__device__ __forceinline__ Pages load_pages(const KvAttnArgs& a, int req, int h, int first, int last, int lane) {
+  return pages_of<kFmt>(a, load_entry(a, req, first, last, lane), h, first);
 }
 
 __device__ __forceinline__ const uint8_t* page_data(const KvAttnArgs& a, const Pages& p, int i) {
@@ -220,23 +228,22 @@ __device__ __forceinline__ KvUnit load_unit(const KvUnit* p) {
 // (269 MB, 31 partial results per row to join) 57.5 us, 4.7 TB/s.  A short chat (777
 // keys) takes 9.5 us, most of it the chain launch, schedule, lengths, block
 // table, scales, codes, join.
+struct StreamUnit {  // (4 bits) a unit and its request's rows and keys
+  int req, kv_begin, kv_end, part, first, parts, q0, q_len, kv_len;
+};
+
 template <int D, int NW>
 struct StreamLds {
   float sum[NW][16][D + 4];  // the waves' results
   float ml[NW][2][16];
   int last;
+  StreamUnit unit[kWave];
 };
 
-template <int D, int kFmt>
+template <int D>
 struct StreamTile {  // 32 keys, two tiles of 16: codes, and their blocks' scales in scalar registers
   uint4 k[2][D / 64], v[2][D / 64];
   float ks[2], lv[2], iv[2];
-  int bad;
-};
-template <int D>
-struct StreamTile<D, NSMLP_KV_E2M1> {
-  Codes4<D> k[2], v[2];
-  uint32_t ks[2], vs[2];  // scale bytes: of the lane's K, of its 4 tokens of V
   int bad;
 };
 
@@ -263,275 +270,14 @@ __device__ __forceinline__ void fill_unseen(const KvAttnArgs& a, int req, int h)
     a.lse[((first + i / a.group) * a.c.heads + h) * a.group + i % a.group] = -INFINITY;
 }
 
-template <int D, int kFmt, bool kBf16, int NW>
-__device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u, int h, StreamLds<D, NW>& lds) {
-  constexpr int NJ = D / 64, KS = D / 32, ND = D / 16;
-  constexpr bool k4 = kFmt == NSMLP_KV_E2M1;
-  // Weights go in two fp16 parts, 22 bits, so that their rounding does not add to
-  // the output's own (fp16: error against 64 bits 2.9e-4 -> 2.1e-4 of the norm, one
-  // rounding; bf16: 64 requests' outputs 7.6e-4 -> 5e-5 from those of fp32 weights).
-  // The products have the time, as the codes' way from memory takes longer:
-  // 131000 keys 57.8 us with one part and with two, 64 requests 82.7 and 82.9.
+// The end of a unit: its waves' results (reference m, sum of weights l of column
+// lane % 16; `put` writes the lane's sums of values times a factor to lds.sum) meet
+// in LDS, and the unit with the others of its rows.
+template <int D, bool kBf16, int NW, typename Put>
+__device__ __forceinline__ void stream_finish(const KvAttnArgs& a, const KvUnit& u, int h, StreamLds<D, NW>& lds, int q0, int rows, float m,
+                                              float l, Put&& put) {
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
-  const int q0 = uniform(a.q_start[u.req]), q_len = uniform(a.q_start[u.req + 1]) - q0, kv_len = uniform(a.kv_len[u.req]);
-  const int rows = q_len > kKvRowsA ? kKvRowsA : min(q_len * a.group, kKvRowsA);
-
-  // this wave's keys
-  const int each = ((u.kv_end - u.kv_begin + NW - 1) / NW + 31) & ~31;
-  const int begin = u.kv_begin + wave * each, end = min(begin + each, u.kv_end);
-  const int last = max(0, (u.kv_end - 1) >> a.c.b_shift);
-
-  // the first tiles' codes are on their way while the queries are made ready
-  unsigned long long bad_seen = 0;
-  Pages pages;
-  // where the lane's scales of 16 tokens are, in 4 bits (K: D/4 dims of a token, V: D/16 dims of 4 tokens)
-  const int ks_at = a.c.B * D + (grp * (D / 4) >> 5) * 16 + col;
-  const int vs_at = a.c.B * D + a.c.B * D / 32 + (grp * (D / 32) + (col * (D / 16) >> 5)) * 4;
-  const auto load = [&](StreamTile<D, kFmt>& t, int pos) {
-    t.bad = 0;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const int at = pos + 16 * s, pg = min(at >> a.c.b_shift, last) - pages.first;
-      if constexpr (k4) {
-        t.bad |= ((int)(pages.bad >> pg) & 1) << s;
-        const uint8_t* base = page_data(a, pages, pg);
-        const int tile = (at & (a.c.B - 1)) >> 4;
-        t.k[s] = load_codes4<D>(base + tile * (8 * D) + lane * (D / 8));
-        t.v[s] = load_codes4<D>(base + a.c.B * D / 2 + tile * (8 * D) + lane * (D / 8));
-        t.ks[s] = base[ks_at + tile * (D / 2)];
-        t.vs[s] = *reinterpret_cast<const uint32_t*>(base + vs_at + tile * (D / 2));
-        continue;
-      } else {
-        t.ks[s] = lane_of(pages.ks, pg), t.lv[s] = lane_of(pages.lv, pg), t.iv[s] = lane_of(pages.iv, pg);
-        t.bad |= ((int)(pages.bad >> pg) & 1) << s;
-        const uint8_t* kb = page_data(a, pages, pg) + ((at & (a.c.B - 1)) >> 4) * (16 * D);
-        const uint8_t* vb = kb + a.c.B * D;
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          t.k[s][j] = *reinterpret_cast<const uint4*>(kb + j * 1024 + lane * 16);
-          t.v[s][j] = *reinterpret_cast<const uint4*>(vb + j * 1024 + lane * 16);
-        }
-      }
-    }
-  };
-  // past the wave's keys its last tile is read again: no branch around a load
-  const int last_tile = begin < end ? begin + ((end - 1 - begin) & ~31) : begin;
-  const auto fetch = [&](StreamTile<D, kFmt>& t, int pos) {
-    pos = min(pos, last_tile);
-    if (min((pos + 31) >> a.c.b_shift, last) - pages.first >= kWave) {
-      pages = load_pages<kFmt>(a, u.req, h, pos >> a.c.b_shift, last, lane);
-      bad_seen |= pages.bad;
-    }
-    load(t, pos);
-  };
-  StreamTile<D, kFmt> t0, t1, t2, t3;  // (in 8 bits the last two are not used)
-  if (begin < end) {
-    pages = load_pages<kFmt>(a, u.req, h, begin >> a.c.b_shift, last, lane);
-    bad_seen = pages.bad;
-    load(t0, begin);
-    if constexpr (k4) fetch(t1, begin + 32), fetch(t2, begin + 64);
-  }
-
-  // queries: columns of the products, 8 dims per lane and step
-  half8_t q[KS];
-  float rowf = a.scale_log2;
-  const int tok = col / a.group;
-  const bool in = col < rows && in_step(a, q0 + tok);
-  const int limit = in ? kv_len - q_len + tok + 1 : 0x7FFFFFFF;  // keys that the row sees
-  {
-    const uint16_t* src = a.q + (long long)(q0 + tok) * a.q_row + (long long)(h * a.group + col % a.group) * a.q_head;
-    uint4 raw[KS];
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-      raw[s] = in ? *reinterpret_cast<const uint4*>(src + (k4 ? (D / 4) * grp + 8 * s : 64 * (s >> 1) + 16 * grp + 8 * (s & 1)))
-                  : uint4{0, 0, 0, 0};
-    if constexpr (kBf16) {
-      uint32_t top = 0;
-#pragma unroll
-      for (int s = 0; s < KS; ++s)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = max(top, max(word(raw[s], i) & 0x7FFFu, (word(raw[s], i) >> 16) & 0x7FFFu));
-      top = max(top, (uint32_t)__shfl_xor((int)top, 16, kWave));
-      top = max(top, (uint32_t)__shfl_xor((int)top, 32, kWave));
-      const int e = row_exponent(top);
-      rowf *= ldexpf(1.0f, e);
-#pragma unroll
-      for (int s = 0; s < KS; ++s) q[s] = as_h8(bf16_to_f16(raw[s], e));
-    } else {
-#pragma unroll
-      for (int s = 0; s < KS; ++s) q[s] = as_h8(raw[s]);
-    }
-  }
-  // keys below this need no mask: every row of the unit sees them
-  const int plain = kv_len - q_len + 1;
-
-  float m = kLowest, l = 0.0f;  // reference, sum of the weights
-  float sum_limit = kSumLimit;  // (below any sum where m is far)
-  float4_t acc[ND];
-#pragma unroll
-  for (int d = 0; d < ND; ++d) acc[d] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-
-  const auto use = [&](auto masked, const StreamTile<D, kFmt>& t, int pos) {
-    constexpr bool kMasked = decltype(masked)::value;
-    float4_t sc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-#pragma unroll
-    for (int i = 0; i < KS; ++i)
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        if constexpr (k4) {
-          const float f = scale4(t.ks[s], 0);
-          const uint32_t c = t.k[s].w[i];
-          sc[s] = mfma16(as_h8(uint4{values4(c, f, 0), values4(c, f, 1), values4(c, f, 2), values4(c, f, 3)}), q[i], sc[s]);
-        } else {
-          sc[s] = mfma16(join4(kv_half4<kFmt>(word(t.k[s][i >> 1], 2 * (i & 1))), kv_half4<kFmt>(word(t.k[s][i >> 1], 2 * (i & 1) + 1))),
-                         q[i], sc[s]);
-        }
-      }
-    mfma_drain();
-    // bit 4 s + i: whether the row sees the lane's key i of the s-th 16
-    uint32_t see = 0xFF;
-    if constexpr (kMasked) {
-      see = 0;
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int n = (t.bad >> s) & 1 ? 0 : min(max(limit - pos - 16 * s - 4 * grp, 0), 4);
-        see |= ((1u << n) - 1u) << (4 * s);
-      }
-    }
-    uint2 w[2], rest[2];  // weights, and what their rounding left
-    float dl;
-    float gs[2], lvs[2], ivs[2];
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      if constexpr (k4) gs[s] = rowf, lvs[s] = 0.0f, ivs[s] = kUnit;
-      else gs[s] = t.ks[s] * rowf, lvs[s] = t.lv[s], ivs[s] = t.iv[s];
-    }
-    const auto weights = [&]() {
-      float sums[2];
-      dl = 0.0f;
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const float g = gs[s], c = lvs[s] - m;
-        float p[4], share = ivs[s];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = exp2_fast(__builtin_fmaf(sc[s][i], g, c));
-        if constexpr (kMasked) {
-          // a hidden key's weight is zero whatever its block's scales are
-#pragma unroll
-          for (int i = 0; i < 4; ++i) p[i] = (see >> (4 * s + i)) & 1 ? p[i] : 0.0f;
-          share = (see >> (4 * s)) & 0xF ? share : 0.0f;
-        }
-        w[s] = uint2{pack_f16(p[0], p[1]), pack_f16(p[2], p[3])};
-        const half2_t a0 = as_half2(w[s].x), a1 = as_half2(w[s].y);
-        rest[s] = uint2{pack_f16(p[0] - (float)a0.x, p[1] - (float)a0.y), pack_f16(p[2] - (float)a1.x, p[3] - (float)a1.y)};
-        sums[s] = (p[0] + p[1]) + (p[2] + p[3]);
-        dl = __builtin_fmaf(sums[s], share, dl);
-      }
-      return fmaxf(sums[0], sums[1]);
-    };
-    const float sum = weights();
-    if (__builtin_expect_with_probability(__any(sum > sum_limit), 0, 0.999)) {
-      float top = kLowest;
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, (see >> (4 * s + i)) & 1 ? __builtin_fmaf(sc[s][i], gs[s], lvs[s]) : kLowest);
-      top = fmaxf(top, __shfl_xor(top, 16, kWave));
-      top = reference_of(fmaxf(top, __shfl_xor(top, 32, kWave)));
-      top = fmaxf(m, top);  // (never down: other rows may have asked)
-      const float scale = exp2_fast(m - top);
-      m = top;
-      sum_limit = is_far(m) ? -1.0f : kSumLimit;
-      l *= scale;
-#pragma unroll
-      for (int d = 0; d < ND; ++d) acc[d] *= scale;
-      if (__builtin_expect_with_probability(__any(is_far(m)), 0, 0.999)) {  // the scores become their weights' exponents
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sc[s][i] = far_exponent(sc[s][i], gs[s], lvs[s], m);
-          gs[s] = 1.0f, lvs[s] = m;
-        }
-      }
-      (void)weights();
-    }
-    l += dl;
-    uint32_t keep[2] = {~0u, ~0u};
-    if (kFmt == NSMLP_KV_E4M3 && kMasked) {
-      // codes past the end may be NaNs: a zero weight does not hide them
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int left = (t.bad >> s) & 1 ? 0 : kv_len - (pos + 16 * s + 4 * grp);
-        keep[s] = left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
-      }
-    }
-    const half8_t wh = join4(w[0], w[1]), wr = join4(rest[0], rest[1]);
-    if constexpr (k4) {
-#pragma unroll
-      for (int m2 = 0; m2 < ND / 2; ++m2) {
-        uint32_t c[2][4];
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) c[s][j] = token_values4<D>(t.v[s], t.vs[s], j, m2);
-        const half8_t lo = join4(lower4(c[0]), lower4(c[1])), hi = join4(upper4(c[0]), upper4(c[1]));
-        acc[2 * m2] = mfma16(lo, wh, acc[2 * m2]);
-        acc[2 * m2] = mfma16(lo, wr, acc[2 * m2]);
-        acc[2 * m2 + 1] = mfma16(hi, wh, acc[2 * m2 + 1]);
-        acc[2 * m2 + 1] = mfma16(hi, wr, acc[2 * m2 + 1]);
-      }
-      return;
-    }
-#pragma unroll
-    for (int d = 0; d < ND; ++d) {
-      if constexpr (!k4) {
-        const half8_t v = join4(kv_half4<kFmt>(word(t.v[0][d >> 2], d & 3) & keep[0]), kv_half4<kFmt>(word(t.v[1][d >> 2], d & 3) & keep[1]));
-        acc[d] = mfma16(v, wh, acc[d]);
-        acc[d] = mfma16(v, wr, acc[d]);
-      }
-    }
-  };
-  if (k4 && begin < end) {
-    // half the bytes of a key: three tiles' codes on their way behind the one in use
-    int pos = begin;
-    while (pos + 128 <= min(end, plain) && bad_seen == 0) {
-      fetch(t3, pos + 96);
-      if (bad_seen != 0) break;  // (of a new window of pages, which may be t3's; t0 to t2 are older or looked at next time)
-      use(std::false_type{}, t0, pos);
-      fetch(t0, pos + 128);
-      use(std::false_type{}, t1, pos + 32);
-      fetch(t1, pos + 160);
-      use(std::false_type{}, t2, pos + 64);
-      fetch(t2, pos + 192);
-      use(std::false_type{}, t3, pos + 96);
-      pos += 128;
-    }
-    while (pos < end) {
-      fetch(t3, pos + 96);
-      use(std::true_type{}, t0, pos);
-      t0 = t1, t1 = t2, t2 = t3;
-      pos += 32;
-    }
-  } else if (begin < end) {
-    int pos = begin;
-    while (pos + 64 <= min(end, plain) && bad_seen == 0) {  // two tiles, the next two's codes behind them
-      fetch(t1, pos + 32);
-      if (bad_seen != 0) break;  // (of a new window of pages, which may be t1's)
-      use(std::false_type{}, t0, pos);
-      fetch(t0, pos + 64);
-      use(std::false_type{}, t1, pos + 32);
-      pos += 64;
-    }
-    while (pos < end) {
-      fetch(t1, pos + 32);
-      use(std::true_type{}, t0, pos);
-      t0 = t1;
-      pos += 32;
-    }
-  }
-  if (bad_seen != 0 && lane == 0) atomicOr(a.status, NSMLP_STATUS_BLOCK_UNAVAILABLE);
-
   mfma_drain();
   // join the waves: each result under the largest reference
   l += __shfl_xor(l, 16, kWave);
@@ -542,21 +288,7 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
     float top = kLowest;
 #pragma unroll
     for (int w = 0; w < NW; ++w) top = fmaxf(top, lds.ml[w][0][col]);
-    const float scale = exp2_fast(m - top);
-    if constexpr (k4) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int n = 0; n < ND; n += 4)
-          *reinterpret_cast<float4_t*>(&lds.sum[wave][col][ND * (4 * grp + i) + n]) =
-              float4_t{acc[n][i], acc[n + 1][i], acc[n + 2][i], acc[n + 3][i]} * scale;
-    }
-#pragma unroll
-    for (int j = 0; !k4 && j < NJ; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<float4_t*>(&lds.sum[wave][col][64 * j + 16 * grp + 4 * i]) =
-            float4_t{acc[4 * j][i], acc[4 * j + 1][i], acc[4 * j + 2][i], acc[4 * j + 3][i]} * scale;
+    put(exp2_fast(m - top));
   }
   __syncthreads();
   constexpr int kPerRow = NW * kWave / 16, kDims = D / kPerRow;
@@ -642,6 +374,217 @@ __device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u,
   }
 }
 
+template <int D, int kFmt, bool kBf16, int NW>
+__device__ __forceinline__ void stream_unit(const KvAttnArgs& a, const KvUnit u, int h, StreamLds<D, NW>& lds) {
+  constexpr int NJ = D / 64, KS = D / 32, ND = D / 16;
+  // Weights go in two fp16 parts, 22 bits, so that their rounding does not add to
+  // the output's own (fp16: error against 64 bits 2.9e-4 -> 2.1e-4 of the norm, one
+  // rounding; bf16: 64 requests' outputs 7.6e-4 -> 5e-5 from those of fp32 weights).
+  // The products have the time, as the codes' way from memory takes longer:
+  // 131000 keys 57.8 us with one part and with two, 64 requests 82.7 and 82.9.
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, grp = lane >> 4;
+  const int q0 = uniform(a.q_start[u.req]), q_len = uniform(a.q_start[u.req + 1]) - q0, kv_len = uniform(a.kv_len[u.req]);
+  const int rows = q_len > kKvRowsA ? kKvRowsA : min(q_len * a.group, kKvRowsA);
+
+  // this wave's keys
+  const int each = ((u.kv_end - u.kv_begin + NW - 1) / NW + 31) & ~31;
+  const int begin = u.kv_begin + wave * each, end = min(begin + each, u.kv_end);
+  const int last = max(0, (u.kv_end - 1) >> a.c.b_shift);
+
+  // the first tiles' codes are on their way while the queries are made ready
+  unsigned long long bad_seen = 0;
+  Pages pages;
+  const auto load = [&](StreamTile<D>& t, int pos) {
+    t.bad = 0;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int at = pos + 16 * s, pg = min(at >> a.c.b_shift, last) - pages.first;
+      t.ks[s] = lane_of(pages.ks, pg), t.lv[s] = lane_of(pages.lv, pg), t.iv[s] = lane_of(pages.iv, pg);
+      t.bad |= ((int)(pages.bad >> pg) & 1) << s;
+      const uint8_t* kb = page_data(a, pages, pg) + ((at & (a.c.B - 1)) >> 4) * (16 * D);
+      const uint8_t* vb = kb + a.c.B * D;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        t.k[s][j] = *reinterpret_cast<const uint4*>(kb + j * 1024 + lane * 16);
+        t.v[s][j] = *reinterpret_cast<const uint4*>(vb + j * 1024 + lane * 16);
+      }
+    }
+  };
+  // past the wave's keys its last tile is read again: no branch around a load
+  const int last_tile = begin < end ? begin + ((end - 1 - begin) & ~31) : begin;
+  const auto fetch = [&](StreamTile<D>& t, int pos) {
+    pos = min(pos, last_tile);
+    if (min((pos + 31) >> a.c.b_shift, last) - pages.first >= kWave) {
+      pages = load_pages<kFmt>(a, u.req, h, pos >> a.c.b_shift, last, lane);
+      bad_seen |= pages.bad;
+    }
+    load(t, pos);
+  };
+  StreamTile<D> t0, t1;
+  if (begin < end) {
+    pages = load_pages<kFmt>(a, u.req, h, begin >> a.c.b_shift, last, lane);
+    bad_seen = pages.bad;
+    load(t0, begin);
+  }
+
+  // queries: columns of the products, 8 dims per lane and step
+  half8_t q[KS];
+  float rowf = a.scale_log2;
+  const int tok = col / a.group;
+  const bool in = col < rows && in_step(a, q0 + tok);
+  const int limit = in ? kv_len - q_len + tok + 1 : 0x7FFFFFFF;  // keys that the row sees
+  {
+    const uint16_t* src = a.q + (long long)(q0 + tok) * a.q_row + (long long)(h * a.group + col % a.group) * a.q_head;
+    uint4 raw[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+      raw[s] = in ? *reinterpret_cast<const uint4*>(src + 64 * (s >> 1) + 16 * grp + 8 * (s & 1)) : uint4{0, 0, 0, 0};
+    if constexpr (kBf16) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = max(top, max(word(raw[s], i) & 0x7FFFu, (word(raw[s], i) >> 16) & 0x7FFFu));
+      top = max(top, (uint32_t)__shfl_xor((int)top, 16, kWave));
+      top = max(top, (uint32_t)__shfl_xor((int)top, 32, kWave));
+      const int e = row_exponent(top);
+      rowf *= ldexpf(1.0f, e);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) q[s] = as_h8(bf16_to_f16(raw[s], e));
+    } else {
+#pragma unroll
+      for (int s = 0; s < KS; ++s) q[s] = as_h8(raw[s]);
+    }
+  }
+  // keys below this need no mask: every row of the unit sees them
+  const int plain = kv_len - q_len + 1;
+
+  float m = kLowest, l = 0.0f;  // reference, sum of the weights
+  float sum_limit = kSumLimit;  // (below any sum where m is far)
+  float4_t acc[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) acc[d] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+
+  const auto use = [&](auto masked, const StreamTile<D>& t, int pos) {
+    constexpr bool kMasked = decltype(masked)::value;
+    float4_t sc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+    for (int i = 0; i < KS; ++i)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        sc[s] = mfma16(join4(kv_half4<kFmt>(word(t.k[s][i >> 1], 2 * (i & 1))), kv_half4<kFmt>(word(t.k[s][i >> 1], 2 * (i & 1) + 1))),
+                       q[i], sc[s]);
+    mfma_drain();
+    // bit 4 s + i: whether the row sees the lane's key i of the s-th 16
+    uint32_t see = 0xFF;
+    if constexpr (kMasked) {
+      see = 0;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int n = (t.bad >> s) & 1 ? 0 : min(max(limit - pos - 16 * s - 4 * grp, 0), 4);
+        see |= ((1u << n) - 1u) << (4 * s);
+      }
+    }
+    uint2 w[2], rest[2];  // weights, and what their rounding left
+    float dl;
+    float gs[2] = {t.ks[0] * rowf, t.ks[1] * rowf}, lvs[2] = {t.lv[0], t.lv[1]};
+    const auto weights = [&]() {
+      float sums[2];
+      dl = 0.0f;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const float g = gs[s], c = lvs[s] - m;
+        float p[4], share = t.iv[s];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = exp2_fast(__builtin_fmaf(sc[s][i], g, c));
+        if constexpr (kMasked) {
+          // a hidden key's weight is zero whatever its block's scales are
+#pragma unroll
+          for (int i = 0; i < 4; ++i) p[i] = (see >> (4 * s + i)) & 1 ? p[i] : 0.0f;
+          share = (see >> (4 * s)) & 0xF ? share : 0.0f;
+        }
+        w[s] = uint2{pack_f16(p[0], p[1]), pack_f16(p[2], p[3])};
+        const half2_t a0 = as_half2(w[s].x), a1 = as_half2(w[s].y);
+        rest[s] = uint2{pack_f16(p[0] - (float)a0.x, p[1] - (float)a0.y), pack_f16(p[2] - (float)a1.x, p[3] - (float)a1.y)};
+        sums[s] = (p[0] + p[1]) + (p[2] + p[3]);
+        dl = __builtin_fmaf(sums[s], share, dl);
+      }
+      return fmaxf(sums[0], sums[1]);
+    };
+    const float sum = weights();
+    if (__builtin_expect_with_probability(__any(sum > sum_limit), 0, 0.999)) {
+      float top = kLowest;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, (see >> (4 * s + i)) & 1 ? __builtin_fmaf(sc[s][i], gs[s], lvs[s]) : kLowest);
+      top = fmaxf(top, __shfl_xor(top, 16, kWave));
+      top = reference_of(fmaxf(top, __shfl_xor(top, 32, kWave)));
+      top = fmaxf(m, top);  // (never down: other rows may have asked)
+      const float scale = exp2_fast(m - top);
+      m = top;
+      sum_limit = is_far(m) ? -1.0f : kSumLimit;
+      l *= scale;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) acc[d] *= scale;
+      if (__builtin_expect_with_probability(__any(is_far(m)), 0, 0.999)) {  // the scores become their weights' exponents
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sc[s][i] = far_exponent(sc[s][i], gs[s], lvs[s], m);
+          gs[s] = 1.0f, lvs[s] = m;
+        }
+      }
+      (void)weights();
+    }
+    l += dl;
+    uint32_t keep[2] = {~0u, ~0u};
+    if (kFmt == NSMLP_KV_E4M3 && kMasked) {
+      // codes past the end may be NaNs: a zero weight does not hide them
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int left = (t.bad >> s) & 1 ? 0 : kv_len - (pos + 16 * s + 4 * grp);
+        keep[s] = left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+      }
+    }
+    const half8_t wh = join4(w[0], w[1]), wr = join4(rest[0], rest[1]);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      const half8_t v = join4(kv_half4<kFmt>(word(t.v[0][d >> 2], d & 3) & keep[0]), kv_half4<kFmt>(word(t.v[1][d >> 2], d & 3) & keep[1]));
+      acc[d] = mfma16(v, wh, acc[d]);
+      acc[d] = mfma16(v, wr, acc[d]);
+    }
+  };
+  if (begin < end) {
+    int pos = begin;
+    while (pos + 64 <= min(end, plain) && bad_seen == 0) {  // two tiles, the next two's codes behind them
+      fetch(t1, pos + 32);
+      if (bad_seen != 0) break;  // (of a new window of pages, which may be t1's)
+      use(std::false_type{}, t0, pos);
+      fetch(t0, pos + 64);
+      use(std::false_type{}, t1, pos + 32);
+      pos += 64;
+    }
+    while (pos < end) {
+      fetch(t1, pos + 32);
+      use(std::true_type{}, t0, pos);
+      t0 = t1;
+      pos += 32;
+    }
+  }
+  if (bad_seen != 0 && lane == 0) atomicOr(a.status, NSMLP_STATUS_BLOCK_UNAVAILABLE);
+
+  stream_finish<D, kBf16, NW>(a, u, h, lds, q0, rows, m, l, [&](float scale) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<float4_t*>(&lds.sum[wave][col][64 * j + 16 * grp + 4 * i]) =
+            float4_t{acc[4 * j][i], acc[4 * j + 1][i], acc[4 * j + 2][i], acc[4 * j + 3][i]} * scale;
+  });
+}
+
 // A workgroup's share of list a: the units from the share's first to the next
 // one's.  The 8 XCDs take shares in turn and all heads of a share: heads of a
 // block have their scales in one line, which one L2 then fetches once.
@@ -661,11 +604,280 @@ __device__ __forceinline__ void stream_share(const KvAttnArgs& a, int block, Str
   }
 }
 
+// The same in 4 bits.  A key is half as many bytes, so what is not its way from
+// memory shows: three tiles are on their way behind the one in use, and the waves
+// go from one unit to the next without a pause: what a share's units are is
+// read once, for all of them at a time, and while a unit's last tiles are in use
+// the next one's first are fetched, its pages and queries before.
+template <int D>
+struct StreamTile4 {
+  Codes4<D> k[2], v[2];
+  uint32_t ks[2], vs[2];  // scale bytes: of the lane's K, of its 4 tokens of V
+  int bad;
+};
+
+template <int D, bool kBf16, int NW, bool kAhead>
+__device__ __forceinline__ void stream_share4(const KvAttnArgs& a, int block, StreamLds<D, NW>& lds) {
+  constexpr int KS = D / 32, ND = D / 16, kFmt = NSMLP_KV_E2M1;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, grp = lane >> 4;
+  const int h = (block >> 3) % a.c.heads, share = (block >> 3) / a.c.heads * 8 + (block & 7);
+  const int shares = min(a.sched[1], a.s.shares), units = min(a.sched[0], a.s.max_units_a);
+  if (share >= shares) return;
+  const int32_t* start = a.sched + a.s.off_shares;
+  const int first = uniform(start[share]), stop = uniform(share + 1 < shares ? min(start[share + 1], units) : units);
+  const KvUnit* list = reinterpret_cast<const KvUnit*>(a.sched + a.s.off_units_a);
+
+  // the tile of 32 keys at `pos`: codes, and scale bytes of the lane's D/4 dims of K and of its 4 tokens' D/16 dims of V
+  Pages pages;
+  unsigned long long bad_seen = 0;
+  const int ks_at = a.c.B * D + (grp * (D / 4) >> 5) * 16 + col;
+  const int vs_at = a.c.B * D + a.c.B * D / 32 + (grp * (D / 32) + (col * (D / 16) >> 5)) * 4;
+  // where the next tile comes from: this wave's keys [., end) of a request, pages up to `last`
+  struct Cursor {
+    int req, pos, end, last;
+  } at = {};
+  const auto span = [&](int i) {  // of unit i
+    const StreamUnit& u = lds.unit[i];
+    const int begin = uniform(u.kv_begin), end = uniform(u.kv_end), each = ((end - begin + NW - 1) / NW + 31) & ~31;
+    const int mine = begin + wave * each;
+    return Cursor{uniform(u.req), mine, min(mine + each, end), max(0, (end - 1) >> a.c.b_shift)};
+  };
+  Cursor next = {};
+  bool next_there = false;  // whether the next unit's keys may follow this one's
+  int next_entry = 0;       // its table entries, one per lane
+  const auto fetch = [&](StreamTile4<D>& t) {
+    if (kAhead && uniform(at.pos >= at.end && next_there)) {
+      at = Cursor{uniform(next.req), uniform(next.pos), uniform(next.end), uniform(next.last)}, next_there = false;
+      pages = pages_of<kFmt>(a, next_entry, h, at.pos >> a.c.b_shift);
+      bad_seen |= pages.bad;
+    }
+    // past the last keys their tile is read again: no branch around a load
+    const int pos = uniform(min(at.pos, (at.end - 1) & ~31));
+    if (min((pos + 31) >> a.c.b_shift, at.last) - pages.first >= kWave) {
+      pages = load_pages<kFmt>(a, at.req, h, pos >> a.c.b_shift, at.last, lane);
+      bad_seen |= pages.bad;
+    }
+    t.bad = 0;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int key = pos + 16 * s, pg = min(key >> a.c.b_shift, at.last) - pages.first, tile = (key & (a.c.B - 1)) >> 4;
+      t.bad |= ((int)(pages.bad >> pg) & 1) << s;
+      const uint8_t* base = page_data(a, pages, pg);
+      t.k[s] = load_codes4<D>(base + tile * (8 * D) + lane * (D / 8));
+      t.v[s] = load_codes4<D>(base + a.c.B * D / 2 + tile * (8 * D) + lane * (D / 8));
+      t.ks[s] = base[ks_at + tile * (D / 2)];
+      t.vs[s] = *reinterpret_cast<const uint32_t*>(base + vs_at + tile * (D / 2));
+    }
+    at.pos += 32;
+  };
+
+  for (int base = first; base < stop; base += kWave) {
+    const int n = min(kWave, stop - base);
+    __syncthreads();
+    if (tid < n) {
+      const KvUnit v = list[base + tid];
+      const int q0 = a.q_start[v.req];
+      lds.unit[tid] = StreamUnit{v.req, v.kv_begin, v.kv_end, v.part, v.first, v.parts, q0, a.q_start[v.req + 1] - q0, a.kv_len[v.req]};
+    }
+    __syncthreads();
+    StreamTile4<D> t0, t1;
+    bool ready = false;  // whether t0 is the unit's first tile
+    uint4 raw[KS];       // the unit's queries
+    for (int i = 0; i < n; ++i) {
+      const StreamUnit m_u = lds.unit[i];
+      const int q0 = uniform(m_u.q0), q_len = uniform(m_u.q_len), kv_len = uniform(m_u.kv_len);
+      const KvUnit u = {uniform(m_u.req), 0, uniform(m_u.kv_begin), uniform(m_u.kv_end), uniform(m_u.part), uniform(m_u.first), uniform(m_u.parts), 0};
+      if (u.kv_end == 0) {
+        fill_unseen<D>(a, u.req, h);
+        ready = false;
+        continue;
+      }
+      const auto load_queries = [&](int from, int len) {  // columns of the products, 8 dims per lane and step
+        const int tok = col / a.group, rows = len > kKvRowsA ? kKvRowsA : min(len * a.group, kKvRowsA);
+        const bool in = col < rows && in_step(a, from + tok);
+        const uint16_t* src = a.q + (long long)(from + tok) * a.q_row + (long long)(h * a.group + col % a.group) * a.q_head;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) raw[s] = in ? *reinterpret_cast<const uint4*>(src + (D / 4) * grp + 8 * s) : uint4{0, 0, 0, 0};
+      };
+      const Cursor mine = span(i);
+      int pos = mine.pos;
+      const int end = mine.end;
+      if (!ready) {
+        at = mine;
+        next_there = false;
+        if (pos < end) {
+          pages = load_pages<kFmt>(a, u.req, h, pos >> a.c.b_shift, at.last, lane);
+          bad_seen |= pages.bad;
+          fetch(t0);
+        }
+        load_queries(q0, q_len);
+      }
+      half8_t q[KS];
+      float rowf = a.scale_log2;
+      const int rows = q_len > kKvRowsA ? kKvRowsA : min(q_len * a.group, kKvRowsA), tok = col / a.group;
+      const int limit = col < rows && in_step(a, q0 + tok) ? kv_len - q_len + tok + 1 : 0x7FFFFFFF;  // keys that the row sees
+      if constexpr (kBf16) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) top = top_of(top, word(raw[s], j));
+        top = max(top, (uint32_t)__shfl_xor((int)top, 16, kWave));
+        top = max(top, (uint32_t)__shfl_xor((int)top, 32, kWave));
+        const int e = row_exponent(top);
+        rowf *= ldexpf(1.0f, e);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) q[s] = as_h8(bf16_to_f16(raw[s], e));
+      } else {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) q[s] = as_h8(raw[s]);
+      }
+      const int plain = kv_len - q_len + 1;  // keys below this need no mask: every row of the unit sees them
+      // what follows this unit's keys
+      next_there = false;
+      if (kAhead && i + 1 < n) {
+        const StreamUnit& v = lds.unit[i + 1];
+        next = span(i + 1);
+        next_there = next.pos < next.end && pos < end;
+        next_entry = load_entry(a, next.req, max(next.pos, 0) >> a.c.b_shift, next.last, lane);
+        load_queries(uniform(v.q0), uniform(v.q_len));
+      }
+      const bool follows = next_there;
+
+      float m = kLowest, l = 0.0f;  // reference, sum of the weights
+      float sum_limit = kSumLimit;  // (below any sum where m is far)
+      float4_t acc[ND];
+#pragma unroll
+      for (int d = 0; d < ND; ++d) acc[d] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      const auto use = [&](auto masked, const StreamTile4<D>& t, int key) {
+        constexpr bool kMasked = decltype(masked)::value;
+        float4_t sc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+        for (int j = 0; j < KS; ++j)
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            const float f = scale4(t.ks[s], 0);
+            const uint32_t c = t.k[s].w[j];
+            sc[s] = mfma16(as_h8(uint4{values4(c, f, 0), values4(c, f, 1), values4(c, f, 2), values4(c, f, 3)}), q[j], sc[s]);
+          }
+        mfma_drain();
+        // bit 4 s + j: whether the row sees the lane's key j of the s-th 16
+        uint32_t see = 0xFF;
+        if constexpr (kMasked) {
+          see = 0;
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            const int count = (t.bad >> s) & 1 ? 0 : min(max(min(limit, end) - key - 16 * s - 4 * grp, 0), 4);
+            see |= ((1u << count) - 1u) << (4 * s);
+          }
+        }
+        uint2 w[2], rest[2];  // weights, and what their rounding left
+        float sums[2], g = rowf, c = -m;
+        const auto weights = [&]() {
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            float p[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) p[j] = exp2_fast(__builtin_fmaf(sc[s][j], g, c));
+            if constexpr (kMasked) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) p[j] = (see >> (4 * s + j)) & 1 ? p[j] : 0.0f;
+            }
+            w[s] = uint2{pack_f16(p[0], p[1]), pack_f16(p[2], p[3])};
+            const half2_t a0 = as_half2(w[s].x), a1 = as_half2(w[s].y);
+            rest[s] = uint2{pack_f16(p[0] - (float)a0.x, p[1] - (float)a0.y), pack_f16(p[2] - (float)a1.x, p[3] - (float)a1.y)};
+            sums[s] = (p[0] + p[1]) + (p[2] + p[3]);
+          }
+        };
+        weights();
+        if (__builtin_expect_with_probability(__any(fmaxf(sums[0], sums[1]) > sum_limit), 0, 0.999)) {
+          float top = kLowest;
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) top = fmaxf(top, (see >> (4 * s + j)) & 1 ? sc[s][j] * rowf : kLowest);
+          top = fmaxf(top, __shfl_xor(top, 16, kWave));
+          top = reference_of(fmaxf(top, __shfl_xor(top, 32, kWave)));
+          top = fmaxf(m, top);  // (never down: other rows may have asked)
+          const float scale = exp2_fast(m - top);
+          m = top, c = -m;
+          sum_limit = is_far(m) ? -1.0f : kSumLimit;
+          l *= scale;
+#pragma unroll
+          for (int d = 0; d < ND; ++d) acc[d] *= scale;
+          if (__builtin_expect_with_probability(__any(is_far(m)), 0, 0.999)) {  // the scores become their weights' exponents
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) sc[s][j] = far_exponent(sc[s][j], rowf, 0.0f, m);
+            g = 1.0f, c = 0.0f;
+          }
+          weights();
+        }
+        l += sums[0] + sums[1];
+        const half8_t wh = join4(w[0], w[1]), wr = join4(rest[0], rest[1]);
+#pragma unroll
+        for (int d = 0; d < ND / 2; ++d) {
+          uint32_t v[2][4];
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[s][j] = token_values4<D>(t.v[s], t.vs[s], j, d);
+          const half8_t lo = join4(lower4(v[0]), lower4(v[1])), hi = join4(upper4(v[0]), upper4(v[1]));
+          acc[2 * d] = mfma16(lo, wh, acc[2 * d]);
+          acc[2 * d] = mfma16(lo, wr, acc[2 * d]);
+          acc[2 * d + 1] = mfma16(hi, wh, acc[2 * d + 1]);
+          acc[2 * d + 1] = mfma16(hi, wr, acc[2 * d + 1]);
+        }
+      };
+      while (pos + 64 <= min(end, plain) && bad_seen == 0) {
+        fetch(t1);
+        if (bad_seen != 0) {  // (of a new window of pages, which may be t1's: fetched again below)
+          at.pos -= 32;
+          break;
+        }
+        use(std::false_type{}, t0, pos);
+        fetch(t0);
+        use(std::false_type{}, t1, pos + 32);
+        pos += 64;
+      }
+      while (pos < end) {
+        fetch(t1);
+        use(std::true_type{}, t0, pos);
+        t0 = t1;
+        pos += 32;
+      }
+      ready = follows;
+      stream_finish<D, kBf16, NW>(a, u, h, lds, q0, rows, m, l * kUnit, [&](float scale) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int d = 0; d < ND; d += 4)
+            *reinterpret_cast<float4_t*>(&lds.sum[wave][col][ND * (4 * grp + j) + d]) =
+                float4_t{acc[d][j], acc[d + 1][j], acc[d + 2][j], acc[d + 3][j]} * scale;
+      });
+      __syncthreads();
+    }
+  }
+  if (bad_seen != 0 && lane == 0) atomicOr(a.status, NSMLP_STATUS_BLOCK_UNAVAILABLE);
+}
+
+template <int D, int kFmt, bool kBf16, int NW, bool kAhead>
+__device__ __forceinline__ void any_share(const KvAttnArgs& a, int block, StreamLds<D, NW>& lds) {
+  if constexpr (kFmt == NSMLP_KV_E2M1) stream_share4<D, kBf16, NW, kAhead>(a, block, lds);
+  else stream_share<D, kFmt, kBf16, NW>(a, block, lds);
+}
+
+template <int kFmt>
+constexpr int kStreamWaves = kFmt == NSMLP_KV_E2M1 ? 8 : 4;
+
 template <int D, int kFmt, bool kBf16>
-__global__ void __launch_bounds__(4 * kWave) k_attn_stream(KvAttnArgs a) {
+__global__ void __launch_bounds__(kStreamWaves<kFmt>* kWave) k_attn_stream(KvAttnArgs a) {
+  constexpr int NW = kStreamWaves<kFmt>;
   kernarg_warm<sizeof(KvAttnArgs)>();
-  __shared__ __attribute__((aligned(16))) StreamLds<D, 4> lds;
-  stream_share<D, kFmt, kBf16, 4>(a, blockIdx.x, lds);
+  __shared__ __attribute__((aligned(16))) StreamLds<D, NW> lds;
+  any_share<D, kFmt, kBf16, NW, true>(a, blockIdx.x, lds);
 }
 
 // ----------------------------------------------------------------- tiles --
@@ -1192,7 +1404,7 @@ __global__ void __launch_bounds__(NW* kWave, 2) k_attn_both(KvAttnArgs a, int bl
       __syncthreads();
     }
   } else {
-    stream_share<D, kFmt, kBf16, NW>(a, block - blocks_b, *reinterpret_cast<StreamLds<D, NW>*>(lds));
+    any_share<D, kFmt, kBf16, NW, false>(a, block - blocks_b, *reinterpret_cast<StreamLds<D, NW>*>(lds));
   }
 }
 
@@ -1307,7 +1519,7 @@ template <int D, int kFmt, bool kBf16>
 void attention_typed(const KvAttnArgs& a, hipStream_t s) {
   const int stream_blocks = (a.s.shares + 7) / 8 * 8 * a.c.heads;
   if (!a.s.list_b) {
-    k_attn_stream<D, kFmt, kBf16><<<dim3(stream_blocks), dim3(4 * kWave), 0, s>>>(a);
+    k_attn_stream<D, kFmt, kBf16><<<dim3(stream_blocks), dim3(kStreamWaves<kFmt> * kWave), 0, s>>>(a);
     return;
   }
   const bool lse = a.lse != nullptr;
