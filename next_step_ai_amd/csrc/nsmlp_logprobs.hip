@@ -50,6 +50,15 @@ __device__ __forceinline__ float value_at(const uint4& v, int i) {
   else if constexpr (T == Logit::kBf16) return __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
   else return h2f((uint16_t)(w[i >> 1] >> (16 * (i & 1))));
 }
+// the same for an index that is not known when compiled
+template <Logit T>
+__device__ __forceinline__ float value_of(const uint4& v, int i) {
+  const int word = T == Logit::kF32 ? i : i >> 1;
+  const uint32_t w = word & 2 ? (word & 1 ? v.w : v.z) : (word & 1 ? v.y : v.x);
+  if constexpr (T == Logit::kF32) return __uint_as_float(w);
+  else if constexpr (T == Logit::kBf16) return __uint_as_float(i & 1 ? w & 0xFFFF0000u : w << 16);
+  else return h2f((uint16_t)(w >> (16 * (i & 1))));
+}
 template <Logit T>
 __device__ __forceinline__ float load_one(const uint8_t* row, long long i) {
   if constexpr (T == Logit::kF32) return reinterpret_cast<const float*>(row)[i];
@@ -80,7 +89,7 @@ struct WaveTop {
   uint64_t* buf;   // [128]
   int n, count;    // (both the same in all lanes)
   uint64_t bound;  // entries at or below it are not among the n largest
-  float least;     // the bound's logit (-inf where every vector is to be looked at)
+  float least;     // what a logit of the next batch has to reach (-inf: any may count)
   int lane;
 
   __device__ __forceinline__ void start(uint64_t* b, int top, int l) {
@@ -88,18 +97,28 @@ struct WaveTop {
   }
 
   // The n largest, in order, and the bound that follows.  An entry's place is the
-  // number of larger ones; 0 stands for none.
+  // number of larger ones; 0 stands for none.  (Four entries are read at a time: one
+  // by one, each read was waited for.)
   __device__ __forceinline__ void settle() {
     wave_sync();
+    if (lane < 4 && count + lane < 2 * kWave) buf[count + lane] = 0;
+    wave_sync();
     const uint64_t a = lane < count ? buf[lane] : 0, b = lane + kWave < count ? buf[lane + kWave] : 0;
+    const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(buf);
     int above_a = 0, above_b = 0;
     if (count > kWave) {
-      for (int j = 0; j < count; ++j) {
-        const uint64_t v = buf[j];
-        above_a += v > a, above_b += v > b;
+#pragma unroll 2
+      for (int j = 0; j < count; j += 4) {
+        const ulonglong2 v = pairs[j >> 1], w = pairs[(j >> 1) + 1];
+        above_a += (v.x > a) + (v.y > a) + (w.x > a) + (w.y > a);
+        above_b += (v.x > b) + (v.y > b) + (w.x > b) + (w.y > b);
       }
     } else {
-      for (int j = 0; j < count; ++j) above_a += buf[j] > a;
+#pragma unroll 2
+      for (int j = 0; j < count; j += 4) {
+        const ulonglong2 v = pairs[j >> 1], w = pairs[(j >> 1) + 1];
+        above_a += (v.x > a) + (v.y > a) + (w.x > a) + (w.y > a);
+      }
     }
     wave_sync();
     if (a != 0 && above_a < n) buf[above_a] = a;
@@ -107,13 +126,25 @@ struct WaveTop {
     wave_sync();
     if (count >= n) {
       count = n;
-      raise(buf[n - 1]);
+      bound = buf[n - 1];
+      // a logit of a later batch stands behind its equals: the next larger one is the least that counts
+      const uint32_t order = (uint32_t)(bound >> 32);
+      least = least_of(order >= 0x007FFFFFu && order < 0xFF800000u ? order + 1 : order);
     }
   }
-  __device__ __forceinline__ void raise(uint64_t to) {
-    bound = to;
-    const uint32_t order = (uint32_t)(to >> 32);
-    least = order < 0x00800000u ? -INFINITY : logit_of(order);  // (-inf and NaN)
+  // the logit of a place in the order, -inf for those of -inf and NaN
+  static __device__ __forceinline__ float least_of(uint32_t order) { return order < 0x00800000u ? -INFINITY : logit_of(order); }
+  // A first bound from the lanes' largest logits: what at least n of them reach, to
+  // 16 bits of the order.
+  __device__ __forceinline__ void expect(float most) {
+    const uint32_t order = order_of(most);
+    uint32_t to = 0;
+#pragma unroll
+    for (int bit = 31; bit >= 16; --bit) {
+      const uint32_t more = to | 1u << bit;
+      to = __popcll(__ballot(order >= more)) >= n ? more : to;
+    }
+    least = least_of(to);
   }
   // Every lane may bring an entry.
   __device__ __forceinline__ void offer(bool mine, uint64_t entry) {
@@ -169,7 +200,7 @@ template <Logit T, bool kTop>
 __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(LogprobArgs a) {
   kernarg_warm<sizeof(LogprobArgs)>();
   constexpr int kPer = kPerVector<T>, kSize = T == Logit::kF32 ? 4 : 2;
-  __shared__ uint64_t bufs[kLpWaves][2 * kWave];
+  __shared__ __attribute__((aligned(16))) uint64_t bufs[kLpWaves][2 * kWave];
   __shared__ uint64_t merged[kLpMaxTop];
   __shared__ float sums[kLpWaves][3];
   __shared__ int last;
@@ -211,15 +242,12 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(LogprobArgs a) {
         raw[u] = uint4{w[0], w[1], w[2], w[3]};
       }
     }
-    float most[kLpBatch], all = s.m;
+    float all = value_at<T>(raw[0], 0);  // (NaN only where every one is)
 #pragma unroll
-    for (int u = 0; u < kLpBatch; ++u) {
-      most[u] = value_at<T>(raw[u], 0);
+    for (int u = 0; u < kLpBatch; ++u)
 #pragma unroll
-      for (int j = 1; j < kPer; ++j) most[u] = fmaxf(most[u], value_at<T>(raw[u], j));
-      all = fmaxf(all, most[u]);
-    }
-    rebase(s, all);
+      for (int j = 0; j < kPer; ++j) all = fmaxf(all, value_at<T>(raw[u], j));
+    rebase(s, fmaxf(s.m, all));
 #pragma unroll
     for (int u = 0; u < kLpBatch; ++u)
 #pragma unroll
@@ -229,36 +257,26 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(LogprobArgs a) {
         s.x = __builtin_fmaf(p, fmaxf(d, -200.0f), s.x);
       }
     if constexpr (kTop) {
-      const auto entry = [&](int u, int j, bool& there) {
-        const int step = at + u * kLpWaves;
-        const long long i = ((long long)step * kWave + lane) * kPer - lead + j;
-        there = step < end && i >= 0 && i < a.vocab;
-        return entry_of(value_at<T>(raw[u], j), (uint32_t)i);
-      };
-      if (at == first + wave) {
-        // the first bound: the n-th largest of the lanes' maxima
-        uint64_t mine = 0;
+      if (at == first + wave) top.expect(all);
+      if (__ballot(!(all < top.least)) != 0) {
+        // which of the lane's logits pass, and those one after the other
+        uint32_t pass = 0;
 #pragma unroll
         for (int u = 0; u < kLpBatch; ++u)
 #pragma unroll
-          for (int j = 0; j < kPer; ++j) {
-            bool there;
-            const uint64_t e = entry(u, j, there);
-            mine = there && e > mine ? e : mine;
-          }
-        top.offer(true, mine);
-        top.settle();
-        if (top.bound != 0) top.raise(top.bound - 1);  // itself among those that pass
-        top.count = 0;
-      }
+          for (int j = 0; j < kPer; ++j) pass |= !(value_at<T>(raw[u], j) < top.least) ? 1u << (u * kPer + j) : 0u;
+        while (__ballot(pass != 0) != 0) {
+          const int k = pass != 0 ? __builtin_ctz(pass) : 0, u = k / kPer, j = k % kPer;
+          uint4 v = raw[0];
 #pragma unroll
-      for (int u = 0; u < kLpBatch; ++u) {
-        if (__ballot(!(most[u] < top.least)) == 0) continue;
-#pragma unroll 1  // (seldom reached: short rather than fast)
-        for (int j = 0; j < kPer; ++j) {
-          bool there;
-          const uint64_t e = entry(u, j, there);
-          top.offer(there, e);
+          for (int w = 1; w < kLpBatch; ++w) {
+            v.x = u == w ? raw[w].x : v.x, v.y = u == w ? raw[w].y : v.y;
+            v.z = u == w ? raw[w].z : v.z, v.w = u == w ? raw[w].w : v.w;
+          }
+          const int step = at + u * kLpWaves;
+          const long long i = ((long long)step * kWave + lane) * kPer - lead + j;
+          top.offer(pass != 0 && step < end && i >= 0 && i < a.vocab, entry_of(value_of<T>(v, j), (uint32_t)i));
+          pass &= pass - 1;
         }
       }
     }
@@ -289,8 +307,10 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(LogprobArgs a) {
       const uint64_t mine = bufs[wave][lane];
       int above = lane;
 #pragma unroll
-      for (int w = 0; w < kLpWaves; ++w)
-        for (int j = 0; w != wave && j < a.top; ++j) above += bufs[w][j] > mine;
+      for (int w = 0; w < kLpWaves; ++w) {
+#pragma unroll 8
+        for (int j = 0; j < a.top; ++j) above += w != wave && bufs[w][j] > mine;
+      }
       if (mine != 0 && above < a.top) merged[above] = mine;
     }
     // (a workgroup with fewer logits than n: none of them has the places behind)
