@@ -66,6 +66,43 @@ __device__ __forceinline__ float load_one(const uint8_t* row, long long i) {
   else return h2f(reinterpret_cast<const uint16_t*>(row)[i]);
 }
 
+// 16 bytes of a row from logit i on, at any address.
+__device__ __forceinline__ uint4 vector_at(const uint8_t* p) {
+  uint4 v;
+  __builtin_memcpy(&v, p, 16);
+  return v;
+}
+// A row of fewer logits than a vector has places: in its last ones.
+template <Logit T>
+__device__ __forceinline__ uint4 short_row(const uint8_t* row, int vocab) {
+  constexpr int kPer = kPerVector<T>;
+  uint32_t w[4] = {};
+#pragma unroll
+  for (int j = 1; j < kPer; ++j) {
+    const int i = j - (kPer - vocab);
+    if (i < 0) continue;
+    if constexpr (T == Logit::kF32) w[j] = reinterpret_cast<const uint32_t*>(row)[i];
+    else w[j >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(row)[i] << (16 * (j & 1));
+  }
+  return uint4{w[0], w[1], w[2], w[3]};
+}
+// -inf in a vector's first `lost` places
+template <Logit T>
+__device__ __forceinline__ uint4 without(const uint4& v, int lost) {
+  constexpr uint32_t kNone = T == Logit::kF32 ? 0xFF800000u : T == Logit::kBf16 ? 0xFF80FF80u : 0xFC00FC00u;
+  uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (T == Logit::kF32) {
+      w[j] = j < lost ? kNone : w[j];
+    } else {
+      const uint32_t gone = 2 * j + 1 < lost ? ~0u : 2 * j < lost ? 0xFFFFu : 0u;
+      w[j] = (w[j] & ~gone) | (kNone & gone);
+    }
+  }
+  return uint4{w[0], w[1], w[2], w[3]};
+}
+
 // A logit's place in the order: larger for a larger one, -0 as +0, 0 for NaN.
 __device__ __forceinline__ uint32_t order_of(float z) {
   const uint32_t b = __float_as_uint(z + 0.0f);
@@ -84,6 +121,40 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_wave_barrier();
 }
 
+// Largest of, and sum over, a wave's lanes: within rows of 16 through DPP, the four
+// rows' through scalar registers (exchanges through LDS took most of the joins).
+template <int kCtrl>
+__device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), kCtrl, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float row_of(float v, int row) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 16 * row)); }
+__device__ __forceinline__ float wave_most(float v) {
+  v = fmaxf(v, dpp<0x128>(v)), v = fmaxf(v, dpp<0x124>(v)), v = fmaxf(v, dpp<0x122>(v)), v = fmaxf(v, dpp<0x121>(v));  // row_ror
+  return fmaxf(fmaxf(row_of(v, 0), row_of(v, 1)), fmaxf(row_of(v, 2), row_of(v, 3)));
+}
+__device__ __forceinline__ float wave_total(float v) {
+  v += dpp<0x128>(v), v += dpp<0x124>(v), v += dpp<0x122>(v), v += dpp<0x121>(v);
+  return (row_of(v, 0) + row_of(v, 1)) + (row_of(v, 2) + row_of(v, 3));
+}
+
+// How many of the entries in LDS (a multiple of 8, 16-byte aligned, 0 for none) are
+// larger than `a`, and than `b`.
+template <bool kBoth>
+__device__ __forceinline__ void count_above(const uint64_t* list, int count, uint64_t a, uint64_t b, int& above_a, int& above_b) {
+  const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(list);
+#pragma unroll 1
+  for (int j = 0; j < count; j += 8) {  // (eight are read at a time: one by one, each read was waited for)
+    ulonglong2 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = pairs[(j >> 1) + i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      above_a += (v[i].x > a) + (v[i].y > a);
+      if (kBoth) above_b += (v[i].x > b) + (v[i].y > b);
+    }
+  }
+}
+
 // Candidates of a wave: up to 128 entries in LDS, of which the n largest count.
 struct WaveTop {
   uint64_t* buf;   // [128]
@@ -97,32 +168,18 @@ struct WaveTop {
   }
 
   // The n largest, in order, and the bound that follows.  An entry's place is the
-  // number of larger ones; 0 stands for none.  (Four entries are read at a time: one
-  // by one, each read was waited for.)
+  // number of larger ones; 0 stands for none.
   __device__ __forceinline__ void settle() {
     wave_sync();
-    if (lane < 4 && count + lane < 2 * kWave) buf[count + lane] = 0;
+    if (lane < 8 && count + lane < 2 * kWave) buf[count + lane] = 0;
     wave_sync();
-    const uint64_t a = lane < count ? buf[lane] : 0, b = lane + kWave < count ? buf[lane + kWave] : 0;
-    const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(buf);
+    const uint64_t a = buf[lane], b = count > kWave ? buf[lane + kWave] : 0;
     int above_a = 0, above_b = 0;
-    if (count > kWave) {
-#pragma unroll 2
-      for (int j = 0; j < count; j += 4) {
-        const ulonglong2 v = pairs[j >> 1], w = pairs[(j >> 1) + 1];
-        above_a += (v.x > a) + (v.y > a) + (w.x > a) + (w.y > a);
-        above_b += (v.x > b) + (v.y > b) + (w.x > b) + (w.y > b);
-      }
-    } else {
-#pragma unroll 2
-      for (int j = 0; j < count; j += 4) {
-        const ulonglong2 v = pairs[j >> 1], w = pairs[(j >> 1) + 1];
-        above_a += (v.x > a) + (v.y > a) + (w.x > a) + (w.y > a);
-      }
-    }
+    if (count > kWave) count_above<true>(buf, count, a, b, above_a, above_b);
+    else count_above<false>(buf, count, a, b, above_a, above_b);
     wave_sync();
-    if (a != 0 && above_a < n) buf[above_a] = a;
-    if (b != 0 && above_b < n) buf[above_b] = b;
+    if (lane < count && above_a < n) buf[above_a] = a;
+    if (lane + kWave < count && above_b < n) buf[above_b] = b;
     wave_sync();
     if (count >= n) {
       count = n;
@@ -134,24 +191,29 @@ struct WaveTop {
   }
   // the logit of a place in the order, -inf for those of -inf and NaN
   static __device__ __forceinline__ float least_of(uint32_t order) { return order < 0x00800000u ? -INFINITY : logit_of(order); }
-  // A first bound from the lanes' largest logits: what at least n of them reach, to
-  // 16 bits of the order.
+  // A first bound from the lanes' largest logits: what at least n of them reach.
   __device__ __forceinline__ void expect(float most) {
+    uint32_t* orders = reinterpret_cast<uint32_t*>(buf);
     const uint32_t order = order_of(most);
-    uint32_t to = 0;
-#pragma unroll
-    for (int bit = 31; bit >= 16; --bit) {
-      const uint32_t more = to | 1u << bit;
-      to = __popcll(__ballot(order >= more)) >= n ? more : to;
+    orders[lane] = order;
+    wave_sync();
+    const uint4* fours = reinterpret_cast<const uint4*>(orders);
+    int above = 0;
+#pragma unroll 4
+    for (int j = 0; j < kWave / 4; ++j) {
+      const uint4 v = fours[j];
+      above += (v.x > order) + (v.y > order) + (v.z > order) + (v.w > order);
     }
-    least = least_of(to);
+    wave_sync();
+    // (the least of those with fewer than n above them)
+    least = -wave_most(above < n ? -least_of(order) : kLowest);
   }
   // Every lane may bring an entry.
   __device__ __forceinline__ void offer(bool mine, uint64_t entry) {
     const bool in = mine && entry > bound;
     const unsigned long long who = __ballot(in);
     if (who == 0) return;
-    if (in) buf[count + __popcll(who & ((1ull << lane) - 1))] = entry;
+    if (in) buf[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] = entry;
     count += __popcll(who);
     if (count > kWave) settle();
   }
@@ -168,8 +230,8 @@ __device__ __forceinline__ void rebase(Sums& s, float m) {
   s.m = m;
 }
 __device__ __forceinline__ Sums join_wave(Sums s) {
-  rebase(s, wave_max(s.m));
-  s.l = wave_sum(s.l), s.x = wave_sum(s.x);
+  rebase(s, wave_most(s.m));
+  s.l = wave_total(s.l), s.x = wave_total(s.x);
   return s;
 }
 
@@ -207,11 +269,7 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(LogprobArgs a) {
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row = (int)(blockIdx.x / (unsigned)a.splits), split = (int)(blockIdx.x % (unsigned)a.splits);
   const uint8_t* logits = a.logits + (long long)row * a.row_bytes;
-  // Vectors start at multiples of 16 bytes, the first one up to 15 bytes before
-  // the row: its elements that are not the row's are not loaded, nor the last one's.
-  const int lead = (int)((uintptr_t)logits & 15) / kSize;
-  const long long vectors = ((long long)lead + a.vocab + kPer - 1) / kPer;
-  const int steps = (int)((vectors + kWave - 1) / kWave);  // of a wave: 64 vectors
+  const int steps = (a.vocab + kPer * kWave - 1) / (kPer * kWave);  // of a wave: 64 vectors
   const int first = (int)((long long)steps * split / a.splits), end = (int)((long long)steps * (split + 1) / a.splits);
 
   WaveTop top;
@@ -219,27 +277,26 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(LogprobArgs a) {
   Sums s = {kLowest, 0.0f, 0.0f};
   for (int at = first + wave; at < end; at += kLpWaves * kLpBatch) {
     uint4 raw[kLpBatch];
+    if (a.vocab >= kPer) {
 #pragma unroll
-    for (int u = 0; u < kLpBatch; ++u) {
-      const int step = at + u * kLpWaves;
-      const long long v = (long long)step * kWave + lane, i0 = v * kPer - lead;
-      if (step < end && i0 >= 0 && i0 + kPer <= a.vocab) {
-        raw[u] = *reinterpret_cast<const uint4*>(logits + i0 * kSize);
-      } else {
-        // -inf where there is no logit
-        uint32_t w[4];
+      for (int u = 0; u < kLpBatch; ++u) {
+        // one that would end past the row ends with it
+        const long long i0 = ((long long)(at + u * kLpWaves) * kWave + lane) * kPer;
+        raw[u] = vector_at(logits + min(i0, (long long)a.vocab - kPer) * kSize);
+      }
+    } else {
+      raw[0] = short_row<T>(logits, a.vocab);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = T == Logit::kF32 ? 0xFF800000u : T == Logit::kBf16 ? 0xFF80FF80u : 0xFC00FC00u;
-        if (step < end) {
+      for (int u = 1; u < kLpBatch; ++u) raw[u] = raw[0];
+    }
+    if (at + (kLpBatch - 1) * kLpWaves >= min(steps - 1, end)) {
+      // -inf where there is no logit, or one that an earlier vector has
 #pragma unroll
-          for (int j = 0; j < kPer; ++j) {
-            if (i0 + j < 0 || i0 + j >= a.vocab) continue;
-            if constexpr (kSize == 4) w[j] = reinterpret_cast<const uint32_t*>(logits)[i0 + j];
-            else w[j >> 1] = (w[j >> 1] & (j & 1 ? 0xFFFFu : 0xFFFF0000u)) |
-                             (uint32_t)reinterpret_cast<const uint16_t*>(logits)[i0 + j] << (16 * (j & 1));
-          }
-        }
-        raw[u] = uint4{w[0], w[1], w[2], w[3]};
+      for (int u = 0; u < kLpBatch; ++u) {
+        const int step = at + u * kLpWaves;
+        const long long i0 = ((long long)step * kWave + lane) * kPer;
+        const int lost = step < end ? (int)min(max(i0 + kPer - a.vocab, 0LL), (long long)kPer) : kPer;
+        raw[u] = without<T>(raw[u], lost);
       }
     }
     float all = value_at<T>(raw[0], 0);  // (NaN only where every one is)
@@ -273,9 +330,8 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(LogprobArgs a) {
             v.x = u == w ? raw[w].x : v.x, v.y = u == w ? raw[w].y : v.y;
             v.z = u == w ? raw[w].z : v.z, v.w = u == w ? raw[w].w : v.w;
           }
-          const int step = at + u * kLpWaves;
-          const long long i = ((long long)step * kWave + lane) * kPer - lead + j;
-          top.offer(pass != 0 && step < end && i >= 0 && i < a.vocab, entry_of(value_of<T>(v, j), (uint32_t)i));
+          const int step = at + u * kLpWaves, i0 = (step * kWave + lane) * kPer, i = min(i0, a.vocab - kPer) + j;
+          top.offer(pass != 0 && step < end && i >= i0 && i >= 0, entry_of(value_of<T>(v, j), (uint32_t)i));
           pass &= pass - 1;
         }
       }
@@ -283,7 +339,7 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(LogprobArgs a) {
   }
   if constexpr (kTop) {
     top.settle();
-    for (int i = top.count + lane; i < a.top; i += kWave) bufs[wave][i] = 0;  // a wave with fewer logits
+    if (lane >= top.count && lane < a.top) bufs[wave][lane] = 0;  // a wave with fewer logits
   }
   s = join_wave(s);
   if (lane == 0) sums[wave][0] = s.m, sums[wave][1] = s.l, sums[wave][2] = s.x;
@@ -303,19 +359,19 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(LogprobArgs a) {
   }
   if constexpr (kTop) {
     // the waves' lists: an entry's place is the number of larger ones in all of them
-    if (lane < a.top) {
-      const uint64_t mine = bufs[wave][lane];
-      int above = lane;
+    const uint64_t mine = lane < a.top ? bufs[wave][lane] : 0;
+    int above = 0, at[kLpWaves] = {};
 #pragma unroll
-      for (int w = 0; w < kLpWaves; ++w) {
-#pragma unroll 8
-        for (int j = 0; j < a.top; ++j) above += w != wave && bufs[w][j] > mine;
-      }
-      if (mine != 0 && above < a.top) merged[above] = mine;
-    }
+    for (int step = kWave; step >= 1; step >>= 1)  // (by halves: the lists are in order)
+#pragma unroll
+      for (int w = 0; w < kLpWaves; ++w)
+        if (at[w] + step <= a.top && bufs[w][at[w] + step - 1] > mine) at[w] += step;
+#pragma unroll
+    for (int w = 0; w < kLpWaves; ++w) above += at[w];
+    if (mine != 0 && above < a.top) merged[above] = mine;
     // (a workgroup with fewer logits than n: none of them has the places behind)
     if (tid < a.top) {
-      const long long here = min((long long)end * kWave * kPer - lead, (long long)a.vocab) - max((long long)first * kWave * kPer - lead, 0LL);
+      const long long here = min((long long)end * kWave * kPer, (long long)a.vocab) - (long long)first * kWave * kPer;
       if (tid >= here) merged[tid] = 0;
     }
     __syncthreads();
@@ -346,14 +402,24 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(LogprobArgs a) {
   }
   p = join_wave(p);
   if constexpr (kTop) {
-    // a lane per workgroup: the lists' first entries, their second ones, and so on,
-    // until none is among the largest
+    // the lists' first entries, their second ones, and so on, 64 at a time: after the
+    // first 64 there is a bound that few of the others pass
     top.start(bufs[0], a.top, lane);
-    const uint64_t* from = a.part_top + (row_at + min(lane, a.splits - 1)) * a.top;
-    for (int i = 0; i < a.top; ++i) {
-      const uint64_t e = __hip_atomic_load(const_cast<uint64_t*>(from + i), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      if (__ballot(lane < a.splits && e > top.bound) == 0) break;
-      top.offer(lane < a.splits && e != 0, e);
+    const uint64_t* from = a.part_top + row_at * a.top;
+    const int all = a.splits * a.top;
+    for (int base = 0; base < all; base += 4 * kWave) {
+      uint64_t e[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int k = base + u * kWave + lane, i = k / a.splits, w = k % a.splits;
+        e[u] = k < all ? __hip_atomic_load(const_cast<uint64_t*>(from + w * a.top + i), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+      }
+#pragma unroll 1
+      for (int u = 0; u < 4; ++u) {
+        const uint64_t mine = u < 2 ? (u == 0 ? e[0] : e[1]) : (u == 2 ? e[2] : e[3]);
+        top.offer(mine != 0, mine);
+        if (base + u == 0) top.settle();
+      }
     }
     top.settle();
     wave_sync();
@@ -361,10 +427,11 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(LogprobArgs a) {
   write_row<T>(a, row, logits, p, bufs[0], lane);
 }
 
+constexpr int kLpTarget = 1024;
 // Workgroups of a row: about a thousand in all, none with less than a batch of vectors per wave.
 int splits_of(int rows, int vocab, int size) {
   const long long steps = ((long long)vocab * size + 16 * kWave - 1) / (16 * kWave);
-  const long long most = (steps + kLpWaves * kLpBatch - 1) / (kLpWaves * kLpBatch), want = (1024 + rows - 1) / rows;
+  const long long most = (steps + kLpWaves * kLpBatch - 1) / (kLpWaves * kLpBatch), want = (kLpTarget + rows - 1) / rows;
   const long long s = most < want ? most : want;
   return (int)(s < 1 ? 1 : s > kLpMaxSplits ? kLpMaxSplits : s);
 }

@@ -33,6 +33,8 @@ __all__ = ["resolve_lm_head_block_size", "lm_head_nf4_meta", "dense_linear_nf4",
 
 _LOGIT_DTYPES = {torch.float16: _lib.NSMLP_DTYPE_F16, torch.bfloat16: _lib.NSMLP_DTYPE_BF16, torch.float32: _lib.NSMLP_DTYPE_F32}
 
+_logprob_bytes: dict[tuple[int, int, int, int], int] = {}  # workspace sizes
+
 
 def resolve_lm_head_block_size(in_features: int) -> int:
     """The column block the reference lists in ``active_idx``: the largest of
@@ -185,30 +187,36 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
         raise RuntimeError(f"logits must be fp16, bf16 or fp32, got {logits.dtype}")
     if logits.dim() < 1:
         raise RuntimeError("logits must have a last dimension, the vocabulary")
-    shape, V = logits.shape[:-1], int(logits.shape[-1])
+    shape, V = logits.shape[:-1], logits.shape[-1]
     z = logits if logits.dim() == 2 else logits.reshape(-1 if V else 0, V)
-    rows = int(z.shape[0])
+    rows = z.shape[0]
     if V > 1 and z.stride(1) != 1:
         z = z.contiguous()
     if tokens is not None and (tokens.dtype != torch.int64 or tokens.device != device or tokens.shape != shape):
         raise RuntimeError(f"tokens must be an int64 {tuple(shape)} tensor on {device}, got {tuple(tokens.shape)} {tokens.dtype} on "
                            f"{tokens.device}")
-    top = int(top)
-    need = int(_lib.lib().nsmlp_token_logprobs_workspace_bytes(rows, V, dtype, max(top, 0)))
-    t = None if tokens is None else tokens.reshape(-1).contiguous()
-    f32 = torch.empty((1 if t is None else 2) * rows + rows * max(top, 0), dtype=torch.float32, device=device)
-    ids = torch.empty(rows * max(top, 0), dtype=torch.int64, device=device)
-    entropy, at = f32[:rows], f32.data_ptr()
-    logprob = None if t is None else f32[rows: 2 * rows]
-    first = rows if t is None else 2 * rows
-    if need and ws is None:
-        ws = workspace(need, device)
-    elif ws is not None and (ws.device != device or not ws.is_contiguous()):
+    key = (rows, V, dtype, int(top))
+    need = _logprob_bytes.get(key)
+    if need is None:
+        if len(_logprob_bytes) >= 1024:
+            _logprob_bytes.clear()
+        need = _logprob_bytes[key] = int(_lib.lib().nsmlp_token_logprobs_workspace_bytes(*key))
+    n = max(key[3], 0)
+    # one buffer for what is fp32: a split into views takes as long as one tensor made anew
+    sizes = [rows, 0 if tokens is None else rows, rows * n]
+    parts = torch.empty(sum(sizes), dtype=torch.float32, device=device).split_with_sizes(sizes)
+    ids = torch.empty((*shape, n), dtype=torch.int64, device=device)
+    if ws is None:
+        ws = workspace(need, device) if need else None
+    elif ws.device != device or not ws.is_contiguous():
         raise RuntimeError(f"ws must be a contiguous tensor on {device}, got one on {ws.device} with strides {ws.stride()}")
-    _lib.call("nsmlp_token_logprobs", z.data_ptr(), z.stride(0) if rows > 1 else V, dtype, rows, V, ptr(t), top,
-              None if t is None else at + 4 * rows, at, ids.data_ptr(), at + 4 * first, None if ws is None else ws.data_ptr(),
-              0 if ws is None else ws.numel() * ws.element_size(), stream_handle(device))
-    out = {} if t is None else {"logprob": logprob.view(shape)}
-    out["entropy"] = entropy.view(shape)
-    out["top_ids"], out["top_logprobs"] = ids.view(*shape, top), f32[first:].view(*shape, top)
+    t = None if tokens is None else tokens.contiguous()
+    at = parts[0].data_ptr()
+    _lib.call("nsmlp_token_logprobs", z.data_ptr(), z.stride(0) if rows > 1 else V, dtype, rows, V, ptr(t), key[3],
+              None if t is None else at + 4 * rows, at, ids.data_ptr(), at + 4 * (sizes[0] + sizes[1]),
+              None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel() * ws.element_size(), stream_handle(device))
+    flat = len(shape) == 1
+    out = {} if t is None else {"logprob": parts[1] if flat else parts[1].view(shape)}
+    out["entropy"] = parts[0] if flat else parts[0].view(shape)
+    out["top_ids"], out["top_logprobs"] = ids, parts[2].view(ids.shape)
     return out
