@@ -14,6 +14,8 @@
 // its n-th largest so far in LDS and drops all but n where they pass 64; the first
 // bound is the n-th largest of the lanes' own maxima of the first batch.  So nearly
 // all vectors cost one comparison.  A NaN counts as below every number.
+#include <algorithm>
+
 #include "nsmlp_internal.h"
 
 namespace nsmlp {
@@ -30,6 +32,8 @@ struct LogprobArgs {
   const uint8_t* logits;
   long long row_bytes;
   int rows, vocab, top, splits;
+  int each;                // wave steps of a workgroup
+  uint32_t per_split;      // ceil(2^20 / splits): k / splits of k < 2^11 + 2^8 as a product
   const int64_t* tokens;   // [rows] or NULL
   float *logprob, *entropy;  // [rows], nullable
   int64_t* top_ids;        // [rows][top]
@@ -54,7 +58,8 @@ __device__ __forceinline__ float value_at(const uint4& v, int i) {
 template <Logit T>
 __device__ __forceinline__ float value_of(const uint4& v, int i) {
   const int word = T == Logit::kF32 ? i : i >> 1;
-  const uint32_t w = word & 2 ? (word & 1 ? v.w : v.z) : (word & 1 ? v.y : v.x);
+  const uint64_t low = (uint64_t)v.y << 32 | v.x, high = (uint64_t)v.w << 32 | v.z;
+  const uint32_t w = (uint32_t)((word & 2 ? high : low) >> (32 * (word & 1)));
   if constexpr (T == Logit::kF32) return __uint_as_float(w);
   else if constexpr (T == Logit::kBf16) return __uint_as_float(i & 1 ? w & 0xFFFF0000u : w << 16);
   else return h2f((uint16_t)(w >> (16 * (i & 1))));
@@ -258,7 +263,7 @@ __device__ __forceinline__ void write_row(const LogprobArgs& a, int row, const u
   }
 }
 
-template <Logit T, bool kTop>
+template <Logit T, bool kTop, bool kShort>
 __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(LogprobArgs a) {
   kernarg_warm<sizeof(LogprobArgs)>();
   constexpr int kPer = kPerVector<T>, kSize = T == Logit::kF32 ? 4 : 2;
@@ -267,17 +272,17 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(LogprobArgs a) {
   __shared__ float sums[kLpWaves][3];
   __shared__ int last;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int row = (int)(blockIdx.x / (unsigned)a.splits), split = (int)(blockIdx.x % (unsigned)a.splits);
+  const int row = blockIdx.x, split = blockIdx.y;
   const uint8_t* logits = a.logits + (long long)row * a.row_bytes;
   const int steps = (a.vocab + kPer * kWave - 1) / (kPer * kWave);  // of a wave: 64 vectors
-  const int first = (int)((long long)steps * split / a.splits), end = (int)((long long)steps * (split + 1) / a.splits);
+  const int first = split * a.each, end = min(first + a.each, steps);
 
   WaveTop top;
   if constexpr (kTop) top.start(bufs[wave], a.top, lane);
   Sums s = {kLowest, 0.0f, 0.0f};
   for (int at = first + wave; at < end; at += kLpWaves * kLpBatch) {
     uint4 raw[kLpBatch];
-    if (a.vocab >= kPer) {
+    if constexpr (!kShort) {
 #pragma unroll
       for (int u = 0; u < kLpBatch; ++u) {
         // one that would end past the row ends with it
@@ -411,7 +416,7 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(LogprobArgs a) {
       uint64_t e[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const int k = base + u * kWave + lane, i = k / a.splits, w = k % a.splits;
+        const int k = base + u * kWave + lane, i = (int)((uint32_t)k * a.per_split >> 20), w = k - i * a.splits;
         e[u] = k < all ? __hip_atomic_load(const_cast<uint64_t*>(from + w * a.top + i), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
       }
 #pragma unroll 1
@@ -429,11 +434,14 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(LogprobArgs a) {
 
 constexpr int kLpTarget = 1024;
 // Workgroups of a row: about a thousand in all, none with less than a batch of vectors per wave.
-int splits_of(int rows, int vocab, int size) {
-  const long long steps = ((long long)vocab * size + 16 * kWave - 1) / (16 * kWave);
-  const long long most = (steps + kLpWaves * kLpBatch - 1) / (kLpWaves * kLpBatch), want = (kLpTarget + rows - 1) / rows;
-  const long long s = most < want ? most : want;
-  return (int)(s < 1 ? 1 : s > kLpMaxSplits ? kLpMaxSplits : s);
+struct Splits {
+  int count, each;
+};
+Splits splits_of(int rows, int vocab, int size) {
+  const int steps = (int)(((long long)vocab * size + 16 * kWave - 1) / (16 * kWave)), least = kLpWaves * kLpBatch;
+  const int most = std::max(1, std::min({(steps + least - 1) / least, (kLpTarget + rows - 1) / rows, kLpMaxSplits}));
+  const int each = (steps + most - 1) / most;
+  return Splits{(steps + each - 1) / each, each};
 }
 constexpr int kLpMaxRows = 1 << 24;
 
@@ -447,15 +455,19 @@ int check_shape(int rows, int vocab, int dtype, int top) {
   return NSMLP_OK;
 }
 size_t workspace_of(int rows, int vocab, int dtype, int top) {
-  const int splits = rows == 0 ? 1 : splits_of(rows, vocab, dtype == NSMLP_DTYPE_F32 ? 4 : 2);
+  const int splits = rows == 0 ? 1 : splits_of(rows, vocab, dtype == NSMLP_DTYPE_F32 ? 4 : 2).count;
   return splits == 1 ? 0 : align_up(kCounterBytes) + (size_t)rows * splits * (16 + 8 * (size_t)top);
 }
 
+template <Logit T, bool kTop>
+void launch(const LogprobArgs& a, hipStream_t s) {
+  const dim3 grid(a.rows, a.splits), block(kLpThreads);
+  if (a.vocab >= kPerVector<T>) k_token_logprobs<T, kTop, false><<<grid, block, 0, s>>>(a);
+  else k_token_logprobs<T, kTop, true><<<grid, block, 0, s>>>(a);
+}
 template <Logit T>
 void launch(const LogprobArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)a.rows * (unsigned)a.splits), block(kLpThreads);
-  if (a.top > 0) k_token_logprobs<T, true><<<grid, block, 0, s>>>(a);
-  else k_token_logprobs<T, false><<<grid, block, 0, s>>>(a);
+  a.top > 0 ? launch<T, true>(a, s) : launch<T, false>(a, s);
 }
 
 }  // namespace
@@ -492,7 +504,8 @@ int nsmlp_token_logprobs(const void* logits, long long row_stride, int dtype, in
   a.logits = (const uint8_t*)logits;
   a.row_bytes = row_stride * size;
   a.rows = rows, a.vocab = vocab, a.top = top;
-  a.splits = splits_of(rows, vocab, size);
+  const Splits s = splits_of(rows, vocab, size);
+  a.splits = s.count, a.each = s.each, a.per_split = ((1u << 20) + s.count - 1) / s.count;
   a.tokens = tokens;
   a.logprob = logprob, a.entropy = entropy;
   a.top_ids = top_ids, a.top_logprobs = top_logprobs;
