@@ -467,6 +467,7 @@ __device__ __forceinline__ void append_run(const KvAppendArgs& a, int t, long lo
     const int tl = lane / kChunks, c = lane % kChunks;
     const uint16_t* x = a.k + (long long)t * a.k_row + (long long)h * a.k_head + c * 16;
     uint4 u[kPass][2];
+    [[maybe_unused]] int pos[kPass];
     uint32_t top = 0;
 #pragma unroll
     for (int p = 0; p < kPass; ++p) {
@@ -476,8 +477,13 @@ __device__ __forceinline__ void append_run(const KvAppendArgs& a, int t, long lo
         const uint4* q = reinterpret_cast<const uint4*>(x + i * a.k_row);
         u[p][0] = q[0], u[p][1] = q[1];
       }
-      if constexpr (kRotate) {
-        // a row's other half is kChunks / 2 lanes away (of tokens past the run, zeros)
+      if (kRotate && i < n) pos[p] = a.rot.positions[t + i];
+    }
+    if constexpr (kRotate) {
+      // a row's other half is kChunks / 2 lanes away (of tokens past the run, zeros)
+#pragma unroll
+      for (int p = 0; p < kPass; ++p) {
+        const int i = p * kTok + tl;
         uint32_t w[8], other[8];
 #pragma unroll
         for (int j = 0; j < 2; ++j)
@@ -485,7 +491,7 @@ __device__ __forceinline__ void append_run(const KvAppendArgs& a, int t, long lo
 #pragma unroll
         for (int j = 0; j < 8; ++j) other[j] = (uint32_t)__shfl_xor((int)w[j], kChunks / 2, kWave);
         if (i < n) {
-          rotate<16, kBf16>(w, other, angles_of<D, 16>(a.rot, a.rot.positions[t + i], c * 16), a.rot.interleaved);
+          rotate<16, kBf16>(w, other, angles_of<D, 16>(a.rot, pos[p], c * 16), a.rot.interleaved);
           u[p][0] = uint4{w[0], w[1], w[2], w[3]}, u[p][1] = uint4{w[4], w[5], w[6], w[7]};
         }
       }
@@ -565,8 +571,12 @@ __device__ __forceinline__ void append_run(const KvAppendArgs& a, int t, long lo
   }
 }
 
+// waves a SIMD, as the rows of a run stay in registers (and the angles of some)
+template <int D, int B, bool kRotate>
+constexpr int kAppendWaves = kRotate ? (B * D > 4096 ? 2 : B * D > 2048 ? 3 : 4) : B == 64 ? 2 : 4;
+
 template <int D, int B, int kFmt, bool kBf16, bool kRotate>
-__global__ void __launch_bounds__(kAppendThreads, B == 64 ? 2 : 4) k_kv_append(KvAppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, (kAppendWaves<D, B, kRotate>)) k_kv_append(KvAppendArgs a) {
   kernarg_warm<sizeof(KvAppendArgs)>();
   const int lane = threadIdx.x & (kWave - 1);
   if (kRotate && blockIdx.x >= a.rot.first) {
