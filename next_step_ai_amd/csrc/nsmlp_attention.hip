@@ -228,16 +228,11 @@ __device__ __forceinline__ KvUnit load_unit(const KvUnit* p) {
 // (269 MB, 31 partial results per row to join) 57.5 us, 4.7 TB/s.  A short chat (777
 // keys) takes 9.5 us, most of it the chain launch, schedule, lengths, block
 // table, scales, codes, join.
-struct StreamUnit {  // (4 bits) a unit and its request's rows and keys
-  int req, kv_begin, kv_end, part, first, parts, q0, q_len, kv_len;
-};
-
 template <int D, int NW>
 struct StreamLds {
   float sum[NW][16][D + 4];  // the waves' results
   float ml[NW][2][16];
   int last;
-  StreamUnit unit[kWave];
 };
 
 template <int D>
@@ -609,6 +604,14 @@ __device__ __forceinline__ void stream_share(const KvAttnArgs& a, int block, Str
 // go from one unit to the next without a pause: what a share's units are is
 // read once, for all of them at a time, and while a unit's last tiles are in use
 // the next one's first are fetched, its pages and queries before.
+struct StreamUnit {  // a unit and its request's rows and keys
+  int req, kv_begin, kv_end, part, first, parts, q0, q_len, kv_len;
+};
+template <int D, int NW>
+struct StreamLds4 : StreamLds<D, NW> {
+  StreamUnit unit[kWave];
+};
+
 template <int D>
 struct StreamTile4 {
   Codes4<D> k[2], v[2];
@@ -617,7 +620,7 @@ struct StreamTile4 {
 };
 
 template <int D, bool kBf16, int NW, bool kAhead>
-__device__ __forceinline__ void stream_share4(const KvAttnArgs& a, int block, StreamLds<D, NW>& lds) {
+__device__ __forceinline__ void stream_share4(const KvAttnArgs& a, int block, StreamLds4<D, NW>& lds) {
   constexpr int KS = D / 32, ND = D / 16, kFmt = NSMLP_KV_E2M1;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
@@ -863,8 +866,11 @@ __device__ __forceinline__ void stream_share4(const KvAttnArgs& a, int block, St
   if (bad_seen != 0 && lane == 0) atomicOr(a.status, NSMLP_STATUS_BLOCK_UNAVAILABLE);
 }
 
+template <int D, int kFmt, int NW>
+using StreamLdsOf = std::conditional_t<kFmt == NSMLP_KV_E2M1, StreamLds4<D, NW>, StreamLds<D, NW>>;
+
 template <int D, int kFmt, bool kBf16, int NW, bool kAhead>
-__device__ __forceinline__ void any_share(const KvAttnArgs& a, int block, StreamLds<D, NW>& lds) {
+__device__ __forceinline__ void any_share(const KvAttnArgs& a, int block, StreamLdsOf<D, kFmt, NW>& lds) {
   if constexpr (kFmt == NSMLP_KV_E2M1) stream_share4<D, kBf16, NW, kAhead>(a, block, lds);
   else stream_share<D, kFmt, kBf16, NW>(a, block, lds);
 }
@@ -876,7 +882,7 @@ template <int D, int kFmt, bool kBf16>
 __global__ void __launch_bounds__(kStreamWaves<kFmt>* kWave) k_attn_stream(KvAttnArgs a) {
   constexpr int NW = kStreamWaves<kFmt>;
   kernarg_warm<sizeof(KvAttnArgs)>();
-  __shared__ __attribute__((aligned(16))) StreamLds<D, NW> lds;
+  __shared__ __attribute__((aligned(16))) StreamLdsOf<D, kFmt, NW> lds;
   any_share<D, kFmt, kBf16, NW, true>(a, blockIdx.x, lds);
 }
 
@@ -1404,7 +1410,7 @@ __global__ void __launch_bounds__(NW* kWave, 2) k_attn_both(KvAttnArgs a, int bl
       __syncthreads();
     }
   } else {
-    any_share<D, kFmt, kBf16, NW, false>(a, block - blocks_b, *reinterpret_cast<StreamLds<D, NW>*>(lds));
+    any_share<D, kFmt, kBf16, NW, false>(a, block - blocks_b, *reinterpret_cast<StreamLdsOf<D, kFmt, NW>*>(lds));
   }
 }
 
@@ -1505,7 +1511,7 @@ __global__ void __launch_bounds__(256) k_attn_join(KvAttnArgs a) {
 
 template <int D, int kFmt, bool kBf16, int NW, bool kLse>
 void launch_both(const KvAttnArgs& a, int stream_blocks, hipStream_t s) {
-  constexpr int kStream = (int)sizeof(StreamLds<D, NW>), kLds = kStream > kTileLds<D> ? kStream : kTileLds<D>;
+  constexpr int kStream = (int)sizeof(StreamLdsOf<D, kFmt, NW>), kLds = kStream > kTileLds<D> ? kStream : kTileLds<D>;
   static std::once_flag once;
   std::call_once(once, [] {
     (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k_attn_both<D, kFmt, kBf16, NW, kLse>),

@@ -24,7 +24,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._runtime import ptr, require_device, stream_handle, workspace
+from ._runtime import current_device, ptr, require_device, stream_handle, workspace
 from .rotary import Rotary
 
 __all__ = ["KvCache", "KvBatch", "KvStep", "paged_attention"]
@@ -73,6 +73,14 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a0 < b1 and b0 < a1
 
 
+def _meets_itself(n: int, row: int, heads: int, head: int, dim: int) -> bool:
+    """Whether rows [n, heads, dim] of these strides have memory in common."""
+    inner, outer = ((heads, head), (n, row)) if head <= row else ((n, row), (heads, head))
+    if inner[0] > 1 and inner[1] < dim:
+        return True
+    return outer[0] > 1 and outer[1] < (max(inner[0], 1) - 1) * inner[1] + dim
+
+
 def _slots(t: torch.Tensor, device: torch.device) -> torch.Tensor:
     if t.dtype != torch.int64 or t.dim() != 1 or t.device != device:
         raise RuntimeError(f"slots must be an int64 [tokens] tensor on {device}")
@@ -104,6 +112,8 @@ class KvCache:
         else:
             self.data = torch.zeros(num_blocks, kv_heads, 2, block_tokens * head_dim, dtype=torch.uint8, device=self.device)
             self.scale = torch.zeros(num_blocks, kv_heads, 2, dtype=torch.float32, device=self.device)
+        # (new tensors from one of their type take 1.2 us; torch.empty with a dtype and a device takes 1.8)
+        self._like = {t: torch.empty(0, dtype=t, device=self.device) for t in _DTYPES}
         self._view = _lib.KvCacheView(num_blocks=self.num_blocks, kv_heads=self.kv_heads, head_dim=self.head_dim,
                                       block_tokens=self.block_tokens, format=_FORMATS[fmt], data=ptr(self.data),
                                       scale=ptr(self.scale))
@@ -114,6 +124,9 @@ class KvCache:
         (a plan's: a block's tokens stand next to each other, in order, none
         twice; a slot of -1 stores nothing).  Where the new rows exceed a block's
         scale in 8 bits its stored codes are rewritten under the larger one."""
+        if current_device() != self.device.index:
+            with torch.cuda.device(self.device):
+                return self.append(k, v, slots)
         k, kp, k_row, k_head = _rows(k, "k", self.kv_heads, self.head_dim, self.device)
         v, vp, v_row, v_head = _rows(v, "v", self.kv_heads, self.head_dim, self.device)
         slots = _slots(slots, self.device)
@@ -135,7 +148,11 @@ class KvCache:
         stored is what ``append`` stores of rows turned in 64 bits and rounded to
         fp32 and to their type; ``k`` is not changed.  A position that is not in
         the table makes its rows NaN; a query row at a negative one (a token of no
-        request) is left as it was in ``q_out``."""
+        request) is left as it was in ``q_out`` (a new one holds anything there).
+        ``q_out`` lies apart from ``k`` and ``v``."""
+        if current_device() != self.device.index:
+            with torch.cuda.device(self.device):
+                return self.append_rotated(k, v, slots, positions, rotary, q=q, q_out=q_out)
         k, kp, k_row, k_head = _rows(k, "k", self.kv_heads, self.head_dim, self.device)
         v, vp, v_row, v_head = _rows(v, "v", self.kv_heads, self.head_dim, self.device)
         slots = _slots(slots, self.device)
@@ -158,14 +175,14 @@ class KvCache:
         if rows.shape[0] != n or rows.dtype != k.dtype or heads < 1:
             raise RuntimeError(f"q must be [{n}, heads, {self.head_dim}] of k's dtype {k.dtype}, got {tuple(q.shape)} {q.dtype}")
         if q_out is None:
-            q_out = torch.empty((n, heads, self.head_dim), dtype=rows.dtype, device=self.device)
+            q_out = rows.new_empty((n, heads, self.head_dim))
             op, o_row, o_head = q_out.data_ptr(), heads * self.head_dim, self.head_dim
         else:
             if q_out.dtype != rows.dtype or q_out.shape != q.shape:
                 raise RuntimeError(f"q_out must be {tuple(q.shape)} {q.dtype}, got {tuple(q_out.shape)} {q_out.dtype}")
             out, op, o_row, o_head = _rows(q_out, "q_out", heads, self.head_dim, self.device)
-            if out is not q_out or (n > 1 and abs(o_row) < self.head_dim) or (heads > 1 and abs(o_head) < self.head_dim):
-                raise RuntimeError("q_out must be 16-byte aligned with strides of whole rows that are multiples of 8 elements")
+            if out is not q_out or _meets_itself(n, o_row, heads, o_head, self.head_dim):
+                raise RuntimeError("q_out must be 16-byte aligned with strides that are multiples of 8 elements, and no element twice")
             same = op == qp and (q_row, q_head) == (o_row, o_head)
             if n and not same and _overlap(rows, q_out):
                 raise RuntimeError("q_out overlaps q: it must be q itself or lie apart from it")
@@ -177,12 +194,16 @@ class KvCache:
     def read(self, slots: torch.Tensor, dtype: torch.dtype = torch.float16) -> dict[str, torch.Tensor]:
         """The stored rows at ``slots``: ``{"k": ..., "v": ...}`` of [tokens,
         kv_heads, head_dim] in ``dtype``; zeros for a slot of -1."""
+        if current_device() != self.device.index:
+            with torch.cuda.device(self.device):
+                return self.read(slots, dtype)
         if dtype not in _DTYPES:
             raise RuntimeError(f"dtype must be fp16 or bf16, got {dtype}")
         slots = _slots(slots, self.device)
         n = slots.shape[0]
         shape = (n, self.kv_heads, self.head_dim)
-        k, v = torch.empty(shape, dtype=dtype, device=self.device), torch.empty(shape, dtype=dtype, device=self.device)
+        like = self._like[dtype]
+        k, v = like.new_empty(shape), like.new_empty(shape)
         _lib.call("nsmlp_kv_read", self._ref, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), _DTYPES[dtype],
                   stream_handle(self.device))
         return {"k": k, "v": v}
@@ -322,6 +343,9 @@ class KvBatch:
         again (with other ``new_tokens``, requests after the first whose need
         of blocks changes get other ones).  ``step``: an earlier step of the same ``total`` and ``max_new``
         whose buffers are written again (a captured graph's)."""
+        if current_device() != self.device.index:
+            with torch.cuda.device(self.device):
+                return self.plan(new_tokens, total, max_new=max_new, step=step)
         total, max_new = int(total), int(max_new)
         if new_tokens.dtype != torch.int32 or new_tokens.device != self.device or new_tokens.numel() != self.requests \
                 or not new_tokens.is_contiguous():
@@ -338,6 +362,9 @@ class KvBatch:
     def commit(self, finished: torch.Tensor | None = None) -> None:
         """Make the last plan's lengths (all of its new tokens) the batch's, and end the requests with
         ``finished`` [requests] (int32, not 0): their blocks become free."""
+        if current_device() != self.device.index:
+            with torch.cuda.device(self.device):
+                return self.commit(finished)
         if finished is not None and (finished.dtype != torch.int32 or finished.device != self.device
                                      or int(finished.numel()) != self.requests or not finished.is_contiguous()):
             raise RuntimeError(f"finished must be a contiguous int32 [{self.requests}] tensor on {self.device}")
@@ -359,6 +386,9 @@ def paged_attention(q: torch.Tensor, cache: KvCache, step: KvStep, *, scale: flo
     b, device, dim = step.batch, cache.device, cache.head_dim
     if b.device != device:
         raise RuntimeError(f"the cache is on {device} and the batch on {b.device}")
+    if current_device() != device.index:
+        with torch.cuda.device(device):
+            return paged_attention(q, cache, step, scale=scale, out=out, lse=lse, ws=ws)
     if not step.planned:  # its lists are what the memory held
         raise RuntimeError("the step has not been planned (KvBatch.plan)")
     total, heads = step.total, b.q_heads

@@ -26,7 +26,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._runtime import aligned16, as_f16, ptr, require_device, stream_handle, workspace
+from ._runtime import aligned16, as_f16, current_device, ptr, require_device, stream_handle, workspace
 from .nested_absmax import NestedAbsmax
 
 __all__ = ["resolve_lm_head_block_size", "lm_head_nf4_meta", "dense_linear_nf4", "lm_head_forward", "token_logprobs"]
@@ -182,6 +182,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     row without one.  ``ws``: a uint8 workspace that ``nsmlp_workspace_init`` has
     cleared, in place of the stream's own."""
     device = require_device(logits, "logits")
+    if current_device() != device.index:
+        with torch.cuda.device(device):
+            return token_logprobs(logits, tokens, top=top, ws=ws)
     dtype = _LOGIT_DTYPES.get(logits.dtype)
     if dtype is None:
         raise RuntimeError(f"logits must be fp16, bf16 or fp32, got {logits.dtype}")
@@ -205,7 +208,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     # one buffer for what is fp32: a split into views takes as long as one tensor made anew
     sizes = [rows, 0 if tokens is None else rows, rows * n]
     parts = torch.empty(sum(sizes), dtype=torch.float32, device=device).split_with_sizes(sizes)
-    ids = torch.empty((*shape, n), dtype=torch.int64, device=device)
+    ids = torch.empty((*shape, n), dtype=torch.int64, device=device) if tokens is None else tokens.new_empty((*shape, n))
     if ws is None:
         ws = workspace(need, device) if need else None
     elif ws.device != device or not ws.is_contiguous():

@@ -32,6 +32,10 @@ def rotary_frequencies(head_dim: int, base: float = 10000.0, scaling: dict | Non
         return f
     if kind not in ("linear", "llama3"):
         raise RuntimeError(f"scaling of type {kind!r} is not offered: give the frequencies instead")
+    need = ["factor"] if kind == "linear" else ["factor", "low_freq_factor", "high_freq_factor", "original_max_position_embeddings"]
+    missing = [k for k in need if k not in scaling]
+    if missing:
+        raise RuntimeError(f"scaling of type {kind!r} needs {', '.join(missing)}")
     factor = float(scaling["factor"])
     if not factor >= 1.0:
         raise RuntimeError(f"scaling factor {factor} must be at least 1")

@@ -391,3 +391,51 @@ def test_a_run_of_them(gpu):
     # the two caches' distributions are close: a code of 4 bits is off by a sixth of its group's largest at most
     kl = (results["int8"].exp() * (results["int8"] - results["e2m1"])).sum(-1)
     assert (kl >= -1e-6).all() and (kl < 0.5).all()
+
+
+def test_tensors_of_a_device_that_is_not_the_current_one(gpu, monkeypatch):
+    """Every call makes its tensors' device current and gives the same (here there is one: the current one is said to be another)."""
+    from next_step_ai_amd import kv_cache, lm_head
+    from next_step_ai_amd.rotary import Rotary
+
+    g = torch.Generator(device=gpu).manual_seed(1)
+    k, v, q = (torch.randn(5, h, 64, device=gpu, generator=g).half() for h in (2, 2, 4))
+    z = torch.randn(3, 500, device=gpu, generator=g)
+    entered = []
+    real = torch.cuda.device
+
+    class Noted(real):
+        def __enter__(self):
+            super().__enter__()
+            entered.append(self.idx)
+            monkeypatch.setattr(kv_cache, "current_device", lambda: 0)
+            monkeypatch.setattr(lm_head, "current_device", lambda: 0)
+
+    def elsewhere():
+        monkeypatch.setattr(kv_cache, "current_device", lambda: 1)
+        monkeypatch.setattr(lm_head, "current_device", lambda: 1)
+
+    results = []
+    for other in (False, True):
+        if other:
+            monkeypatch.setattr(torch.cuda, "device", Noted)
+        away = elsewhere if other else lambda: None
+        b = kv_cache.KvBatch(4, 16, max_requests=1, max_blocks=4, q_heads=4, kv_heads=2, head_dim=64)
+        c = kv_cache.KvCache(4, 2, 64, fmt="e2m1")
+        rotary = Rotary(64, 10)
+        away()
+        st = b.plan(ints([5], gpu), 5)
+        away()
+        c.append(k, v, st.slots)
+        away()
+        turned = c.append_rotated(k, v, st.slots, st.positions, rotary, q=q)
+        away()
+        got = c.read(st.slots)
+        away()
+        out = kv_cache.paged_attention(turned, c, st)
+        away()
+        b.commit()
+        away()
+        lp = lm_head.token_logprobs(z, top=3)
+        results.append([turned, got["k"], out, b.cached.clone(), *lp.values()])
+    assert all(torch.equal(x, y) for x, y in zip(*results)) and entered == [0] * 7

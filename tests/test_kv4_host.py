@@ -100,7 +100,8 @@ def test_frequencies():
 
 
 @pytest.mark.parametrize("kw", [dict(base=0.0), dict(base=float("inf")), dict(scaling={"rope_type": "other", "factor": 2}),
-                                dict(scaling={"rope_type": "linear", "factor": 0.5}),
+                                dict(scaling={"rope_type": "linear", "factor": 0.5}), dict(scaling={"rope_type": "linear"}),
+                                dict(scaling={"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0}),
                                 dict(scaling={"rope_type": "llama3", "factor": 8, "low_freq_factor": 4, "high_freq_factor": 4,
                                               "original_max_position_embeddings": 8192})])
 def test_frequencies_refused(kw):
@@ -128,6 +129,17 @@ def test_overlap_of_rows():
     a, b = t[:1024].view(8, 2, 64), t[1024:2048].view(8, 2, 64)
     assert not _overlap(a, b) and not _overlap(b, a) and _overlap(a, a) and _overlap(a, t[1023:2047].view(8, 2, 64))
     assert _overlap(t.as_strided((4, 2, 64), (256, 64, 1)), t.as_strided((4, 2, 64), (256, 64, 1), 128))  # (between each other's rows)
+
+
+@pytest.mark.parametrize("n,row,heads,head,meets", [
+    (3, 128, 2, 64, False), (3, 127, 2, 64, True), (3, 64, 2, 64, True), (3, 64, 2, 192, False), (3, 64, 2, 128, True), (1, 0, 2, 64, False),
+    (3, 0, 1, 64, True), (3, 64, 1, 64, False), (1, 8, 1, 8, False), (3, 1000, 2, 500, False), (3, 1000, 2, 32, True), (0, 0, 2, 64, False)])
+def test_rows_that_meet_themselves(n, row, heads, head, meets):
+    from next_step_ai_amd.kv_cache import _meets_itself
+
+    assert _meets_itself(n, row, heads, head, 64) == meets
+    places = [r * row + h * head + d for r in range(n) for h in range(heads) for d in range(64)]
+    assert (len(set(places)) < len(places)) <= meets
 
 
 def test_codes_of_the_oracle():
