@@ -248,7 +248,9 @@ __device__ __forceinline__ float log_prob(float z, const Sums& s, float log_l) {
 template <Logit T>
 __device__ __forceinline__ void write_row(const LogprobArgs& a, int row, const uint8_t* logits, const Sums& s, const uint64_t* list,
                                           int tid) {
-  const float log_l = logf(s.l);
+  // the weights were 2^(d kLog2e) = e^(d (1 + kOff)), so that l is off by kOff x
+  constexpr float kOff = -1.3349758e-8f;  // kLog2e as rounded, over log2 e, less 1
+  const float log_l = logf(s.l == 0.0f ? 0.0f : __builtin_fmaf(-kOff, s.x, s.l));
   if (tid == 0) {
     if (a.logprob != nullptr) {
       const int64_t t = a.tokens[row];
@@ -311,13 +313,16 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(LogprobArgs a) {
       for (int j = 0; j < kPer; ++j) all = fmaxf(all, value_at<T>(raw[u], j));
     rebase(s, fmaxf(s.m, all));
 #pragma unroll
-    for (int u = 0; u < kLpBatch; ++u)
+    for (int u = 0; u < kLpBatch; ++u) {
+      float l = 0.0f, x = 0.0f;  // (a vector's sums first: fewer roundings on the way of each weight)
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
         const float d = value_at<T>(raw[u], j) - s.m, p = __builtin_amdgcn_exp2f(d * kLog2e);
-        s.l += p;
-        s.x = __builtin_fmaf(p, fmaxf(d, -200.0f), s.x);
+        l += p;
+        x = __builtin_fmaf(p, fmaxf(d, -200.0f), x);
       }
+      s.l += l, s.x += x;
+    }
     if constexpr (kTop) {
       if (at == first + wave) top.expect(all);
       if (__ballot(!(all < top.least)) != 0) {
