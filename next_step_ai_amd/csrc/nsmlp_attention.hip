@@ -173,7 +173,10 @@ __device__ __forceinline__ Codes4<D> load_codes4(const uint8_t* p) {
   }
   return o;
 }
-__device__ __forceinline__ float scale4(uint32_t bytes, int i) { return __uint_as_float(((bytes >> (8 * i)) & 0xFFu) << 23); }
+// A scale byte's float, byte i of four.  The conversions look at a scale's exponent
+// alone (all 256 of them with other bits set give the same values), so what the
+// shift leaves in the other bits may stay.
+__device__ __forceinline__ float scale4(uint32_t bytes, int i) { return __uint_as_float(i == 3 ? bytes >> 1 : bytes << (23 - 8 * i)); }
 
 // the two values of byte i (known when compiled) under a scale
 __device__ __forceinline__ uint32_t values4(uint32_t w, float scale, int i) {
