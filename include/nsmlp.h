@@ -568,7 +568,8 @@ typedef struct nsmlp_kv_cache {
 /* Stores K and V rows k, v [n][kv_heads][head_dim] (strides in elements,
  * multiples of 8; the last dimension contiguous) at slots[n] (block *
  * block_tokens + offset; a slot outside the cache, such as -1, stores nothing).
- * No slot stands twice in a call.  In 8 bits the tokens of one block stand next
+ * n is at most 2^24, and n * kv_heads at most 2^28, in 4 bits 2^27.  No slot
+ * stands twice in a call.  In 8 bits the tokens of one block stand next
  * to each other in the call, in the order of their offsets, as nsmlp_kv_plan
  * lists them. */
 int nsmlp_kv_append(const nsmlp_kv_cache* cache, const void* k, long long k_row_stride, long long k_head_stride,

@@ -603,10 +603,16 @@ __device__ __forceinline__ void stream_share(const KvAttnArgs& a, int block, Str
 }
 
 // The same in 4 bits.  A key is half as many bytes, so what is not its way from
-// memory shows: three tiles are on their way behind the one in use, and the waves
-// go from one unit to the next without a pause: what a share's units are is
-// read once, for all of them at a time, and while a unit's last tiles are in use
-// the next one's first are fetched, its pages and queries before.
+// memory shows: there are 8 waves, and they go from one unit to the next without a
+// pause (kAhead; next to tiles, where registers are short, they do not): what 64 of
+// a share's units are is read at once, and while a unit's last tile is in use the
+// next one's first is fetched, its pages and queries before.
+//
+// What bounds it: the codes' way from HBM, and about 2.8 us at a unit's end, where
+// its waves meet.  64 uneven requests (228 MB) 58 us, 5.2 TB/s beyond the 7 us of
+// the chain above (66 us with a pause between units); one token over 131000 keys
+// (143 MB) 37 us, 777 keys 10 us.  Vector instructions are issued in 56% of the
+// cycles (decoding and the weights), the matrix cores are busy in 17%.
 struct StreamUnit {  // a unit and its request's rows and keys
   int req, kv_begin, kv_end, part, first, parts, q0, q_len, kv_len;
 };
@@ -878,6 +884,9 @@ __device__ __forceinline__ void any_share(const KvAttnArgs& a, int block, Stream
   else stream_share<D, kFmt, kBf16, NW>(a, block, lds);
 }
 
+// In 8 bits 4 waves with two tiles each fill the memory's queues.  In 4 bits a wave
+// has half the bytes on their way: 4 waves with four tiles in turn 69 us for the 64
+// requests above, 8 with two 58, 8 with four 97 (their registers spill).
 template <int kFmt>
 constexpr int kStreamWaves = kFmt == NSMLP_KV_E2M1 ? 8 : 4;
 
@@ -979,7 +988,10 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
   const auto at_of = [&](int i) { return u.kv_begin + min(i, tiles - 1) * kTileKeys + 16 * part; };
   const auto page_of = [&](int i) { return min(at_of(i) >> a.c.b_shift, last) - pages.first; };
   uint4 raw[kRoles][2];
-  // In 4 bits every wave decodes K and V of its 16 keys, with 8 waves a half of
+  // In 4 bits, where there is more to decode and a lane's operands have scales of
+  // their own, every wave has the same share of K and of V (as in 8 bits, two copies
+  // of the products spilled: 2048 tokens over 14336 cached 3655 us, so 1890, 1.09
+  // PFLOP/s, matrix cores busy 53%).  It decodes K and V of 16 keys, with 8 waves a half of
   // either: K lane: token l % 16, dims D/4 (l / 16) + D/8 o + 0..D/8-1 (half o); V
   // lane: tokens 8 o + 4 (l / 32) + 0..3, dims D/16 (l % 16) + D/32 (l / 16 % 2) +
   // 0..D/32-1, which are its own places in the D/32 fragments of 32 dims.
@@ -1283,7 +1295,8 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
   //   2 i + 1  weights of tile i
   // K(i + 1) takes the place of K(i - 1), last read in step 2 i - 1, and V(i)
   // that of V(i - 2), last read in step 2 i - 1.  The tile's scales are written
-  // in the vector half before, four tiles' in turn.
+  // in the vector half before, four tiles' in turn.  In 4 bits both are written by
+  // all waves, halves of them in 2 i and in 2 i + 1.
   if (tiles > 0) {
     char* const buf0 = lds;
     char* const buf1 = lds + kTileBytes<D>;

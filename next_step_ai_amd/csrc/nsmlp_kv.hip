@@ -571,7 +571,9 @@ __device__ __forceinline__ void append_run(const KvAppendArgs& a, int t, long lo
   }
 }
 
-// waves a SIMD, as the rows of a run stay in registers (and the angles of some)
+// Waves a SIMD, as the rows of a run stay in registers, and with a rotation the
+// angles of some.  12071 tokens of 8 heads of 128 in blocks of 32 with a rotation:
+// 4 waves (their registers spill) 43 us, with 32 heads of queries 83; 3 waves 33, 62.
 template <int D, int B, bool kRotate>
 constexpr int kAppendWaves = kRotate ? (B * D > 4096 ? 2 : B * D > 2048 ? 3 : 4) : B == 64 ? 2 : 4;
 

@@ -75,12 +75,18 @@ int check_batch(const nsmlp_kv_batch* b) {
 
 constexpr int kMaxTokens = 1 << 24;
 
+// Heads' rows of a call: in 4 bits 16 threads have one, and a launch has fewer than 2^32.
+int check_count(const KvView& c, int n) {
+  const int log2 = c.fmt == NSMLP_KV_E2M1 ? 27 : 28;
+  if (n < 0 || n > kMaxTokens || (long long)n * c.heads > (1LL << log2))
+    return set_error(NSMLP_EINVAL, "n = %d rows of %d heads: at most 2^24 rows and 2^%d heads' rows", n, c.heads, log2);
+  return NSMLP_OK;
+}
+
 int append_args(const nsmlp_kv_cache* cache, const void* k, long long k_row, long long k_head, const void* v, long long v_row,
                 long long v_head, int dtype, const int64_t* slots, int n, KvAppendArgs& a) {
   int rc = cache_view(cache, a.c);
-  if (rc || (rc = check_dtype(dtype))) return rc;
-  if (n < 0 || n > kMaxTokens || (long long)n * a.c.heads > (1 << 28))
-    return set_error(NSMLP_EINVAL, "n = %d rows of %d heads: at most 2^24 rows and 2^28 heads' rows", n, a.c.heads);
+  if (rc || (rc = check_dtype(dtype)) || (rc = check_count(a.c, n))) return rc;
   if (n == 0) return NSMLP_OK;
   if (slots == nullptr) return set_error(NSMLP_EINVAL, "slots must be non-NULL");
   if ((rc = check_rows("k", k, k_row, k_head)) || (rc = check_rows("v", v, v_row, v_head))) return rc;
@@ -190,9 +196,7 @@ int nsmlp_kv_read(const nsmlp_kv_cache* cache, const int64_t* slots, int n, void
   NSMLP_FAULT_POINT("kv_read");
   KvReadArgs a;
   int rc = cache_view(cache, a.c);
-  if (rc || (rc = check_dtype(dtype))) return rc;
-  if (n < 0 || n > kMaxTokens || (long long)n * a.c.heads > (1 << 28))
-    return set_error(NSMLP_EINVAL, "n = %d rows of %d heads: at most 2^24 rows and 2^28 heads' rows", n, a.c.heads);
+  if (rc || (rc = check_dtype(dtype)) || (rc = check_count(a.c, n))) return rc;
   if (n == 0) return NSMLP_OK;
   if (slots == nullptr) return set_error(NSMLP_EINVAL, "slots must be non-NULL");
   if ((rc = check_rows("k_out", k_out, 0, 0)) || (rc = check_rows("v_out", v_out, 0, 0))) return rc;

@@ -117,7 +117,9 @@ __device__ __forceinline__ void rotate_part(RowPart<D>& x, const Angles<D / 16>&
 }
 
 // Query rows: 16 lanes turn kQueryHeads heads of a token under one set of
-// angles.  `unit` counts tokens times groups of heads.
+// angles (8 bytes a pair: a token's are as much as two heads' rows).  `unit` counts
+// tokens times groups of heads.  HBM bounds it: an append of 12071 tokens takes 20
+// us without and 49 us with 32 heads of 128 (198 MB in and out).
 constexpr int kQueryHeads = 4;
 __host__ __device__ __forceinline__ long long query_units(const KvRotateArgs& r, int n) {
   return (long long)n * ((r.q_heads + kQueryHeads - 1) / kQueryHeads);

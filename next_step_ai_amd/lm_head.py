@@ -193,18 +193,20 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     shape, V = logits.shape[:-1], logits.shape[-1]
     z = logits if logits.dim() == 2 else logits.reshape(-1 if V else 0, V)
     rows = z.shape[0]
+    key = (rows, V, dtype, int(top))
+    if not 0 <= key[3] <= V < 1 << 31 or rows >= 1 << 31:  # (before they become 32-bit numbers)
+        raise RuntimeError(f"top {top} must be in [0, 64] and at most the vocabulary: got {rows} rows of {V} logits")
     if V > 1 and z.stride(1) != 1:
         z = z.contiguous()
     if tokens is not None and (tokens.dtype != torch.int64 or tokens.device != device or tokens.shape != shape):
         raise RuntimeError(f"tokens must be an int64 {tuple(shape)} tensor on {device}, got {tuple(tokens.shape)} {tokens.dtype} on "
                            f"{tokens.device}")
-    key = (rows, V, dtype, int(top))
     need = _logprob_bytes.get(key)
     if need is None:
         if len(_logprob_bytes) >= 1024:
             _logprob_bytes.clear()
         need = _logprob_bytes[key] = int(_lib.lib().nsmlp_token_logprobs_workspace_bytes(*key))
-    n = max(key[3], 0)
+    n = key[3]
     # one buffer for what is fp32: a split into views takes as long as one tensor made anew
     sizes = [rows, 0 if tokens is None else rows, rows * n]
     parts = torch.empty(sum(sizes), dtype=torch.float32, device=device).split_with_sizes(sizes)

@@ -201,6 +201,14 @@ def test_refusals(gpu):
             token_logprobs(*args, **kw)
 
 
+@pytest.mark.parametrize("rows,vocab,top", [(1, (1 << 32) + 5, 0), (1, 100, 1 << 32), (1, 100, -(1 << 32)), ((1 << 32) + 1, 1, 0)])
+def test_sizes_past_32_bits(gpu, rows, vocab, top):
+    """Numbers that would be small ones in 32 bits (broadcast logits: nothing is stored)."""
+    z = torch.zeros(1, 1, dtype=torch.float16, device=gpu).expand(rows, vocab)
+    with pytest.raises(RuntimeError, match="top"):
+        token_logprobs(z, top=top)
+
+
 def test_in_a_graph(gpu):
     """Captured and replayed with other logits, eager calls on the same stream between the replays."""
     from next_step_ai_amd.lm_head import token_logprobs

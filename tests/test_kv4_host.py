@@ -60,6 +60,16 @@ def test_refusals(L, kw, text):
     assert call(L, **kw) == EINVAL and text in L.nsmlp_last_error(), L.nsmlp_last_error()
 
 
+def test_more_rows_than_a_launch_has_threads(L):
+    """In 4 bits 16 threads have a row: 2^28 rows, which the 8-bit formats take, would be 2^32 threads."""
+    from next_step_ai_amd import _lib
+
+    assert call(L, n=1 << 24, kv_heads=16, q=None) == EINVAL and b"2^27" in L.nsmlp_last_error()
+    c = _lib.KvCacheView(num_blocks=8, kv_heads=16, head_dim=64, block_tokens=16, format=_lib.NSMLP_KV_E2M1, data=MEM, scale=None)
+    assert L.nsmlp_kv_append(ctypes.byref(c), MEM, 1024, 64, MEM, 1024, 64, 0, MEM, 1 << 24, None) == EINVAL
+    assert L.nsmlp_kv_read(ctypes.byref(c), MEM, 1 << 24, MEM, MEM, 0, None) == EINVAL and b"2^27" in L.nsmlp_last_error()
+
+
 def test_nothing_to_store(L):
     assert call(L, n=0, q=None) == 0 and call(L, n=0, positions=None, slots=None, k=None, v=None, q_out=None) == 0
     assert call(L, n=0, interleaved=5) == EINVAL
