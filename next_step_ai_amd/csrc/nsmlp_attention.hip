@@ -991,7 +991,7 @@ __device__ __forceinline__ void tile_unit(const KvAttnArgs& a, const KvUnit u, i
   // In 4 bits, where there is more to decode and a lane's operands have scales of
   // their own, every wave has the same share of K and of V (as in 8 bits, two copies
   // of the products spilled: 2048 tokens over 14336 cached 3655 us, so 1890, 1.09
-  // PFLOP/s, matrix cores busy 53%).  It decodes K and V of 16 keys, with 8 waves a half of
+  // PFLOP/s, matrix cores busy 52%).  It decodes K and V of 16 keys, with 8 waves a half of
   // either: K lane: token l % 16, dims D/4 (l / 16) + D/8 o + 0..D/8-1 (half o); V
   // lane: tokens 8 o + 4 (l / 32) + 0..3, dims D/16 (l % 16) + D/32 (l / 16 % 2) +
   // 0..D/32-1, which are its own places in the D/32 fragments of 32 dims.

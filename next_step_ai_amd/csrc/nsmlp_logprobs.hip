@@ -11,7 +11,7 @@
 //
 // The top n of a row are found as whole numbers (order of the logit, then the
 // lower index first): 64 bits, all different.  A wave keeps the candidates above
-// its n-th largest so far in LDS and drops all but n where they pass 64; the first
+// its n-th largest so far in LDS and drops all but n where they pass 2 n or 64; the first
 // bound is the n-th largest of the lanes' own maxima of the first batch.  So nearly
 // all vectors cost one comparison.  A NaN counts as below every number.
 //
@@ -19,7 +19,7 @@
 // vector instructions (an exp2 and seven others for a logit): 2048 rows of 128256 in
 // bf16 with 5 alternatives (525 MB) 105 us, 5.0 TB/s.  One row, the chain of a
 // load, the selection and the joins: 128256 in fp16 4.4 us without alternatives,
-// 8.3 with one, 10.8 with 20, 32 with 64, where candidates are counted against each
+// 8.3 with one, 10.8 with 20, 25 with 64, where candidates are counted against each
 // other.
 #include <algorithm>
 
@@ -150,9 +150,9 @@ __device__ __forceinline__ float wave_total(float v) {
 }
 
 // How many of the entries in LDS (a multiple of 8, 16-byte aligned, 0 for none) are
-// larger than `a`, and than `b`.
-template <bool kBoth>
-__device__ __forceinline__ void count_above(const uint64_t* list, int count, uint64_t a, uint64_t b, int& above_a, int& above_b) {
+// larger than each of `mine`.
+template <int N>
+__device__ __forceinline__ void count_above(const uint64_t* list, int count, const uint64_t (&mine)[N], int (&above)[N]) {
   const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(list);
 #pragma unroll 1
   for (int j = 0; j < count; j += 8) {  // (eight are read at a time: one by one, each read was waited for)
@@ -160,38 +160,49 @@ __device__ __forceinline__ void count_above(const uint64_t* list, int count, uin
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = pairs[(j >> 1) + i];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      above_a += (v[i].x > a) + (v[i].y > a);
-      if (kBoth) above_b += (v[i].x > b) + (v[i].y > b);
-    }
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int k = 0; k < N; ++k) above[k] += (v[i].x > mine[k]) + (v[i].y > mine[k]);
   }
 }
 
-// Candidates of a wave: up to 128 entries in LDS, of which the n largest count.
+// Candidates of a wave: entries in LDS, of which the n largest count.  They are
+// settled where they pass `limit`: late enough for as many as n new ones (with a
+// limit of 64 candidates, 64 alternatives of 1200 rows of 50257 took 117 us, so 82;
+// one row of 128256 32, so 25), and no later, as the bound rises then.
+constexpr int kLpList = 3 * kWave;
 struct WaveTop {
-  uint64_t* buf;   // [128]
-  int n, count;    // (both the same in all lanes)
+  uint64_t* buf;          // [kLpList]
+  int n, count, limit;    // (the same in all lanes)
   uint64_t bound;  // entries at or below it are not among the n largest
   float least;     // what a logit of the next batch has to reach (-inf: any may count)
   int lane;
 
   __device__ __forceinline__ void start(uint64_t* b, int top, int l) {
-    buf = b, n = top, count = 0, bound = 0, least = -INFINITY, lane = l;
+    buf = b, n = top, count = 0, limit = max(kWave, 2 * n), bound = 0, least = -INFINITY, lane = l;
   }
 
   // The n largest, in order, and the bound that follows.  An entry's place is the
   // number of larger ones; 0 stands for none.
+  template <int N>
+  __device__ __forceinline__ void rank() {
+    uint64_t mine[N];
+    int above[N] = {};
+#pragma unroll
+    for (int k = 0; k < N; ++k) mine[k] = buf[lane + k * kWave];
+    count_above<N>(buf, count, mine, above);
+    wave_sync();
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (lane + k * kWave < count && above[k] < n) buf[above[k]] = mine[k];
+  }
   __device__ __forceinline__ void settle() {
     wave_sync();
-    if (lane < 8 && count + lane < 2 * kWave) buf[count + lane] = 0;
+    if (lane < 8 && count + lane < kLpList) buf[count + lane] = 0;
     wave_sync();
-    const uint64_t a = buf[lane], b = count > kWave ? buf[lane + kWave] : 0;
-    int above_a = 0, above_b = 0;
-    if (count > kWave) count_above<true>(buf, count, a, b, above_a, above_b);
-    else count_above<false>(buf, count, a, b, above_a, above_b);
-    wave_sync();
-    if (lane < count && above_a < n) buf[above_a] = a;
-    if (lane + kWave < count && above_b < n) buf[above_b] = b;
+    if (count > 2 * kWave) rank<3>();
+    else if (count > kWave) rank<2>();
+    else rank<1>();
     wave_sync();
     if (count >= n) {
       count = n;
@@ -227,7 +238,7 @@ struct WaveTop {
     if (who == 0) return;
     if (in) buf[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] = entry;
     count += __popcll(who);
-    if (count > kWave) settle();
+    if (count > limit) settle();
   }
 };
 
@@ -276,7 +287,7 @@ template <Logit T, bool kTop, bool kShort>
 __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(LogprobArgs a) {
   kernarg_warm<sizeof(LogprobArgs)>();
   constexpr int kPer = kPerVector<T>, kSize = T == Logit::kF32 ? 4 : 2;
-  __shared__ __attribute__((aligned(16))) uint64_t bufs[kLpWaves][2 * kWave];
+  __shared__ __attribute__((aligned(16))) uint64_t bufs[kLpWaves][kLpList];
   __shared__ uint64_t merged[kLpMaxTop];
   __shared__ float sums[kLpWaves][3];
   __shared__ int last;
@@ -444,8 +455,11 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(LogprobArgs a) {
   write_row<T>(a, row, logits, p, bufs[0], lane);
 }
 
-constexpr int kLpTarget = 1024;  // four a CU
-// Workgroups of a row: about a thousand in all, none with less than a batch of vectors per wave.
+// Workgroups of a row: about kLpTarget in all, four a CU, none with less than a batch
+// of vectors per wave.  With 512, 1024 and 2048, 5 alternatives of 300 rows of 128256
+// in bf16 take 30, 27 and 32 us, of 700 rows 46.5, 48.4 and 50.3, of 256 rows of 32000
+// 11.7, 12.0 and 11.9; fewer rows have their most in all three.
+constexpr int kLpTarget = 1024;
 struct Splits {
   int count, each;
 };

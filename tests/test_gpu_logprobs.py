@@ -204,6 +204,8 @@ def test_refusals(gpu):
 @pytest.mark.parametrize("rows,vocab,top", [(1, (1 << 32) + 5, 0), (1, 100, 1 << 32), (1, 100, -(1 << 32)), ((1 << 32) + 1, 1, 0)])
 def test_sizes_past_32_bits(gpu, rows, vocab, top):
     """Numbers that would be small ones in 32 bits (broadcast logits: nothing is stored)."""
+    from next_step_ai_amd.lm_head import token_logprobs
+
     z = torch.zeros(1, 1, dtype=torch.float16, device=gpu).expand(rows, vocab)
     with pytest.raises(RuntimeError, match="top"):
         token_logprobs(z, top=top)
