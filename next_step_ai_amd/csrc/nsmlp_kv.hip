@@ -673,9 +673,13 @@ void append_typed(KvAppendArgs a, hipStream_t s) {
   // are then one wave's, one after the other.  With 1, 8 and 16 tokens per wave,
   // 8 heads: prompts of 4096 tokens (65536 pairs) 32.6, 10.5, 9.6 us, of 8192 62.5,
   // 17.0, 13.9; single tokens, 1024 of them 16.0, 17.7, 28.2 us, 2048 29.0, 23.0, 32.1,
-  // 4096 53.9, 41.1, 41.7; 290 next to 7000 of prompts 46.9, 18.3, 30.2.
+  // 4096 53.9, 41.1, 41.7; 290 next to 7000 of prompts 46.9, 18.3, 30.2.  In between,
+  // with 1, 2 and 4, without and with a rotation (blocks of 64, heads of 64): 256
+  // single tokens 5.9, 6.8, 9.4 and 7.7, 8.1, 10.8; 512 9.6, 9.0, 10.9 and 12.7, 12.3,
+  // 12.9; 1024 16.9, 15.3, 14.8 and 22.7, 20.3, 20.9; a prompt of 1024 9.4, 7.9, 7.5 and
+  // 14.5, 12.1, 10.9; 21 next to 1858 of prompts 12.5, 9.2, 9.5 and 18.6, 13.1, 12.0.
   const long long pairs = (long long)a.n * a.c.heads * 2;
-  a.take = pairs >= 128 * 1024 ? 16 : pairs >= 32 * 1024 ? 8 : 1;
+  a.take = pairs >= 128 * 1024 ? 16 : pairs >= 32 * 1024 ? 8 : pairs >= 16 * 1024 ? 4 : pairs >= 8 * 1024 ? 2 : 1;
   const long long waves = (long long)((a.n + a.take - 1) / a.take) * a.c.heads * 2, per = kAppendThreads / kWave;
   a.rot.first = (unsigned)((waves + per - 1) / per);
   if (a.rot.table == nullptr) {
