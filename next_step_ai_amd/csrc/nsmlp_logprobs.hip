@@ -3,11 +3,14 @@
 //
 // With m the largest logit of a row (finite), l = sum e^(z - m) and x = sum e^(z - m) (z - m):
 //   log p_t = (z_t - m) - log l          entropy = log l - x / l
-// Neither subtracts large numbers from each other, as z - log sum e^z would.
-// Every lane keeps its own m, l, x (fp32), raises m once per batch of
-// vectors, and lanes, waves and workgroups join theirs under the largest m.  A
-// NaN or +inf makes l NaN; -inf adds nothing to l, and to x neither, as the
-// factor z - m is held above -200, below which e^(z - m) is zero.
+// Neither subtracts large numbers from each other, as z - log sum e^z would.  What
+// the largest logit itself adds to l, 1, is kept apart, so that where one token has
+// nearly all of a row log l = log(1 + r) is known to its own size (a log probability
+// of -0.005 to 2e-7 of it; with the 1 in the sum to 1e-5).
+// A wave's lanes have their sums (fp32) under one m, raised at most once per batch of
+// vectors; waves and workgroups join theirs under the largest m.  A NaN or +inf makes
+// l NaN; -inf adds nothing to l, and to x neither, as the factor z - m is held above
+// -200, below which e^(z - m) is zero.
 //
 // The top n of a row are found as whole numbers (order of the logit, then the
 // lower index first): 64 bits, all different.  A wave keeps the candidates above
@@ -17,11 +20,12 @@
 //
 // What bounds it: many rows, the logits' way from HBM and, nearly as much, the
 // vector instructions (an exp2 and seven others for a logit): 2048 rows of 128256 in
-// bf16 with 5 alternatives (525 MB) 105 us, 5.0 TB/s.  One row, the chain of a
-// load, the selection and the joins: 128256 in fp16 4.4 us without alternatives,
-// 8.3 with one, 10.8 with 20, 25 with 64, where candidates are counted against each
+// bf16 with 5 alternatives (525 MB) 113 us, 4.6 TB/s.  One row, the chain of a
+// load, the selection and the joins: 128256 in fp16 5.0 us without alternatives,
+// 9.9 with 5, 11.5 with 20, 26 with 64, where candidates are counted against each
 // other.
 #include <algorithm>
+#include <type_traits>
 
 #include "nsmlp_internal.h"
 
@@ -45,7 +49,7 @@ struct LogprobArgs {
   float *logprob, *entropy;  // [rows], nullable
   int64_t* top_ids;        // [rows][top]
   float* top_logprobs;
-  float* part_sums;        // [rows][splits][4]: m, l, x
+  float* part_sums;        // [rows][splits][4]: m, l, x, ones
   uint64_t* part_top;      // [rows][splits][top]
   int* count;              // [rows] workgroups of a row that have ended (zero, left zero)
 };
@@ -242,24 +246,28 @@ struct WaveTop {
   }
 };
 
-// Sums under a largest logit m.
+// Sums under a largest logit m: of the weights that are in `ones` (logits equal to m,
+// some or all) and of the others.
 struct Sums {
-  float m, l, x;
+  float m, l, x, ones;
+  __device__ __forceinline__ float all() const { return l + ones; }
 };
 __device__ __forceinline__ void rebase(Sums& s, float m) {
-  const float d = s.m - m, f = __builtin_amdgcn_exp2f(d * kLog2e);
-  s.x = f * __builtin_fmaf(fmaxf(d, -200.0f), s.l, s.x);
-  s.l *= f;
+  const float d = s.m - m;
+  if (d != 0.0f) {  // (NaN where both are inf)
+    const float f = __builtin_amdgcn_exp2f(d * kLog2e), l = s.all();
+    s.x = f * __builtin_fmaf(fmaxf(d, -200.0f), l, s.x);
+    s.l = f * l;
+    s.ones = 0.0f;
+  }
   s.m = m;
 }
-__device__ __forceinline__ Sums join_wave(Sums s) {
-  rebase(s, wave_most(s.m));
-  s.l = wave_total(s.l), s.x = wave_total(s.x);
-  return s;
+__device__ __forceinline__ Sums join_lanes(const Sums& s) {  // of one m
+  return Sums{s.m, wave_total(s.l), wave_total(s.x), wave_total(s.ones)};
 }
 
 __device__ __forceinline__ float log_prob(float z, const Sums& s, float log_l) {
-  return s.l == 0.0f ? -INFINITY : (z - s.m) - log_l;  // (nothing but -inf in the row)
+  return s.all() == 0.0f ? -INFINITY : (z - s.m) - log_l;  // (nothing but -inf in the row)
 }
 
 // The row's results from its sums and, in `list`, its n largest.
@@ -268,13 +276,14 @@ __device__ __forceinline__ void write_row(const LogprobArgs& a, int row, const u
                                           int tid) {
   // the weights were 2^(d kLog2e) = e^(d (1 + kOff)), so that l is off by kOff x
   constexpr float kOff = -1.3349758e-8f;  // kLog2e as rounded, over log2 e, less 1
-  const float log_l = logf(s.l == 0.0f ? 0.0f : __builtin_fmaf(-kOff, s.x, s.l));
+  const float l = s.all(), others = l == 0.0f ? 0.0f : __builtin_fmaf(-kOff, s.x, s.l);
+  const float log_l = s.ones == 1.0f ? log1pf(others) : logf(others + s.ones);
   if (tid == 0) {
     if (a.logprob != nullptr) {
       const int64_t t = a.tokens[row];
       a.logprob[row] = t >= 0 && t < a.vocab ? log_prob(load_one<T>(logits, t), s, log_l) : __uint_as_float(0x7FC00000u);
     }
-    if (a.entropy != nullptr) a.entropy[row] = s.l == 0.0f ? 0.0f : log_l - s.x / s.l;
+    if (a.entropy != nullptr) a.entropy[row] = l == 0.0f ? 0.0f : log_l - s.x / l;
   }
   if (tid < a.top) {
     const uint64_t e = list[tid];
@@ -284,12 +293,12 @@ __device__ __forceinline__ void write_row(const LogprobArgs& a, int row, const u
 }
 
 template <Logit T, bool kTop, bool kShort>
-__global__ void __launch_bounds__(kLpThreads) k_token_logprobs(LogprobArgs a) {
+__global__ void __launch_bounds__(kLpThreads, 5) k_token_logprobs(LogprobArgs a) {
   kernarg_warm<sizeof(LogprobArgs)>();
   constexpr int kPer = kPerVector<T>, kSize = T == Logit::kF32 ? 4 : 2;
   __shared__ __attribute__((aligned(16))) uint64_t bufs[kLpWaves][kLpList];
   __shared__ uint64_t merged[kLpMaxTop];
-  __shared__ float sums[kLpWaves][3];
+  __shared__ float sums[kLpWaves][4];
   __shared__ int last;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row = blockIdx.x, split = blockIdx.y;
@@ -299,7 +308,8 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(LogprobArgs a) {
 
   WaveTop top;
   if constexpr (kTop) top.start(bufs[wave], a.top, lane);
-  Sums s = {kLowest, 0.0f, 0.0f};
+  Sums s = {kLowest, 0.0f, 0.0f, 0.0f};
+  int ones = 0;  // of the wave
   for (int at = first + wave; at < end; at += kLpWaves * kLpBatch) {
     uint4 raw[kLpBatch];
     if constexpr (!kShort) {
@@ -324,22 +334,47 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(LogprobArgs a) {
         raw[u] = without<T>(raw[u], lost);
       }
     }
-    float all = value_at<T>(raw[0], 0);  // (NaN only where every one is)
-#pragma unroll
-    for (int u = 0; u < kLpBatch; ++u)
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) all = fmaxf(all, value_at<T>(raw[u], j));
-    rebase(s, fmaxf(s.m, all));
+    float most[kLpBatch];  // of a vector (NaN only where every one is)
 #pragma unroll
     for (int u = 0; u < kLpBatch; ++u) {
+      most[u] = value_at<T>(raw[u], 0);
+#pragma unroll
+      for (int j = 1; j < kPer; ++j) most[u] = fmaxf(most[u], value_at<T>(raw[u], j));
+    }
+    const float all = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+    if (__ballot(all > s.m) != 0) {
+      s.ones = lane == 0 ? (float)ones : 0.0f;
+      rebase(s, wave_most(all));
+      ones = 0;
+    }
+    const auto add = [&](auto has_most, int u) {
       float l = 0.0f, x = 0.0f;  // (a vector's sums first: fewer roundings on the way of each weight)
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
         const float d = value_at<T>(raw[u], j) - s.m, p = __builtin_amdgcn_exp2f(d * kLog2e);
-        l += p;
+        if constexpr (decltype(has_most)::value) {
+          ones += __popcll(__ballot(d == 0.0f));
+          l += d == 0.0f ? 0.0f : p;
+        } else {
+          l += p;
+        }
         x = __builtin_fmaf(p, fmaxf(d, -200.0f), x);
       }
       s.l += l, s.x += x;
+    };
+    // Few batches of a long row hold an m (1 + log n of n, as a wave has one): those that
+    // do not have no branch between their vectors.  (700 rows of 128256 with 5
+    // alternatives 51.7 us, with a branch per vector in all batches 52.3, every vector of
+    // a batch that raises m counted 53.7, with the 1 in the sum 48.5.)
+    if (__builtin_expect_with_probability(__ballot(all == s.m) != 0, 0, 0.9)) {
+#pragma unroll
+      for (int u = 0; u < kLpBatch; ++u) {
+        if (__ballot(most[u] == s.m) != 0) add(std::true_type{}, u);
+        else add(std::false_type{}, u);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < kLpBatch; ++u) add(std::false_type{}, u);
     }
     if constexpr (kTop) {
       if (at == first + wave) top.expect(all);
@@ -369,19 +404,20 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(LogprobArgs a) {
     top.settle();
     if (lane >= top.count && lane < a.top) bufs[wave][lane] = 0;  // a wave with fewer logits
   }
-  s = join_wave(s);
-  if (lane == 0) sums[wave][0] = s.m, sums[wave][1] = s.l, sums[wave][2] = s.x;
+  s.ones = lane == 0 ? (float)ones : 0.0f;
+  s = join_lanes(s);
+  if (lane == 0) sums[wave][0] = s.m, sums[wave][1] = s.l, sums[wave][2] = s.x, sums[wave][3] = s.ones;
   __syncthreads();
   {
     float m = sums[0][0];
 #pragma unroll
     for (int w = 1; w < kLpWaves; ++w) m = fmaxf(m, sums[w][0]);
-    Sums r = {m, 0.0f, 0.0f};
+    Sums r = {m, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int w = 0; w < kLpWaves; ++w) {
-      Sums p = {sums[w][0], sums[w][1], sums[w][2]};
+      Sums p = {sums[w][0], sums[w][1], sums[w][2], sums[w][3]};
       rebase(p, m);
-      r.l += p.l, r.x += p.x;
+      r.l += p.l, r.x += p.x, r.ones += p.ones;
     }
     s = r;
   }
@@ -414,6 +450,7 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(LogprobArgs a) {
     st_coherent(a.part_sums + at * 4, s.m);
     st_coherent(a.part_sums + at * 4 + 1, s.l);
     st_coherent(a.part_sums + at * 4 + 2, s.x);
+    st_coherent(a.part_sums + at * 4 + 3, s.ones);
   }
   if (kTop && tid < a.top) __hip_atomic_store(a.part_top + at * a.top + tid, merged[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   wait_stores();
@@ -423,12 +460,13 @@ __global__ void __launch_bounds__(kLpThreads) k_token_logprobs(LogprobArgs a) {
   if (!last || wave != 0) return;
   if (lane == 0) atomicExch(a.count + row, 0);
   const long long row_at = (long long)row * a.splits;
-  Sums p = {kLowest, 0.0f, 0.0f};
+  Sums p = {kLowest, 0.0f, 0.0f, 0.0f};
   if (lane < a.splits) {
     const float* from = a.part_sums + (row_at + lane) * 4;
-    p = {ld_coherent(from), ld_coherent(from + 1), ld_coherent(from + 2)};
+    p = {ld_coherent(from), ld_coherent(from + 1), ld_coherent(from + 2), ld_coherent(from + 3)};
   }
-  p = join_wave(p);
+  rebase(p, wave_most(p.m));
+  p = join_lanes(p);
   if constexpr (kTop) {
     // the lists' first entries, their second ones, and so on, 64 at a time: after the
     // first 64 there is a bound that few of the others pass

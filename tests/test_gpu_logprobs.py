@@ -201,6 +201,39 @@ def test_refusals(gpu):
             token_logprobs(*args, **kw)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,vocab", [(1, 3), (3, 40), (2, 1000), (1, 70001), (300, 2000)])
+def test_rows_of_one_token(gpu, dtype, rows, vocab):
+    """One token has nearly all of a row: log p and the entropy to their own size, not to that of 1.
+
+    With the others d = -12 to -20 below it (exact in fp32) and log p = -log(1 + r), r = sum e^d: a weight's
+    exponent d log2 e is rounded once and its exp2 to an ulp, (20 * 1.45 + 2) 2^-24; the sums take at most 8 terms of a
+    vector, 35 batches of 4 vectors, 6 joins of lanes, 3 of waves, 6 of workgroups: 60 roundings, r as it grows;
+    log1p two ulps.  The entropy has x = sum e^d d next to it, with one rounding more each."""
+    from next_step_ai_amd.lm_head import token_logprobs
+
+    g = torch.Generator().manual_seed(vocab)
+    z = (torch.randint(0, 33, (rows, vocab), generator=g) * 0.25 - 20.0).to(dtype)  # exact in all three
+    at = torch.randint(vocab, (rows,), generator=g)
+    z[torch.arange(rows), at] = 0.0
+    got = token_logprobs(z.to(gpu), at.to(gpu), top=1)
+    lp = z.double().log_softmax(-1)
+    d = z.double()
+    r = (d.exp() * (d < 0)).sum(-1)
+    want = -torch.log1p(r)
+    entropy = -(lp.exp() * lp).sum(-1)
+    tol = (20 * 1.45 + 2 + 60 + 4) * 2.0 ** -24
+    for name, w in (("logprob", want), ("entropy", torch.log1p(r) - (d.exp() * d).sum(-1) / (1 + r))):
+        e = (got[name].double().cpu() - w).abs() / w.abs()
+        assert float(e.max()) <= tol * (1 if name == "logprob" else 1.5), (name, float(e.max()), tol)
+    assert torch.allclose(entropy, torch.log1p(r) - (d.exp() * d).sum(-1) / (1 + r), rtol=1e-9, atol=1e-13)
+    assert torch.equal(got["top_ids"][:, 0].cpu(), at) and torch.equal(got["top_logprobs"][:, 0], got["logprob"])
+    # several of the same: their logits are 1 each
+    tied = token_logprobs(torch.zeros(2, vocab, dtype=dtype, device=gpu), torch.zeros(2, dtype=torch.int64, device=gpu))
+    for name, sign in (("logprob", -1), ("entropy", 1)):
+        assert torch.allclose(tied[name].double().cpu(), torch.full((2,), sign * math.log(vocab), dtype=torch.float64), rtol=2.0 ** -22, atol=0)
+
+
 @pytest.mark.parametrize("rows,vocab,top", [(1, (1 << 32) + 5, 0), (1, 100, 1 << 32), (1, 100, -(1 << 32)), ((1 << 32) + 1, 1, 0)])
 def test_sizes_past_32_bits(gpu, rows, vocab, top):
     """Numbers that would be small ones in 32 bits (broadcast logits: nothing is stored)."""
