@@ -669,8 +669,9 @@ int nsmlp_kv_commit(const nsmlp_kv_batch* batch, const nsmlp_kv_step* step, cons
  * A token that sees no key (a refused request's) gets zeros and -inf; rows past
  * the step's tokens are left as they are.  A table entry that is not a block
  * (or past max_blocks) hides its keys and sets
- * NSMLP_STATUS_BLOCK_UNAVAILABLE in the workspace's status word.  fp32 scores
- * and sums; a softmax weight is an fp16 operand of the products, or two (22 bits)
+ * NSMLP_STATUS_BLOCK_UNAVAILABLE in the workspace's status word.  A row that sees
+ * a key that is not finite is NaN, whatever the other scores are, and so is one
+ * with a score past fp32's range.  fp32 scores and sums; a softmax weight is an fp16 operand of the products, or two (22 bits)
  * where a request has up to 16 rows per K/V head; the result does not depend on
  * how the work is scheduled, only on the batch's lengths.  scale > 0.  The step
  * is one that nsmlp_kv_plan has written; ws is cleared once by

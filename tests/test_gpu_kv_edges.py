@@ -451,6 +451,56 @@ def test_scores_of_any_size(gpu, fmt, size, Hq, H, D, block, cached, new):
     assert ((lse.double() - top).abs() <= (2.0 ** -11 + 2.0 ** -16) * top).all()
 
 
+@pytest.mark.parametrize("fmt", ["e2m1", "int8", "e4m3"])
+@pytest.mark.parametrize("which,value", [("k", float("nan")), ("k", float("inf")), ("v", -float("inf"))])
+@pytest.mark.parametrize("Hq,H,D,block,cached,new,bad", [
+    (4, 2, 128, 16, 600, 1, 0),       # single tokens: in a wave's first tile, in a later one, in the last
+    (4, 2, 128, 16, 600, 1, 333),
+    (4, 2, 64, 32, 600, 1, 600),
+    (4, 2, 64, 16, 200, 6, 70),       # drafts
+    (4, 2, 64, 16, 200, 6, 203),
+    (4, 2, 128, 32, 200, 60, 5),      # tiles of 128 rows
+    (4, 2, 128, 32, 200, 60, 236),
+    (8, 8, 64, 16, 0, 40, 17),
+    (256, 128, 64, 16, 100, 520, 40),  # of 256
+    (256, 128, 64, 16, 100, 520, 433),
+])
+def test_a_value_that_is_not_finite_among_far_scores(gpu, fmt, which, value, Hq, H, D, block, cached, new, bad):
+    """Queries that are keys of the cache, of size 3000, so that scores pass 2^20: rows that see the token (in 8 bits its
+    block, whose scale is NaN) are NaN, the others their key's value."""
+    from next_step_ai_amd.kv_cache import KvBatch, KvCache, paged_attention
+
+    n, G, head = cached + new, Hq // H, H - 1
+    pool = n // block + 1
+    b = KvBatch(pool, block, max_requests=1, max_blocks=pool, q_heads=Hq, kv_heads=H, head_dim=D)
+    c = KvCache(pool, H, D, block_tokens=block, fmt=fmt)
+    g = torch.Generator(device=gpu).manual_seed(3)
+    k = ((torch.randint(0, 2, (n, H, D), device=gpu, generator=g) * 2 - 1) * 3000.0).half()
+    v = torch.randn(n, H, D, device=gpu, generator=g).half()
+    ask = (7 * torch.arange(new, device=gpu)) % (cached + 1 + torch.arange(new, device=gpu))
+    q = k[ask].repeat_interleave(G, 1)
+    kv = {"k": k, "v": v}
+    kv[which][bad, head, 3] = value
+    if cached:
+        st = b.plan(ints([cached], gpu), cached)
+        c.append(k[:cached], v[:cached], st.slots)
+        b.commit()
+    st = b.plan(ints([new], gpu), new, max_new=new)
+    c.append(k[cached:], v[cached:], st.slots)
+    lse = torch.empty(new, Hq, device=gpu)
+    out = paged_attention(q, c, st, lse=lse)
+    first = bad if fmt == "e2m1" else bad // block * block  # the first key that is not a number
+    sees = (cached + torch.arange(new, device=gpu) >= first)[:, None] & (torch.arange(Hq, device=gpu) >= head * G)[None]
+    assert sees.any() and not sees.all()
+    assert torch.equal(out.isnan().all(-1), sees) and torch.equal(out.isnan().any(-1), sees)
+    assert torch.equal(lse.isnan(), sees)
+    at = torch.arange(n, device=gpu)
+    slots = st.table[0][at // block].long() * block + at % block
+    want = c.read(slots[ask])["v"].repeat_interleave(G, 1).double()
+    off = (out.double() - want).abs() <= 2.0 ** -10 * want.abs() + 2.0 ** -24  # read and row rounded once each
+    assert off.all(-1)[~sees].all()
+
+
 @pytest.mark.parametrize("new", [1, 60])
 def test_scores_of_any_size_in_bf16(gpu, new):
     """The same with bf16 magnitudes of 2^40, whose scores pass 2^80."""
