@@ -56,6 +56,44 @@ int check_rows(const char* what, const void* p, long long row, long long head) {
   return NSMLP_OK;
 }
 
+// Rows [n][heads][dim] of 16-bit elements, strides in elements.
+struct RowSet {
+  const void* p;
+  long long n, row, heads, head;
+  int dim;
+};
+
+// Whether two sets of rows may have memory in common.  They have none where one ends
+// before the other begins, or where both repeat with a period (a stride) that every
+// other stride is a multiple of, or that holds the rest, and lie apart within it: as
+// slices of one projection do.
+bool rows_meet(const RowSet& a, const RowSet& b) {
+  struct Span {
+    __int128 first, size;
+  };
+  const auto span = [](const RowSet& s, __int128 period) {  // of the strides that are no multiples of it (0: of all)
+    Span o = {(__int128)((uintptr_t)s.p / 2), s.dim};
+    const __int128 count[2] = {s.n, s.heads}, stride[2] = {s.row, s.head};
+    for (int i = 0; i < 2; ++i) {
+      if (count[i] < 2 || (period != 0 && stride[i] % period == 0)) continue;
+      const __int128 way = (count[i] - 1) * stride[i];
+      o.size += way < 0 ? -way : way;
+      if (way < 0) o.first += way;
+    }
+    return o;
+  };
+  const Span all_a = span(a, 0), all_b = span(b, 0);
+  if (all_a.first + all_a.size <= all_b.first || all_b.first + all_b.size <= all_a.first) return false;
+  for (const long long stride : {a.row, a.head, b.row, b.head}) {
+    const __int128 period = stride < 0 ? -(__int128)stride : stride;
+    if (period == 0) continue;
+    const Span sa = span(a, period), sb = span(b, period);
+    const __int128 to_b = ((sb.first - sa.first) % period + period) % period;
+    if (to_b >= sa.size && period - to_b >= sb.size) return false;
+  }
+  return true;
+}
+
 int check_batch(const nsmlp_kv_batch* b) {
   if (b == nullptr) return set_error(NSMLP_EINVAL, "batch must be non-NULL");
   if (b->requests < 1 || b->requests > kKvMaxRequests)
@@ -177,6 +215,11 @@ int nsmlp_kv_append_rotated(const nsmlp_kv_cache* cache, const nsmlp_rotary* rot
       return rc;
     if (q == q_out && (q_row_stride != out_row_stride || q_head_stride != out_head_stride))
       return set_error(NSMLP_EINVAL, "queries that are rotated in place keep their strides");
+    // (other workgroups of the launch read K and V)
+    const RowSet out = {q_out, n, out_row_stride, q_heads, out_head_stride, a.c.D};
+    if (rows_meet(out, RowSet{k, n, k_row_stride, a.c.heads, k_head_stride, a.c.D}) ||
+        rows_meet(out, RowSet{v, n, v_row_stride, a.c.heads, v_head_stride, a.c.D}))
+      return set_error(NSMLP_EINVAL, "q_out overlaps k or v");
   }
   if ((rc = check_device())) return rc;
   a.rot.table = rotary->table;

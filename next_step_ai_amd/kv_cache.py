@@ -149,7 +149,8 @@ class KvCache:
         fp32 and to their type; ``k`` is not changed.  A position that is not in
         the table makes its rows NaN; a query row at a negative one (a token of no
         request) is left as it was in ``q_out`` (a new one holds anything there).
-        ``q_out`` lies apart from ``k`` and ``v``."""
+        A ``q_out`` that overlaps ``k`` or ``v`` is refused; slices of one
+        projection do not."""
         if current_device() != self.device.index:
             with torch.cuda.device(self.device):
                 return self.append_rotated(k, v, slots, positions, rotary, q=q, q_out=q_out)

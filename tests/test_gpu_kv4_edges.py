@@ -337,6 +337,41 @@ def test_step_in_a_graph(gpu, fmt):
             assert torch.equal(b.cached, plain[0].cached)
 
 
+@pytest.mark.parametrize("fmt", ["e2m1", "int8"])
+@pytest.mark.parametrize("n,H,D,layout", [(1, 3, 64, "rows"), (37, 1, 128, "rows"), (37, 4, 64, "rows"), (70, 4, 128, "heads"),
+                                          (21, 3, 64, "stacked"), (21, 3, 64, "turned")])
+def test_queries_turned_next_to_keys_and_values(gpu, fmt, n, H, D, layout):
+    """In place in a buffer that holds K and V too, whatever the order of its dimensions; over K or V it is refused."""
+    from next_step_ai_amd.kv_cache import KvCache
+    from next_step_ai_amd.rotary import Rotary
+
+    g = torch.Generator(device=gpu).manual_seed(n)
+    if layout == "rows":  # [n, 3 H, D]
+        both = torch.randn(n, 3 * H, D, device=gpu, generator=g).half()
+        q, k, v = both.split(H, 1)
+    elif layout == "heads":  # [n, H, 3, D]
+        both = torch.randn(n, H, 3, D, device=gpu, generator=g).half()
+        q, k, v = both.unbind(2)
+    elif layout == "stacked":  # [3, n, H, D]
+        both = torch.randn(3, n, H, D, device=gpu, generator=g).half()
+        q, k, v = both.unbind(0)
+    else:  # [3 H, n, D]
+        both = torch.randn(3 * H, n, D, device=gpu, generator=g).half()
+        q, k, v = (t.transpose(0, 1) for t in both.split(H, 0))
+    rotary = Rotary(D, 100, interleaved=layout == "heads")
+    slots, pos = torch.arange(n, device=gpu), torch.arange(5, 5 + n, dtype=torch.int32, device=gpu)
+    apart, cache = (KvCache(5, H, D, fmt=fmt) for _ in range(2))
+    q0, k0, v0 = (t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
+    want = apart.append_rotated(k0, v0, slots, pos, rotary, q=q0)
+    for over in (k, v):
+        with pytest.raises(RuntimeError, match="overlaps k or v"):
+            cache.append_rotated(k, v, slots, pos, rotary, q=q0, q_out=over)
+    assert torch.equal(q, q0) and torch.equal(k, k0) and not cache.data.any()
+    assert cache.append_rotated(k, v, slots, pos, rotary, q=q, q_out=q) is q
+    assert torch.equal(q, want) and torch.equal(k, k0) and torch.equal(v, v0)
+    assert torch.equal(cache.data, apart.data)
+
+
 def test_a_run_of_them(gpu):
     """Steps of a small model's layer as a server makes them: fused projection, rotated append in place, attention, a head,
     log probabilities; against the same in 64 bits from what the cache gives back, and against the 8-bit cache's."""

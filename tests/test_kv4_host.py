@@ -70,6 +70,21 @@ def test_more_rows_than_a_launch_has_threads(L):
     assert L.nsmlp_kv_read(ctypes.byref(c), MEM, 1 << 24, MEM, MEM, 0, None) == EINVAL and b"2^27" in L.nsmlp_last_error()
 
 
+@pytest.mark.parametrize("kw", [
+    dict(q_out=MEM + 4096, k=MEM + 4096), dict(q_out=MEM + 4096, v=MEM + 4096),            # the same rows
+    dict(q_out=MEM + 4096, k=MEM + 4096 + 2 * (2 * 256 + 3 * 64)),                          # the last query row, the first of K
+    dict(q_out=MEM + 4096, v=MEM + 4096 - 2 * (2 * 128 + 64)),                              # the last row of V, the first query row
+    dict(q_out=MEM + 4096, o_row=512, k=MEM + 4096 + 2 * 192, k_row=512),                   # in every row of one projection
+    dict(q_out=MEM + 4096, o_row=512, k=MEM + 4096 + 2 * 512 * 2 - 2 * 64, k_row=512),      # K's rows begin before the queries'
+    dict(q_out=MEM + 4096, o_head=192, o_row=768, v=MEM + 4096 + 2 * 56, v_head=192, v_row=768),  # in every head's
+    dict(q_out=MEM + 4096, o_row=0, q_heads=1, k=MEM + 4096, k_row=0, n=1)])
+def test_queries_over_keys_or_values(L, kw):
+    """Other workgroups read K and V while rows of q_out are written."""
+    x = dict(q=MEM + 32768, k=MEM + 16384, v=MEM + 16384)
+    x.update(kw)
+    assert call(L, **x) == EINVAL and b"q_out overlaps k or v" in L.nsmlp_last_error(), L.nsmlp_last_error()
+
+
 def test_nothing_to_store(L):
     assert call(L, n=0, q=None) == 0 and call(L, n=0, positions=None, slots=None, k=None, v=None, q_out=None) == 0
     assert call(L, n=0, interleaved=5) == EINVAL
