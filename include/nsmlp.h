@@ -667,6 +667,7 @@ int nsmlp_kv_commit(const nsmlp_kv_batch* batch, const nsmlp_kv_step* step, cons
  * first kv_len - n + i + 1 keys:
  *   out = sum_j softmax_j(scale q . k_j) v_j     [total][q_heads][head_dim]
  *   lse = log sum_j exp(scale q . k_j)           [total][q_heads] fp32, nullable
+ * out may be q itself, of contiguous rows, and must not overlap it otherwise.
  * A token that sees no key (a refused request's) gets zeros and -inf; rows past
  * the step's tokens are left as they are.  A table entry that is not a block
  * (or past max_blocks) hides its keys and sets

@@ -380,7 +380,8 @@ def paged_attention(q: torch.Tensor, cache: KvCache, step: KvStep, *, scale: flo
     """Attention of a step's queries ``q`` [total, q_heads, head_dim] (fp16 or
     bf16) over the cache, causal at the end of each request (its new tokens'
     K and V are appended before the call).  ``scale`` defaults to
-    1/sqrt(head_dim).  Returns ``out`` [total, q_heads, head_dim]; ``lse``
+    1/sqrt(head_dim).  Returns ``out`` [total, q_heads, head_dim], contiguous,
+    which may be ``q`` itself and overlaps it in no other way; ``lse``
     ([total, q_heads] fp32) receives the log of the softmax sums.  ``ws``: a
     uint8 workspace of ``step.workspace_bytes(head_dim)`` that
     ``nsmlp_workspace_init`` has cleared, in place of the stream's own."""
@@ -402,6 +403,9 @@ def paged_attention(q: torch.Tensor, cache: KvCache, step: KvStep, *, scale: flo
     elif out.dtype != dtype or out.device != device or tuple(out.shape) != (total, heads, dim) or not out.is_contiguous() \
             or out.data_ptr() % 16:
         raise RuntimeError(f"out must be a contiguous, 16-byte aligned {dtype} tensor {(total, heads, dim)} on {device}")
+    elif total and _overlap(q, out) and not (out.data_ptr() == qp and q.is_contiguous()):
+        # (a row of q is read by the workgroups that write the same row of out, and by no others)
+        raise RuntimeError("out overlaps q: it must be q's own memory, both contiguous, or lie apart from it")
     if lse is not None and (lse.dtype != torch.float32 or lse.device != device or tuple(lse.shape) != (total, heads)
                             or not lse.is_contiguous()):
         raise RuntimeError(f"lse must be a contiguous fp32 tensor {(total, heads)} on {device}")

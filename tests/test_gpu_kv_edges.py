@@ -501,6 +501,41 @@ def test_a_value_that_is_not_finite_among_far_scores(gpu, fmt, which, value, Hq,
     assert off.all(-1)[~sees].all()
 
 
+@pytest.mark.parametrize("fmt", ["e2m1", "int8"])
+@pytest.mark.parametrize("Hq,H,D,cached,new", [(16, 2, 128, [9000, 40, 3], [1, 1, 1]), (8, 2, 64, [5000, 0, 17], [3, 1, 40]),
+                                               (256, 128, 64, [100], [520])])
+def test_outputs_over_queries(gpu, fmt, Hq, H, D, cached, new):
+    """In the queries' own memory: the same bits.  Anywhere else over them: refused, as other rows' queries would be lost."""
+    from next_step_ai_amd.kv_cache import KvBatch, KvCache, paged_attention
+
+    pool = sum(-(-(c + n) // 16) for c, n in zip(cached, new))
+    b = KvBatch(pool, 16, max_requests=len(new), max_blocks=pool, q_heads=Hq, kv_heads=H, head_dim=D)
+    c = KvCache(pool, H, D, fmt=fmt)
+    g = torch.Generator(device=gpu).manual_seed(5)
+    for lengths in (cached, new):
+        T = sum(lengths)
+        st = b.plan(ints(lengths, gpu), T, max_new=max(lengths))
+        k, v = (torch.randn(T, H, D, device=gpu, generator=g).half() for _ in range(2))
+        c.append(k, v, st.slots)
+        if lengths is cached:
+            b.commit()
+    wide = torch.randn(T + 1, Hq, D, device=gpu, generator=g).half()
+    q = wide[:T]
+    want = paged_attention(q, c, st)
+    for over in (wide[1:], wide.view(-1)[8: 8 + q.numel()].view_as(q)):
+        before = wide.clone()
+        with pytest.raises(RuntimeError, match="overlaps q"):
+            paged_attention(q, c, st, out=over)
+        assert torch.equal(wide, before)
+    fused = torch.randn(T, Hq + 2, D, device=gpu, generator=g).half()
+    if T > 1:
+        with pytest.raises(RuntimeError, match="overlaps q"):
+            paged_attention(fused[:, :Hq], c, st, out=fused.view(-1)[: q.numel()].view_as(q))
+    for _ in range(3):
+        mine = q.clone()
+        assert paged_attention(mine, c, st, out=mine) is mine and torch.equal(mine, want)
+
+
 @pytest.mark.parametrize("new", [1, 60])
 def test_scores_of_any_size_in_bf16(gpu, new):
     """The same with bf16 magnitudes of 2^40, whose scores pass 2^80."""
