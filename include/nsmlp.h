@@ -590,8 +590,8 @@ typedef struct nsmlp_rotary {
  * that what is stored is what nsmlp_kv_append stores of such rows.
  * positions[n]: a row of K whose position is not in the table becomes NaN.
  * q [n][q_heads][head_dim] (strides as k's; NULL: none) goes to q_out, which
- * may be q itself with the same strides and must not overlap it otherwise.  A
- * q_out that overlaps k or v is refused (slices of one projection do not).  A
+ * may be q itself with the same strides.  A q_out that overlaps q otherwise, k or
+ * v is refused (slices of one projection or buffer do not).  A
  * row whose position is negative (a token of no request) is left as it was in
  * q_out, one past the table becomes NaN.  k is not changed. */
 int nsmlp_kv_append_rotated(const nsmlp_kv_cache* cache, const nsmlp_rotary* rotary, const void* k, long long k_row_stride,

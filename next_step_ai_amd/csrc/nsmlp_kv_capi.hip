@@ -213,10 +213,14 @@ int nsmlp_kv_append_rotated(const nsmlp_kv_cache* cache, const nsmlp_rotary* rot
       return set_error(NSMLP_EINVAL, "q_heads %d of %d tokens: at least 1 and at most 2^28 heads' rows", q_heads, n);
     if ((rc = check_rows("q", q, q_row_stride, q_head_stride)) || (rc = check_rows("q_out", q_out, out_row_stride, out_head_stride)))
       return rc;
-    if (q == q_out && (q_row_stride != out_row_stride || q_head_stride != out_head_stride))
-      return set_error(NSMLP_EINVAL, "queries that are rotated in place keep their strides");
-    // (other workgroups of the launch read K and V)
     const RowSet out = {q_out, n, out_row_stride, q_heads, out_head_stride, a.c.D};
+    if (q == q_out) {
+      if (q_row_stride != out_row_stride || q_head_stride != out_head_stride)
+        return set_error(NSMLP_EINVAL, "queries that are rotated in place keep their strides");
+    } else if (rows_meet(out, RowSet{q, n, q_row_stride, q_heads, q_head_stride, a.c.D})) {
+      return set_error(NSMLP_EINVAL, "q_out overlaps q: it must be q itself or lie apart from it");
+    }
+    // (other workgroups of the launch read K and V)
     if (rows_meet(out, RowSet{k, n, k_row_stride, a.c.heads, k_head_stride, a.c.D}) ||
         rows_meet(out, RowSet{v, n, v_row_stride, a.c.heads, v_head_stride, a.c.D}))
       return set_error(NSMLP_EINVAL, "q_out overlaps k or v");

@@ -149,8 +149,8 @@ class KvCache:
         fp32 and to their type; ``k`` is not changed.  A position that is not in
         the table makes its rows NaN; a query row at a negative one (a token of no
         request) is left as it was in ``q_out`` (a new one holds anything there).
-        A ``q_out`` that overlaps ``k`` or ``v`` is refused; slices of one
-        projection do not."""
+        A ``q_out`` that overlaps ``q`` otherwise, ``k`` or ``v`` is refused; slices
+        of one projection or buffer do not."""
         if current_device() != self.device.index:
             with torch.cuda.device(self.device):
                 return self.append_rotated(k, v, slots, positions, rotary, q=q, q_out=q_out)
@@ -184,9 +184,6 @@ class KvCache:
             out, op, o_row, o_head = _rows(q_out, "q_out", heads, self.head_dim, self.device)
             if out is not q_out or _meets_itself(n, o_row, heads, o_head, self.head_dim):
                 raise RuntimeError("q_out must be 16-byte aligned with strides that are multiples of 8 elements, and no element twice")
-            same = op == qp and (q_row, q_head) == (o_row, o_head)
-            if n and not same and _overlap(rows, q_out):
-                raise RuntimeError("q_out overlaps q: it must be q itself or lie apart from it")
         _lib.call("nsmlp_kv_append_rotated", self._ref, rotary._ref, kp, k_row, k_head, vp, v_row, v_head, _DTYPES[k.dtype],
                   slots.data_ptr(), positions.data_ptr(), n, qp, q_row, q_head, heads, op, o_row, o_head,
                   stream_handle(self.device))

@@ -372,6 +372,29 @@ def test_queries_turned_next_to_keys_and_values(gpu, fmt, n, H, D, layout):
     assert torch.equal(cache.data, apart.data)
 
 
+@pytest.mark.parametrize("fmt", ["e2m1", "int8"])
+def test_queries_turned_into_the_other_half_of_their_buffer(gpu, fmt):
+    """Slices of one buffer that have no element in common, in rows, in heads and in dims."""
+    from next_step_ai_amd.kv_cache import KvCache
+    from next_step_ai_amd.rotary import Rotary
+
+    n, Hq, H, D = 19, 4, 2, 64
+    g = torch.Generator(device=gpu).manual_seed(2)
+    rotary = Rotary(D, 100)
+    slots, pos = torch.arange(n, device=gpu), torch.arange(n, dtype=torch.int32, device=gpu)
+    k, v = (torch.randn(n, H, D, device=gpu, generator=g).half() for _ in range(2))
+    q = torch.randn(n, Hq, D, device=gpu, generator=g).half()
+    cache = KvCache(2, H, D, fmt=fmt)
+    want = cache.append_rotated(k, v, slots, pos, rotary, q=q)
+    for shape, parts in (((n, 2 * Hq, D), lambda t: (t[:, :Hq], t[:, Hq:])), ((n, 2 * Hq, D), lambda t: (t[:, ::2], t[:, 1::2])),
+                         ((n, Hq, 2 * D), lambda t: (t[:, :, D:], t[:, :, :D])), ((2 * n, Hq, D), lambda t: (t[::2], t[1::2]))):
+        both = torch.full(shape, 7.0, dtype=torch.float16, device=gpu)
+        mine, out = parts(both)
+        mine.copy_(q)
+        assert cache.append_rotated(k, v, slots, pos, rotary, q=mine, q_out=out) is out
+        assert torch.equal(out, want) and torch.equal(mine, q)
+
+
 def test_a_run_of_them(gpu):
     """Steps of a small model's layer as a server makes them: fused projection, rotated append in place, attention, a head,
     log probabilities; against the same in 64 bits from what the cache gives back, and against the 8-bit cache's."""

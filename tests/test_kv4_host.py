@@ -85,6 +85,17 @@ def test_queries_over_keys_or_values(L, kw):
     assert call(L, **x) == EINVAL and b"q_out overlaps k or v" in L.nsmlp_last_error(), L.nsmlp_last_error()
 
 
+@pytest.mark.parametrize("kw", [
+    dict(q_out=MEM + 4096 + 16), dict(q_out=MEM + 4096 + 2 * 64), dict(q_out=MEM + 4096 - 2 * (2 * 256 + 3 * 64)),
+    dict(q_out=MEM + 4096 + 2 * 192, q_row=512, o_row=512), dict(q_out=MEM + 4096 + 2 * 56, q_head=128, o_head=128, q_row=512, o_row=512),
+    dict(q_out=MEM + 4096 + 2 * 56, q_row=0, q_head=0), dict(q_out=MEM + 4096 + 2 * 64, q_head=-64, o_row=256),
+    dict(q_out=MEM + 4096 + 2 * 320, q_row=512, o_row=520)])  # (strides without a period: as if they met)
+def test_queries_over_queries(L, kw):
+    x = dict(q=MEM + 4096, k=MEM + 16384, v=MEM + 16384)
+    x.update(kw)
+    assert call(L, **x) == EINVAL and b"q_out overlaps q:" in L.nsmlp_last_error(), L.nsmlp_last_error()
+
+
 def test_nothing_to_store(L):
     assert call(L, n=0, q=None) == 0 and call(L, n=0, positions=None, slots=None, k=None, v=None, q_out=None) == 0
     assert call(L, n=0, interleaved=5) == EINVAL
