@@ -507,10 +507,10 @@ Splits splits_of(int rows, int vocab, int size) {
   const int each = (steps + most - 1) / most;
   return Splits{(steps + each - 1) / each, each};
 }
-constexpr int kLpMaxRows = 1 << 24;
+constexpr int kLpMaxRows = (1 << 24) - 1;  // (a launch has fewer than 2^32 threads in a dimension)
 
 int check_shape(int rows, int vocab, int dtype, int top) {
-  if (rows < 0 || rows > kLpMaxRows) return set_error(NSMLP_EINVAL, "rows %d out of range [0, 2^24]", rows);
+  if (rows < 0 || rows > kLpMaxRows) return set_error(NSMLP_EINVAL, "rows %d out of range [0, 2^24 - 1]", rows);
   if (vocab < 1 || vocab > (1 << 30)) return set_error(NSMLP_EINVAL, "vocabulary %d out of range [1, 2^30]", vocab);
   if (dtype != NSMLP_DTYPE_F16 && dtype != NSMLP_DTYPE_BF16 && dtype != NSMLP_DTYPE_F32)
     return set_error(NSMLP_EINVAL, "unknown dtype %d", dtype);

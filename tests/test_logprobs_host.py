@@ -44,6 +44,15 @@ def test_refusals(L, kw, code, text):
     assert call(L, **kw) == code and text in L.nsmlp_last_error(), L.nsmlp_last_error()
 
 
+def test_more_rows_than_a_launch_has_threads(L):
+    """256 threads have a row: 2^24 rows would be 2^32 threads."""
+    assert call(L, rows=1 << 24) == EINVAL and b"rows" in L.nsmlp_last_error()
+    with_ws = L.nsmlp_token_logprobs_workspace_bytes
+    assert with_ws(1 << 24, 1000, 0, 3) == 0 and b"rows" in L.nsmlp_last_error()
+    # one fewer is taken as far as its other arguments go
+    assert call(L, rows=(1 << 24) - 1, logits=None) == EINVAL and b"logits" in L.nsmlp_last_error()
+
+
 def test_no_rows(L):
     assert call(L, rows=0) == 0 and call(L, rows=0, logits=None, ws=None, ws_bytes=0) == 0
 
