@@ -170,6 +170,13 @@ def lm_head_forward(hidden: torch.Tensor, meta: dict) -> torch.Tensor:
     return logits.view(*hidden.shape[:-1], V)
 
 
+def _check_sizes(rows: int, vocab: int, top: int) -> None:
+    """Before they become 32-bit numbers and outputs of their size are made."""
+    if rows >= 1 << 24 or not 1 <= vocab <= 1 << 30 or not 0 <= top <= min(vocab, 64):
+        raise RuntimeError(f"fewer than 2^24 rows, a vocabulary of 1 to 2^30 and a top of 0 to 64, at most the vocabulary: got {rows} rows "
+                           f"of {vocab} logits and top {top}")
+
+
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, top: int = 0,
                    ws: torch.Tensor | None = None) -> dict[str, torch.Tensor]:
     """What ``logits`` [..., V] (fp16, bf16 or fp32) say about ``tokens`` [...]
@@ -194,8 +201,6 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     z = logits if logits.dim() == 2 else logits.reshape(-1 if V else 0, V)
     rows = z.shape[0]
     key = (rows, V, dtype, int(top))
-    if not 0 <= key[3] <= V < 1 << 31 or rows >= 1 << 31:  # (before they become 32-bit numbers)
-        raise RuntimeError(f"top {top} must be in [0, 64] and at most the vocabulary: got {rows} rows of {V} logits")
     if V > 1 and z.stride(1) != 1:
         z = z.contiguous()
     if tokens is not None and (tokens.dtype != torch.int64 or tokens.device != device or tokens.shape != shape):
@@ -203,6 +208,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
                            f"{tokens.device}")
     need = _logprob_bytes.get(key)
     if need is None:
+        _check_sizes(rows, V, key[3])
         if len(_logprob_bytes) >= 1024:
             _logprob_bytes.clear()
         need = _logprob_bytes[key] = int(_lib.lib().nsmlp_token_logprobs_workspace_bytes(*key))

@@ -264,3 +264,17 @@ def test_in_a_graph(gpu):
             want = token_logprobs(z, tokens, top=5)
             stream.synchronize()
             assert all(torch.equal(out[k], want[k]) for k in want)
+
+
+def test_alternatives_refused_before_memory_is_taken(gpu):
+    """More of them than there may be: no outputs are made for them."""
+    from next_step_ai_amd.lm_head import token_logprobs
+
+    z = torch.zeros(200, 100000, dtype=torch.float16, device=gpu)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.max_memory_allocated()
+    for top in (65, 100000):
+        with pytest.raises(RuntimeError, match=f"top {top}"):
+            token_logprobs(z, top=top)
+    assert torch.cuda.max_memory_allocated() == before

@@ -79,3 +79,22 @@ def test_python_wants_a_gpu():
 
     with pytest.raises(RuntimeError, match="GPU"):
         token_logprobs(torch.zeros(2, 5))
+
+
+@pytest.mark.parametrize("rows,vocab,top,text", [
+    (1 << 24, 10, 1, "16777216 rows"), (1 << 31, 1, 0, "2147483648 rows"), ((1 << 32) + 1, 1, 0, "4294967297 rows"),
+    (1, (1 << 30) + 1, 0, "of 1073741825 logits"), (1, (1 << 32) + 5, 0, "of 4294967301 logits"), (2, 0, 0, "of 0 logits"),
+    (1, 1000, 65, "top 65"), (1, 10, 11, "top 11"), (1, 100, -1, "top -1"), (1, 100, 1 << 32, "top 4294967296")])
+def test_sizes_refused_before_anything_is_made(rows, vocab, top, text):
+    """Each by what is wrong with it."""
+    from next_step_ai_amd.lm_head import _check_sizes
+
+    with pytest.raises(RuntimeError, match=text):
+        _check_sizes(rows, vocab, top)
+
+
+def test_sizes_taken():
+    from next_step_ai_amd.lm_head import _check_sizes
+
+    for sizes in ((0, 5, 5), ((1 << 24) - 1, 1 << 30, 64), (1, 1, 1), (3, 64, 64), (3, 1000, 0)):
+        _check_sizes(*sizes)
