@@ -201,17 +201,17 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     z = logits if logits.dim() == 2 else logits.reshape(-1 if V else 0, V)
     rows = z.shape[0]
     key = (rows, V, dtype, int(top))
-    if V > 1 and z.stride(1) != 1:
-        z = z.contiguous()
-    if tokens is not None and (tokens.dtype != torch.int64 or tokens.device != device or tokens.shape != shape):
-        raise RuntimeError(f"tokens must be an int64 {tuple(shape)} tensor on {device}, got {tuple(tokens.shape)} {tokens.dtype} on "
-                           f"{tokens.device}")
     need = _logprob_bytes.get(key)
     if need is None:
         _check_sizes(rows, V, key[3])
         if len(_logprob_bytes) >= 1024:
             _logprob_bytes.clear()
         need = _logprob_bytes[key] = int(_lib.lib().nsmlp_token_logprobs_workspace_bytes(*key))
+    if V > 1 and z.stride(1) != 1:
+        z = z.contiguous()
+    if tokens is not None and (tokens.dtype != torch.int64 or tokens.device != device or tokens.shape != shape):
+        raise RuntimeError(f"tokens must be an int64 {tuple(shape)} tensor on {device}, got {tuple(tokens.shape)} {tokens.dtype} on "
+                           f"{tokens.device}")
     n = key[3]
     # one buffer for what is fp32: a split into views takes as long as one tensor made anew
     sizes = [rows, 0 if tokens is None else rows, rows * n]

@@ -277,4 +277,7 @@ def test_alternatives_refused_before_memory_is_taken(gpu):
     for top in (65, 100000):
         with pytest.raises(RuntimeError, match=f"top {top}"):
             token_logprobs(z, top=top)
+    # nor is a row of one broadcast logit written out
+    with pytest.raises(RuntimeError, match="logits"):
+        token_logprobs(z[:1, :1].expand(1, (1 << 30) + 1))
     assert torch.cuda.max_memory_allocated() == before
