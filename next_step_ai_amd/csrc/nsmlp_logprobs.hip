@@ -493,8 +493,10 @@ __global__ void __launch_bounds__(kLpThreads, 5) k_token_logprobs(LogprobArgs a)
   write_row<T>(a, row, logits, p, bufs[0], lane);
 }
 
-// Workgroups of a row: about kLpTarget in all, four a CU, none with less than a batch
-// of vectors per wave.  With 512, 1024 and 2048, 5 alternatives of 300 rows of 128256
+// Workgroups of a row: about kLpTarget in all, four a CU, with whole batches of vectors
+// for every wave (but the row's last: what a batch has past its workgroup's share is
+// read and weighed all the same; 5 alternatives of 150 rows of 128256 in bf16 19 us, in
+// even shares 24, of 900 rows of 10000 in fp16 19.1 and 19.7).  With 512, 1024 and 2048, 5 alternatives of 300 rows of 128256
 // in bf16 take 30, 27 and 32 us, of 700 rows 46.5, 48.4 and 50.3, of 256 rows of 32000
 // 11.7, 12.0 and 11.9; fewer rows have their most in all three.
 constexpr int kLpTarget = 1024;
@@ -504,7 +506,7 @@ struct Splits {
 Splits splits_of(int rows, int vocab, int size) {
   const int steps = (int)(((long long)vocab * size + 16 * kWave - 1) / (16 * kWave)), least = kLpWaves * kLpBatch;
   const int most = std::max(1, std::min({(steps + least - 1) / least, (kLpTarget + rows - 1) / rows, kLpMaxSplits}));
-  const int each = (steps + most - 1) / most;
+  const int each = ((steps + most - 1) / most + least - 1) / least * least;
   return Splits{(steps + each - 1) / each, each};
 }
 constexpr int kLpMaxRows = (1 << 24) - 1;  // (a launch has fewer than 2^32 threads in a dimension)

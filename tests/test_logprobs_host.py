@@ -65,6 +65,19 @@ def test_sizes(L):
     assert size(1, 128256, 0, 65) == 0 and size(1, 10, 0, 11) == 0 and size(1, 128256, 7, 1) == 0
 
 
+@pytest.mark.parametrize("vocab", [5000, 10000, 16000, 20001, 32000, 50257, 100003, 128256, 262144])
+@pytest.mark.parametrize("dtype,size", [(0, 2), (1, 2), (2, 4)])
+def test_shares_of_whole_batches(L, vocab, dtype, size):
+    """The workgroups of a row (16 + 8 top bytes of workspace for each) have 16 steps of 64 vectors, or a multiple."""
+    bytes_of = L.nsmlp_token_logprobs_workspace_bytes
+    steps = -(-vocab * size // 1024)
+    for rows in (1, 2, 7, 61, 100, 205, 230, 256, 300, 511, 700, 1023, 1024, 5000):
+        more = bytes_of(rows, vocab, dtype, 1) - bytes_of(rows, vocab, dtype, 0)
+        shares = max(1, more // (8 * rows))
+        assert shares == 1 or rows * shares < 1024 + rows
+        assert shares <= 32 and any(-(-steps // each) == shares for each in range(16, steps + 17, 16)), (rows, shares)
+
+
 @pytest.mark.parametrize("kind,code", [("hip", EIO), ("nospc", ENOSPC), ("nodev", ENODEV)])
 def test_fault_point(L, kind, code):
     from next_step_ai_amd import _lib
