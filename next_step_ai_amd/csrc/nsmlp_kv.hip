@@ -673,13 +673,22 @@ void append_typed(KvAppendArgs a, hipStream_t s) {
   // are then one wave's, one after the other.  With 1, 8 and 16 tokens per wave,
   // 8 heads: prompts of 4096 tokens (65536 pairs) 32.6, 10.5, 9.6 us, of 8192 62.5,
   // 17.0, 13.9; single tokens, 1024 of them 16.0, 17.7, 28.2 us, 2048 29.0, 23.0, 32.1,
-  // 4096 53.9, 41.1, 41.7; 290 next to 7000 of prompts 46.9, 18.3, 30.2.  In between,
-  // with 1, 2 and 4, without and with a rotation (blocks of 64, heads of 64): 256
-  // single tokens 5.9, 6.8, 9.4 and 7.7, 8.1, 10.8; 512 9.6, 9.0, 10.9 and 12.7, 12.3,
-  // 12.9; 1024 16.9, 15.3, 14.8 and 22.7, 20.3, 20.9; a prompt of 1024 9.4, 7.9, 7.5 and
-  // 14.5, 12.1, 10.9; 21 next to 1858 of prompts 12.5, 9.2, 9.5 and 18.6, 13.1, 12.0.
+  // 4096 53.9, 41.1, 41.7; 290 next to 7000 of prompts 46.9, 18.3, 30.2.  In between
+  // with 1, 2 and 4, without and with a rotation.  16384 pairs of 8 heads of 128 in
+  // blocks of 16: single tokens 15.7, 13.6, 12.9 and 18.1, 16.7, 16.1 us; a prompt of
+  // 1024 11.6, 9.4, 6.1 and 18.7, 15.7, 9.6; 64 next to 960 of prompts 10.4, 7.6, 8.3 and
+  // 15.7, 10.4, 10.2.  8192: 8.8, 7.9, 9.9 and 10.6, 9.6, 11.7; 7.4, 5.8, 4.9 and 11.5,
+  // 9.2, 6.9; 7.1, 5.5, 8.2 and 9.5, 6.9, 10.0.  A wave's tokens are more of a call's
+  // chain where they are few: 512 tokens of 16 heads of 64, 32 of them single ones, 6.7,
+  // 5.4, 7.4; 256 of 32 heads, 16 of them, 6.4, 5.4, 7.5; a prompt of 128 of 32 heads of
+  // 128 in blocks of 64 with a rotation 14.4, 16.3, 16.1.  (Heads of 64 and 128, blocks of
+  // 16 to 64, 2 to 64 of them, int8 and e4m3: none slower than with 1 by more than 4%.)
   const long long pairs = (long long)a.n * a.c.heads * 2;
-  a.take = pairs >= 128 * 1024 ? 16 : pairs >= 32 * 1024 ? 8 : pairs >= 16 * 1024 ? 4 : pairs >= 8 * 1024 ? 2 : 1;
+  a.take = pairs >= 128 * 1024                  ? 16
+           : pairs >= 32 * 1024                 ? 8
+           : pairs >= 16 * 1024 && a.n >= 1024 ? 4
+           : pairs >= 8 * 1024 && a.n >= 256   ? 2
+                                               : 1;
   const long long waves = (long long)((a.n + a.take - 1) / a.take) * a.c.heads * 2, per = kAppendThreads / kWave;
   a.rot.first = (unsigned)((waves + per - 1) / per);
   if (a.rot.table == nullptr) {

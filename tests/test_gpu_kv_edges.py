@@ -655,6 +655,51 @@ def test_append_of_many_tokens(gpu, fmt, block, D, lengths):
         assert torch.equal(whole.data, single.data) and torch.equal(whole.scale, single.scale)
 
 
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("H,block,D,lengths", [
+    (32, 64, 64, [128]), (64, 16, 128, [1] * 100),                         # 1 token a wave, as tokens are few
+    (16, 64, 64, [1] * 20 + [130, 107]), (32, 16, 128, [1] * 30 + [240]),  # 2
+    (8, 32, 64, [1] * 70 + [300, 300, 355]), (4, 64, 128, [1] * 2049), (8, 16, 128, [1100]),  # 4
+])
+def test_append_of_some_tokens(gpu, fmt, H, block, D, lengths):
+    """Calls between a few tokens and many, whose waves look at one to four: what the same rows store request by request,
+    with a rotation too."""
+    from next_step_ai_amd.kv_cache import KvBatch, KvCache
+    from next_step_ai_amd.rotary import Rotary
+
+    R = len(lengths)
+    cached = [(7 * r) % 40 for r in range(R)]
+    need = [-(-(a + b) // block) for a, b in zip(cached, lengths)]
+    pool = sum(need)
+    rotary = Rotary(D, 1200)
+    g = torch.Generator(device=gpu).manual_seed(11)
+    b = KvBatch(pool, block, max_requests=R, max_blocks=max(need), q_heads=H, kv_heads=H, head_dim=D,
+                free_blocks=torch.randperm(pool, generator=torch.Generator().manual_seed(1)))
+    whole, single, turned, turned1 = (KvCache(pool, H, D, block_tokens=block, fmt=fmt) for _ in range(4))
+    for new in (cached, lengths):
+        if sum(new) == 0:
+            continue
+        st = b.plan(ints(new, gpu), sum(new))
+        st.check()
+        k, v = ((torch.randn(sum(new), H, D, device=gpu, generator=g) * torch.randn(sum(new), 1, 1, device=gpu, generator=g).exp2())
+                .bfloat16() for _ in range(2))
+        whole.append(k, v, st.slots)
+        turned.append_rotated(k, v, st.slots, st.positions, rotary)
+        at = 0
+        for m in new:
+            first = at
+            while first < at + m:  # whole blocks at a time, few tokens in a call
+                last = min(at + m, first + 64 - int(st.slots[first]) % block)
+                part = slice(first, last)
+                single.append(k[part], v[part], st.slots[part])
+                turned1.append_rotated(k[part], v[part], st.slots[part], st.positions[part], rotary)
+                first = last
+            at += m
+        b.commit()
+        for x, y in ((whole, single), (turned, turned1)):
+            assert torch.equal(x.data, y.data) and torch.equal(x.scale, y.scale)
+
+
 @pytest.mark.parametrize("fmt,Hq,H,D", [("e4m3", 32, 8, 128), ("int8", 16, 1, 64)])
 def test_weights_of_single_tokens_are_not_rounded_in_bf16(gpu, fmt, Hq, H, D):
     """Streamed rows are the bf16 roundings of numbers within 2^-14 of the weights (fp32 scores up to 64 and sums) of the
