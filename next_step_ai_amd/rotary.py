@@ -4,7 +4,9 @@ The frequencies are base^(-2 i / head_dim), i < head_dim / 2, or the caller's;
 ``scaling`` stretches them as a model's configuration says ("linear": all by
 ``factor``; "llama3": waves longer than original_max_position_embeddings /
 low_freq_factor by ``factor``, those shorter than it over high_freq_factor not
-at all, those between by a share of it).  The reference leaves the encoding to
+at all, those between by a share of it).  Whole heads are turned.  Scalings that
+multiply cos and sin by a factor take their own frequencies and, as q and k have
+the factor each, its square times the softmax scale.  The reference leaves the encoding to
 its model library (RT:5927-7142 call it with precomputed cos and sin).
 """
 from __future__ import annotations
@@ -27,11 +29,17 @@ def rotary_frequencies(head_dim: int, base: float = 10000.0, scaling: dict | Non
     f = float(base) ** -(torch.arange(0, head_dim, 2, dtype=torch.float64) / head_dim)
     if scaling is None:
         return f
+    # (what a configuration may say next to the scaling: left out, it would turn all rows by wrong angles)
+    if scaling.get("partial_rotary_factor") not in (None, 1):
+        raise RuntimeError(f"partial_rotary_factor {scaling['partial_rotary_factor']}: a part of a head's dims is not offered")
+    if scaling.get("rope_theta") not in (None, base):
+        raise RuntimeError(f"the scaling's rope_theta {scaling['rope_theta']} is not the base {base}")
     kind = scaling.get("rope_type", scaling.get("type"))
     if kind in (None, "default"):
         return f
     if kind not in ("linear", "llama3"):
-        raise RuntimeError(f"scaling of type {kind!r} is not offered: give the frequencies instead")
+        raise RuntimeError(f"scaling of type {kind!r} is not offered: give its frequencies instead, and where it multiplies cos and "
+                           "sin by a factor, the attention a softmax scale times that factor's square")
     need = ["factor"] if kind == "linear" else ["factor", "low_freq_factor", "high_freq_factor", "original_max_position_embeddings"]
     missing = [k for k in need if k not in scaling]
     if missing:

@@ -147,6 +147,23 @@ def test_frequencies_refused(kw):
         rotary_frequencies(128, **kw)
 
 
+def test_configurations_with_more_than_a_scaling():
+    """What stands next to it in a model's configuration is checked: other angles than asked for come out of neither."""
+    from next_step_ai_amd.rotary import rotary_frequencies
+
+    plain = rotary_frequencies(64, 500000.0)
+    for kind in ("default", None):
+        same = {"rope_type": kind, "rope_theta": 500000, "partial_rotary_factor": 1.0}
+        assert torch.equal(rotary_frequencies(64, 500000.0, same), plain)
+    for other, text in (({"rope_theta": 10000.0}, "rope_theta"), ({"partial_rotary_factor": 0.5}, "part of a head")):
+        for kind in ({"rope_type": "default"}, {"rope_type": "linear", "factor": 2.0}):
+            with pytest.raises(RuntimeError, match=text):
+                rotary_frequencies(64, 500000.0, {**kind, **other})
+    # a factor on cos and sin, which frequencies do not hold, is named
+    with pytest.raises(RuntimeError, match="square"):
+        rotary_frequencies(64, 500000.0, {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 4096})
+
+
 def test_rotary_refusals():
     from next_step_ai_amd.rotary import Rotary
 
