@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from oracle import kv_reference as ref
+from test_gpu_kv_edges import rows_against_formula
 from test_gpu_paged_attention import Served
 
 pytestmark = pytest.mark.gpu
@@ -239,6 +240,73 @@ def test_bf16_of_far_exponents(gpu):
         assert out.isfinite().all()
         # (scores of 2^40: which of two close ones is larger is fp32's to say; there the row is a mix of values all the same)
         assert q_size > 1 or within(out, want, spread, 200 + new)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D,block", [(128, 16), (128, 64), (64, 32)])
+def test_tiles_of_256_rows(gpu, dtype, D, block):
+    """What long prompts run (128 K/V heads: from 1024 rows a head on, 8 waves a workgroup): a chunk with more than 64 blocks
+    of 16 tokens behind it, next to a draft, single tokens and a request that waits; with and without log sums, the same
+    bits. The bound is the output's rounding, the weights' to fp16 (2^-11 each, 2^-25 of the largest value where one is
+    subnormal) and fp32 scores."""
+    from next_step_ai_amd.kv_cache import KvBatch, KvCache, paged_attention
+
+    Hq, H, cached, new = 256, 128, [1500, 700, 0, 40, 0], [520, 1, 0, 6, 1]
+    pool = sum(-(-(c + n) // block) for c, n in zip(cached, new)) + 2
+    b = KvBatch(pool, block, max_requests=5, max_blocks=pool, q_heads=Hq, kv_heads=H, head_dim=D,
+                free_blocks=torch.randperm(pool, generator=torch.Generator().manual_seed(1)))
+    c = KvCache(pool, H, D, block_tokens=block, fmt="e2m1")
+    g = torch.Generator(device=gpu).manual_seed(D + block)
+    for lengths in (cached, new):
+        T = sum(lengths)
+        st = b.plan(ints(lengths, gpu), T, max_new=max(lengths))
+        k, v = ((torch.randn(T, H, D, device=gpu, generator=g) * torch.randn(T, H, 1, device=gpu, generator=g).exp2()).to(dtype)
+                for _ in range(2))
+        c.append(k, v, st.slots)
+        if lengths is cached:
+            b.commit()
+    assert T * 2 // 256 * H >= 512
+    q = (torch.randn(T, Hq, D, device=gpu, generator=g) * 1.5).to(dtype)
+    lse = torch.full((T, Hq), 7.0, device=gpu)
+    out = paged_attention(q, c, st, lse=lse)
+    assert torch.equal(paged_attention(q, c, st), out)
+    starts, u = st.q_start.tolist(), 2.0 ** -11 if dtype == torch.float16 else 2.0 ** -8
+    for r, (have, n) in enumerate(zip(cached, new)):
+        if n == 0:
+            continue
+        at, rows = torch.arange(have + n, device=gpu), slice(starts[r], starts[r + 1])
+        got = c.read(st.table[r][at // block].long() * block + at % block)  # (every value is an fp16 number)
+        rows_against_formula(q[rows], got["k"], got["v"], out[rows], have, u, 2)
+        hidden = at[None] > have + torch.arange(n, device=gpu)[:, None]
+        for h in range(0, Hq, 15):
+            e = (q[rows, h].double() @ got["k"][:, h // 2].double().t().contiguous() * D ** -0.5).masked_fill(hidden, -math.inf)
+            want = torch.logsumexp(e, 1)
+            assert ((lse[rows, h].double() - want).abs() <= 2.0 ** -14 + 2.0 ** -20 * want.abs()).all(), (r, h)
+
+
+@pytest.mark.parametrize("size", [2.0 ** 60, 2.0 ** 100])
+@pytest.mark.parametrize("Hq,H,D,block,cached,new", [(4, 2, 128, 16, 300, 1), (4, 2, 64, 16, 200, 6), (4, 2, 128, 32, 200, 60),
+                                                     (256, 128, 64, 16, 100, 520), (256, 128, 128, 16, 100, 520)])
+def test_bf16_queries_far_above_their_keys(gpu, size, Hq, H, D, block, cached, new):
+    """Queries of 2^60 and 2^100 along a key each: that key's value, which 4 bits and a power of two make exact."""
+    from next_step_ai_amd.kv_cache import KvBatch, KvCache, paged_attention
+
+    n = cached + new
+    pool = n // block + 1
+    b = KvBatch(pool, block, max_requests=1, max_blocks=pool, q_heads=Hq, kv_heads=H, head_dim=D)
+    c = KvCache(pool, H, D, block_tokens=block, fmt="e2m1")
+    g = torch.Generator(device=gpu).manual_seed(6)
+    k = (torch.randint(0, 2, (n, H, D), device=gpu, generator=g) * 2 - 1).bfloat16()
+    v = torch.randn(n, H, D, device=gpu, generator=g).bfloat16()
+    st = b.plan(ints([cached], gpu), cached)
+    c.append(k[:cached], v[:cached], st.slots)
+    b.commit()
+    st = b.plan(ints([new], gpu), new, max_new=new)
+    c.append(k[cached:], v[cached:], st.slots)
+    ask = (7 * torch.arange(new, device=gpu)) % (cached + 1 + torch.arange(new, device=gpu))
+    out = paged_attention((k[ask].float() * size).bfloat16().repeat_interleave(Hq // H, 1), c, st)
+    slots = st.table[0][ask // block].long() * block + ask % block
+    assert torch.equal(out, c.read(slots, torch.bfloat16)["v"].repeat_interleave(Hq // H, 1))
 
 
 def test_streams(gpu):

@@ -281,3 +281,21 @@ def test_alternatives_refused_before_memory_is_taken(gpu):
     with pytest.raises(RuntimeError, match="logits"):
         token_logprobs(z[:1, :1].expand(1, (1 << 30) + 1))
     assert torch.cuda.max_memory_allocated() == before
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [3, 300, 70000])
+@pytest.mark.parametrize("top", [0, 3, 64])
+def test_rows_of_nothing_but_minus_infinity(gpu, dtype, vocab, top):
+    """Log probabilities of -inf, an entropy of 0, alternatives by index; and one logit among them has all of the row."""
+    from next_step_ai_amd.lm_head import token_logprobs
+
+    top = min(top, vocab)
+    z = torch.full((4, vocab), -math.inf, dtype=dtype, device=gpu)
+    z[1, vocab - 1] = z[3, 0] = -3.0
+    tokens = torch.tensor([vocab - 1, vocab - 1, 0, vocab - 1], device=gpu)
+    got = {k: v.cpu() for k, v in token_logprobs(z, tokens, top=top).items()}
+    assert got["logprob"].tolist() == [-math.inf, 0.0, -math.inf, -math.inf] and got["entropy"].tolist() == [0.0] * 4
+    for r, order in enumerate(([*range(vocab)], [vocab - 1, *range(vocab - 1)], [*range(vocab)], [*range(vocab)])):
+        assert got["top_ids"][r].tolist() == order[:top]
+        assert got["top_logprobs"][r].tolist() == ([0.0 if r % 2 else -math.inf] + [-math.inf] * (top - 1))[:top]
