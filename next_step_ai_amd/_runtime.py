@@ -34,10 +34,10 @@ def stream_handle(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if idx is None else idx)
 
 
-def current_device() -> int:
-    """The current device's index.  A kernel is launched for the current device:
-    calls for tensors of another one make it current first."""
-    return torch._C._cuda_getDevice()
+# The current device's index.  A kernel is launched for the current device: calls for
+# tensors of another one make it current first.  (torch's own accessor without a frame
+# around it: each call asks.)
+current_device = torch._C._cuda_getDevice
 
 
 def require_device(t: torch.Tensor, what: str = "input") -> torch.device:

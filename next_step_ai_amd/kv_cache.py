@@ -104,6 +104,7 @@ class KvCache:
         if num_blocks < 1 or kv_heads < 1:
             raise RuntimeError(f"num_blocks and kv_heads must be at least 1, got {num_blocks} and {kv_heads}")
         self.device = _device(device)
+        self._index = self.device.index
         self.num_blocks, self.kv_heads, self.head_dim = int(num_blocks), int(kv_heads), int(head_dim)
         self.block_tokens, self.fmt = int(block_tokens), fmt
         if fmt == "e2m1":
@@ -124,7 +125,7 @@ class KvCache:
         (a plan's: a block's tokens stand next to each other, in order, none
         twice; a slot of -1 stores nothing).  Where the new rows exceed a block's
         scale in 8 bits its stored codes are rewritten under the larger one."""
-        if current_device() != self.device.index:
+        if current_device() != self._index:
             with torch.cuda.device(self.device):
                 return self.append(k, v, slots)
         k, kp, k_row, k_head = _rows(k, "k", self.kv_heads, self.head_dim, self.device)
@@ -151,7 +152,7 @@ class KvCache:
         request) is left as it was in ``q_out`` (a new one holds anything there).
         A ``q_out`` that overlaps ``q`` otherwise, ``k`` or ``v`` is refused; slices
         of one projection or buffer do not."""
-        if current_device() != self.device.index:
+        if current_device() != self._index:
             with torch.cuda.device(self.device):
                 return self.append_rotated(k, v, slots, positions, rotary, q=q, q_out=q_out)
         k, kp, k_row, k_head = _rows(k, "k", self.kv_heads, self.head_dim, self.device)
@@ -192,7 +193,7 @@ class KvCache:
     def read(self, slots: torch.Tensor, dtype: torch.dtype = torch.float16) -> dict[str, torch.Tensor]:
         """The stored rows at ``slots``: ``{"k": ..., "v": ...}`` of [tokens,
         kv_heads, head_dim] in ``dtype``; zeros for a slot of -1."""
-        if current_device() != self.device.index:
+        if current_device() != self._index:
             with torch.cuda.device(self.device):
                 return self.read(slots, dtype)
         if dtype not in _DTYPES:
@@ -210,7 +211,7 @@ class KvCache:
 class _StepLayout:
     """Sizes of a step's buffers, which depend on its total and max_new alone."""
 
-    __slots__ = ("ints", "sizes", "schedule_bytes", "ws_bytes")
+    __slots__ = ("ints", "positions_at", "sizes", "offsets", "schedule_bytes", "ws_bytes")
 
     def __init__(self, batch: "KvBatch", total: int, max_new: int):
         self.schedule_bytes = int(_lib.lib().nsmlp_kv_schedule_bytes(batch._ref, total, max_new))
@@ -218,7 +219,9 @@ class _StepLayout:
             raise RuntimeError(f"nsmlp_kv_schedule_bytes: {_lib.last_error()}")
         R = batch.requests
         self.ints = (3 * R + 5 + 3) // 4 * 4
-        self.sizes = [R + 1, R, R, 4, self.ints - 3 * R - 5 + self.schedule_bytes // 4, total]
+        self.positions_at = self.ints + self.schedule_bytes // 4
+        self.sizes = [R + 1, R, R, 4, self.positions_at - 3 * R - 5 + total]
+        self.offsets = tuple(4 * i for i in (R + 1, 2 * R + 1, 3 * R + 1, self.ints, self.positions_at))
         self.ws_bytes: dict[int, int] = {}
 
 
@@ -230,20 +233,20 @@ class KvStep:
     block table.  ``info`` and the others are device tensors: reading them
     waits for the stream.  ``planned``: whether a plan has written them."""
 
-    __slots__ = ("batch", "total", "max_new", "slots", "planned", "_buf", "_layout", "_view", "_ref", "_split")
+    __slots__ = ("batch", "total", "max_new", "slots", "planned", "_buf", "_layout", "_view", "_ref", "_split", "_positions")
 
     def __init__(self, batch: "KvBatch", total: int, max_new: int):
         lay = batch._layout(total, max_new)
         self.batch, self.total, self.max_new, self._layout = batch, total, max_new, lay
         self.slots = batch._slot.new_empty(total)  # (1.2 us; torch.empty with a dtype and a device takes 1.7)
         # q_start, kv_len, next and info, then the schedule at the next 16 bytes, then positions
-        self._buf = batch.state.new_empty(lay.ints + lay.schedule_bytes // 4 + total)
-        base, R = self._buf.data_ptr(), batch.requests
-        self._view = _lib.KvStepView(total, max_new, self.slots.data_ptr(), base, base + 4 * (R + 1), base + 4 * (2 * R + 1),
-                                     base + 4 * (3 * R + 1), base + 4 * lay.ints, lay.schedule_bytes,
-                                     base + 4 * lay.ints + lay.schedule_bytes)
+        self._buf = batch.state.new_empty(lay.positions_at + total)
+        base = self._buf.data_ptr()
+        kv_len, following, info, schedule, positions = lay.offsets
+        self._view = _lib.KvStepView(total, max_new, self.slots.data_ptr(), base, base + kv_len, base + following, base + info,
+                                     base + schedule, lay.schedule_bytes, base + positions)
         self._ref = ctypes.byref(self._view)
-        self._split = None
+        self._split = self._positions = None
         self.planned = False
 
     def _part(self, i: int) -> torch.Tensor:
@@ -265,7 +268,9 @@ class KvStep:
 
     @property
     def positions(self) -> torch.Tensor:
-        return self._part(5)
+        if self._positions is None:  # (a view of its own: steps without a rotation do not make it)
+            self._positions = self._buf[self._layout.positions_at:]
+        return self._positions
 
     @property
     def table(self) -> torch.Tensor:
@@ -298,6 +303,7 @@ class KvBatch:
                  head_dim: int = 128, free_blocks: torch.Tensor | None = None, device=None):
         """``free_blocks``: the ids to hand out, in this order (default all, ascending)."""
         self.device = _device(device)
+        self._index = self.device.index
         self.requests, self.max_blocks, self.num_blocks = int(max_requests), int(max_blocks), int(num_blocks)
         self.block_tokens, self.q_heads, self.kv_heads, self.head_dim = int(block_tokens), int(q_heads), int(kv_heads), \
             int(head_dim)
@@ -341,7 +347,7 @@ class KvBatch:
         again (with other ``new_tokens``, requests after the first whose need
         of blocks changes get other ones).  ``step``: an earlier step of the same ``total`` and ``max_new``
         whose buffers are written again (a captured graph's)."""
-        if current_device() != self.device.index:
+        if current_device() != self._index:
             with torch.cuda.device(self.device):
                 return self.plan(new_tokens, total, max_new=max_new, step=step)
         total, max_new = int(total), int(max_new)
@@ -360,7 +366,7 @@ class KvBatch:
     def commit(self, finished: torch.Tensor | None = None) -> None:
         """Make the last plan's lengths (all of its new tokens) the batch's, and end the requests with
         ``finished`` [requests] (int32, not 0): their blocks become free."""
-        if current_device() != self.device.index:
+        if current_device() != self._index:
             with torch.cuda.device(self.device):
                 return self.commit(finished)
         if finished is not None and (finished.dtype != torch.int32 or finished.device != self.device
@@ -385,7 +391,7 @@ def paged_attention(q: torch.Tensor, cache: KvCache, step: KvStep, *, scale: flo
     b, device, dim = step.batch, cache.device, cache.head_dim
     if b.device != device:
         raise RuntimeError(f"the cache is on {device} and the batch on {b.device}")
-    if current_device() != device.index:
+    if current_device() != cache._index:
         with torch.cuda.device(device):
             return paged_attention(q, cache, step, scale=scale, out=out, lse=lse, ws=ws)
     if not step.planned:  # its lists are what the memory held

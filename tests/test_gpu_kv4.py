@@ -223,6 +223,18 @@ def test_positions_of_a_plan(gpu):
     assert batch.plan(ints([0] * 4), 0).positions.numel() == 0
 
 
+def test_positions_are_a_view_of_their_own(gpu):
+    """Looking at a step's other outputs makes no view for them, as steps without a rotation have no use for one."""
+    from next_step_ai_amd.kv_cache import KvBatch
+
+    batch = KvBatch(10, 16, max_requests=2, max_blocks=3, q_heads=4, kv_heads=4)
+    step = batch.plan(torch.tensor([3, 4], dtype=torch.int32, device=gpu), 7)
+    assert step.q_start.tolist() == [0, 3, 7] and step.kv_len.tolist() == [3, 4] and step.info.tolist()[2:] == [0, 7]
+    assert len(step._split) == 5 and step._positions is None
+    assert step.positions is step.positions and step.positions.tolist() == [0, 1, 2, 0, 1, 2, 3]
+    assert step.positions.data_ptr() == step._view.positions
+
+
 def test_refusals(gpu):
     from next_step_ai_amd.kv_cache import KvCache
     from next_step_ai_amd.rotary import Rotary
