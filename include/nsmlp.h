@@ -455,7 +455,8 @@ int nsmlp_dense_linear_nf4_f16(const nsmlp_nf4_matrix* w, const void* x, int row
  *   top_ids, top_logprobs [rows][top]: the `top` (at most 64) largest logits'
  *   indices, largest first, the lower index first among equals (-0 equals +0),
  *   and their log p.
- * rows is at most 2^24 - 1 and vocab 2^30.  fp32 sums.  A logit of -inf has p =
+ * rows is at most 2^24 - 1 and vocab 2^30.  fp32 sums, whose order, and with it a
+ * number's last bits, depends on rows and vocab.  A logit of -inf has p =
  * 0; where a row has nothing else, its log probabilities are -inf and its entropy is 0.  A NaN or +inf in a row makes all
  * its numbers NaN; a NaN is below every number in the order of top_ids.  A token
  * outside [0, vocab), such as -1 for a row without one, gives NaN.  No

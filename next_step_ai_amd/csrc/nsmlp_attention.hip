@@ -609,9 +609,10 @@ __device__ __forceinline__ void stream_share(const KvAttnArgs& a, int block, Str
 // next one's first is fetched, its pages and queries before.
 //
 // What bounds it: the codes' way from HBM, and about 2.8 us at a unit's end, where
-// its waves meet.  64 uneven requests (228 MB) 58 us, 5.2 TB/s beyond the 7 us of
+// its waves meet.  64 uneven requests (228 MB) 57.5 us, 4.5 TB/s beyond the 7 us of
 // the chain above (66 us with a pause between units); one token over 131000 keys
-// (143 MB) 37 us, 777 keys 10 us.  Vector instructions are issued in 56% of the
+// (143 MB) 38 us, 777 keys 10 us; 12 requests of 5 drafts over 29166 keys, 24 heads on 8
+// of 128 (32 MB) 22 us, of 64 17.5.  Vector instructions are issued in 56% of the
 // cycles (decoding and the weights), the matrix cores are busy in 17%.
 struct StreamUnit {  // a unit and its request's rows and keys
   int req, kv_begin, kv_end, part, first, parts, q0, q_len, kv_len;

@@ -572,8 +572,10 @@ __device__ __forceinline__ void append_run(const KvAppendArgs& a, int t, long lo
 }
 
 // Waves a SIMD, as the rows of a run stay in registers, and with a rotation the
-// angles of some.  12071 tokens of 8 heads of 128 in blocks of 32 with a rotation:
-// 4 waves (their registers spill) 43 us, with 32 heads of queries 83; 3 waves 33, 62.
+// angles of some.  12071 tokens of 8 heads of 128 with a rotation, in blocks of 32:
+// 4 waves (their registers spill) 43 us, with 32 heads of queries 83; 3 waves (3 to 5 of
+// them spill) 34, 65; 2 waves (none) 38, 76.  In blocks of 64: 2 waves (19 spill) 51, 91;
+// 1 wave (none) 88, 144.  Without a rotation 20 and 30 us, in blocks of 16 18, rotated 26.
 template <int D, int B, bool kRotate>
 constexpr int kAppendWaves = kRotate ? (B * D > 4096 ? 2 : B * D > 2048 ? 3 : 4) : B == 64 ? 2 : 4;
 

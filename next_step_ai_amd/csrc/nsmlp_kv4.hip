@@ -23,9 +23,11 @@ typedef __bf16 bf2_t __attribute__((ext_vector_type(2)));
 // of their own.
 //
 // What bounds it: the rows' way from HBM, and the queries' way in and out.  12071
-// tokens of 8 heads of 128 (49 MB in, 13 MB out) 13.7 us, 4.6 TB/s; K rotated on
-// the way 20 us (the angles, and products in 64 bits); with 32 heads of queries
-// (198 MB more) 49 us, 5.3 TB/s.  Few tokens take one chain of slot, rows,
+// tokens of 8 heads of 128 (49 MB in, 13 MB out) 14 us, 4.4 TB/s; K rotated on
+// the way 20.9 us (6 MB of angles, and position and angles one after the other before a
+// row can be stored; a kernel without the query branch, whose 40 registers leave room for
+// all eight waves a SIMD where 109 leave it for four, 20.2); with 32 heads of queries (198
+// MB more) 50 us, 5.2 TB/s.  Few tokens take one chain of slot, rows,
 // positions, angles: 1 token 2.8 us, 64 tokens with their queries 3.5.
 constexpr int kAppend4Threads = 256;
 

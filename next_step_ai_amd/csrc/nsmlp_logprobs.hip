@@ -18,12 +18,17 @@
 // bound is the n-th largest of the lanes' own maxima of the first batch.  So nearly
 // all vectors cost one comparison.  A NaN counts as below every number.
 //
-// What bounds it: many rows, the logits' way from HBM and, nearly as much, the
-// vector instructions (an exp2 and seven others for a logit): 2048 rows of 128256 in
-// bf16 with 5 alternatives (525 MB) 113 us, 4.6 TB/s.  One row, the chain of a
-// load, the selection and the joins: 128256 in fp16 5.0 us without alternatives,
-// 9.9 with 5, 11.5 with 20, 26 with 64, where candidates are counted against each
-// other.
+// What bounds it: many rows, the vector instructions, an exp2 and nine others for a
+// logit, which are issued in 94% of the cycles: 2048 rows of 128256 in bf16 with 5
+// alternatives (525 MB) 113 to 116 us, 4.6 TB/s, without alternatives 101, where a kernel
+// that only reads takes 84 (6.25 TB/s).  In fp32, twice the bytes, 192 us (5.5 TB/s; in
+// 75%).  One row, the chain of a load, the selection and the joins: 128256 in fp16 5.4 us
+// without alternatives, 10.2 with 5, 26 with 64, where candidates are counted against
+// each other.
+//
+// The sums are joined in the order of their workgroups, whoever ends last.  How many
+// workgroups a row has depends on the number of rows, and with it the order of the
+// fp32 sums: a row's numbers may differ in their last bits between calls of other rows.
 #include <algorithm>
 #include <type_traits>
 
@@ -496,9 +501,10 @@ __global__ void __launch_bounds__(kLpThreads, 5) k_token_logprobs(LogprobArgs a)
 // Workgroups of a row: about kLpTarget in all, four a CU, with whole batches of vectors
 // for every wave (but the row's last: what a batch has past its workgroup's share is
 // read and weighed all the same; 5 alternatives of 150 rows of 128256 in bf16 19 us, in
-// even shares 24, of 900 rows of 10000 in fp16 19.1 and 19.7).  With 512, 1024 and 2048, 5 alternatives of 300 rows of 128256
-// in bf16 take 30, 27 and 32 us, of 700 rows 46.5, 48.4 and 50.3, of 256 rows of 32000
-// 11.7, 12.0 and 11.9; fewer rows have their most in all three.
+// even shares 24, of 900 rows of 10000 in fp16 19.1 and 19.7).  In even shares, with
+// 512, 1024 and 2048, 5 alternatives of 300 rows of 128256 in bf16 took 30, 27 and 32
+// us, of 700 rows 46.5, 48.4 and 50.3, of 256 rows of 32000 11.7, 12.0 and 11.9; fewer
+// rows have their most in all three.
 constexpr int kLpTarget = 1024;
 struct Splits {
   int count, each;

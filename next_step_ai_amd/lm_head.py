@@ -186,7 +186,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     logit on, the lower id first among equals.  A logit of -inf has no
     probability; a row of nothing else gives -inf and an entropy of 0, one with a
     NaN or +inf gives NaN, and so does a token outside [0, V), such as -1 for a
-    row without one.  ``ws``: a uint8 workspace that ``nsmlp_workspace_init`` has
+    row without one.  Equal calls give equal bits; a row's numbers may differ in
+    their last bits between calls of other numbers of rows, as few rows' fp32 sums
+    are shared out.  ``ws``: a uint8 workspace that ``nsmlp_workspace_init`` has
     cleared, in place of the stream's own."""
     device = require_device(logits, "logits")
     if current_device() != device.index:
