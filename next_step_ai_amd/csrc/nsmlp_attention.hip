@@ -105,8 +105,8 @@ __device__ __forceinline__ float reference_of(float top) {
 }
 __device__ __forceinline__ float far_exponent(float s, float g, float lv, float m) {
 #pragma clang fp contract(off)
-  const float e = (s * g - m) + lv;
-  return is_far(m) && e > 15.0f ? 15.0f : e;  // (a NaN stays one, which fminf would not keep)
+  const float t = s * g;
+  return is_far(m) ? __builtin_elementwise_minimum((t - m) + lv, 15.0f) : (t - m) + lv;  // (a NaN stays one)
 }
 
 // Pages of a range of keys, held one per lane: 64 pages from page `first`.  (In 4
