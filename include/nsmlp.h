@@ -456,12 +456,13 @@ int nsmlp_dense_linear_nf4_f16(const nsmlp_nf4_matrix* w, const void* x, int row
  *   indices, largest first, the lower index first among equals (-0 equals +0),
  *   and their log p.
  * rows is at most 2^24 - 1 and vocab 2^30.  fp32 sums, whose order, and with it a
- * number's last bits, depends on rows and vocab.  A logit of -inf has p =
- * 0; where a row has nothing else, its log probabilities are -inf and its entropy is 0.  A NaN or +inf in a row makes all
- * its numbers NaN; a NaN is below every number in the order of top_ids.  A token
- * outside [0, vocab), such as -1 for a row without one, gives NaN.  No
- * counterpart in the reference, whose samplers work on the logits in torch.  ws
- * (needed where nsmlp_token_logprobs_workspace_bytes is not 0) is cleared once
+ * number's last bits, depends on rows and vocab.  A logit of -inf has p = 0; where
+ * a row has nothing else, its log probabilities are -inf and its entropy is 0.  A
+ * NaN or +inf in a row makes all its numbers NaN; a NaN is below every number in
+ * the order of top_ids.  A token outside [0, vocab), such as -1 for a row without
+ * one, gives NaN.  No counterpart in the reference, whose samplers work on the
+ * logits in torch.  ws (needed where nsmlp_token_logprobs_workspace_bytes is not
+ * 0) is cleared once
  * by nsmlp_workspace_init. */
 size_t nsmlp_token_logprobs_workspace_bytes(int rows, int vocab, int dtype, int top);
 int nsmlp_token_logprobs(const void* logits, long long row_stride, int dtype, int rows, int vocab, const int64_t* tokens, int top,
@@ -592,9 +593,9 @@ typedef struct nsmlp_rotary {
  * positions[n]: a row of K whose position is not in the table becomes NaN.
  * q [n][q_heads][head_dim] (strides as k's; NULL: none) goes to q_out, which
  * may be q itself with the same strides.  A q_out that overlaps q otherwise, k or
- * v is refused (slices of one projection or buffer do not).  A
- * row whose position is negative (a token of no request) is left as it was in
- * q_out, one past the table becomes NaN.  k is not changed. */
+ * v is refused (slices of one projection or buffer do not).  A row whose position
+ * is negative (a token of no request) is left as it was in q_out, one past the
+ * table becomes NaN.  k is not changed. */
 int nsmlp_kv_append_rotated(const nsmlp_kv_cache* cache, const nsmlp_rotary* rotary, const void* k, long long k_row_stride,
                             long long k_head_stride, const void* v, long long v_row_stride, long long v_head_stride, int dtype,
                             const int64_t* slots, const int32_t* positions, int n, const void* q, long long q_row_stride,
@@ -674,11 +675,11 @@ int nsmlp_kv_commit(const nsmlp_kv_batch* batch, const nsmlp_kv_step* step, cons
  * (or past max_blocks) hides its keys and sets
  * NSMLP_STATUS_BLOCK_UNAVAILABLE in the workspace's status word.  A row that sees
  * a key that is not finite is NaN, whatever the other scores are, and so is one
- * with a score past fp32's range.  fp32 scores and sums; a softmax weight is an fp16 operand of the products, or two (22 bits)
- * where a request has up to 16 rows per K/V head; the result does not depend on
- * how the work is scheduled, only on the batch's lengths.  scale > 0.  The step
- * is one that nsmlp_kv_plan has written; ws is cleared once by
- * nsmlp_workspace_init. */
+ * with a score past fp32's range.  fp32 scores and sums; a softmax weight is an
+ * fp16 operand of the products, or two (22 bits) where a request has up to 16 rows
+ * per K/V head; the result does not depend on how the work is scheduled, only on
+ * the batch's lengths.  scale > 0.  The step is one that nsmlp_kv_plan has written;
+ * ws is cleared once by nsmlp_workspace_init. */
 size_t nsmlp_paged_attention_workspace_bytes(const nsmlp_kv_batch* batch, int total, int max_new, int head_dim);
 int nsmlp_paged_attention(const nsmlp_kv_cache* cache, const nsmlp_kv_batch* batch, const nsmlp_kv_step* step, const void* q,
                           long long q_row_stride, long long q_head_stride, int dtype, float scale, void* out, float* lse,

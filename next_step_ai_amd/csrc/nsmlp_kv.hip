@@ -684,7 +684,7 @@ void append_typed(KvAppendArgs a, hipStream_t s) {
   // chain where they are few: 512 tokens of 16 heads of 64, 32 of them single ones, 6.7,
   // 5.4, 7.4; 256 of 32 heads, 16 of them, 6.4, 5.4, 7.5; a prompt of 128 of 32 heads of
   // 128 in blocks of 64 with a rotation 14.4, 16.3, 16.1.  (Heads of 64 and 128, blocks of
-  // 16 to 64, 2 to 64 of them, int8 and e4m3: none slower than with 1 by more than 4%.)
+  // 16 to 64, 2 to 64 of them, int8 and e4m3: none slower than with 1 by more than 2%.)
   const long long pairs = (long long)a.n * a.c.heads * 2;
   a.take = pairs >= 128 * 1024                  ? 16
            : pairs >= 32 * 1024                 ? 8

@@ -407,7 +407,7 @@ def paged_attention(q: torch.Tensor, cache: KvCache, step: KvStep, *, scale: flo
             or out.data_ptr() % 16:
         raise RuntimeError(f"out must be a contiguous, 16-byte aligned {dtype} tensor {(total, heads, dim)} on {device}")
     elif total and _overlap(q, out) and not (out.data_ptr() == qp and q.is_contiguous()):
-        # (a row of q is read by the workgroups that write the same row of out, and by no others)
+        # (in place: a row of out is written when all that read the same row of q have done so)
         raise RuntimeError("out overlaps q: it must be q's own memory, both contiguous, or lie apart from it")
     if lse is not None and (lse.dtype != torch.float32 or lse.device != device or tuple(lse.shape) != (total, heads)
                             or not lse.is_contiguous()):
